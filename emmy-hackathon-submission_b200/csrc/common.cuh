@@ -1,0 +1,82 @@
+// What the hand-written CUDA entry points share: the error channel, launches that overlap the
+// kernel before them, and the descriptions of a paged cache as the kernels see it.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/ptxgen_b200.h"
+
+// Records `msg` as the calling thread's last error (launcher.cpp) and returns `code`.
+int pg_detail_fail(int code, const char *msg);
+
+namespace pg {
+
+inline int runtime_fail(cudaError_t e, const char *what) {
+  char buf[512];
+  snprintf(buf, sizeof buf, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
+  return pg_detail_fail(PG_ERR_RUNTIME, buf);
+}
+
+__attribute__((format(printf, 1, 2))) inline int argument_fail(const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return pg_detail_fail(PG_ERR_ARGUMENT, buf);
+}
+
+// Launches with programmatic stream serialization: the kernel's blocks may become resident
+// while the kernel ahead of it on the stream drains, which hides a launch's set-up. Every kernel
+// launched this way calls cudaGridDependencySynchronize() before its first access to memory, in
+// every thread and on every path, so it still sees all that came before it and a kernel behind
+// it cannot run ahead of what this one waits for.
+template <class... P, class... A>
+int launch(const char *name, void (*kernel)(P...), dim3 grid, int block, int smem,
+           cudaStream_t stream, A... args) {
+  cudaError_t e;
+  if (smem > 48 * 1024) {
+    e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return runtime_fail(e, name);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  if (e != cudaSuccess) return runtime_fail(e, name);
+  return PG_OK;
+}
+
+inline int sm_count(int *out) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, device);
+  return e == cudaSuccess ? PG_OK : runtime_fail(e, "cudaDeviceGetAttribute");
+}
+
+__device__ __forceinline__ void wait_for_earlier_kernels() {
+#if defined(__CUDA_ARCH__)
+  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
+#endif
+}
+
+__device__ __forceinline__ uint4 load16(const void *p) {
+  return *reinterpret_cast<const uint4 *>(p);
+}
+
+}  // namespace pg

@@ -1,0 +1,126 @@
+"""Attention over a paged key-value cache: one new token a sequence, or several.
+
+    ws = Workspace()                                     # once, one per stream
+    out = decode(q, k, v, table, lens, workspace=ws)     # q [batch, heads, dim]
+    out = prompt(q, starts, k, v, table, lens, workspace=ws)   # q [tokens, heads, dim]
+
+``k`` and ``v`` are one layer's pages [pages, kv_heads, page_size, dim] (``PagedCache.k[layer]``),
+``table`` [slots, width] and ``lens`` [slots] the cache's; sequence b of the batch is row
+``slots[b]`` of them, or row b. The queries are a sequence's last tokens, already written to the
+cache: row b of q for ``decode``, rows ``starts[b]`` to ``starts[b + 1]`` for ``prompt``. A query
+at position p sees key j when j <= p and, with a ``window``, j > p - window or j < ``sinks``. A
+query that sees no key gives zeros; what lies past a sequence's length or in a masked place is
+never part of a result. Each group of heads / kv_heads query heads reads one kv head.
+
+q, k and v have one dtype (f32, bf16 or f16) and a head size of up to 256 whose rows are a
+multiple of 16 bytes; q may be a slice of a fused projection. Sums and the softmax are held in 32
+bits. Nothing waits for the GPU; what only the device can see (a slot or page id out of range) is
+left out and sets bits that ``Workspace.check`` raises as ``CacheError``. The kernels are
+``csrc/attention*.cu`` (``pg_attention``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Any
+
+from .cache import CacheError, int32_list
+from .logprob import _dtype_code
+from .runtime import AttentionArgs, _check, library, torch_stream
+
+WORKSPACE_BYTES = 64 << 20  # PG_ATTENTION_WORKSPACE
+DIM_MAX = 256  # PG_ATTENTION_DIM
+
+
+class Workspace:
+    """The device memory in which attention leaves the parts of a long sequence's result until
+    they are joined. One per stream: calls that overlap on the GPU must not share it."""
+
+    def __init__(self, device: Any = None):
+        import torch
+
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None \
+            else torch.device(device)
+        self.buffer = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.int32, device=self.device)
+
+    def check(self) -> None:
+        """Wait for the GPU and raise ``CacheError`` if an earlier call met a slot, page id or
+        starts out of range (the bits are cleared)."""
+        bits = int(self.buffer[0].item())
+        if bits:
+            self.buffer[0].zero_()
+            raise CacheError(bits)
+
+
+def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any,
+          scale: float | None, window: int, sinks: int, max_len: int | None, workspace: Workspace,
+          out: Any, stream: int | None) -> Any:
+    import torch
+
+    dev, dtype, size = q.device, q.dtype, q.element_size()
+    if q.dim() != 3 or not q.is_cuda or q.stride(2) != 1:
+        raise ValueError(f"q: want [tokens, heads, dim] on a CUDA device with contiguous rows, "
+                         f"got {tuple(q.shape)} {q.stride()} on {dev}")
+    tokens, hq, dim = q.shape
+    for name, t in (("k", k), ("v", v)):
+        if t.dim() != 4 or t.dtype != dtype or t.device != dev or t.shape != k.shape or \
+                t.shape[3] != dim or t.stride(3) != 1 or t.stride(2) != dim:
+            raise ValueError(f"{name}: want {dtype} [pages, kv_heads, page_size, {dim}] on {dev} "
+                             f"with a head's rows of one page one after another, got {t.dtype} "
+                             f"{tuple(t.shape)} {t.stride()} on {t.device}")
+    pages, heads, page_size = k.shape[:3]
+    if hq % heads:
+        raise ValueError(f"{hq} query heads are no multiple of {heads} kv heads")
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1 or \
+            table.device != dev:
+        raise ValueError(f"table: want int32 [slots, width] on {dev} with contiguous rows")
+    rows, width = table.shape
+    if slots is not None:
+        batch = slots.shape[0]
+        slots = int32_list("slots", slots, dev)
+    else:
+        batch = rows if starts is None else starts.shape[0] - 1
+        slots = 0
+        if batch > rows:
+            raise ValueError(f"{batch} sequences, but table has {rows} rows")
+    if starts is None:
+        if batch != tokens:
+            raise ValueError(f"q has {tokens} tokens for {batch} sequences")
+    else:
+        starts = int32_list("starts", starts, dev, batch + 1)
+    if workspace.device != dev:
+        raise ValueError(f"the workspace is on {workspace.device}, q on {dev}")
+    if out is None:
+        out = torch.empty((tokens, hq, dim), dtype=dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(2) != 1:
+        raise ValueError(f"out: want {dtype} {tuple(q.shape)} on {dev} with contiguous rows")
+    qs, os_, ks, vs = q.stride(), out.stride(), k.stride(), v.stride()
+    args = AttentionArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts or 0, slots,
+        table.data_ptr(), int32_list("lens", lens, dev, rows), workspace.buffer.data_ptr(),
+        WORKSPACE_BYTES, qs[0] * size, qs[1] * size, os_[0] * size, os_[1] * size,
+        ks[0] * size, ks[1] * size, vs[0] * size, vs[1] * size, table.stride(0),
+        _dtype_code(dtype), batch, tokens, heads, hq // heads, dim, page_size, pages, width, rows,
+        window, sinks, max_len or 0, dim ** -0.5 if scale is None else scale)
+    with torch_stream(dev, stream) as s:
+        _check(library().pg_attention(ctypes.byref(args), s), "pg_attention")
+    return out
+
+
+def decode(q: Any, k: Any, v: Any, table: Any, lens: Any, *, workspace: Workspace,
+           slots: Any = None, scale: float | None = None, window: int = 0, sinks: int = 0,
+           max_len: int | None = None, out: Any = None, stream: int | None = None) -> Any:
+    """Attention of one new token a sequence, ``q`` [batch, heads, dim]: the last of each
+    sequence's ``lens`` tokens. ``max_len`` may name the longest length (it only shapes the
+    launch); ``scale`` is dim ** -0.5 by default."""
+    return _call(q, None, k, v, table, lens, slots, scale, window, sinks, max_len, workspace, out,
+                 stream)
+
+
+def prompt(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, *, workspace: Workspace,
+           slots: Any = None, scale: float | None = None, window: int = 0, sinks: int = 0,
+           max_len: int | None = None, out: Any = None, stream: int | None = None) -> Any:
+    """Causal attention of each sequence's last tokens, ``q`` [tokens, heads, dim] with sequence
+    b's in rows ``starts[b]`` to ``starts[b + 1]`` (int32, on the device)."""
+    return _call(q, starts, k, v, table, lens, slots, scale, window, sinks, max_len, workspace,
+                 out, stream)

@@ -1,7 +1,7 @@
 """Builds the native launcher library in-tree (``ptxgen/_lib/libptxgen_b200.so``).
 
 The launcher is host C++ over the CUDA driver API (``csrc/launcher.cpp``); the library also
-holds one hand-written sm_100a kernel pair (``csrc/noalloc_sum.cu``, compiled by nvcc and linked
+holds the hand-written sm_100a kernels (``csrc/*.cu``, compiled by nvcc side by side and linked
 with the static CUDA runtime, which loads libcuda only at its first call). Both build on a
 machine without a GPU.
 """
@@ -11,6 +11,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -37,7 +38,8 @@ def stale() -> bool:
         return True
     built = LIB.stat().st_mtime
     header = ROOT.parent / "include" / "ptxgen_b200.h"
-    return any(p.stat().st_mtime > built for p in [*sources(), *cuda_sources(), header]
+    return any(p.stat().st_mtime > built
+               for p in [*sources(), *cuda_sources(), *CSRC.glob("*.cuh"), header]
                if p.exists())
 
 
@@ -51,16 +53,17 @@ def build_library(force: bool = False) -> Path:
     LIB_DIR.mkdir(exist_ok=True)
     tmp = LIB.with_suffix(f".so.tmp{os.getpid()}")
     nvcc = CUDA_HOME / "bin" / "nvcc"
-    objs = []
-    for cu in cuda_sources():
-        obj = LIB_DIR / f"{cu.stem}.o.tmp{os.getpid()}"
-        _run([str(nvcc), NVCC_ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-              "-c", str(cu), "-o", str(obj)])
-        objs.append(obj)
+    objs = [LIB_DIR / f"{cu.stem}.o.tmp{os.getpid()}" for cu in cuda_sources()]
+    with ThreadPoolExecutor(max_workers=os.cpu_count()) as pool:
+        done = [pool.submit(_run, [str(nvcc), NVCC_ARCH, "-lineinfo", "-O3", "-std=c++17",
+                                   "-Xcompiler", "-fPIC", "-c", str(cu), "-o", str(obj)])
+                for cu, obj in zip(cuda_sources(), objs)]
     cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-Wextra",
            f"-I{CUDA_HOME / 'include'}", *map(str, sources()), *map(str, objs), "-o", str(tmp),
            f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static", "-lrt", "-lpthread", "-ldl"]
     try:
+        for d in done:
+            d.result()
         _run(cmd)
     finally:
         for obj in objs:

@@ -1,0 +1,111 @@
+"""Log probabilities of given tokens, with the distribution's entropy and its top alternatives.
+
+    r = logprobs(logits, tokens, top=5)          # r.logp, r.entropy, r.top_logp, r.top_ids
+    d_logits = logprobs_grad(logits, tokens, r, d_logp, d_entropy)
+
+For a row x of ``logits`` [rows, vocab] (f32, bf16 or f16; rows may lie apart) and p =
+softmax(x): ``logp`` = log p[token], ``entropy`` = -sum p log p, ``norm`` = (max x, log sum
+exp(x - max x)), and the ``top`` largest log probabilities with their columns, ties to the lowest column. All are f32 from
+32-bit sums. Token -1 means there is none: its ``logp`` is 0 and has no gradient. A token outside
+[-1, vocab) gives NaN, as does a row with a NaN, a +inf or nothing but -inf; a column of -inf has
+probability 0. ``logprobs_grad`` is the gradient of ``logp`` and ``entropy`` with respect to the
+logits, in their type; either incoming gradient may be None.
+
+The kernels are ``csrc/logprob.cu`` (``pg_logprobs``, ``pg_logprobs_grad``); calls run on the
+current stream, or on ``stream`` (a ``cudaStream_t`` as an integer).
+"""
+
+from __future__ import annotations
+
+from typing import Any, NamedTuple
+
+from .runtime import _check, library, torch_stream
+
+TOP_MAX = 32  # PG_LOGPROB_TOP
+
+
+class LogProbs(NamedTuple):
+    logp: Any  # [rows] f32
+    entropy: Any  # [rows] f32
+    norm: Any  # [rows, 2] f32: the largest logit m, and log sum exp(x - m)
+    top_logp: Any  # [rows, top] f32, largest first
+    top_ids: Any  # [rows, top] int32
+
+
+def _dtype_code(dtype: Any) -> int:
+    import torch
+
+    code = {torch.float16: 1, torch.bfloat16: 2, torch.float32: 3}.get(dtype)
+    if code is None:
+        raise ValueError(f"dtype {dtype}: want float32, bfloat16 or float16")
+    return code
+
+
+def _inputs(logits: Any, tokens: Any) -> tuple[int, int, int, int, int, int, int]:
+    import torch
+
+    if logits.dim() != 2 or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits: want [rows, vocab] on a CUDA device with contiguous rows, got "
+                         f"{tuple(logits.shape)} {logits.stride()} on {logits.device}")
+    rows, vocab = logits.shape
+    if tokens.dtype not in (torch.int64, torch.int32) or tuple(tokens.shape) != (rows,) or \
+            not tokens.is_contiguous() or tokens.device != logits.device:
+        raise ValueError(f"tokens: want contiguous int64 or int32 [{rows}] on {logits.device}, "
+                         f"got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
+    return (logits.data_ptr(), logits.stride(0), _dtype_code(logits.dtype), tokens.data_ptr(),
+            tokens.element_size(), rows, vocab)
+
+
+def _per_row(name: str, t: Any, logits: Any, *more: int) -> int:
+    import torch
+
+    if t is None:
+        return 0
+    shape = (logits.shape[0], *more)
+    if t.dtype is not torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or \
+            t.device != logits.device:
+        raise ValueError(f"{name}: want contiguous float32 {list(shape)} on {logits.device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def logprobs(logits: Any, tokens: Any, top: int = 0, stream: int | None = None) -> LogProbs:
+    """``LogProbs`` of ``tokens`` [rows] under ``logits`` [rows, vocab], with the ``top`` (at
+    most 32) largest log probabilities of each row."""
+    import torch
+
+    args = _inputs(logits, tokens)
+    rows, vocab = logits.shape
+    if not 0 <= top <= min(TOP_MAX, vocab):
+        raise ValueError(f"top {top}: want 0 to {min(TOP_MAX, vocab)}")
+    logp, entropy = torch.empty((2, rows), dtype=torch.float32, device=logits.device).unbind(0)
+    norm = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
+    top_logp = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+    top_ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+    with torch_stream(logits.device, stream) as s:
+        _check(library().pg_logprobs(
+            *args, top, logp.data_ptr(), entropy.data_ptr(), norm.data_ptr(), top_logp.data_ptr(),
+            top_ids.data_ptr(), s), "pg_logprobs")
+    return LogProbs(logp, entropy, norm, top_logp, top_ids)
+
+
+def logprobs_grad(logits: Any, tokens: Any, result: LogProbs, d_logp: Any, d_entropy: Any = None,
+                  out: Any = None, stream: int | None = None) -> Any:
+    """The gradient of sum(d_logp * logp + d_entropy * entropy) with respect to ``logits``, given
+    ``result`` = ``logprobs(logits, tokens)``; into ``out`` (which may be ``logits``) if given."""
+    import torch
+
+    args = _inputs(logits, tokens)
+    if out is None:
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \
+            or (out.shape[1] > 1 and out.stride(1) != 1):
+        raise ValueError(f"out: want {logits.dtype} {tuple(logits.shape)} on {logits.device} "
+                         "with contiguous rows")
+    with torch_stream(logits.device, stream) as s:
+        _check(library().pg_logprobs_grad(
+            *args, _per_row("norm", result.norm, logits, 2),
+            _per_row("entropy", result.entropy, logits), _per_row("d_logp", d_logp, logits),
+            _per_row("d_entropy", d_entropy, logits), out.data_ptr(), out.stride(0), s),
+            "pg_logprobs_grad")
+    return out

@@ -39,6 +39,38 @@ class KernelStatusError(LaunchError):
     """A kernel reported a failure through its status word (a bounded wait gave up)."""
 
 
+class Cache(ctypes.Structure):
+    """``pg_cache``: a paged key-value cache (``ptxgen.cache``)."""
+
+    _fields_ = [*((n, ctypes.c_uint64) for n in ("k", "v")),
+                *((n, ctypes.c_int64) for n in ("layer_stride", "page_stride", "head_stride")),
+                *((n, ctypes.c_uint64) for n in ("refs", "table", "lens", "status", "scratch")),
+                *((n, ctypes.c_int64) for n in ("table_stride", "scratch_words")),
+                *((n, ctypes.c_int32) for n in ("layers", "pages", "heads", "page_size",
+                                                "row_bytes", "slots", "width"))]
+
+
+class Rows(ctypes.Structure):
+    """``pg_rows``: rows of new keys or values."""
+
+    _fields_ = [("data", ctypes.c_uint64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """``pg_attention_args``: attention over a paged cache (``ptxgen.attention``)."""
+
+    _fields_ = [*((n, ctypes.c_uint64) for n in ("q", "k", "v", "out", "starts", "slots", "table",
+                                                 "lens", "workspace")),
+                *((n, ctypes.c_int64) for n in ("workspace_bytes", "q_token", "q_head",
+                                                "out_token", "out_head", "k_page", "k_head",
+                                                "v_page", "v_head", "table_stride")),
+                *((n, ctypes.c_int32) for n in ("dtype", "batch", "queries", "heads", "group",
+                                                "dim", "page_size", "pages", "width",
+                                                "slot_rows", "window", "sinks", "max_len")),
+                ("scale", ctypes.c_float)]
+
+
 _lib: ctypes.CDLL | None = None
 _lock = threading.Lock()
 _initialised: set[int] = set()
@@ -80,6 +112,18 @@ def library() -> ctypes.CDLL:
                 "pg_ipc_open": [vp, pu64],
                 "pg_ipc_close": [u64],
                 "pg_grid_sum_f32_noalloc": [u64, u64, u64, u32, u64],
+                "pg_cache_extend": [ctypes.POINTER(Cache), u64, u64, i32, u64],
+                "pg_cache_write": [ctypes.POINTER(Cache), i32, u64, u64, i32, i32, ctypes.POINTER(Rows),
+                                   ctypes.POINTER(Rows), u64],
+                "pg_cache_free": [ctypes.POINTER(Cache), u64, i32, u64],
+                "pg_cache_copy": [ctypes.POINTER(Cache), u64, u64, i32, u64],
+                "pg_cache_fork": [ctypes.POINTER(Cache), u64, u64, i32, u64],
+                "pg_cache_compact": [ctypes.POINTER(Cache), u64],
+                "pg_attention": [ctypes.POINTER(AttentionArgs), u64],
+                "pg_logprobs": [u64, ctypes.c_int64, i32, u64, i32, i32, i32, i32, u64, u64, u64,
+                                u64, u64, u64],
+                "pg_logprobs_grad": [u64, ctypes.c_int64, i32, u64, i32, i32, i32, u64, u64, u64,
+                                     u64, u64, ctypes.c_int64, u64],
             }
             for name, args in sig.items():
                 fn = getattr(lib, name)
@@ -101,6 +145,31 @@ def init(device: int = 0) -> None:
     lib = library()
     _check(lib.pg_init(device), f"pg_init({device})")
     _initialised.add(device)
+
+
+class torch_stream:
+    """``with torch_stream(device, stream) as s``: the stream to launch on, as an integer
+    (``device``'s current one where ``stream`` is None), with ``device`` current inside."""
+
+    def __init__(self, device: Any, stream: int | None = None):
+        self.device, self.stream, self.before = device, stream, None
+
+    def __enter__(self) -> int:
+        import torch
+
+        index = self.device.index
+        now = torch.cuda.current_device()
+        if now != index:
+            self.before = now
+            torch.cuda.set_device(index)
+        return torch.cuda.current_stream(index).cuda_stream if self.stream is None \
+            else self.stream
+
+    def __exit__(self, *exc: Any) -> None:
+        if self.before is not None:
+            import torch
+
+            torch.cuda.set_device(self.before)
 
 
 def header_notes(ptx: str) -> dict[str, list[str]]:

@@ -181,6 +181,133 @@ int pg_run_host(pg_kernel *kernel, uint32_t grid, uint32_t block, uint32_t smem_
 int pg_grid_sum_f32_noalloc(uint64_t x, uint64_t n, uint64_t out, uint32_t blocks,
                             uint64_t stream);
 
+/* --- the paged key-value cache --------------------------------------------------------------
+ *
+ * No counterpart in the reference, whose attention kernels read whole K and V matrices. A cache
+ * holds the keys and values of `slots` sequences in `pages` pages of `page_size` tokens. Element
+ * (layer, page, head, row, byte) of the keys is at k + layer * layer_stride + page * page_stride +
+ * head * head_stride + row * row_bytes + byte, and the values are laid out the same from v. Slot s
+ * holds lens[s] tokens; token t is row t % page_size of page table[s * table_stride + t /
+ * page_size]. refs[p] counts the table rows that name page p; a page whose count is 0 is free,
+ * and a call that takes pages takes the lowest free ones, in the order of its slots.
+ *
+ * The calls are asynchronous on `stream` and never wait for the host. What only the device can
+ * see (no page left, a slot listed twice, a page id out of range) sets PG_CACHE_* bits of the
+ * status word, which the caller clears: extend and fork then change nothing, free, write and
+ * copy skip the entry. All calls on one cache share its scratch words and so belong on one
+ * stream at a time. */
+typedef struct pg_cache {
+  uint64_t k, v;                                    /* device addresses, 16-byte aligned */
+  int64_t layer_stride, page_stride, head_stride;   /* bytes, multiples of 16 */
+  uint64_t refs, table, lens;                       /* int32: [pages], [slots, width], [slots] */
+  uint64_t status;                                  /* one uint32 */
+  uint64_t scratch;                                 /* int32[scratch_words], any contents */
+  int64_t table_stride, scratch_words;              /* words */
+  int32_t layers, pages, heads, page_size;
+  int32_t row_bytes;                                /* one token's keys of one head */
+  int32_t slots, width;
+} pg_cache;
+
+/* Rows of new keys or values: token t's head h is row_bytes bytes at data + t * token_stride +
+ * h * head_stride (bytes, multiples of 16). */
+typedef struct pg_rows {
+  uint64_t data;
+  int64_t token_stride, head_stride;
+} pg_rows;
+
+#define PG_CACHE_SCRATCH(pages, slots) (4 + 3 * (int64_t)(pages) + 2 * (int64_t)(slots) + 2)
+
+#define PG_CACHE_NO_PAGES 1u /* fewer free pages than a call needs */
+#define PG_CACHE_BAD_SLOT 2u /* a slot out of range, listed twice, or a fork's child in use */
+#define PG_CACHE_BAD_PAGE 4u /* a page id or count that cannot be */
+#define PG_CACHE_TOO_LONG 8u /* more tokens than a table row has pages for */
+
+/* Makes room for the new tokens of n sequences: slots[i] grows by starts[i + 1] - starts[i]
+ * tokens (starts: n + 1 ascending int32 on the device), taking pages as needed. */
+int pg_cache_extend(const pg_cache *cache, uint64_t slots, uint64_t starts, int32_t n,
+                    uint64_t stream);
+
+/* Writes one layer's rows of the last tokens of n sequences: token t of the `tokens` rows, with
+ * starts[i] <= t < starts[i + 1], lands at position lens[slots[i]] - starts[i + 1] + t. */
+int pg_cache_write(const pg_cache *cache, int32_t layer, uint64_t slots, uint64_t starts,
+                   int32_t n, int32_t tokens, const pg_rows *k, const pg_rows *v,
+                   uint64_t stream);
+
+/* Each of n slots lets go of its pages: counts go down, its table row becomes -1, its length 0. */
+int pg_cache_free(const pg_cache *cache, uint64_t slots, int32_t n, uint64_t stream);
+
+/* Copies page from[i] to page to[i], whole, in every layer. No page may be both a source and a
+ * destination, nor a destination twice. Counts and tables stay as they are. */
+int pg_cache_copy(const pg_cache *cache, uint64_t from, uint64_t to, int32_t n, uint64_t stream);
+
+/* children[i] (an empty slot) becomes a continuation of parents[i]: it shares the parent's full
+ * pages and gets its own copy of the rows in use of a last page that is not full. */
+int pg_cache_fork(const pg_cache *cache, uint64_t parents, uint64_t children, int32_t n,
+                  uint64_t stream);
+
+/* Moves the L live pages to ids 0..L-1: the k-th free page below L takes the k-th live page at
+ * or above L. Tables and counts follow; every other page stays where it is. */
+int pg_cache_compact(const pg_cache *cache, uint64_t stream);
+
+/* --- log probabilities ------------------------------------------------------------------------
+ *
+ * No counterpart in the reference. For each row x of `rows` rows of `vocab` logits (dtype
+ * PG_DT_F32, PG_DT_BF16 or PG_DT_F16; rows row_stride elements apart) and p = softmax(x):
+ * logp[i] = log p[tokens[i]], entropy[i] = -sum p log p, norm[i] = (m, log sum exp(x - m)) with m
+ * = max x, and the `top` (at most PG_LOGPROB_TOP) largest log probabilities with their columns in top_logp and
+ * top_ids [rows, top], ties to the lowest column. Tokens are int32 or int64 (token_bytes 4 or
+ * 8); token -1 means there is none: logp 0. A token outside [-1, vocab) gives NaN, as does a row
+ * with a NaN, a +inf or nothing but -inf. Outputs are f32, top_ids int32. Asynchronous. */
+#define PG_LOGPROB_TOP 32
+int pg_logprobs(uint64_t logits, int64_t row_stride, int32_t dtype, uint64_t tokens,
+                int32_t token_bytes, int32_t rows, int32_t vocab, int32_t top, uint64_t logp,
+                uint64_t entropy, uint64_t lse, uint64_t top_logp, uint64_t top_ids,
+                uint64_t stream);
+
+/* The gradient of sum_i d_logp[i] logp[i] + d_entropy[i] entropy[i] with respect to the logits,
+ * into out (the logits' type, rows out_stride elements apart; out may be the logits). norm and
+ * entropy are pg_logprobs's; d_logp or d_entropy may be 0 (no such gradient). Asynchronous. */
+int pg_logprobs_grad(uint64_t logits, int64_t row_stride, int32_t dtype, uint64_t tokens,
+                     int32_t token_bytes, int32_t rows, int32_t vocab, uint64_t norm,
+                     uint64_t entropy, uint64_t d_logp, uint64_t d_entropy, uint64_t out,
+                     int64_t out_stride, uint64_t stream);
+
+/* --- attention over a paged cache -------------------------------------------------------------
+ *
+ * No counterpart in the reference. Sequence b of the batch is table row s = slots[b] (b where
+ * slots is 0) with lens[s] tokens. Its queries are its last tokens: rows starts[b] to
+ * starts[b + 1] of q, or row b alone where starts is 0 (one new token a sequence). The query at
+ * position p sees key j when j <= p and (window == 0 or j > p - window or j < sinks);
+ * out = softmax(scale q . k) v over the keys it sees. A query that sees none (a length of 0, or
+ * fewer tokens than queries) gives zeros, and what lies in masked places, pages past the length
+ * or unused rows of a page is never part of a result, whatever it is. Query head h reads kv head
+ * h / group. q and out are [queries, heads * group, dim], k and v [pages, heads, page_size, dim]
+ * with a head's rows of one page one after another; all of one dtype (PG_DT_F32, PG_DT_BF16 or
+ * PG_DT_F16), with sums and softmax in 32 bits and one rounding of the result.
+ *
+ * max_len, if not 0, is at least the longest length; it only shapes the launch. The workspace
+ * must be zeroed once, belongs to one stream at a time and is left as a next call needs it. Its
+ * first word gets PG_CACHE_* bits for what only the device can see (a slot, a page id or starts
+ * out of range: such keys and queries are left out); the caller clears it. Asynchronous. */
+typedef struct pg_attention_args {
+  uint64_t q, k, v, out;
+  uint64_t starts, slots, table, lens;           /* int32 on the device; starts, slots may be 0 */
+  uint64_t workspace;                            /* 256-byte aligned */
+  int64_t workspace_bytes;                       /* at least PG_ATTENTION_WORKSPACE */
+  int64_t q_token, q_head, out_token, out_head;  /* byte strides, multiples of 16 */
+  int64_t k_page, k_head, v_page, v_head;        /* byte strides, multiples of 16 */
+  int64_t table_stride;                          /* words */
+  int32_t dtype, batch, queries, heads, group, dim;
+  int32_t page_size, pages, width, slot_rows;    /* slot_rows: rows of table and lens */
+  int32_t window, sinks, max_len;
+  float scale;
+} pg_attention_args;
+
+#define PG_ATTENTION_DIM 256
+#define PG_ATTENTION_WORKSPACE (64 << 20)
+
+int pg_attention(const pg_attention_args *args, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif
