@@ -132,6 +132,9 @@ __device__ __forceinline__ float factor(float a, float b) {
   return a == -INFINITY ? 0.0f : exp2_fast(a - b);
 }
 
+// Kernels for the 16-bit types at head sizes of up to 128 (attention_decode.cu).
+int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream);
+
 // --- host side -------------------------------------------------------------------------------
 
 constexpr int kCounters = 4096;  // (tile, kv head) pairs that may be cut in parts

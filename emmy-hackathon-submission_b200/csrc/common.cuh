@@ -41,7 +41,7 @@ template <class... P, class... A>
 int launch(const char *name, void (*kernel)(P...), dim3 grid, int block, int smem,
            cudaStream_t stream, A... args) {
   cudaError_t e;
-  if (smem > 48 * 1024) {
+  if (smem > 32 * 1024) {  // with a kernel's static shared memory more than the default 48 KiB
     e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                              cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return runtime_fail(e, name);
