@@ -310,7 +310,7 @@ int run(Attention a, int max_len, int64_t partial_bytes, int sms, cudaStream_t s
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
   const int size = rows <= 16ll * a.batch ? 16 : 64;
   const int tiles = pg::tile_bound(a, size);
-  a.parts = pg::choose_parts(a, tiles, size, kKeys, max_len, 2 * sms, partial_bytes);
+  a.parts = pg::choose_parts(a, tiles, size, a.dim, kKeys, max_len, 2 * sms, partial_bytes);
   return size == 16 ? launch_dim<T, 16>(a, tiles, stream) : launch_dim<T, 64>(a, tiles, stream);
 }
 
@@ -386,8 +386,9 @@ extern "C" int pg_attention(const pg_attention_args *p, uint64_t stream) {
   const int max_len = static_cast<int>(p->max_len && p->max_len < most ? p->max_len : most);
   const int64_t partial_bytes = p->workspace_bytes - 256 - pg::kCounters * 4ll;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
-  if (dtype != PG_DT_F32 && !p->starts && a.dim <= 128)
-    return pg::decode_16bit(a, dtype == PG_DT_BF16, sms, s);
+  if (dtype != PG_DT_F32 && a.dim <= 128)
+    return a.starts ? pg::prompt_16bit(a, dtype == PG_DT_BF16, max_len, partial_bytes, sms, s)
+                    : pg::decode_16bit(a, dtype == PG_DT_BF16, sms, s);
   if (dtype == PG_DT_F32) return run<float>(a, max_len, partial_bytes, sms, s);
   if (dtype == PG_DT_BF16) return run<__nv_bfloat16>(a, max_len, partial_bytes, sms, s);
   return run<__half>(a, max_len, partial_bytes, sms, s);

@@ -132,8 +132,11 @@ __device__ __forceinline__ float factor(float a, float b) {
   return a == -INFINITY ? 0.0f : exp2_fast(a - b);
 }
 
-// Kernels for the 16-bit types at head sizes of up to 128 (attention_decode.cu).
+// Kernels for the 16-bit types at head sizes of up to 128: one query a sequence
+// (attention_decode.cu), and several (attention_prompt.cu).
 int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream);
+int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
+                 cudaStream_t stream);
 
 // --- host side -------------------------------------------------------------------------------
 
@@ -148,8 +151,8 @@ inline int tile_bound(const Attention &a, int rows_per_tile) {
 
 // Parts that each tile's keys are cut in: enough to give `blocks` blocks work, each part at
 // least four steps of `keys` keys at the longest length, no more than the workspace holds.
-inline int choose_parts(const Attention &a, int tiles, int rows_per_tile, int keys, int max_len,
-                        int blocks, int64_t partial_bytes) {
+inline int choose_parts(const Attention &a, int tiles, int rows_per_tile, int columns, int keys,
+                        int max_len, int blocks, int64_t partial_bytes) {
   const int64_t pairs = static_cast<int64_t>(tiles) * a.heads;
   if (pairs * 2 > blocks || pairs > kCounters) return 1;
   int64_t seen = max_len;
@@ -160,7 +163,7 @@ inline int choose_parts(const Attention &a, int tiles, int rows_per_tile, int ke
   int64_t parts = blocks / pairs;
   const int64_t steps = (seen + 4ll * keys - 1) / (4ll * keys);
   parts = steps < parts ? steps : parts;
-  const int64_t each = pairs * rows_per_tile * (a.dim + 2) * 4ll;
+  const int64_t each = pairs * rows_per_tile * (columns + 2) * 4ll;
   parts = partial_bytes / each < parts ? partial_bytes / each : parts;
   return static_cast<int>(parts < 1 ? 1 : parts);
 }

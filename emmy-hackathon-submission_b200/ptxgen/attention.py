@@ -14,9 +14,10 @@ never part of a result. Each group of heads / kv_heads query heads reads one kv 
 
 q, k and v have one dtype (f32, bf16 or f16) and a head size of up to 256 whose rows are a
 multiple of 16 bytes; q may be a slice of a fused projection. Sums and the softmax are held in 32
-bits. Nothing waits for the GPU; what only the device can see (a slot or page id out of range) is
-left out and sets bits that ``Workspace.check`` raises as ``CacheError``. The kernels are
-``csrc/attention*.cu`` (``pg_attention``).
+bits. Nothing waits for the GPU; where only the device can see that a slot, page id or length is
+out of range, nothing is read, that sequence's result is not defined, and bits are set that
+``Workspace.check`` raises as ``CacheError``. The kernels are ``csrc/attention*.cu``
+(``pg_attention``).
 """
 
 from __future__ import annotations

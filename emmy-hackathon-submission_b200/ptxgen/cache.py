@@ -26,11 +26,12 @@ from typing import Any
 
 from .runtime import Cache, LaunchError, Rows, _check, library, torch_stream
 
-NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG = 1, 2, 4, 8
+NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG, WAIT = 1, 2, 4, 8, 16
 _WHY = {NO_PAGES: "fewer free pages than a call needed",
         BAD_SLOT: "a slot out of range, listed twice, or a fork's child in use",
         BAD_PAGE: "a page id or count out of range",
-        TOO_LONG: "more tokens than a table row has pages for"}
+        TOO_LONG: "more tokens than a table row has pages for",
+        WAIT: "a bounded wait inside an attention kernel gave up"}
 
 
 class CacheError(LaunchError):

@@ -288,7 +288,8 @@ int pg_logprobs_grad(uint64_t logits, int64_t row_stride, int32_t dtype, uint64_
  * max_len, if not 0, is at least the longest length; it only shapes the launch. The workspace
  * must be zeroed once, belongs to one stream at a time and is left as a next call needs it. Its
  * first word gets PG_CACHE_* bits for what only the device can see (a slot, a page id or starts
- * out of range: such keys and queries are left out); the caller clears it. Asynchronous. */
+ * out of range: nothing is read there, and that sequence's result is not defined); the caller
+ * clears it. Asynchronous. */
 typedef struct pg_attention_args {
   uint64_t q, k, v, out;
   uint64_t starts, slots, table, lens;           /* int32 on the device; starts, slots may be 0 */
@@ -303,6 +304,7 @@ typedef struct pg_attention_args {
   float scale;
 } pg_attention_args;
 
+#define PG_ATTENTION_WAIT 16u /* in the status word: a bounded wait inside a kernel gave up */
 #define PG_ATTENTION_DIM 256
 #define PG_ATTENTION_WORKSPACE (64 << 20)
 
