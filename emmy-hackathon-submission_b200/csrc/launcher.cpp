@@ -165,6 +165,27 @@ __attribute__((visibility("hidden"))) int pg_detail_fail(int code, const char *m
   return fail(code, "%s", msg);
 }
 
+// Encodes a tiled tensor map (128-byte swizzle, cuTensorMapEncodeTiled) of 2-byte elements into
+// the 128 bytes at `map`, for kernels that take theirs as a parameter. Not exported.
+__attribute__((visibility("hidden"))) int pg_detail_tensormap(void *map, int rank, uint64_t base,
+                                                              const uint64_t *dims,
+                                                              const uint64_t *strides_bytes,
+                                                              const uint32_t *box) {
+  {
+    std::lock_guard<std::mutex> lock(g_mu);
+    int rc = load_driver();
+    if (rc) return rc;
+  }
+  const cuuint32_t estride[5] = {1, 1, 1, 1, 1};
+  PG_CU(g_drv.TensorMapEncodeTiled(
+            static_cast<CUtensorMap *>(map), CU_TENSOR_MAP_DATA_TYPE_UINT16,
+            static_cast<cuuint32_t>(rank), reinterpret_cast<void *>(base), dims, strides_bytes,
+            box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+        "cuTensorMapEncodeTiled");
+  return PG_OK;
+}
+
 struct pg_module {
   CUmodule mod = nullptr;
   std::unordered_map<std::string, TmapKey> filled;
