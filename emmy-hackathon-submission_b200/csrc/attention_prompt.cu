@@ -9,13 +9,13 @@
 // tensor cores work for the other.
 //
 //   warps 0-3, 4-7  the rows' threads of tile 0 and tile 1
-//   warp 8          issues the products (one thread)
-//   warps 9-11      bring keys and values, page by page, into a ring in shared memory
+//   warp 8          issues the products, the two tiles' strictly in turn: issued as they come,
+//                   they mix, and both tiles then wait for both
+//   warps 9, 10     bring keys and values, page by page, into a ring in shared memory
 //
-// Where pages are whole groups of eight keys, one warp brings them with TMA (a box is the run of
-// keys that a page and a block of 128 always share, 128-byte swizzled as the products read it) and
-// the other two look after the blocks that some row must not see in full. Pages of other sizes
-// come in 16-byte pieces through cp.async from all three warps, whose address arithmetic then
+// Where pages are whole groups of eight keys, two warps bring them with TMA (a box is the run of
+// keys that a page and a block of 128 always share, 128-byte swizzled as the products read it).
+// Pages of other sizes come in 16-byte pieces through cp.async, whose arithmetic then
 // bounds the kernel: 4096 new tokens of up to 8192 with 32 heads take 1370 us that way, 579 with TMA.
 //
 // Exponentials bound it beside the products: 128 x 128 of them take the 16 lanes an SM has
@@ -26,10 +26,10 @@
 // Rounding: weights go into the second product in the values' type (2^-9 or 2^-12 of each, at
 // random), as the tensor cores take both operands in one type; S, m, l and O are in 32 bits.
 //
-// A masked place has weight 0, and 0 times a value that is not finite would be NaN. So the
-// warps that copy look through the values of each block that some row must not see in full,
-// zero what is not finite and raise a flag; at the end a row adds the ones it does see again.
-// Rows past the sequence's length are zeroed by the copy.
+// A masked place has weight 0, and 0 times a value that is not finite would be NaN. So the values
+// of each block that some row must not see in full are looked through before they are used: what
+// is not finite is zeroed and a flag raised, and at the end a row adds the ones it does see again.
+// Rows past the sequence's length are zeroed.
 //
 // Every wait is bounded: one that takes over two seconds sets PG_ATTENTION_WAIT in the status
 // word, and all roles leave their loops; the block then frees its tensor memory and returns.
@@ -51,17 +51,16 @@ using pg::Tile;
 
 constexpr int kKeys = 128, kRows = 256, kHalf = 128;
 constexpr int kThreads = 384;
-constexpr int kCopyWarps = 3, kCopyThreads = 32 * kCopyWarps;
-constexpr int kCleanThreads = 64;
+constexpr int kCopyWarps = 2, kCopyThreads = 32 * kCopyWarps;  // without TMA
 constexpr int kLag = 2;  // tiles whose cp.async copies are in flight before the oldest is waited for
 constexpr float kGrow = 8.0f;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 template <int DIM>
 struct Plan {
-  static constexpr int chunk = 128 * 128;         // 128 rows of 64 columns, 128-byte swizzled
-  static constexpr int chunks = DIM / 64;
-  static constexpr int tile = chunks * chunk;     // 128 queries, keys or values
+  // 128 queries, keys or values: by eight rows, then by 64 columns, each such 1024 bytes swizzled
+  static constexpr int atom = 1024, chunks = DIM / 64, group = chunks * atom;
+  static constexpr int tile = 16 * group;
   static constexpr int stages = DIM == 128 ? 5 : 8;
   static constexpr int q = 0, ring = 2 * tile, bars = ring + stages * tile;
   // over half an SM's shared memory, so that no other block that takes all its tensor memory
@@ -69,7 +68,7 @@ struct Plan {
   static constexpr int bytes = 1024 + bars + 256;
   static_assert(bytes > 116 * 1024 && bytes <= 232448 && stages > kLag + 1, "shared memory");
   __device__ static int at(int r, int piece) {    // 16-byte piece of a row
-    return (piece >> 3) * chunk + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+    return (r >> 3) * group + (piece >> 3) * atom + (r & 7) * 128 + (((piece & 7) ^ (r & 7)) << 4);
   }
 };
 
@@ -87,11 +86,18 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
                : "memory");
 }
 // One box of a tensor map into shared memory; its bytes count at the barrier.
-__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap *map, int x, int row,
-                                         int head, int page, uint32_t bar) {
+__device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap *map, int x, int y,
+                                            int z, int w, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-               "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(row),
-               "r"(head), "r"(page), "r"(bar)
+               "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z),
+               "r"(w), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t to, const CUtensorMap *map, int z, int w,
+                                            uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+               "[%0], [%1, {%2, %2, %2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(0), "r"(z),
+               "r"(w), "r"(bar)
                : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
@@ -108,7 +114,7 @@ __device__ __forceinline__ unsigned long long now_ns() {
   return t;
 }
 // Waits for a phase of a barrier; false once a wait of this block has run out of time.
-__device__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, unsigned *status) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, unsigned *status) {
   if (bar_try(bar, parity)) return true;
   const unsigned long long begin = now_ns();
   while (!bar_try(bar, parity)) {
@@ -136,24 +142,26 @@ __device__ __forceinline__ void fence_after() {
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
+// The products are issued by one lane of a warp that runs as a whole, so that operands stay in
+// uniform registers: issued from a branch of one thread's, each took longer than its work.
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t elected) {
+  asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %1, 0;\n@q tcgen05.commit.cta_group::1."
+               "mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar), "r"(elected)
                : "memory");
 }
 // D (tensor memory) = A B (+ D): both from shared memory, or A from tensor memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc,
-                                       bool add) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-               "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add,
+                                       uint32_t elected) {
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+               "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "r"(elected)
                : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc,
-                                       bool add) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
-               "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add,
+                                       uint32_t elected) {
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
+               "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "r"(elected)
                : "memory");
 }
 
@@ -183,8 +191,49 @@ __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t *v) {
 __device__ __forceinline__ void wait_loads() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+// What was loaded is used after this point only.
+__device__ __forceinline__ void tie(uint32_t *v) {
+#define PG_TIE(i) "+r"(v[i])
+  asm volatile("" : PG_R32(PG_TIE));
+#undef PG_TIE
+}
 __device__ __forceinline__ void wait_stores() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// The largest of three; NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The largest score of a row of a block, and m.
+__device__ __forceinline__ float largest(const float *s, float m) {
+  float top[4] = {m, s[0], s[1], s[2]};
+#pragma unroll
+  for (int k = 3; k < kKeys - 1; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
+  return max3(max3(top[0], top[1], top[2]), top[3], s[kKeys - 1]);
+}
+
+// Two 32-bit numbers that one instruction multiplies and adds.
+struct Two {
+  uint64_t v;
+  __device__ Two(uint64_t x) : v(x) {}
+  __device__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ void get(float &x, float &y) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+  }
+};
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two add(Two a, Two b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+  return r;
 }
 
 template <class T> struct Type;
@@ -211,11 +260,11 @@ template <> struct Type<__half> {
   }
 };
 
-// A shared-memory operand of 128-byte swizzled rows: eight rows every 1024 bytes; `apart` is the
-// distance of its 64-column chunks where columns are the product's M or N.
-__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t apart) {
-  const uint32_t lo = ((at >> 4) & 0x3fff) | ((apart >> 4) << 16);
-  const uint32_t hi = (1024 >> 4) | (1u << 14) | (2u << 29);
+// A shared-memory operand of 128-byte swizzled rows: `rows` is the distance of its groups of
+// eight, `columns` that of its 64-column chunks where columns are the product's N.
+__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t rows, uint32_t columns) {
+  const uint32_t lo = ((at >> 4) & 0x3fff) | ((columns >> 4) << 16);
+  const uint32_t hi = (rows >> 4) | (1u << 14) | (2u << 29);
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
 // 32-bit sums, M = 128, N columns; B with its N side contiguous or its K side
@@ -226,14 +275,23 @@ __device__ constexpr uint32_t product(int n, bool n_contiguous) {
          (128u >> 4 << 24);
 }
 
-// Whether every row of a tile, with queries at positions lo..hi, sees every key of the block.
-struct Range {
-  int lo, hi;
+// Which blocks of keys every row of a tile, with queries at positions lo..hi, sees in full.
+struct Seen {
+  int low, high, sinks;  // those that start in low..high, or end within the sinks
+  __device__ Seen(const Attention &a, int lo, int hi, int length)
+      : low(a.window ? hi - a.window + 1 : 0), high(min(lo + 1, length) - kKeys), sinks(a.sinks) {}
+  __device__ bool all(int key0) const {
+    return key0 <= high && (key0 >= low || key0 + kKeys <= sinks);
+  }
 };
-__device__ __forceinline__ bool all_see(const Attention &a, Range r, int key0, int length) {
-  if (key0 + kKeys > length || key0 + kKeys - 1 > r.lo) return false;
-  return !a.window || key0 > r.hi - a.window || key0 + kKeys <= a.sinks;
-}
+
+// How the tensor maps name a page's rows of a kv head: by five coordinates with heads and pages
+// in one (`per_page` of it a page), so that one box is eight rows by all columns by the rest of
+// the run, or (per_page 0) by four, a box eight rows of 64 columns.
+struct Boxes {
+  int keys;  // the keys that a page and a block always share
+  int k_per_page, v_per_page;
+};
 
 struct Head {  // what the roles share
   uint32_t tmem;
@@ -257,11 +315,11 @@ __device__ __forceinline__ bool clean(uint4 *at) {
   return any;
 }
 
-// With TMA a box is `box` keys; without, `box` is 0 and the maps are empty.
+// Without TMA the maps and `boxes` are empty.
 template <class T, int DIM, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(Attention a, const __grid_constant__ CUtensorMap k_map,
-                  const __grid_constant__ CUtensorMap v_map, int box) {
+                  const __grid_constant__ CUtensorMap v_map, Boxes boxes) {
   using P = Plan<DIM>;
   extern __shared__ char smem_raw[];
   __shared__ Head sh;
@@ -274,8 +332,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!t.rows) return;
   const int first_pos = t.length - t.count;
   const int tiles = t.rows > kHalf ? 2 : 1;
-  const Range both{first_pos + t.row / a.group, first_pos + (t.row + t.rows - 1) / a.group};
-  const Blocks blocks = pg::blocks_of(a, both.lo, both.hi, kKeys);
+  const int lo = first_pos + t.row / a.group, hi = first_pos + (t.row + t.rows - 1) / a.group;
+  const Blocks blocks = pg::blocks_of(a, lo, hi, kKeys);
+  const Seen both(a, lo, hi, t.length);
   const int b0 = static_cast<int>(static_cast<int64_t>(blocks.count) * part / a.parts);
   const int steps =
       static_cast<int>(static_cast<int64_t>(blocks.count) * (part + 1) / a.parts) - b0;
@@ -286,8 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t q_full = bars + 16 * P::stages;
   const auto s_full = [&](int i) { return q_full + 8 + 8 * i; };
   const auto p_full = [&](int i) { return q_full + 24 + 8 * i; };
-  const uint32_t o_full = q_full + 40;
-  const uint32_t to_clean = o_full + 8, cleaned = o_full + 16;
+  const uint32_t o_full = q_full + 40, cleaned = q_full + 48;
   if (tid == 0) {
     for (int s = 0; s < P::stages; ++s) {
       bar_init(full(s), TMA ? 1 : kCopyThreads);
@@ -299,8 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(p_full(i), kHalf);
     }
     bar_init(o_full, 1);
-    bar_init(to_clean, 1);
-    bar_init(cleaned, kCleanThreads);
+    bar_init(cleaned, kHalf * tiles);
     sh.failed = sh.odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -316,73 +373,59 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sh.tmem;  // S and P of tile i at 128 i, O at 256 + 128 i
   volatile int *failed = &sh.failed;
 
-  // registers: 3 x 128 threads start with 168 each; the rows' threads, which hold a row of S,
-  // take 32 more from the others' (2 x 200 + 104 = 3 x 168)
+  // Registers: three groups of 128 threads start with 168 each; the rows' threads, which hold a
+  // row of S and what is made of it, take what the third group can do without (2 x 232 + 40 or
+  // 2 x 200 + 104 = 3 x 168).
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (TMA && warp == 9) {
-      // --- copies: K and V of each block in turn, lane i the i-th box of a tile ----------------
-      const int boxes = kKeys / box;
-      const auto page_for = [&](int j) {  // -1: the box lies past the length
-        const int key = blocks.key_block(b0 + j) * kKeys + lane * box;
-        if (j >= steps || lane >= boxes || key >= t.length) return -1;
-        const int page = t.pages[key / a.page_size];
-        if (page >= 0 && page < a.pages) return page;
-        atomicOr(a.status, PG_CACHE_BAD_PAGE);
-        return a.pages;  // past the last page: the copy fills in zeros
+    if (TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (TMA && (warp == 9 || warp == 10)) {
+      // --- copies: one warp the keys of each block, one the values; lane i the i-th page run ----
+      const int half = warp - 9, runs = kKeys / boxes.keys;
+      const CUtensorMap *map = half ? &v_map : &k_map;
+      const int per_page = half ? boxes.v_per_page : boxes.k_per_page;
+      const auto key_of = [&](int j) { return blocks.key_block(b0 + j) * kKeys + lane * boxes.keys; };
+      const auto page_for = [&](int j) {  // -1: the run lies past the length
+        if (j >= steps || lane >= runs || key_of(j) >= t.length) return -1;
+        return t.pages[key_of(j) / a.page_size];
       };
-      int page = page_for(0), n = 0;
+      int next = page_for(0), j = 0;
       bool ok = true;
-      for (int j = 0; j < steps && ok; ++j) {
-        const int next = page_for(j + 1);
-        const int row = (blocks.key_block(b0 + j) * kKeys + lane * box) % a.page_size;
-        const int held = __popc(__ballot_sync(0xffffffffu, page >= 0));
-        for (int half = 0; half < 2; ++half, ++n) {
-          const int s = n % P::stages;
-          if (n >= P::stages) ok = bar_wait(empty(s), (n / P::stages - 1) & 1, failed, a.status);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) bar_expect(full(s), held * box * 128 * P::chunks);
-          __syncwarp();
-          if (page >= 0) {
-            const uint32_t to = smem_at + P::ring + s * P::tile + lane * box * 128;
+      for (; j < steps; ++j) {
+        const bool real = lane < runs && key_of(j) < t.length;
+        int page = next;
+        next = page_for(j + 1);
+        if (real && (page < 0 || page >= a.pages)) {
+          atomicOr(a.status, PG_CACHE_BAD_PAGE);
+          page = a.pages;  // past the last page: the copy fills in zeros
+        }
+        const int row = key_of(j) % a.page_size, n = 2 * j + half, s = n % P::stages;
+        const int held = __popc(__ballot_sync(0xffffffffu, real));
+        if (n >= P::stages) ok = bar_wait(empty(s), (n / P::stages - 1) & 1, failed, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) bar_expect(full(s), held * boxes.keys * 128 * P::chunks);
+        __syncwarp();
+        if (real) {
+          const uint32_t to = smem_at + P::ring + s * P::tile + lane * (boxes.keys / 8) * P::group;
+          if (per_page) {
+            // an index past the map's last head and page too where the page is not one
+            tma_load_5d(to, map, row / 8, page * per_page + head, full(s));
+          } else {
+            for (int g = 0; g < boxes.keys / 8; ++g)
 #pragma unroll
-            for (int k = 0; k < P::chunks; ++k)
-              tma_load(to + k * P::chunk, half ? &v_map : &k_map, 64 * k, row, head, page, full(s));
+              for (int k = 0; k < P::chunks; ++k)
+                tma_load_4d(to + g * P::group + k * P::atom, map, 64 * k, row + 8 * g, head, page,
+                            full(s));
           }
         }
-        page = next;
       }
       // no copy is in flight when the block's shared memory goes
-      for (int k = max(0, n - P::stages); k < n; ++k)
-        bar_drain(full(k % P::stages), k / P::stages & 1, a.status);
-    } else if (TMA && warp > 9) {
-      // --- values of blocks that some row must not see in full ---------------------------------
-      // In turn with the thread that issues the products, which holds the slot meanwhile.
-      const int mine = tid - 320;
-      bool ok = true;
-      uint32_t phase = 0;
-      for (int j = 0; j < steps && ok; ++j) {
-        const int key0 = blocks.key_block(b0 + j) * kKeys, n = 2 * j + 1, s = n % P::stages;
-        if (all_see(a, both, key0, t.length)) continue;
-        ok = bar_wait(to_clean, phase, failed, a.status) &&
-             bar_wait(full(s), n / P::stages & 1, failed, a.status);
-        if (!ok) break;
-        phase ^= 1;
-        bool odd = false;
-        for (int r = mine; r < kKeys; r += kCleanThreads)
-#pragma unroll
-          for (int piece = 0; piece < DIM / 8; ++piece) {
-            uint4 *at =
-                reinterpret_cast<uint4 *>(smem + P::ring + s * P::tile + P::at(r, piece));
-            if (key0 + r >= t.length) *at = make_uint4(0, 0, 0, 0);
-            else odd |= clean<T>(at);
-          }
-        if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
-        fence_async();
-        bar_arrive(cleaned);
+      for (int k = max(0, j - P::stages); k < j; ++k) {
+        const int n = 2 * k + half;
+        if (n + P::stages >= 2 * j + half) bar_drain(full(n % P::stages), n / P::stages & 1, a.status);
       }
-    } else if (!TMA && warp > 8) {
+    } else if (!TMA && (warp == 9 || warp == 10)) {
       // --- copies: K and V of each block in turn ----------------------------------------------
       const int w = warp - 9;
       constexpr int kPieces = DIM / 8, kPer = 32 / kPieces;  // rows a warp copies at once
@@ -406,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s = n % P::stages;
         if (n & 1) {
           const int key0 = blocks.key_block(b0 + (n >> 1)) * kKeys;
-          if (!all_see(a, both, key0, t.length)) {
+          if (!both.all(key0)) {
             bool odd = false;
             for (int i = w; i < kKeys / kPer; i += kCopyWarps) {  // the pieces it has copied
               odd |= clean<T>(reinterpret_cast<uint4 *>(smem + P::ring + s * P::tile +
@@ -459,61 +502,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       while (ok && done < n) finish(done++);
-    } else if (warp == 8 && lane == 0 && steps) {
-      // --- products ----------------------------------------------------------------------------
+    } else if (warp == 8 && steps) {
+      // --- products --------------------------------------------------------------------------
+      const uint32_t elected = lane == 0;
       constexpr uint32_t s_desc = product<T>(kKeys, false), o_desc = product<T>(DIM, true);
       const auto scores = [&](int i, int s) {  // S_i = Q_i K^T
         const uint32_t q_at = smem_at + P::q + i * P::tile, k_at = smem_at + P::ring + s * P::tile;
 #pragma unroll
         for (int k = 0; k < DIM / 16; ++k) {
-          const uint32_t off = (k >> 2) * P::chunk + (k & 3) * 32;
-          mma_ss(tmem + 128 * i, operand(q_at + off, 16), operand(k_at + off, 16), s_desc, k > 0);
+          const uint32_t off = (k >> 2) * P::atom + (k & 3) * 32;
+          mma_ss(tmem + 128 * i, operand(q_at + off, P::group, 16),
+                 operand(k_at + off, P::group, 16), s_desc, k > 0, elected);
         }
-        commit(s_full(i));
+        commit(s_full(i), elected);
       };
       const auto values = [&](int i, int s, bool add) {  // O_i (+)= P_i V
         const uint32_t v_at = smem_at + P::ring + s * P::tile;
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
           mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k,
-                 operand(v_at + k * 16 * 128, P::chunk), o_desc, add || k > 0);
+                 operand(v_at + k * 2 * P::group, P::group, P::atom), o_desc, add || k > 0,
+                 elected);
       };
-      bool ok = bar_wait(q_full, 0, failed, a.status) && bar_wait(full(0), 0, failed, a.status);
+      const auto wait = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, a.status));
+      };
+      uint32_t phase = 0;  // of `cleaned`
+      bool ok = wait(q_full, 0) && wait(full(0), 0);
       if (ok) {
         fence_after();
         for (int i = 0; i < tiles; ++i) scores(i, 0);
-        commit(empty(0));
+        commit(empty(0), elected);
       }
-      uint32_t phase = 0;  // of `cleaned`
       for (int j = 0; j < steps && ok; ++j) {
         const int nv = 2 * j + 1, nk = 2 * j + 2, sv = nv % P::stages, sk = nk % P::stages;
         const bool more = j + 1 < steps;
-        ok = bar_wait(full(sv), nv / P::stages & 1, failed, a.status);
-        if (TMA && ok && !all_see(a, both, blocks.key_block(b0 + j) * kKeys, t.length)) {
-          bar_arrive(to_clean);
-          ok = bar_wait(cleaned, phase, failed, a.status);
+        ok = wait(full(sv), nv / P::stages & 1) && (!more || wait(full(sk), nk / P::stages & 1));
+        if (TMA && ok && !both.all(blocks.key_block(b0 + j) * kKeys)) {
+          ok = wait(cleaned, phase);
           phase ^= 1;
         }
         for (int i = 0; i < tiles && ok; ++i) {
-          ok = bar_wait(p_full(i), j & 1, failed, a.status);
-          if (ok && more && i == 0) ok = bar_wait(full(sk), nk / P::stages & 1, failed, a.status);
+          ok = wait(p_full(i), j & 1);
           if (!ok) break;
           fence_after();
           values(i, sv, j > 0);
           if (more) scores(i, sk);
         }
         if (!ok) break;
-        commit(empty(sv));
-        if (more) commit(empty(sk));
+        commit(empty(sv), elected);
+        if (more) commit(empty(sk), elected);
       }
-      commit(o_full);
+      commit(o_full, elected);
       // whatever was issued ends before the block's shared and tensor memory go
       bar_drain(o_full, 0, a.status);
     }
     __syncwarp();
   } else {
     // --- a row's thread --------------------------------------------------------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    if (TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int i = warp >> 2, r = tid & 127, row = i * kHalf + r;
     const bool real = row < t.rows;
     const int at = t.row + row, token = at / a.group, h = head * a.group + at - token * a.group;
@@ -537,8 +585,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes a warp, lane at 16
     const uint32_t s_at = tmem + lanes + 128 * i, o_at = tmem + lanes + 256 + 128 * i;
     const int row_last = min(t.rows - 1, i * kHalf + kHalf - 1);
-    const Range mine{first_pos + (t.row + i * kHalf) / a.group,
-                     first_pos + (t.row + row_last) / a.group};
+    const Seen mine(a, first_pos + (t.row + i * kHalf) / a.group,
+                    first_pos + (t.row + row_last) / a.group, t.length);
     float m = -INFINITY, l = 0.0f;
     const bool active = i < tiles;
     bool ok = true;
@@ -547,24 +595,53 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       fence_after();
       float s[kKeys];
+      uint32_t *const s_bits = reinterpret_cast<uint32_t *>(s);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        tmem_load(s_at + 32 * k, reinterpret_cast<uint32_t *>(s) + 32 * k);
+      for (int k = 0; k < 4; ++k) tmem_load(s_at + 32 * k, s_bits + 32 * k);
       wait_loads();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tie(s_bits + 32 * k);
       const int key0 = blocks.key_block(b0 + j) * kKeys;
-      if (!all_see(a, mine, key0, t.length)) {
-#pragma unroll
-        for (int k = 0; k < kKeys; ++k)
-          if (!pg::sees(a, pos, key0 + k)) s[k] = -INFINITY;
+      if (TMA && !both.all(key0)) {
+        // the values of a block that some row must not see in full, before their first product:
+        // a thread of each tile takes a part of row r
+        const int n = 2 * j + 1, slot = n % P::stages;
+        ok = bar_wait(full(slot), n / P::stages & 1, failed, a.status);
+        bool odd = false;
+        char *const values = smem + P::ring + slot * P::tile;
+        for (int piece = i; piece < DIM / 8; piece += tiles) {
+          uint4 *at16 = reinterpret_cast<uint4 *>(values + P::at(r, piece));
+          if (key0 + r >= t.length) *at16 = make_uint4(0, 0, 0, 0);
+          else odd |= clean<T>(at16);
+        }
+        if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
+        fence_async();
+        bar_arrive(cleaned);
       }
-      float top[4] = {s[0], s[1], s[2], s[3]};
+      float most;
+      if (mine.all(key0)) {
+        most = largest(s, m);
+      } else {
+        asm volatile("" ::: "memory");  // a branch, not predicated instructions in every block
+        const int to = pos - key0, from = a.window ? to - a.window : -1, sink = a.sinks - key0;
 #pragma unroll
-      for (int k = 4; k < kKeys; ++k) top[k & 3] = fmaxf(top[k & 3], s[k]);
-      const float most = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-      // the first block's maximum stands until a row's has grown by 2^8
+        for (int k = 0; k < 4; ++k) {
+          // bit e: key 32 k + e is seen
+          const auto below = [&](int n) {  // the bits of keys below n
+            n -= 32 * k;
+            return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+          };
+          const uint32_t seen = below(to + 1) & (~below(from + 1) | below(sink));
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1)) s[32 * k + e] = -INFINITY;
+        }
+        most = largest(s, m);
+      }
+      // the first block's maximum stands until a row's has grown by 2^8 (or is NaN)
       if (j == 0) {
         m = most;
-      } else if (__any_sync(0xffffffffu, most > m && !((most - m) * c <= kGrow))) {
+      } else if (__any_sync(0xffffffffu, !((most - m) * c <= kGrow))) {
         const float f = m == -INFINITY ? 0.0f : pg::exp2_fast((m - most) * c);
         m = most;
         l *= f;
@@ -573,26 +650,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t x[32];
           tmem_load(o_at + 32 * k, x);
           wait_loads();
+          tie(x);
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
           tmem_store(o_at + 32 * k, x);
         }
       }
-      const float base = m == -INFINITY ? 0.0f : -m * c;
-      float sum[4] = {0, 0, 0, 0};
+      // an infinite maximum gives NaN, as the formula does, in every weight
+      const float base = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : -m * c;
+      Two sum[2] = {Two(l, 0.0f), Two(0.0f, 0.0f)};
+      const Two c2(c, c), base2(base, base);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         uint32_t x[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float y = pg::exp2_fast(fmaf(s[64 * k + 2 * e], c, base));
-          const float z = pg::exp2_fast(fmaf(s[64 * k + 2 * e + 1], c, base));
-          sum[e & 3] += y + z;
+          float y, z;
+          fma(Two(s[64 * k + 2 * e], s[64 * k + 2 * e + 1]), c2, base2).get(y, z);
+          y = pg::exp2_fast(y);
+          z = pg::exp2_fast(z);
+          sum[e & 1] = add(sum[e & 1], Two(y, z));
           x[e] = Type<T>::pack(y, z);
         }
         tmem_store(s_at + 32 * k, x);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      {
+        float y, z;
+        add(sum[0], sum[1]).get(y, z);
+        l = y + z;
+      }
       wait_stores();
       fence_before();
       bar_arrive(p_full(i));
@@ -611,11 +697,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tmem_load(o_at + 32 * k, reinterpret_cast<uint32_t *>(x));
       wait_loads();
+      tie(reinterpret_cast<uint32_t *>(x));
       if (!*const_cast<volatile int *>(&sh.odd)) return;
       // values that are not finite, in blocks that some row must not see in full
       for (int j = 0; j < steps; ++j) {
         const int key0 = blocks.key_block(b0 + j) * kKeys;
-        if (all_see(a, both, key0, t.length)) continue;
+        if (both.all(key0)) continue;
         for (int key = key0; key < min(key0 + kKeys, t.length); ++key) {
           if (!pg::sees(a, pos, key)) continue;
           const int page = pg::page_of(a, t, key);
@@ -720,6 +807,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// The tensor map of the keys or values (see Boxes). One box a run of keys, where head size and
+// strides allow, takes half the copies: 4096 new tokens of up to 8192 @FOLD@
+int encode(CUtensorMap *map, int *per_page, const Attention &a, const char *base, int64_t head,
+           int64_t page, int dim, int keys) {
+  const uint64_t row = 2ull * a.dim, at = reinterpret_cast<uintptr_t>(base);
+  const int64_t unit = a.heads > 1 ? head : page;
+  if (a.dim == dim && unit > 0 && page % unit == 0 &&
+      (a.pages + 1ll) * (page / unit) < INT32_MAX) {
+    *per_page = static_cast<int>(page / unit);
+    const uint64_t dims[5] = {64, 8, static_cast<uint64_t>(dim / 64),
+                              static_cast<uint64_t>(a.page_size / 8),
+                              static_cast<uint64_t>(a.pages - 1) * *per_page + a.heads};
+    const uint64_t strides[4] = {row, 128, 8 * row, static_cast<uint64_t>(unit)};
+    const uint32_t box[5] = {64, 8, static_cast<uint32_t>(dim / 64),
+                             static_cast<uint32_t>(keys / 8), 1};
+    return pg_detail_tensormap(map, 5, at, dims, strides, box);
+  }
+  *per_page = 0;
+  const uint64_t dims[4] = {static_cast<uint64_t>(a.dim), static_cast<uint64_t>(a.page_size),
+                            static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.pages)};
+  const uint64_t strides[3] = {row, static_cast<uint64_t>(head), static_cast<uint64_t>(page)};
+  const uint32_t box[4] = {64, 8, 1, 1};
+  return pg_detail_tensormap(map, 4, at, dims, strides, box);
+}
+
 template <class T, int DIM>
 int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cudaStream_t stream) {
   a.rows_per_tile = kRows;
@@ -731,24 +843,16 @@ int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cuda
   CUtensorMap k_map = {}, v_map = {};
   // a kv head's tiles of the latest queries, which see the most keys, go first
   const dim3 grid(a.heads, tiles, a.parts);
-  const int box = std::gcd(a.page_size, kKeys);
-  if (box < 8)
+  const int keys = std::gcd(a.page_size, kKeys);
+  if (keys < 8)
     return pg::launch("prompt_kernel", prompt_kernel<T, DIM, false>, grid, kThreads,
-                      Plan<DIM>::bytes, stream, a, k_map, v_map, 0);
-  const uint64_t dims[4] = {static_cast<uint64_t>(a.dim), static_cast<uint64_t>(a.page_size),
-                            static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.pages)};
-  const uint32_t boxes[4] = {64, static_cast<uint32_t>(box), 1, 1};
-  const uint64_t row = 2ull * a.dim;
-  const uint64_t k_strides[3] = {row, static_cast<uint64_t>(a.k_head),
-                                 static_cast<uint64_t>(a.k_page)};
-  const uint64_t v_strides[3] = {row, static_cast<uint64_t>(a.v_head),
-                                 static_cast<uint64_t>(a.v_page)};
-  int rc = pg_detail_tensormap(&k_map, 4, reinterpret_cast<uintptr_t>(a.k), dims, k_strides, boxes);
-  if (!rc)
-    rc = pg_detail_tensormap(&v_map, 4, reinterpret_cast<uintptr_t>(a.v), dims, v_strides, boxes);
+                      Plan<DIM>::bytes, stream, a, k_map, v_map, Boxes{});
+  Boxes boxes{keys, 0, 0};
+  int rc = encode(&k_map, &boxes.k_per_page, a, a.k, a.k_head, a.k_page, DIM, keys);
+  if (!rc) rc = encode(&v_map, &boxes.v_per_page, a, a.v, a.v_head, a.v_page, DIM, keys);
   if (rc) return rc;
   return pg::launch("prompt_kernel", prompt_kernel<T, DIM, true>, grid, kThreads,
-                    Plan<DIM>::bytes, stream, a, k_map, v_map, box);
+                    Plan<DIM>::bytes, stream, a, k_map, v_map, boxes);
 }
 
 }  // namespace
