@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t q_full = bars + 16 * P::stages;
   const auto s_full = [&](int i) { return q_full + 8 + 8 * i; };
   const auto p_full = [&](int i) { return q_full + 24 + 8 * i; };
-  const uint32_t o_full = q_full + 40, cleaned = q_full + 48;
+  const uint32_t o_full = q_full + 40;
   if (tid == 0) {
     for (int s = 0; s < P::stages; ++s) {
       bar_init(full(s), TMA ? 1 : kCopyThreads);
@@ -357,7 +357,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(p_full(i), kHalf);
     }
     bar_init(o_full, 1);
-    bar_init(cleaned, kHalf * tiles);
     sh.failed = sh.odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -527,7 +526,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const auto wait = [&](uint32_t bar, uint32_t parity) {
         return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, a.status));
       };
-      uint32_t phase = 0;  // of `cleaned`
       bool ok = wait(q_full, 0) && wait(full(0), 0);
       if (ok) {
         fence_after();
@@ -538,10 +536,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nv = 2 * j + 1, nk = 2 * j + 2, sv = nv % P::stages, sk = nk % P::stages;
         const bool more = j + 1 < steps;
         ok = wait(full(sv), nv / P::stages & 1) && (!more || wait(full(sk), nk / P::stages & 1));
-        if (TMA && ok && !both.all(blocks.key_block(b0 + j) * kKeys)) {
-          ok = wait(cleaned, phase);
-          phase ^= 1;
-        }
         for (int i = 0; i < tiles && ok; ++i) {
           ok = wait(p_full(i), j & 1);
           if (!ok) break;
@@ -587,6 +581,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row_last = min(t.rows - 1, i * kHalf + kHalf - 1);
     const Seen mine(a, first_pos + (t.row + i * kHalf) / a.group,
                     first_pos + (t.row + row_last) / a.group, t.length);
+    // Steps whole.. (as many as wholes) are blocks of the window that every row sees in full. What
+    // the others need is worked out only there: two numbers are what the registers have room for.
+    const int at_first = blocks.first - blocks.sink + b0;  // the key block at step 0
+    const int whole =
+        max(max(0, blocks.sink - b0), (max(both.low, 0) + kKeys - 1) / kKeys - at_first);
+    const int whole_end = both.high < 0 ? 0 : min(steps, both.high / kKeys + 1 - at_first);
+    const unsigned wholes = max(0, whole_end - whole);
     float m = -INFINITY, l = 0.0f;
     const bool active = i < tiles;
     bool ok = true;
@@ -602,42 +603,41 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < 4; ++k) tie(s_bits + 32 * k);
       const int key0 = blocks.key_block(b0 + j) * kKeys;
-      if (TMA && !both.all(key0)) {
-        // the values of a block that some row must not see in full, before their first product:
-        // a thread of each tile takes a part of row r
-        const int n = 2 * j + 1, slot = n % P::stages;
-        ok = bar_wait(full(slot), n / P::stages & 1, failed, a.status);
-        bool odd = false;
-        char *const values = smem + P::ring + slot * P::tile;
-        for (int piece = i; piece < DIM / 8; piece += tiles) {
-          uint4 *at16 = reinterpret_cast<uint4 *>(values + P::at(r, piece));
-          if (key0 + r >= t.length) *at16 = make_uint4(0, 0, 0, 0);
-          else odd |= clean<T>(at16);
-        }
-        if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
-        fence_async();
-        bar_arrive(cleaned);
-      }
-      float most;
-      if (mine.all(key0)) {
-        most = largest(s, m);
-      } else {
+      if (static_cast<unsigned>(j - whole) >= wholes) {
         asm volatile("" ::: "memory");  // a branch, not predicated instructions in every block
-        const int to = pos - key0, from = a.window ? to - a.window : -1, sink = a.sinks - key0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // bit e: key 32 k + e is seen
-          const auto below = [&](int n) {  // the bits of keys below n
-            n -= 32 * k;
-            return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
-          };
-          const uint32_t seen = below(to + 1) & (~below(from + 1) | below(sink));
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(seen >> e & 1)) s[32 * k + e] = -INFINITY;
+        if (TMA && i == 0 && !both.all(key0)) {
+          // The values of a block that some row must not see in full, before this step's weights
+          // are handed on: tile 0's are used first. A thread takes row r.
+          const int n = 2 * j + 1, slot = n % P::stages;
+          ok = bar_wait(full(slot), n / P::stages & 1, failed, a.status);
+          bool odd = false;
+          char *const values = smem + P::ring + slot * P::tile;
+#pragma unroll 4
+          for (int piece = 0; piece < DIM / 8; ++piece) {
+            uint4 *at16 = reinterpret_cast<uint4 *>(values + P::at(r, piece));
+            if (key0 + r >= t.length) *at16 = make_uint4(0, 0, 0, 0);
+            else odd |= clean<T>(at16);
+          }
+          if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
+          fence_async();
         }
-        most = largest(s, m);
+        if (!mine.all(key0)) {
+          const int to = pos - key0, from = a.window ? to - a.window : -1, sink = a.sinks - key0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // bit e: key 32 k + e is seen
+            const auto below = [&](int n) {  // the bits of keys below n
+              n -= 32 * k;
+              return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+            };
+            const uint32_t seen = below(to + 1) & (~below(from + 1) | below(sink));
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen >> e & 1)) s[32 * k + e] = -INFINITY;
+          }
+        }
       }
+      const float most = largest(s, m);
       // the first block's maximum stands until a row's has grown by 2^8 (or is NaN)
       if (j == 0) {
         m = most;
