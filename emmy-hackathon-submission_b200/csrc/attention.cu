@@ -292,8 +292,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(Attention a) {
 template <class T, int ROWS, int DIM>
 int launch_tiles(Attention a, int tiles, cudaStream_t stream) {
   a.rows_per_tile = ROWS;
-  return pg::launch("attention_kernel", attention_kernel<T, ROWS, DIM>,
-                    dim3(tiles, a.heads, a.parts), kThreads, Layout<ROWS, DIM>::bytes, stream, a);
+  return pg::launch<attention_kernel<T, ROWS, DIM>>("attention_kernel", dim3(tiles, a.heads, a.parts), kThreads, Layout<ROWS, DIM>::bytes, stream, a);
 }
 
 template <class T, int ROWS>

@@ -447,7 +447,7 @@ template <class T, int DIM>
 int launch_decode(const Attention &a, int sms, cudaStream_t stream) {
   // a block per 4 units (256 keys) at least, below which the joining costs more than it gives
   constexpr int kLeast = 4;
-  return pg::launch("decode_kernel", decode_kernel<T, DIM>, dim3(kPerSm * sms), kThreads,
+  return pg::launch<decode_kernel<T, DIM>>("decode_kernel", dim3(kPerSm * sms), kThreads,
                     Ring<DIM>::bytes, stream, a, kLeast);
 }
 

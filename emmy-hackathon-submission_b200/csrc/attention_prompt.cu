@@ -845,13 +845,13 @@ int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cuda
   const dim3 grid(a.heads, tiles, a.parts);
   const int keys = std::gcd(a.page_size, kKeys);
   if (keys < 8)
-    return pg::launch("prompt_kernel", prompt_kernel<T, DIM, false>, grid, kThreads,
+    return pg::launch<prompt_kernel<T, DIM, false>>("prompt_kernel", grid, kThreads,
                       Plan<DIM>::bytes, stream, a, k_map, v_map, Boxes{});
   Boxes boxes{keys, 0, 0};
   int rc = encode(&k_map, &boxes.k_per_page, a, a.k, a.k_head, a.k_page, DIM, keys);
   if (!rc) rc = encode(&v_map, &boxes.v_per_page, a, a.v, a.v_head, a.v_page, DIM, keys);
   if (rc) return rc;
-  return pg::launch("prompt_kernel", prompt_kernel<T, DIM, true>, grid, kThreads,
+  return pg::launch<prompt_kernel<T, DIM, true>>("prompt_kernel", grid, kThreads,
                     Plan<DIM>::bytes, stream, a, k_map, v_map, boxes);
 }
 

@@ -511,7 +511,7 @@ extern "C" int pg_cache_extend(const pg_cache *c, uint64_t slots, uint64_t start
                                uint64_t stream) {
   int rc = check_list("pg_cache_extend", c, slots, starts, n, c ? c->slots : 0);
   if (rc || !n) return rc;
-  return pg::launch("cache_extend", cache_extend, dim3(1), kPlan, 0, stream_of(stream), *c,
+  return pg::launch<cache_extend>("cache_extend", dim3(1), kPlan, 0, stream_of(stream), *c,
                     ints(slots), ints(starts), n);
 }
 
@@ -527,7 +527,7 @@ extern "C" int pg_cache_write(const pg_cache *c, int32_t layer, uint64_t slots, 
   if ((rc = check_rows("pg_cache_write", k)) || (rc = check_rows("pg_cache_write", v))) return rc;
   int grid;
   if ((rc = copy_grid((tokens + kCopy / 32 - 1) / (kCopy / 32), &grid))) return rc;
-  return pg::launch("cache_write", cache_write, dim3(grid), kCopy, 0, stream_of(stream), *c,
+  return pg::launch<cache_write>("cache_write", dim3(grid), kCopy, 0, stream_of(stream), *c,
                     layer, ints(slots), ints(starts), n, tokens, *k, *v);
 }
 
@@ -536,7 +536,7 @@ extern "C" int pg_cache_free(const pg_cache *c, uint64_t slots, int32_t n, uint6
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(n, &grid))) return rc;
-  return pg::launch("cache_free", cache_free, dim3(grid), kCopy, 0, stream_of(stream), *c,
+  return pg::launch<cache_free>("cache_free", dim3(grid), kCopy, 0, stream_of(stream), *c,
                     ints(slots), n);
 }
 
@@ -546,7 +546,7 @@ extern "C" int pg_cache_copy(const pg_cache *c, uint64_t from, uint64_t to, int3
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(static_cast<int64_t>(n) * c->layers * 2, &grid))) return rc;
-  return pg::launch("cache_copy", cache_copy, dim3(grid), kCopy, 0, stream_of(stream), *c,
+  return pg::launch<cache_copy>("cache_copy", dim3(grid), kCopy, 0, stream_of(stream), *c,
                     ints(from), ints(to), n);
 }
 
@@ -556,10 +556,10 @@ extern "C" int pg_cache_fork(const pg_cache *c, uint64_t parents, uint64_t child
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(static_cast<int64_t>(n) * (2 * c->layers + 1), &grid))) return rc;
-  rc = pg::launch("cache_fork_plan", cache_fork_plan, dim3(1), kPlan, 0, stream_of(stream), *c,
+  rc = pg::launch<cache_fork_plan>("cache_fork_plan", dim3(1), kPlan, 0, stream_of(stream), *c,
                   ints(parents), ints(children), n);
   if (rc) return rc;
-  return pg::launch("cache_fork_copy", cache_fork_copy, dim3(grid), kCopy, 0, stream_of(stream),
+  return pg::launch<cache_fork_copy>("cache_fork_copy", dim3(grid), kCopy, 0, stream_of(stream),
                     *c, ints(parents), ints(children), n);
 }
 
@@ -568,9 +568,9 @@ extern "C" int pg_cache_compact(const pg_cache *c, uint64_t stream) {
   if (rc) return rc;
   int grid;
   if ((rc = copy_grid(c->slots + static_cast<int64_t>(c->pages) * c->layers, &grid))) return rc;
-  rc = pg::launch("cache_compact_plan", cache_compact_plan, dim3(1), kPlan, 0, stream_of(stream),
+  rc = pg::launch<cache_compact_plan>("cache_compact_plan", dim3(1), kPlan, 0, stream_of(stream),
                   *c);
   if (rc) return rc;
-  return pg::launch("cache_compact_move", cache_compact_move, dim3(grid), kCopy, 0,
+  return pg::launch<cache_compact_move>("cache_compact_move", dim3(grid), kCopy, 0,
                     stream_of(stream), *c);
 }

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -32,19 +33,32 @@ __attribute__((format(printf, 1, 2))) inline int argument_fail(const char *fmt, 
   return pg_detail_fail(PG_ERR_ARGUMENT, buf);
 }
 
+// Arguments take the kernel's own types on the way.
+template <class... P, class... A>
+cudaError_t launch_kernel(const cudaLaunchConfig_t &cfg, void (*kernel)(P...), A... args) {
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Launches with programmatic stream serialization: the kernel's blocks may become resident
 // while the kernel ahead of it on the stream drains, which hides a launch's set-up. Every kernel
 // launched this way calls cudaGridDependencySynchronize() before its first access to memory, in
 // every thread and on every path, so it still sees all that came before it and a kernel behind
 // it cannot run ahead of what this one waits for.
-template <class... P, class... A>
-int launch(const char *name, void (*kernel)(P...), dim3 grid, int block, int smem,
-           cudaStream_t stream, A... args) {
+// `Kernel` always has the same `smem`, so the opt-in above the default 48 KiB is made once a device.
+template <auto Kernel, class... A>
+int launch(const char *name, dim3 grid, int block, int smem, cudaStream_t stream, A... args) {
   cudaError_t e;
-  if (smem > 32 * 1024) {  // with a kernel's static shared memory more than the default 48 KiB
-    e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return runtime_fail(e, name);
+  if (smem > 32 * 1024) {  // with a kernel's static shared memory more than the default
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    if ((e = cudaGetDevice(&device)) != cudaSuccess) return runtime_fail(e, name);
+    const uint64_t bit = 1ull << (device & 63);
+    if (device > 63 || !(done.load(std::memory_order_relaxed) & bit)) {
+      e = cudaFuncSetAttribute(reinterpret_cast<const void *>(Kernel),
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return runtime_fail(e, name);
+      done.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -56,16 +70,20 @@ int launch(const char *name, void (*kernel)(P...), dim3 grid, int block, int sme
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-  if (e != cudaSuccess) return runtime_fail(e, name);
-  return PG_OK;
+  e = launch_kernel(cfg, Kernel, args...);
+  return e == cudaSuccess ? PG_OK : runtime_fail(e, name);
 }
 
 inline int sm_count(int *out) {
+  static std::atomic<int> known[64];
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && device < 64 && (*out = known[device].load(std::memory_order_relaxed)))
+    return PG_OK;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, device);
-  return e == cudaSuccess ? PG_OK : runtime_fail(e, "cudaDeviceGetAttribute");
+  if (e != cudaSuccess) return runtime_fail(e, "cudaDeviceGetAttribute");
+  if (device < 64) known[device].store(*out, std::memory_order_relaxed);
+  return PG_OK;
 }
 
 __device__ __forceinline__ void wait_for_earlier_kernels() {

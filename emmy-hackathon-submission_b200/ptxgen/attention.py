@@ -23,14 +23,20 @@ out of range, nothing is read, that sequence's result is not defined, and bits a
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Any
 
-from .cache import CacheError, int32_list
-from .logprob import _dtype_code
-from .runtime import AttentionArgs, _check, library, torch_stream
+import torch
+
+from .cache import CacheError
+from .launch import call, dtype_code, int32_list
+from .runtime import AttentionArgs, library
 
 WORKSPACE_BYTES = 64 << 20  # PG_ATTENTION_WORKSPACE
 DIM_MAX = 256  # PG_ATTENTION_DIM
+# pg_attention_args at once: setting its fields one by one takes longer than a short call
+_PACK = struct.Struct("=9Q10q13if")
+assert _PACK.size == ctypes.sizeof(AttentionArgs)
 
 
 class Workspace:
@@ -38,8 +44,6 @@ class Workspace:
     they are joined. One per stream: calls that overlap on the GPU must not share it."""
 
     def __init__(self, device: Any = None):
-        import torch
-
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None \
             else torch.device(device)
         self.buffer = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.int32, device=self.device)
@@ -56,20 +60,20 @@ class Workspace:
 def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any,
           scale: float | None, window: int, sinks: int, max_len: int | None, workspace: Workspace,
           out: Any, stream: int | None) -> Any:
-    import torch
-
     dev, dtype, size = q.device, q.dtype, q.element_size()
-    if q.dim() != 3 or not q.is_cuda or q.stride(2) != 1:
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if len(qs) != 3 or not q.is_cuda or qs[2] != 1:
         raise ValueError(f"q: want [tokens, heads, dim] on a CUDA device with contiguous rows, "
                          f"got {tuple(q.shape)} {q.stride()} on {dev}")
     tokens, hq, dim = q.shape
-    for name, t in (("k", k), ("v", v)):
-        if t.dim() != 4 or t.dtype != dtype or t.device != dev or t.shape != k.shape or \
-                t.shape[3] != dim or t.stride(3) != 1 or t.stride(2) != dim:
+    shape = k.shape
+    for name, t, s in (("k", k, ks), ("v", v, vs)):
+        if len(s) != 4 or t.dtype is not dtype or t.device != dev or t.shape != shape or \
+                shape[3] != dim or s[3] != 1 or s[2] != dim:
             raise ValueError(f"{name}: want {dtype} [pages, kv_heads, page_size, {dim}] on {dev} "
                              f"with a head's rows of one page one after another, got {t.dtype} "
                              f"{tuple(t.shape)} {t.stride()} on {t.device}")
-    pages, heads, page_size = k.shape[:3]
+    pages, heads, page_size, _ = shape
     if hq % heads:
         raise ValueError(f"{hq} query heads are no multiple of {heads} kv heads")
     if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1 or \
@@ -95,16 +99,19 @@ def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any
         out = torch.empty((tokens, hq, dim), dtype=dtype, device=dev)
     elif out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(2) != 1:
         raise ValueError(f"out: want {dtype} {tuple(q.shape)} on {dev} with contiguous rows")
-    qs, os_, ks, vs = q.stride(), out.stride(), k.stride(), v.stride()
-    args = AttentionArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts or 0, slots,
-        table.data_ptr(), int32_list("lens", lens, dev, rows), workspace.buffer.data_ptr(),
-        WORKSPACE_BYTES, qs[0] * size, qs[1] * size, os_[0] * size, os_[1] * size,
-        ks[0] * size, ks[1] * size, vs[0] * size, vs[1] * size, table.stride(0),
-        _dtype_code(dtype), batch, tokens, heads, hq // heads, dim, page_size, pages, width, rows,
-        window, sinks, max_len or 0, dim ** -0.5 if scale is None else scale)
-    with torch_stream(dev, stream) as s:
-        _check(library().pg_attention(ctypes.byref(args), s), "pg_attention")
+    os_ = out.stride()
+    args = AttentionArgs()
+    try:
+        _PACK.pack_into(
+            args, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts or 0, slots,
+            table.data_ptr(), int32_list("lens", lens, dev, rows), workspace.buffer.data_ptr(),
+            WORKSPACE_BYTES, qs[0] * size, qs[1] * size, os_[0] * size, os_[1] * size,
+            ks[0] * size, ks[1] * size, vs[0] * size, vs[1] * size, table.stride(0),
+            dtype_code(dtype), batch, tokens, heads, hq // heads, dim, page_size, pages, width, rows,
+            window, sinks, max_len or 0, dim ** -0.5 if scale is None else scale)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"window, sinks, max_len, scale or a size is out of range: {e}") from e
+    call(library().pg_attention, dev, stream, args)
     return out
 
 

@@ -24,7 +24,10 @@ from __future__ import annotations
 import ctypes
 from typing import Any
 
-from .runtime import Cache, LaunchError, Rows, _check, library, torch_stream
+import torch
+
+from .launch import call, int32_list
+from .runtime import Cache, LaunchError, Rows, library
 
 NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG, WAIT = 1, 2, 4, 8, 16
 _WHY = {NO_PAGES: "fewer free pages than a call needed",
@@ -42,26 +45,12 @@ class CacheError(LaunchError):
         super().__init__("; ".join(w for b, w in _WHY.items() if bits & b))
 
 
-def int32_list(name: str, t: Any, device: Any, n: int | None = None) -> int:
-    """The address of a contiguous 1-D int32 tensor on ``device`` (with ``n`` entries)."""
-    import torch
-
-    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name}: want a contiguous 1-D int32 tensor on {device}, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    if n is not None and t.shape[0] != n:
-        raise ValueError(f"{name}: {t.shape[0]} entries, want {n}")
-    return t.data_ptr()
-
-
 class PagedCache:
     """The cache over ``k`` and ``v`` [layers, pages, heads, page_size, dim], ``refs`` [pages],
     ``table`` [slots, width] and ``lens`` [slots] (int32). A head's rows of one page lie one
     after another; the other strides are free but multiples of 16 bytes and the same for both."""
 
     def __init__(self, k: Any, v: Any, refs: Any, table: Any, lens: Any):
-        import torch
-
         if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
             raise ValueError("k and v: want one shape [layers, pages, heads, page_size, dim], "
                              f"dtype and strides, got {k.dtype} {tuple(k.shape)} {k.stride()} "
@@ -76,7 +65,7 @@ class PagedCache:
         if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1:
             raise ValueError("table: want int32 [slots, width] with contiguous rows")
         self.k, self.v, self.refs, self.table, self.lens = k, v, refs, table, lens
-        self.device = k.device
+        self.device, self._size, self._row_shape = k.device, size, torch.Size((heads, dim))
         slots, width = table.shape
         words = 4 + 3 * pages + 2 * slots + 2
         self._scratch = torch.empty(words, dtype=torch.int32, device=k.device)
@@ -94,8 +83,6 @@ class PagedCache:
     def allocate(cls, layers: int, pages: int, heads: int, page_size: int, dim: int, slots: int,
                  width: int, dtype: Any = None, device: Any = None) -> PagedCache:
         """An empty cache: ``pages`` free pages, ``slots`` empty slots of up to ``width`` pages."""
-        import torch
-
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None \
             else torch.device(device)
         shape = (layers, pages, heads, page_size, dim)
@@ -105,64 +92,53 @@ class PagedCache:
         return cls(k, v, refs, table, torch.zeros(slots, dtype=torch.int32, device=dev))
 
     def _rows(self, name: str, t: Any) -> Rows:
-        shape = (self._c.heads, self.k.shape[4])
-        if t.dtype != self.k.dtype or t.dim() != 3 or tuple(t.shape[1:]) != shape or \
-                t.device != self.device or (shape[1] > 1 and t.stride(2) != 1):
-            raise ValueError(f"{name}: want {self.k.dtype} [tokens, {shape[0]}, {shape[1]}] on "
-                             f"{self.device} with contiguous rows, got {t.dtype} "
-                             f"{tuple(t.shape)} on {t.device}")
-        size = t.element_size()
+        if t.dtype is not self.k.dtype or t.dim() != 3 or t.shape[1:] != self._row_shape or \
+                t.device != self.device or t.stride(2) != 1:
+            raise ValueError(f"{name}: want {self.k.dtype} [tokens, {self._row_shape[0]}, "
+                             f"{self._row_shape[1]}] on {self.device} with contiguous rows, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        size = self._size
         return Rows(t.data_ptr(), t.stride(0) * size, t.stride(1) * size)
 
     def extend(self, slots: Any, starts: Any, stream: int | None = None) -> None:
         """Make room for new tokens: ``slots[i]`` grows by ``starts[i + 1] - starts[i]`` tokens."""
-        n = slots.shape[0]
-        with torch_stream(self.device, stream) as s:
-            _check(self._lib.pg_cache_extend(self._ref, int32_list("slots", slots, self.device),
-                                             int32_list("starts", starts, self.device, n + 1), n,
-                                             s), "pg_cache_extend")
+        n, dev = slots.shape[0], self.device
+        call(self._lib.pg_cache_extend, dev, stream, self._ref, int32_list("slots", slots, dev),
+             int32_list("starts", starts, dev, n + 1), n)
 
     def write(self, layer: int, slots: Any, starts: Any, k: Any, v: Any,
               stream: int | None = None) -> None:
         """Write one layer's ``k`` and ``v`` [tokens, heads, dim] of the slots' last tokens:
         rows ``starts[i]`` to ``starts[i + 1]`` are the last ones of ``slots[i]``."""
-        n = slots.shape[0]
+        n, dev = slots.shape[0], self.device
         if k.shape[0] != v.shape[0]:
             raise ValueError(f"k has {k.shape[0]} tokens, v has {v.shape[0]}")
-        with torch_stream(self.device, stream) as s:
-            _check(self._lib.pg_cache_write(
-                self._ref, layer, int32_list("slots", slots, self.device),
-                int32_list("starts", starts, self.device, n + 1), n, k.shape[0],
-                self._rows("k", k), self._rows("v", v), s), "pg_cache_write")
+        call(self._lib.pg_cache_write, dev, stream, self._ref, layer,
+             int32_list("slots", slots, dev), int32_list("starts", starts, dev, n + 1), n,
+             k.shape[0], self._rows("k", k), self._rows("v", v))
 
     def free(self, slots: Any, stream: int | None = None) -> None:
         """Let go of the slots' pages: their lengths become 0."""
-        with torch_stream(self.device, stream) as s:
-            _check(self._lib.pg_cache_free(self._ref, int32_list("slots", slots, self.device),
-                                           slots.shape[0], s), "pg_cache_free")
+        call(self._lib.pg_cache_free, self.device, stream, self._ref,
+             int32_list("slots", slots, self.device), slots.shape[0])
 
     def fork(self, parents: Any, children: Any, stream: int | None = None) -> None:
         """Make each empty slot ``children[i]`` a continuation of ``parents[i]``: it shares the
         full pages and gets a copy of a last page that is not full, in every layer."""
-        n = parents.shape[0]
-        with torch_stream(self.device, stream) as s:
-            _check(self._lib.pg_cache_fork(
-                self._ref, int32_list("parents", parents, self.device),
-                int32_list("children", children, self.device, n), n, s), "pg_cache_fork")
+        n, dev = parents.shape[0], self.device
+        call(self._lib.pg_cache_fork, dev, stream, self._ref,
+             int32_list("parents", parents, dev), int32_list("children", children, dev, n), n)
 
     def copy_pages(self, source: Any, destination: Any, stream: int | None = None) -> None:
         """Copy whole pages in every layer; counts and tables stay as they are. No page may be
         both a source and a destination, nor a destination twice."""
-        n = source.shape[0]
-        with torch_stream(self.device, stream) as s:
-            _check(self._lib.pg_cache_copy(
-                self._ref, int32_list("source", source, self.device),
-                int32_list("destination", destination, self.device, n), n, s), "pg_cache_copy")
+        n, dev = source.shape[0], self.device
+        call(self._lib.pg_cache_copy, dev, stream, self._ref, int32_list("source", source, dev),
+             int32_list("destination", destination, dev, n), n)
 
     def compact(self, stream: int | None = None) -> None:
         """Move the live pages to the lowest ids, with the tables and counts."""
-        with torch_stream(self.device, stream) as s:
-            _check(self._lib.pg_cache_compact(self._ref, s), "pg_cache_compact")
+        call(self._lib.pg_cache_compact, self.device, stream, self._ref)
 
     def check(self) -> None:
         """Wait for the GPU and raise ``CacheError`` if an earlier call could not be met (the

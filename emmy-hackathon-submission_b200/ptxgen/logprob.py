@@ -19,7 +19,10 @@ from __future__ import annotations
 
 from typing import Any, NamedTuple
 
-from .runtime import _check, library, torch_stream
+import torch
+
+from .launch import call, dtype_code
+from .runtime import library
 
 TOP_MAX = 32  # PG_LOGPROB_TOP
 
@@ -32,18 +35,7 @@ class LogProbs(NamedTuple):
     top_ids: Any  # [rows, top] int32
 
 
-def _dtype_code(dtype: Any) -> int:
-    import torch
-
-    code = {torch.float16: 1, torch.bfloat16: 2, torch.float32: 3}.get(dtype)
-    if code is None:
-        raise ValueError(f"dtype {dtype}: want float32, bfloat16 or float16")
-    return code
-
-
 def _inputs(logits: Any, tokens: Any) -> tuple[int, int, int, int, int, int, int]:
-    import torch
-
     if logits.dim() != 2 or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits: want [rows, vocab] on a CUDA device with contiguous rows, got "
                          f"{tuple(logits.shape)} {logits.stride()} on {logits.device}")
@@ -52,13 +44,11 @@ def _inputs(logits: Any, tokens: Any) -> tuple[int, int, int, int, int, int, int
             not tokens.is_contiguous() or tokens.device != logits.device:
         raise ValueError(f"tokens: want contiguous int64 or int32 [{rows}] on {logits.device}, "
                          f"got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
-    return (logits.data_ptr(), logits.stride(0), _dtype_code(logits.dtype), tokens.data_ptr(),
+    return (logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), tokens.data_ptr(),
             tokens.element_size(), rows, vocab)
 
 
 def _per_row(name: str, t: Any, logits: Any, *more: int) -> int:
-    import torch
-
     if t is None:
         return 0
     shape = (logits.shape[0], *more)
@@ -72,29 +62,25 @@ def _per_row(name: str, t: Any, logits: Any, *more: int) -> int:
 def logprobs(logits: Any, tokens: Any, top: int = 0, stream: int | None = None) -> LogProbs:
     """``LogProbs`` of ``tokens`` [rows] under ``logits`` [rows, vocab], with the ``top`` (at
     most 32) largest log probabilities of each row."""
-    import torch
-
     args = _inputs(logits, tokens)
     rows, vocab = logits.shape
     if not 0 <= top <= min(TOP_MAX, vocab):
         raise ValueError(f"top {top}: want 0 to {min(TOP_MAX, vocab)}")
-    logp, entropy = torch.empty((2, rows), dtype=torch.float32, device=logits.device).unbind(0)
-    norm = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
-    top_logp = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    top_ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-    with torch_stream(logits.device, stream) as s:
-        _check(library().pg_logprobs(
-            *args, top, logp.data_ptr(), entropy.data_ptr(), norm.data_ptr(), top_logp.data_ptr(),
-            top_ids.data_ptr(), s), "pg_logprobs")
-    return LogProbs(logp, entropy, norm, top_logp, top_ids)
+    # the results in one allocation, which costs as much as each of theirs would
+    both = torch.empty((4 + 2 * top) * rows, dtype=torch.float32, device=logits.device)
+    norm, logp, entropy, top_logp, top_ids = both.split_with_sizes(
+        (2 * rows, rows, rows, top * rows, top * rows))
+    at = both.data_ptr()
+    call(library().pg_logprobs, logits.device, stream, *args, top, at + 8 * rows, at + 12 * rows,
+         at, at + 16 * rows, at + (16 + 4 * top) * rows)
+    return LogProbs(logp, entropy, norm.view(rows, 2), top_logp.view(rows, top),
+                    top_ids.view(torch.int32).view(rows, top))
 
 
 def logprobs_grad(logits: Any, tokens: Any, result: LogProbs, d_logp: Any, d_entropy: Any = None,
                   out: Any = None, stream: int | None = None) -> Any:
     """The gradient of sum(d_logp * logp + d_entropy * entropy) with respect to ``logits``, given
     ``result`` = ``logprobs(logits, tokens)``; into ``out`` (which may be ``logits``) if given."""
-    import torch
-
     args = _inputs(logits, tokens)
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
@@ -102,10 +88,8 @@ def logprobs_grad(logits: Any, tokens: Any, result: LogProbs, d_logp: Any, d_ent
             or (out.shape[1] > 1 and out.stride(1) != 1):
         raise ValueError(f"out: want {logits.dtype} {tuple(logits.shape)} on {logits.device} "
                          "with contiguous rows")
-    with torch_stream(logits.device, stream) as s:
-        _check(library().pg_logprobs_grad(
-            *args, _per_row("norm", result.norm, logits, 2),
-            _per_row("entropy", result.entropy, logits), _per_row("d_logp", d_logp, logits),
-            _per_row("d_entropy", d_entropy, logits), out.data_ptr(), out.stride(0), s),
-            "pg_logprobs_grad")
+    call(library().pg_logprobs_grad, logits.device, stream, *args,
+         _per_row("norm", result.norm, logits, 2), _per_row("entropy", result.entropy, logits),
+         _per_row("d_logp", d_logp, logits), _per_row("d_entropy", d_entropy, logits),
+         out.data_ptr(), out.stride(0))
     return out

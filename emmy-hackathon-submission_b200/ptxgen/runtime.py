@@ -147,31 +147,6 @@ def init(device: int = 0) -> None:
     _initialised.add(device)
 
 
-class torch_stream:
-    """``with torch_stream(device, stream) as s``: the stream to launch on, as an integer
-    (``device``'s current one where ``stream`` is None), with ``device`` current inside."""
-
-    def __init__(self, device: Any, stream: int | None = None):
-        self.device, self.stream, self.before = device, stream, None
-
-    def __enter__(self) -> int:
-        import torch
-
-        index = self.device.index
-        now = torch.cuda.current_device()
-        if now != index:
-            self.before = now
-            torch.cuda.set_device(index)
-        return torch.cuda.current_stream(index).cuda_stream if self.stream is None \
-            else self.stream
-
-    def __exit__(self, *exc: Any) -> None:
-        if self.before is not None:
-            import torch
-
-            torch.cuda.set_device(self.before)
-
-
 def header_notes(ptx: str) -> dict[str, list[str]]:
     notes: dict[str, list[str]] = {}
     for key, rest in _NOTE.findall(ptx):
