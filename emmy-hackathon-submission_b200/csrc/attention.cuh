@@ -134,6 +134,7 @@ __device__ __forceinline__ float factor(float a, float b) {
 
 // Kernels for the 16-bit types at head sizes of up to 128: one query a sequence
 // (attention_decode.cu), and several (attention_prompt.cu).
+bool decode_fits(const Attention &a, int max_len);  // its blocks of keys count in 31 bits
 int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream);
 int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                  cudaStream_t stream);

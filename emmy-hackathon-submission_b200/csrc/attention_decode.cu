@@ -3,8 +3,8 @@
 //
 // HBM bounds it: every key and value is read once and used for the query heads of its group
 // only. So the work is cut evenly by keys, not by sequences: the blocks of 64 keys of all
-// (sequence, kv head) pairs form one line, and block c of C takes the c-th of C equal pieces of
-// it. A pair whose keys lie in several pieces is joined by the last block that finishes one, in
+// (sequence, kv head) pairs form one line, and block c takes the c-th of as many equal pieces of
+// it as there are blocks. A pair whose keys lie in several pieces is joined by the last block that finishes one, in
 // the pieces' order.
 //
 // Within a block each of four warps takes every fourth 16 keys by itself: it copies their rows
@@ -24,9 +24,8 @@ using pg::Blocks;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kStep = 16;             // keys a warp takes at a time
 constexpr int kKeys = kStep * kWarps; // keys of a block's step
-constexpr int kStages = 3;
 constexpr int kRows = 16;
-constexpr int kPerSm = 2;
+constexpr int kPerSm = 2;             // blocks an SM holds
 
 template <class T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
@@ -87,16 +86,11 @@ struct Ring {
   static constexpr int row = DIM * 2, chunks = DIM / 8;
   static constexpr int tile = kStep * row;        // 16 keys, or 16 values
   static constexpr int stage = 2 * tile;
-  static constexpr int warp = kStages * stage;
+  static constexpr int stages = 384 / DIM;
+  static constexpr int warp = stages * stage;
   static constexpr int bytes = kWarps * warp;
   static_assert(warp >= kRows * (DIM + 2) * 4, "a warp's result takes its ring's place");
   __device__ static int at(int r, int chunk) { return r * row + ((chunk ^ (r & 7)) << 4); }
-};
-
-// What every block works out for itself: how many blocks of keys each sequence has.
-struct Line {
-  int64_t total;   // blocks of keys of the whole batch, over all heads and row groups
-  int pieces;      // how many equal pieces the line is cut in
 };
 
 __device__ __forceinline__ int length_of(const Attention &a, int b, int *slot) {
@@ -118,66 +112,60 @@ __device__ __forceinline__ int blocks_in(const Attention &a, int length) {
   return pg::blocks_of(a, length - 1, length - 1, kKeys).count;
 }
 
-// The piece that unit u of the line lies in: piece c is [c total / C, (c + 1) total / C).
-__device__ __forceinline__ int piece_of(const Line &line, int64_t u) {
-  return static_cast<int>(((u + 1) * line.pieces - 1) / line.total);
-}
-
 template <class T, int DIM>
-__global__ void __launch_bounds__(kThreads, kPerSm)
-    decode_kernel(Attention a, int least_units) {
+__global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(Attention a) {
   using R = Ring<DIM>;
   extern __shared__ float4 smem4[];
-  __shared__ int64_t scan[kThreads];
+  __shared__ uint32_t warp_sum[kWarps];
   __shared__ int found_b;
-  __shared__ int64_t found_before;
+  __shared__ uint32_t found_before;
   __shared__ unsigned last;
   pg::wait_for_earlier_kernels();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int row_groups = (a.group + kRows - 1) / kRows, per_block = a.heads * row_groups;
+  const uint32_t row_groups = (a.group + kRows - 1) / kRows, per_block = a.heads * row_groups;
+  const uint32_t c = blockIdx.x;
 
-  // the line: thread i counts a run of sequences
+  // Every block works the line out for itself: thread i counts the units (blocks of keys of a
+  // head and row group) of a run of sequences.
   const int run = (a.batch + kThreads - 1) / kThreads;
   const int first_b = min(tid * run, a.batch), end_b = min(first_b + run, a.batch);
-  int64_t mine = 0;
+  uint32_t mine = 0;
   for (int b = first_b; b < end_b; ++b) {
     int slot;
-    mine += blocks_in(a, length_of(a, b, &slot));
+    const int n = length_of(a, b, &slot);
+    mine += blocks_in(a, n);
+    if (!n && b % gridDim.x == c)  // no key: zeros
+      for (int h = 0; h < a.heads * a.group; ++h)
+        for (int j = 0; j < a.dim / 8; ++j)
+          *reinterpret_cast<uint4 *>(a.out + b * a.out_token + h * a.out_head + j * 16) =
+              make_uint4(0, 0, 0, 0);
   }
   mine *= per_block;
-  scan[tid] = mine;
+  uint32_t upto = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += o;
+  }
+  if (lane == 31) warp_sum[warp] = upto;
   __syncthreads();
-  for (int off = 1; off < kThreads; off <<= 1) {
-    const int64_t o = tid >= off ? scan[tid - off] : 0;
-    __syncthreads();
-    scan[tid] += o;
-    __syncthreads();
+  uint32_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += warp_sum[w];
+    total += warp_sum[w];
   }
-  Line line;
-  line.total = scan[kThreads - 1];
-  const int64_t wanted = (line.total + least_units - 1) / least_units;
-  line.pieces = static_cast<int>(wanted < gridDim.x ? wanted : gridDim.x);
-  const int c = blockIdx.x;
-
-  // sequences without a key: zeros
-  for (int b = c; b < a.batch; b += gridDim.x) {
-    int slot;
-    if (length_of(a, b, &slot) > 0) continue;
-    for (int i = tid; i < a.heads * a.group * (a.dim / 8); i += kThreads) {
-      const int h = i / (a.dim / 8), j = i % (a.dim / 8);
-      *reinterpret_cast<uint4 *>(a.out + b * a.out_token + h * a.out_head + j * 16) =
-          make_uint4(0, 0, 0, 0);
-    }
-  }
-  if (c >= line.pieces) return;
-  int64_t u = line.total * c / line.pieces;
-  const int64_t u_end = line.total * (c + 1) / line.pieces;
-  const int64_t upto = scan[tid], before = upto - mine;
+  // The units of a piece; piece c is [c per, (c + 1) per). One is not too few: four sequences of
+  // up to 777 keys take 12 us, with at least two 16.5, with four 19.5.
+  const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
+  if (static_cast<uint64_t>(c) * per >= total) return;
+  uint32_t u = c * per;
+  const uint32_t u_end = min(total, u + per), before = upto - mine;
   if (u >= before && u < upto) {
-    int64_t at = before;
+    uint32_t at = before;
     for (int b = first_b; b < end_b; ++b) {
       int slot;
-      const int64_t units = static_cast<int64_t>(blocks_in(a, length_of(a, b, &slot))) * per_block;
+      const uint32_t units = blocks_in(a, length_of(a, b, &slot)) * per_block;
       if (u < at + units) {
         found_b = b;
         found_before = at;
@@ -188,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   }
   __syncthreads();
   int b = found_b;
-  int64_t seq_before = found_before;
+  uint32_t seq_before = found_before;
 
   char *ring = reinterpret_cast<char *>(smem4) + warp * R::warp;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
@@ -201,13 +189,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       ++b;
       continue;
     }
-    const int pair = static_cast<int>((u - seq_before) / blocks.count);
+    const uint32_t pair = (u - seq_before) / blocks.count;
     const int head = pair / row_groups, row0 = (pair % row_groups) * kRows;
     const int rows = min(kRows, a.group - row0);
-    const int64_t pair_first = seq_before + static_cast<int64_t>(pair) * blocks.count;
-    const int block0 = static_cast<int>(u - pair_first);
-    const int64_t stop = min(u_end, pair_first + blocks.count);
-    const int block1 = static_cast<int>(stop - pair_first);
+    const uint32_t pair_first = seq_before + pair * blocks.count;
+    const int block0 = u - pair_first;
+    const uint32_t stop = min(u_end, pair_first + blocks.count);
+    const int block1 = stop - pair_first;
     const int *pages = a.table + slot * a.table_row;
     const int pos = length - 1;
 
@@ -229,50 +217,85 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
 
-    // the warp's steps are the blocks' 16 keys at 16 warp; lane r < 16 knows key r's page
+    // The warp's steps are the blocks' 16 keys at 16 warp. A step whose keys all are seen and lie
+    // in one page, as they do where pages are whole groups of 16, needs one look at the table and
+    // one address; else lane r < 16 knows key r's page and row.
     const int steps = block1 - block0;
-    const auto first_key = [&](int i) { return blocks.key_block(block0 + i) * kKeys + kStep * warp; };
-    const auto page_for = [&](int i) {  // this lane's page and row for step i; -1: not seen
-      int2 p = make_int2(-1, 0);
-      if (i < steps) {
-        const int key = first_key(i) + (lane & 15);
-        if (pg::sees(a, pos, key)) {
-          const int entry = key / a.page_size;
-          p = make_int2(pages[entry], key - entry * a.page_size);
-          if (p.x < 0 || p.x >= a.pages) {
-            atomicOr(a.status, PG_CACHE_BAD_PAGE);
-            p.x = -1;
-          }
-        }
-      }
-      return p;
+    const bool whole_pages = a.page_size % kStep == 0;
+    const auto first_key = [&](int i) {
+      return blocks.key_block(block0 + i) * kKeys + kStep * warp;
     };
-    const auto issue = [&](int i, int2 p) {
+    const auto all_seen = [&](int key) {
+      return key + kStep - 1 <= pos &&
+             (!a.window || key > pos - a.window || key + kStep <= a.sinks);
+    };
+    const auto page_for = [&](int i) {  // as the table names it; -1: not seen
+      if (i >= steps) return -1;
+      const int key = first_key(i);
+      if (whole_pages && all_seen(key)) return pages[key / a.page_size];
+      return pg::sees(a, pos, key + (lane & 15)) ? pages[(key + (lane & 15)) / a.page_size] : -1;
+    };
+    const int sub = lane / R::chunks, chunk = lane % R::chunks;
+    const bool column = chunk * 8 < a.dim;
+    const int64_t row_bytes = 2ll * a.dim;
+    const char *const k_head = a.k + head * a.k_head + chunk * 16;
+    const char *const v_head = a.v + head * a.v_head + chunk * 16;
+    constexpr int kCopies = kStep * R::chunks / 32, kRowsEach = 32 / R::chunks;
+    const auto issue = [&](int i, int page) {
       if (i < steps) {
-        const uint32_t to = ring_at + (i % kStages) * R::stage;
+        const uint32_t to = ring_at + (i % R::stages) * R::stage;
+        const int key = first_key(i);
+        if (whole_pages && all_seen(key)) {
+          bool real = column;
+          if (page < 0 || page >= a.pages) {
+            atomicOr(a.status, PG_CACHE_BAD_PAGE);
+            real = false, page = 0;
+          }
+          const int64_t in = (key % a.page_size + sub) * row_bytes;
+          const char *k = k_head + page * a.k_page + in, *v = v_head + page * a.v_page + in;
 #pragma unroll
-        for (int j = 0; j < kStep * R::chunks / 32; ++j) {
-          const int r = j * (32 / R::chunks) + lane / R::chunks, chunk = lane % R::chunks;
-          const int page = __shfl_sync(0xffffffffu, p.x, r);
-          const int row = __shfl_sync(0xffffffffu, p.y, r);
-          const bool real = page >= 0 && chunk * 8 < a.dim;
-          const int64_t in = real ? static_cast<int64_t>(row) * a.dim * 2 + chunk * 16 : 0;
-          const int64_t pg = real ? page : 0;
-          copy16(to + R::at(r, chunk), a.k + pg * a.k_page + head * a.k_head + in, real);
-          copy16(to + R::tile + R::at(r, chunk), a.v + pg * a.v_page + head * a.v_head + in, real);
+          for (int j = 0; j < kCopies; ++j) {
+            const uint32_t at = to + R::at(j * kRowsEach + sub, chunk);
+            copy16(at, k, real);
+            copy16(at + R::tile, v, real);
+            k += kRowsEach * row_bytes;
+            v += kRowsEach * row_bytes;
+          }
+        } else {
+          const int mine_key = key + (lane & 15);
+          if (pg::sees(a, pos, mine_key) && (page < 0 || page >= a.pages)) {
+            atomicOr(a.status, PG_CACHE_BAD_PAGE);
+            page = -1;
+          }
+          const int mine_row = mine_key % a.page_size;
+#pragma unroll
+          for (int j = 0; j < kCopies; ++j) {
+            const int r = j * kRowsEach + sub;
+            const int at_page = __shfl_sync(0xffffffffu, page, r);
+            const int row = __shfl_sync(0xffffffffu, mine_row, r);
+            const bool real = at_page >= 0 && column;
+            const int64_t in = real ? row * row_bytes : 0, pg = real ? at_page : 0;
+            copy16(to + R::at(r, chunk), k_head + pg * a.k_page + in, real);
+            copy16(to + R::tile + R::at(r, chunk), v_head + pg * a.v_page + in, real);
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    int next = page_for(0);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i, page_for(i));
-    int2 next = page_for(kStages - 1);
+    for (int i = 0; i < R::stages - 1; ++i) {
+      const int page = next;
+      next = page_for(i + 1);
+      issue(i, page);
+    }
     for (int i = 0; i < steps; ++i) {
-      issue(i + kStages - 1, next);
-      next = page_for(i + kStages);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      const int page = next;
+      next = page_for(i + R::stages);
+      issue(i + R::stages - 1, page);
+      asm volatile("cp.async.wait_group %0;" ::"n"(R::stages - 1) : "memory");
       __syncwarp();
-      const uint32_t ks = ring_at + (i % kStages) * R::stage, vs = ks + R::tile;
+      const uint32_t ks = ring_at + (i % R::stages) * R::stage, vs = ks + R::tile;
       float s[2][4] = {};
 #pragma unroll
       for (int k = 0; k < DIM / 32; ++k)
@@ -283,14 +306,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
           Mma<T>::run(s[n], q[2 * k], x[0], x[1]);
           Mma<T>::run(s[n], q[2 * k + 1], x[2], x[3]);
         }
-      const int key = first_key(i) + 2 * t4;
+      const int key = first_key(i);
+      const bool masked = !all_seen(key);
       float top[2] = {m[0], m[1]};
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool seen = pg::sees(a, pos, key + 8 * n + (e & 1));
-          s[n][e] = seen ? s[n][e] * a.scale_log2 : -INFINITY;
+          s[n][e] *= a.scale_log2;
+          if (masked && !pg::sees(a, pos, key + 2 * t4 + 8 * n + (e & 1))) s[n][e] = -INFINITY;
           top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
         }
 #pragma unroll
@@ -357,13 +381,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     }
     __syncthreads();
 
-    const int c0 = piece_of(line, pair_first), c1 = piece_of(line, pair_first + blocks.count - 1);
+    const uint32_t c0 = pair_first / per, c1 = (pair_first + blocks.count - 1) / per;
     const bool alone = c0 == c1;
     constexpr int kPartial = kRows * (DIM + 2);
-    // a block has at most two pairs that others share: one it starts in the middle of (or at
-    // the start of its piece), and one it leaves in the middle of
-    const auto slot_of = [&](int piece) {
-      return a.partial + (2ll * piece + (pair_first > line.total * piece / line.pieces)) * kPartial;
+    // a block has at most two pairs that others share: one that its piece starts with, and one
+    // it leaves in the middle of
+    const auto slot_of = [&](uint32_t piece) {
+      return a.partial + (2ll * piece + (pair_first > piece * per)) * kPartial;
     };
     // thread's columns: four of row `warp`, `warp + 4`, ...
     const int lanes = DIM / 4;
@@ -405,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       __threadfence();
       __syncthreads();
       // the counter of the piece that the pair starts in: no other pair's
-      if (tid == 0) last = atomicInc(a.arrived + c0, c1 - c0) == static_cast<unsigned>(c1 - c0);
+      if (tid == 0) last = atomicInc(a.arrived + c0, c1 - c0) == c1 - c0;
       __syncthreads();
       if (last) {
         __threadfence();
@@ -413,10 +437,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
           const int r = i / lanes, col = 4 * (i % lanes);
           float top = -INFINITY, sum = 0.0f;
           float4 acc = make_float4(0, 0, 0, 0);
-          for (int p = c0; p <= c1; ++p) top = fmaxf(top, __ldcg(slot_of(p) + kRows * DIM + r));
+          for (uint32_t p = c0; p <= c1; ++p) top = fmaxf(top, __ldcg(slot_of(p) + kRows * DIM + r));
           const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
-          for (int p = c0; p <= c1; ++p) {
+          for (uint32_t p = c0; p <= c1; ++p) {
             const float *from = slot_of(p);
             const float f = pg::factor(__ldcg(from + kRows * DIM + r), base);
             const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + r * DIM + col));
@@ -436,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     }
     __syncthreads();  // the rings are free again
     u = stop;
-    if (u == seq_before + static_cast<int64_t>(blocks.count) * per_block) {
+    if (u == seq_before + blocks.count * per_block) {
       seq_before = u;
       ++b;
     }
@@ -445,15 +469,18 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
 
 template <class T, int DIM>
 int launch_decode(const Attention &a, int sms, cudaStream_t stream) {
-  // a block per 4 units (256 keys) at least, below which the joining costs more than it gives
-  constexpr int kLeast = 4;
   return pg::launch<decode_kernel<T, DIM>>("decode_kernel", dim3(kPerSm * sms), kThreads,
-                    Ring<DIM>::bytes, stream, a, kLeast);
+                                           Ring<DIM>::bytes, stream, a);
 }
 
 }  // namespace
 
 namespace pg {
+
+bool decode_fits(const Attention &a, int max_len) {
+  const int64_t pairs = static_cast<int64_t>(a.batch) * a.heads * ((a.group + kRows - 1) / kRows);
+  return pairs * (max_len / kKeys + 2ll) < INT32_MAX;
+}
 
 int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream) {
   if (bf16)

@@ -47,7 +47,9 @@ namespace {
 
 using pg::Attention;
 using pg::Blocks;
+using pg::max3;
 using pg::Tile;
+using pg::Two;
 
 constexpr int kKeys = 128, kRows = 256, kHalf = 128;
 constexpr int kThreads = 384;
@@ -201,39 +203,12 @@ __device__ __forceinline__ void wait_stores() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// The largest of three; NaN if one is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // The largest score of a row of a block, and m.
 __device__ __forceinline__ float largest(const float *s, float m) {
   float top[4] = {m, s[0], s[1], s[2]};
 #pragma unroll
   for (int k = 3; k < kKeys - 1; k += 2) top[k / 2 & 3] = max3(top[k / 2 & 3], s[k], s[k + 1]);
   return max3(max3(top[0], top[1], top[2]), top[3], s[kKeys - 1]);
-}
-
-// Two 32-bit numbers that one instruction multiplies and adds.
-struct Two {
-  uint64_t v;
-  __device__ Two(uint64_t x) : v(x) {}
-  __device__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
-  __device__ void get(float &x, float &y) const {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
-  }
-};
-__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Two add(Two a, Two b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
-  return r;
 }
 
 template <class T> struct Type;

@@ -93,6 +93,38 @@ __device__ __forceinline__ void wait_for_earlier_kernels() {
 #endif
 }
 
+// The largest of three; NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two 32-bit numbers that one instruction multiplies and adds.
+struct Two {
+  uint64_t v;
+  __device__ Two(uint64_t x) : v(x) {}
+  __device__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ void get(float &x, float &y) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+  }
+};
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two add(Two a, Two b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 __device__ __forceinline__ uint4 load16(const void *p) {
   return *reinterpret_cast<const uint4 *>(p);
 }

@@ -4,10 +4,10 @@
 // With m the row's largest logit, s = sum exp(x - m) and t = sum (x - m) exp(x - m):
 //   log p_j = (x_j - m) - log s,  entropy H = log s - t / s,
 //   d x_j = a ([j = token] - p_j) - b p_j (log p_j + H)   for gradients a of log p_token, b of H.
-// One pass keeps m, s and t in 32 bits a thread, rescaling s and t when m grows:
+// One pass keeps m, s and t in 32 bits a thread (t in powers of two), rescaling s and t when m
+// grows:
 //   s' = s f,  t' = (t + (m - m') s) f,  f = exp(m - m').
-// x - m is cut off at -1e4, where exp is 0 long since, so a logit of -inf adds 0 to t and not
-// 0 * inf; m starts at the lowest finite number, so a row of lowest numbers is an even
+// x - m is cut off where exp is 0 long since, so a logit of -inf adds 0 to t and not 0 * inf; m starts at the lowest finite number, so a row of lowest numbers is an even
 // distribution and only a row of nothing but -inf (s = 0) has none: it gives NaN, as does a row
 // with a NaN or +inf. The gradient goes by the pair (m, log s), not by their sum, which would lose
 // log s beside a large m.
@@ -25,8 +25,8 @@ constexpr int kBatch = 4;            // 16-byte loads a thread has in flight
 constexpr int kTopMax = PG_LOGPROB_TOP;
 constexpr int kCandidates = 1024;    // elements the selection of the top ones may look at
 constexpr float kLowest = -3.402823466e38f;
-constexpr float kCut = -1e4f;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kCut = -1e4f;        // of x - m in powers of two, below which exp is 0
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -34,16 +34,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ float exp_fast(float x) {
+__device__ __forceinline__ float exp2_fast(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * kLog2e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
-// ... with results below 2^-126 kept: the factor of a probability in the gradient may be large
-__device__ __forceinline__ float exp_small(float x) {
+// ... with results below 2^-126 kept
+__device__ __forceinline__ float exp2_small(float x) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x * kLog2e));
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -109,13 +109,13 @@ __device__ __forceinline__ void from_float(float x, __nv_bfloat16 *to) {
 }
 __device__ __forceinline__ void from_float(float x, __half *to) { *to = __float2half_rn(x); }
 
-// Row sums: the largest logit, the sum of exp(x - m) and of (x - m) exp(x - m).
+// Row sums: the largest logit m, and with d = (x - m) log2 e the sums of 2^d and of d 2^d.
 struct Sums {
-  float m = kLowest, s = 0.0f, t = 0.0f;
+  float m, s, t;
 };
 
 __device__ __forceinline__ void rescale(Sums &a, float m) {
-  const float d = max_nan(a.m - m, kCut), f = exp_fast(d);
+  const float d = max_nan((a.m - m) * kLog2e, kCut), f = exp2_fast(d);
   a.t = (a.t + d * a.s) * f;
   a.s *= f;
   a.m = m;
@@ -130,19 +130,31 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   return a;
 }
 
+// One vector more. The subtraction comes before the scaling, so that it is exact for the large
+// numbers of a mask; two at a time otherwise, since instructions bound this, not memory.
 template <int N>
 __device__ __forceinline__ void add(Sums &a, const float *x) {
-  float top = x[0];
+  float top = a.m;
 #pragma unroll
-  for (int i = 1; i < N; ++i) top = max_nan(top, x[i]);
-  top = max_nan(a.m, top);
+  for (int i = 0; i < N; i += 2) top = pg::max3(top, x[i], x[i + 1]);
   if (top != a.m) rescale(a, top);
+  const pg::Two m(-a.m, -a.m), scale(kLog2e, kLog2e);
+  pg::Two s(a.s, 0.0f), t(a.t, 0.0f);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = max_nan(x[i] - a.m, kCut), e = exp_fast(d);
-    a.s += e;
-    a.t = fmaf(d, e, a.t);
+  for (int i = 0; i < N; i += 2) {
+    float d, e;
+    mul(add(pg::Two(x[i], x[i + 1]), m), scale).get(d, e);
+    d = max_nan(d, kCut);
+    e = max_nan(e, kCut);
+    const pg::Two p(exp2_fast(d), exp2_fast(e));
+    s = add(s, p);
+    t = fma(pg::Two(d, e), p, t);
   }
+  float u, v;
+  s.get(u, v);
+  a.s = u + v;
+  t.get(u, v);
+  a.t = u + v;
 }
 
 // A key whose order as a whole number is the logits' order, NaN above all, -0 equal to 0; 0 is
@@ -290,23 +302,40 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int64_t v64 = vocab;
   const Part<T> part(x_row, static_cast<int>(v64 * rank / parts),
                      static_cast<int>(v64 * (rank + 1) / parts));
-  Sums mine;
+  Sums mine{kLowest, 0.0f, 0.0f};
   int v = tid;
-  for (; v + (kBatch - 1) * kThreads < part.vectors; v += kBatch * kThreads) {
-    float x[kBatch][Vec<T>::n];
-    if (part.whole(v) && part.whole(v + (kBatch - 1) * kThreads)) {
-      uint4 raw[kBatch];
+  // whole batches, the next one's loads on their way while one is added up
+  const auto batch_here = [&](int at) {
+    return at + (kBatch - 1) * kThreads < part.vectors && part.whole(at) &&
+           part.whole(at + (kBatch - 1) * kThreads);
+  };
+  const T *const vectors = part.row + part.base;
+  if (v < part.vectors && !part.whole(v)) {  // the first vector may start before the part
+    float x[Vec<T>::n];
+    part.load(v, x);
+    add<Vec<T>::n>(mine, x);
+    v += kThreads;
+  }
+  if (batch_here(v)) {
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      raw[u] = pg::load16(vectors + static_cast<int64_t>(v + u * kThreads) * Vec<T>::n);
+    for (bool more = true; more;) {
+      v += kBatch * kThreads;
+      more = batch_here(v);
+      uint4 next[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        raw[u] = pg::load16(part.row + part.base + (v + u * kThreads) * Vec<T>::n);
+        if (more) next[u] = pg::load16(vectors + static_cast<int64_t>(v + u * kThreads) * Vec<T>::n);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) Vec<T>::get(raw[u], x[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) part.load(v + u * kThreads, x[u]);
+      for (int u = 0; u < kBatch; ++u) {
+        float x[Vec<T>::n];
+        Vec<T>::get(raw[u], x);
+        add<Vec<T>::n>(mine, x);
+        raw[u] = next[u];
+      }
     }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) add<Vec<T>::n>(mine, x[u]);
   }
   for (; v < part.vectors; v += kThreads) {
     float x[Vec<T>::n];
@@ -346,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (token != -1)
         lp = token < 0 || token >= vocab || none ? NAN : (to_float(x_row[token]) - r.m) - log_s;
       logp[row] = lp;
-      entropy[row] = none ? NAN : log_s - r.t / r.s;
+      entropy[row] = none ? NAN : log_s - kLn2 * (r.t / r.s);
       norm[row] = make_float2(r.m, log_s);
     }
     for (int i = tid; i < parts * top; i += kThreads) {
@@ -388,11 +417,21 @@ __global__ void __launch_bounds__(kThreads)
   if (token < -1 || token >= vocab) a = NAN;
   const float b = d_entropy ? d_entropy[row] : 0.0f;
   const float c = fmaf(b, h, a);
-  // -p (a + b (log p + H)), and a more at the token
-  const auto grad = [&](float x, int column) {
-    const float lp = max_nan((x - l.x) - l.y, kCut), p = exp_small(lp);
-    const float g = -p * fmaf(b, lp, c);
-    return column == token ? g + a : g;
+  // -p (a + b (log p + H)) of two columns; the token's a is added after. Probabilities below
+  // 2^-126 become 0 but for f32 results, which can hold such numbers times a large factor.
+  const pg::Two m(-l.x, -l.x), log_s(-l.y, -l.y), scale(kLog2e, kLog2e), b2(-b, -b), c2(-c, -c);
+  const auto grad = [&](float &x, float &y) {
+    add(add(pg::Two(x, y), m), log_s).get(x, y);
+    const pg::Two lp(max_nan(x, kCut), max_nan(y, kCut));
+    mul(lp, scale).get(x, y);
+    const pg::Two p = sizeof(T) == 4 ? pg::Two(exp2_small(x), exp2_small(y))
+                                     : pg::Two(exp2_fast(x), exp2_fast(y));
+    mul(p, fma(b2, lp, c2)).get(x, y);
+  };
+  const auto grad_one = [&](int column) {
+    float x = to_float(x_row[column]), y = x;
+    grad(x, y);
+    from_float(column == token ? x + a : x, y_row + column);
   };
   const int over_x = static_cast<int>((reinterpret_cast<uintptr_t>(x_row) & 15) / sizeof(T));
   const int over_y = static_cast<int>((reinterpret_cast<uintptr_t>(y_row) & 15) / sizeof(T));
@@ -411,19 +450,25 @@ __global__ void __launch_bounds__(kThreads)
         float x[n];
         Vec<T>::get(raw[u], x);
 #pragma unroll
-        for (int i = 0; i < n; ++i) x[i] = grad(x[i], at + i);
+        for (int i = 0; i < n; i += 2) grad(x[i], x[i + 1]);
+        const int64_t here = token - at;
+        if (here >= 0 && here < n) {
+#pragma unroll
+          for (int i = 0; i < n; ++i)
+            if (i == here) x[i] += a;
+        }
         *reinterpret_cast<uint4 *>(y_row + at) = Vec<T>::put(x);
       } else {
         for (int i = 0; i < n; ++i)
           if (at + i >= 0 && at + i < vocab)
-            from_float(grad(to_float(x_row[at + i]), at + i), y_row + at + i);
+            grad_one(at + i);
       }
     }
     return;
   }
   // logits and gradients lie differently on 16-byte boundaries: one element at a time
   for (int at = first + static_cast<int>(threadIdx.x); at < first + span; at += kThreads)
-    if (at >= 0 && at < vocab) from_float(grad(to_float(x_row[at]), at), y_row + at);
+    if (at >= 0 && at < vocab) grad_one(at);
 }
 
 template <class T>
