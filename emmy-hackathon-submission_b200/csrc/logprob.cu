@@ -25,6 +25,7 @@ constexpr int kThreads = 256, kPerSm = 4;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;            // 16-byte loads a thread has in flight
 constexpr int kTopMax = PG_LOGPROB_TOP;
+constexpr int kParts = 8;            // blocks a row is cut in at most (a portable cluster)
 constexpr int kCandidates = 1024;    // elements the selection of the top ones may look at
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kCut = -1e4f;        // of x - m in powers of two, below which exp is 0
@@ -206,6 +207,7 @@ struct Part {
 struct Shared {
   Sums warp[kWarps];
   Sums row;                          // the part's sums
+  Sums part[kParts];                 // the parts' sums
   uint32_t chosen[kThreads];         // the threads whose strips are looked at again
   uint64_t found[kCandidates];
   uint64_t top[kTopMax];             // the part's top entries, best first; 0 where there is none
@@ -368,38 +370,46 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     sh.row = all;
   }
   if (top) select_top(part, largest, any, top, sh);
-  cluster.sync();
-  if (rank == 0) {
-    // every thread joins the parts' sums in the same order
-    Sums r = sh.row;
-    for (int p = 1; p < parts; ++p) r = join(r, cluster.map_shared_rank(&sh, p)->row);
-    const float log_s = logf(r.s);
-    const bool none = r.s == 0.0f;
-    if (tid == 0) {
-      const int64_t token = token_bytes == 8 ? static_cast<const int64_t *>(tokens)[row]
-                                             : static_cast<const int32_t *>(tokens)[row];
-      float lp = 0.0f;
-      if (token != -1)
-        lp = token < 0 || token >= vocab || none ? NAN : (to_float(x_row[token]) - r.m) - log_s;
-      logp[row] = lp;
-      entropy[row] = none ? NAN : log_s - kLn2 * (r.t / r.s);
-      norm[row] = make_float2(r.m, log_s);
+  if (parts > 1) {
+    // the first block copies the others' sums and lists, and only then do those end
+    cluster.sync();
+    if (rank == 0) {
+      if (tid < parts) sh.part[tid] = cluster.map_shared_rank(&sh, tid)->row;
+      for (int i = tid; i < parts * top; i += kThreads)
+        sh.found[i] = cluster.map_shared_rank(&sh, i / top)->top[i % top];
     }
-    for (int i = tid; i < parts * top; i += kThreads) {
-      const uint64_t e = cluster.map_shared_rank(&sh, i / top)->top[i % top];
-      int place = 0;
-      for (int p = 0; p < parts; ++p) {
-        const uint64_t *list = cluster.map_shared_rank(&sh, p)->top;
-        for (int j = 0; j < top; ++j) place += list[j] > e;
-      }
-      if (e && place < top) {
-        const int64_t at = static_cast<int64_t>(row) * top + place;
-        top_ids[at] = static_cast<int32_t>(~static_cast<uint32_t>(e));
-        top_logp[at] = none ? NAN : (logit_of(static_cast<uint32_t>(e >> 32)) - r.m) - log_s;
-      }
+    cluster.sync();
+    if (rank) return;
+  } else {
+    if (tid < top) sh.found[tid] = sh.top[tid];
+    if (tid == 0) sh.part[0] = all;
+    __syncthreads();
+  }
+  // every thread joins the parts' sums in the same order
+  Sums r = sh.part[0];
+  for (int p = 1; p < parts; ++p) r = join(r, sh.part[p]);
+  const float log_s = logf(r.s);
+  const bool none = r.s == 0.0f;
+  if (tid == 0) {
+    const int64_t token = token_bytes == 8 ? static_cast<const int64_t *>(tokens)[row]
+                                           : static_cast<const int32_t *>(tokens)[row];
+    float lp = 0.0f;
+    if (token != -1)
+      lp = token < 0 || token >= vocab || none ? NAN : (to_float(x_row[token]) - r.m) - log_s;
+    logp[row] = lp;
+    entropy[row] = none ? NAN : log_s - kLn2 * (r.t / r.s);
+    norm[row] = make_float2(r.m, log_s);
+  }
+  for (int i = tid; i < parts * top; i += kThreads) {
+    const uint64_t e = sh.found[i];
+    int place = 0;
+    for (int j = 0; j < parts * top; ++j) place += sh.found[j] > e;
+    if (e && place < top) {
+      const int64_t at = static_cast<int64_t>(row) * top + place;
+      top_ids[at] = static_cast<int32_t>(~static_cast<uint32_t>(e));
+      top_logp[at] = none ? NAN : (logit_of(static_cast<uint32_t>(e >> 32)) - r.m) - log_s;
     }
   }
-  cluster.sync();  // a block's shared memory stays until the first one has read it
 }
 
 // Reads each logit once and writes its gradient; HBM bounds it. Rows go last to first, so that
@@ -485,11 +495,11 @@ int run_logprobs(uint64_t logits, int64_t row_stride, uint64_t tokens, int token
   int sms;
   int rc = pg::sm_count(&sms);
   if (rc) return rc;
-  // blocks a row: as many as still give every SM a block, up to a portable cluster, and no part
+  // blocks a row: as many as the SMs hold at once, up to a portable cluster, and no part
   // shorter than one batch of a block's loads
   int parts = 1;
   const int least = kThreads * Vec<T>::n;
-  while (parts < 8 && rows * 2ll * parts <= kPerSm * sms && vocab / (2 * parts) >= least) parts *= 2;
+  while (parts < kParts && rows * 2ll * parts <= kPerSm * sms && vocab / (2 * parts) >= least) parts *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
   cfg.blockDim = dim3(kThreads);

@@ -17,7 +17,7 @@ current stream, or on ``stream`` (a ``cudaStream_t`` as an integer).
 
 from __future__ import annotations
 
-from typing import Any, NamedTuple
+from typing import Any
 
 import torch
 
@@ -27,12 +27,42 @@ from .runtime import library
 TOP_MAX = 32  # PG_LOGPROB_TOP
 
 
-class LogProbs(NamedTuple):
-    logp: Any  # [rows] f32
-    entropy: Any  # [rows] f32
-    norm: Any  # [rows, 2] f32: the largest logit m, and log sum exp(x - m)
-    top_logp: Any  # [rows, top] f32, largest first
-    top_ids: Any  # [rows, top] int32
+class LogProbs:
+    """What ``logprobs`` returns. Its tensors are parts of one allocation, made when asked for: five
+    allocations would take the host longer than a short call takes the GPU."""
+
+    __slots__ = ("_all", "_rows", "_top")
+
+    def __init__(self, device: torch.device, rows: int, top: int):
+        # norm, logp, entropy, top_logp, top_ids
+        self._all = torch.empty((4 + 2 * top) * rows, dtype=torch.float32, device=device)
+        self._rows, self._top = rows, top
+
+    @property
+    def logp(self) -> Any:
+        """[rows] f32: log p[token]."""
+        return self._all.narrow(0, 2 * self._rows, self._rows)
+
+    @property
+    def entropy(self) -> Any:
+        """[rows] f32."""
+        return self._all.narrow(0, 3 * self._rows, self._rows)
+
+    @property
+    def norm(self) -> Any:
+        """[rows, 2] f32: the largest logit m, and log sum exp(x - m)."""
+        return self._all.as_strided((self._rows, 2), (2, 1))
+
+    @property
+    def top_logp(self) -> Any:
+        """[rows, top] f32, largest first."""
+        return self._all.as_strided((self._rows, self._top), (self._top, 1), 4 * self._rows)
+
+    @property
+    def top_ids(self) -> Any:
+        """[rows, top] int32: their columns."""
+        return self._all.as_strided((self._rows, self._top), (self._top, 1),
+                                    (4 + self._top) * self._rows).view(torch.int32)
 
 
 def _inputs(logits: Any, tokens: Any) -> tuple[int, int, int, int, int, int, int]:
@@ -40,7 +70,7 @@ def _inputs(logits: Any, tokens: Any) -> tuple[int, int, int, int, int, int, int
         raise ValueError(f"logits: want [rows, vocab] on a CUDA device with contiguous rows, got "
                          f"{tuple(logits.shape)} {logits.stride()} on {logits.device}")
     rows, vocab = logits.shape
-    if tokens.dtype not in (torch.int64, torch.int32) or tuple(tokens.shape) != (rows,) or \
+    if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != logits.shape[:1] or \
             not tokens.is_contiguous() or tokens.device != logits.device:
         raise ValueError(f"tokens: want contiguous int64 or int32 [{rows}] on {logits.device}, "
                          f"got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
@@ -48,14 +78,13 @@ def _inputs(logits: Any, tokens: Any) -> tuple[int, int, int, int, int, int, int
             tokens.element_size(), rows, vocab)
 
 
-def _per_row(name: str, t: Any, logits: Any, *more: int) -> int:
+def _per_row(name: str, t: Any, logits: Any) -> int:
     if t is None:
         return 0
-    shape = (logits.shape[0], *more)
-    if t.dtype is not torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or \
+    if t.dtype is not torch.float32 or t.shape != logits.shape[:1] or not t.is_contiguous() or \
             t.device != logits.device:
-        raise ValueError(f"{name}: want contiguous float32 {list(shape)} on {logits.device}, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        raise ValueError(f"{name}: want contiguous float32 [{logits.shape[0]}] on "
+                         f"{logits.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -66,15 +95,11 @@ def logprobs(logits: Any, tokens: Any, top: int = 0, stream: int | None = None) 
     rows, vocab = logits.shape
     if not 0 <= top <= min(TOP_MAX, vocab):
         raise ValueError(f"top {top}: want 0 to {min(TOP_MAX, vocab)}")
-    # the results in one allocation, which costs as much as each of theirs would
-    both = torch.empty((4 + 2 * top) * rows, dtype=torch.float32, device=logits.device)
-    norm, logp, entropy, top_logp, top_ids = both.split_with_sizes(
-        (2 * rows, rows, rows, top * rows, top * rows))
-    at = both.data_ptr()
+    result = LogProbs(logits.device, rows, top)
+    at = result._all.data_ptr()
     call(library().pg_logprobs, logits.device, stream, *args, top, at + 8 * rows, at + 12 * rows,
          at, at + 16 * rows, at + (16 + 4 * top) * rows)
-    return LogProbs(logp, entropy, norm.view(rows, 2), top_logp.view(rows, top),
-                    top_ids.view(torch.int32).view(rows, top))
+    return result
 
 
 def logprobs_grad(logits: Any, tokens: Any, result: LogProbs, d_logp: Any, d_entropy: Any = None,
@@ -88,8 +113,12 @@ def logprobs_grad(logits: Any, tokens: Any, result: LogProbs, d_logp: Any, d_ent
             or (out.shape[1] > 1 and out.stride(1) != 1):
         raise ValueError(f"out: want {logits.dtype} {tuple(logits.shape)} on {logits.device} "
                          "with contiguous rows")
-    call(library().pg_logprobs_grad, logits.device, stream, *args,
-         _per_row("norm", result.norm, logits, 2), _per_row("entropy", result.entropy, logits),
+    rows, of = logits.shape[0], result._all
+    if result._rows != rows or of.device != logits.device:
+        raise ValueError(f"result: of {result._rows} rows on {of.device}, logits have {rows} on "
+                         f"{logits.device}")
+    at = of.data_ptr()
+    call(library().pg_logprobs_grad, logits.device, stream, *args, at, at + 12 * rows,
          _per_row("d_logp", d_logp, logits), _per_row("d_entropy", d_entropy, logits),
          out.data_ptr(), out.stride(0))
     return out
