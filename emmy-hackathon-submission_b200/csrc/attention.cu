@@ -292,7 +292,9 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(Attention a) {
 template <class T, int ROWS, int DIM>
 int launch_tiles(Attention a, int tiles, cudaStream_t stream) {
   a.rows_per_tile = ROWS;
-  return pg::launch<attention_kernel<T, ROWS, DIM>>("attention_kernel", dim3(tiles, a.heads, a.parts), kThreads, Layout<ROWS, DIM>::bytes, stream, a);
+  return pg::launch<attention_kernel<T, ROWS, DIM>>(
+      "attention_kernel", dim3(tiles, a.heads, a.parts), kThreads, Layout<ROWS, DIM>::bytes, stream,
+      a);
 }
 
 template <class T, int ROWS>
@@ -386,9 +388,9 @@ extern "C" int pg_attention(const pg_attention_args *p, uint64_t stream) {
   const int64_t partial_bytes = p->workspace_bytes - 256 - pg::kCounters * 4ll;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
   if (dtype != PG_DT_F32 && a.dim <= 128) {
-    if (a.starts) return pg::prompt_16bit(a, dtype == PG_DT_BF16, max_len, partial_bytes, sms, s);
-    if (pg::decode_fits(a, static_cast<int>(most)))
+    if (pg::decode_takes(a, static_cast<int>(most)))
       return pg::decode_16bit(a, dtype == PG_DT_BF16, sms, s);
+    if (a.starts) return pg::prompt_16bit(a, dtype == PG_DT_BF16, max_len, partial_bytes, sms, s);
   }
   if (dtype == PG_DT_F32) return run<float>(a, max_len, partial_bytes, sms, s);
   if (dtype == PG_DT_BF16) return run<__nv_bfloat16>(a, max_len, partial_bytes, sms, s);

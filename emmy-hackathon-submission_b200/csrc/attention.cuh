@@ -121,6 +121,22 @@ __device__ __forceinline__ int page_of(const Attention &a, const Tile &t, int ke
   return -1;
 }
 
+// Zeroes the 16-bit numbers at `at` that are not finite (their exponent's bits are EXPONENT);
+// whether there were any.
+template <uint32_t EXPONENT>
+__device__ __forceinline__ bool clean(uint4 *at) {
+  const uint4 x = *at;
+  uint32_t u[4] = {x.x, x.y, x.z, x.w};
+  bool any = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if ((u[k] & EXPONENT) == EXPONENT) u[k] &= 0xffff0000u, any = true;
+    if ((u[k] >> 16 & EXPONENT) == EXPONENT) u[k] &= 0x0000ffffu, any = true;
+  }
+  if (any) *at = make_uint4(u[0], u[1], u[2], u[3]);
+  return any;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -132,9 +148,9 @@ __device__ __forceinline__ float factor(float a, float b) {
   return a == -INFINITY ? 0.0f : exp2_fast(a - b);
 }
 
-// Kernels for the 16-bit types at head sizes of up to 128: one query a sequence
-// (attention_decode.cu), and several (attention_prompt.cu).
-bool decode_fits(const Attention &a, int max_len);  // its blocks of keys count in 31 bits
+// Kernels for the 16-bit types at head sizes of up to 128: few rows a sequence
+// (attention_decode.cu), and many (attention_prompt.cu).
+bool decode_takes(const Attention &a, int max_len);
 int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream);
 int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                  cudaStream_t stream);

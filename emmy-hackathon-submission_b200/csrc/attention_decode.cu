@@ -1,10 +1,10 @@
-// Attention of one new token a sequence for the 16-bit types at head sizes of up to 128
-// (pg_attention without starts).
+// Attention of one new token a sequence, or a few, for the 16-bit types at head sizes of up to
+// 128 (pg_attention).
 //
 // HBM bounds it: every key and value is read once and used for the query heads of its group
 // only. So the work is cut evenly by keys, not by sequences: the blocks of 64 keys of all
-// (sequence, kv head) pairs form one line, and block c takes the c-th of as many equal pieces of
-// it as there are blocks. A pair whose keys lie in several pieces is joined by the last block that finishes one, in
+// (sequence, kv head) pairs form one line, each pair with a few more for what it costs by itself,
+// and block c takes the c-th of as many equal pieces of it as there are blocks. A pair whose keys lie in several pieces is joined by the last block that finishes one, in
 // the pieces' order.
 //
 // Within a block each of four warps takes every fourth 16 keys by itself: it copies their rows
@@ -14,6 +14,10 @@
 // each key the memory is slower by far). A weight goes into the second product as the sum of two
 // numbers of the values' type, the rounded weight and what the rounding left, so that the
 // result is rounded once; that doubles the second product, which the memory hides.
+//
+// Several queries' heads make more rows, 16 to a pair of their own, so each of their groups of 16
+// reads the keys again, from L2. What some row of a step must not see has weight 0 there; values
+// that are not finite are zeroed in such steps, and added again at the end for rows that see them.
 #include "attention.cuh"
 
 namespace {
@@ -26,6 +30,10 @@ constexpr int kStep = 16;             // keys a warp takes at a time
 constexpr int kKeys = kStep * kWarps; // keys of a block's step
 constexpr int kRows = 16;
 constexpr int kPerSm = 2;             // blocks an SM holds
+// What a pair costs by itself, in blocks of keys (64 sequences of up to 8000 keys: 160 us with 8,
+// 190 with 4, 220 with 0).
+constexpr int kPair = 8;
+constexpr float kCut = 2.0f;
 
 template <class T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
@@ -35,6 +43,9 @@ template <> struct Mma<__nv_bfloat16> {
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  static constexpr uint32_t exponent = 0x7f80;
+  __device__ static float low(uint32_t w) { return __uint_as_float(w << 16); }
+  __device__ static float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
   // two weights rounded, and the two that rounding left
   __device__ static void split(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
@@ -49,6 +60,13 @@ template <> struct Mma<__nv_bfloat16> {
   }
 };
 template <> struct Mma<__half> {
+  static constexpr uint32_t exponent = 0x7c00;
+  __device__ static float low(uint32_t w) {
+    return __low2float(*reinterpret_cast<const __half2 *>(&w));
+  }
+  __device__ static float high(uint32_t w) {
+    return __high2float(*reinterpret_cast<const __half2 *>(&w));
+  }
   __device__ static void run(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, "
                  "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -93,124 +111,332 @@ struct Ring {
   __device__ static int at(int r, int chunk) { return r * row + ((chunk ^ (r & 7)) << 4); }
 };
 
-__device__ __forceinline__ int length_of(const Attention &a, int b, int *slot) {
-  const int s = a.slots ? a.slots[b] : b;
-  *slot = s;
-  if (s < 0 || s >= a.slot_rows) {
-    atomicOr(a.status, PG_CACHE_BAD_SLOT);
-    return 0;
-  }
-  const int n = a.lens[s], most = a.width * a.page_size;
-  if (n < 0 || n > most) {
+// A sequence as the kernel takes it: `count` queries from row `query` on, the last of `length`
+// tokens, which makes `pairs` of a head and 16 rows.
+struct Sequence {
+  int slot, length, query, count, row_groups;
+  Blocks blocks;
+  uint32_t pairs;
+};
+
+template <bool MANY>
+__device__ __forceinline__ Sequence sequence_of(const Attention &a, int b) {
+  Sequence s;
+  s.slot = a.slots ? a.slots[b] : b;
+  s.query = MANY ? a.starts[b] : b;
+  s.count = MANY ? max(0, a.starts[b + 1] - s.query) : 1;
+  s.length = 0;
+  if (MANY && (s.query < 0 || s.count > a.queries - s.query)) {
     atomicOr(a.status, PG_CACHE_TOO_LONG);
-    return n < 0 ? 0 : most;
+    s.count = 0;
   }
-  return n;
+  if (s.slot < 0 || s.slot >= a.slot_rows) {
+    atomicOr(a.status, PG_CACHE_BAD_SLOT);
+  } else {
+    const int most = a.width * a.page_size;
+    s.length = a.lens[s.slot];
+    if (s.length < 0 || s.length > most) {
+      atomicOr(a.status, PG_CACHE_TOO_LONG);
+      s.length = s.length < 0 ? 0 : most;
+    }
+  }
+  s.row_groups = (s.count * a.group + kRows - 1) / kRows;
+  s.blocks = pg::blocks_of(a, s.length - s.count, s.length - 1, kKeys);
+  s.pairs = s.blocks.count ? a.heads * s.row_groups : 0;
+  return s;
 }
 
-__device__ __forceinline__ int blocks_in(const Attention &a, int length) {
-  return pg::blocks_of(a, length - 1, length - 1, kKeys).count;
-}
+// A pair of a kv head and 16 rows, as far as a block has a piece of it.
+struct Pair {
+  int query, row0, rows, head, lo, hi;  // lo..hi: the positions of the sequence's queries
+  int block0, block1;                   // of its blocks of keys
+  uint32_t first, c0, c1;               // its place on the line, the pieces that it lies in
+  Blocks blocks;
+  const int *pages;
+  unsigned last;
+  // whether all rows see all of a step's keys
+  __device__ bool all_see(const Attention &a, int key) const {
+    return key + kStep - 1 <= lo &&
+           (!a.window || key > hi - a.window || key + kStep <= a.sinks);
+  }
+};
 
-template <class T, int DIM>
-__global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(Attention a) {
+// What the warps of a block have of a pair, from their rings' places: joined, and written as the
+// result, or left for the block that finishes the pair last, which joins all. A function of its own
+// for the registers: what is needed here only would otherwise be held through the loop over the
+// keys, whose loads of operands then wait for one another (a tenth of the whole).
+template <class T, int DIM, bool MANY>
+__device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t per, int odd) {
   using R = Ring<DIM>;
   extern __shared__ float4 smem4[];
-  __shared__ uint32_t warp_sum[kWarps];
-  __shared__ int found_b;
-  __shared__ uint32_t found_before;
-  __shared__ unsigned last;
+  const Pair p = sh;
+  const int tid = threadIdx.x;
+  const auto query_of = [&](int r) { return MANY ? (p.row0 + r) / a.group : 0; };
+  const auto head_of = [&](int r) {
+    return p.head * a.group + (MANY ? (p.row0 + r) % a.group : p.row0 + r);
+  };
+  const bool alone = p.c0 == p.c1;
+  constexpr int kPartial = kRows * (DIM + 2);
+  // a block has at most two pairs that others share: one that its piece starts with, and one
+  // it leaves in the middle of
+  const auto slot_of = [&](uint32_t piece) {
+    return a.partial + (2ll * piece + (p.first > piece * per)) * kPartial;
+  };
+  const auto write = [&](int r, int col, float4 x, float sum) {
+    if (r >= p.rows || col >= a.dim) return;
+    // a query before the sequence's start sees no key: zeros
+    const float inv = 1.0f / sum;
+    const bool none = p.lo + query_of(r) < 0;
+    *reinterpret_cast<uint2 *>(a.out + (p.query + query_of(r)) * a.out_token +
+                               head_of(r) * a.out_head + col * 2) =
+        none ? make_uint2(0, 0)
+             : make_uint2(Mma<T>::pack(x.x * inv, x.y * inv), Mma<T>::pack(x.z * inv, x.w * inv));
+  };
+  // thread's columns: four of row `warp`, `warp + 4`, ...
+  constexpr int lanes = DIM / 4;
+  for (int i = tid; i < p.rows * lanes; i += kThreads) {
+    const int r = i / lanes, col = 4 * (i % lanes);
+    float top = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      top = fmaxf(top, reinterpret_cast<float *>(smem4)[w * (R::warp / 4) + kRows * DIM + r]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float *from = reinterpret_cast<float *>(smem4) + w * (R::warp / 4);
+      const float f = pg::factor(from[kRows * DIM + r], base);
+      const float4 x = *reinterpret_cast<const float4 *>(from + r * DIM + col);
+      sum += f * from[kRows * DIM + kRows + r];
+      acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y);
+      acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
+    }
+    if (MANY && odd && col < a.dim)
+      for (int i = 0; i < p.block1 - p.block0; ++i)
+        for (int j = 0; j < kKeys; ++j) {
+          const int key = p.blocks.key_block(p.block0 + i) * kKeys + j;
+          if (p.all_see(a, key / kStep * kStep) || !pg::sees(a, p.lo + query_of(r), key)) continue;
+          const int page = p.pages[key / a.page_size];
+          if (page < 0 || page >= a.pages) continue;
+          const uint2 w = *reinterpret_cast<const uint2 *>(
+              a.v + page * a.v_page + p.head * a.v_head +
+              static_cast<int64_t>(key % a.page_size) * a.dim * 2 + col * 2);
+          const float x[4] = {Mma<T>::low(w.x), Mma<T>::high(w.x), Mma<T>::low(w.y),
+                              Mma<T>::high(w.y)};
+          if (!(fabsf(x[0]) < INFINITY)) acc.x += x[0];
+          if (!(fabsf(x[1]) < INFINITY)) acc.y += x[1];
+          if (!(fabsf(x[2]) < INFINITY)) acc.z += x[2];
+          if (!(fabsf(x[3]) < INFINITY)) acc.w += x[3];
+        }
+    if (alone) {
+      write(r, col, acc, sum);
+    } else {
+      float *to = slot_of(blockIdx.x);
+      *reinterpret_cast<float4 *>(to + r * DIM + col) = acc;
+      if (col == 0) {
+        to[kRows * DIM + r] = top;
+        to[kRows * DIM + kRows + r] = sum;
+      }
+    }
+  }
+  if (!alone) {
+    __threadfence();
+    __syncthreads();
+    // the counter of the piece that the pair starts in: no other pair's
+    if (tid == 0) sh.last = atomicInc(a.arrived + p.c0, p.c1 - p.c0) == p.c1 - p.c0;
+    __syncthreads();
+    if (sh.last) {
+      __threadfence();
+      // as many pieces as the rings have room for at a time, all their loads in flight together
+      constexpr int kBatch = R::bytes / (kPartial * 4), kPieces16 = kPartial / 4;
+      constexpr int kEach = kThreads / lanes, kMine = kRows / kEach;
+      const int col = 4 * (tid % lanes), first_r = tid / lanes;
+      const int used = p.rows * lanes;  // 16-byte pieces of the rows there are
+      float *const stage = reinterpret_cast<float *>(smem4);
+      const uint32_t stage_at = static_cast<uint32_t>(__cvta_generic_to_shared(stage));
+      float top[kMine], sum[kMine];
+      float4 acc[kMine];
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        top[k] = -INFINITY, sum[k] = 0.0f;
+        acc[k] = make_float4(0, 0, 0, 0);
+      }
+      for (uint32_t at = p.c0; at <= p.c1; at += kBatch) {
+        const int here = min(static_cast<uint32_t>(kBatch), p.c1 - at + 1);
+        __syncthreads();
+        for (int i = 0; i < here; ++i) {
+          const float *from = slot_of(at + i);
+          for (int j = tid; j < used + kRows / 2; j += kThreads) {
+            const int piece = j < used ? j : j - used + kRows * lanes;  // rows, then m and l
+            copy16(stage_at + (i * kPieces16 + piece) * 16, from + 4 * piece, true);
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        for (int i = 0; i < here; ++i) {
+          const float *from = stage + i * kPartial;
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) {
+            const int r = first_r + k * kEach;
+            if (r >= p.rows) continue;
+            const float m_here = from[kRows * DIM + r], most = fmaxf(top[k], m_here);
+            const float base = most == -INFINITY ? 0.0f : most;
+            const float f = pg::factor(m_here, base), old = pg::factor(top[k], base);
+            const float4 x = *reinterpret_cast<const float4 *>(from + r * DIM + col);
+            top[k] = most;
+            sum[k] = fmaf(f, from[kRows * DIM + kRows + r], old * sum[k]);
+            acc[k].x = fmaf(f, x.x, old * acc[k].x), acc[k].y = fmaf(f, x.y, old * acc[k].y);
+            acc[k].z = fmaf(f, x.z, old * acc[k].z), acc[k].w = fmaf(f, x.w, old * acc[k].w);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) write(first_r + k * kEach, col, acc[k], sum[k]);
+    }
+  }
+}
+
+// A block's piece of the line: up to which place it goes and how long a piece is; and the pair it is
+// at: its sequence, and the sequence's place on the line.
+struct Plan {
+  uint32_t end, per, before;
+  int sequence, turn;
+};
+
+// MANY: sequences have any number of queries, not one each.
+template <class T, int DIM, bool MANY>
+__global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_constant__ Attention a) {
+  using R = Ring<DIM>;
+  extern __shared__ float4 smem4[];
+  __shared__ uint3 warp_sum[kWarps];
+  __shared__ Pair sh;
+  __shared__ Plan plan_here;
+  // read each time: held in registers, it would crowd the loop over the keys
+  volatile Plan &plan = plan_here;
+  __shared__ int odds[2];  // whether a value that is not finite was zeroed, by turns of pairs
   pg::wait_for_earlier_kernels();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const uint32_t row_groups = (a.group + kRows - 1) / kRows, per_block = a.heads * row_groups;
   const uint32_t c = blockIdx.x;
+  if (tid < 2) odds[tid] = 0;
 
-  // Every block works the line out for itself: thread i counts the units (blocks of keys of a
-  // head and row group) of a run of sequences.
+  // Every block works the line out for itself: thread i counts the pairs and their blocks of keys
+  // of a run of sequences.
   const int run = (a.batch + kThreads - 1) / kThreads;
   const int first_b = min(tid * run, a.batch), end_b = min(first_b + run, a.batch);
-  uint32_t mine = 0;
+  uint32_t pairs = 0, keys = 0, longest = 0;
   for (int b = first_b; b < end_b; ++b) {
-    int slot;
-    const int n = length_of(a, b, &slot);
-    mine += blocks_in(a, n);
-    if (!n && b % gridDim.x == c)  // no key: zeros
-      for (int h = 0; h < a.heads * a.group; ++h)
+    const Sequence s = sequence_of<MANY>(a, b);
+    pairs += s.pairs;
+    keys += s.pairs * s.blocks.count;
+    longest = max(longest, static_cast<uint32_t>(s.blocks.count));
+    if (!s.length && b % gridDim.x == c)  // no key: zeros
+      for (int i = 0; i < s.count * a.heads * a.group; ++i)
         for (int j = 0; j < a.dim / 8; ++j)
-          *reinterpret_cast<uint4 *>(a.out + b * a.out_token + h * a.out_head + j * 16) =
+          *reinterpret_cast<uint4 *>(a.out + (s.query + i / (a.heads * a.group)) * a.out_token +
+                                     i % (a.heads * a.group) * a.out_head + j * 16) =
               make_uint4(0, 0, 0, 0);
   }
-  mine *= per_block;
-  uint32_t upto = mine;
+  uint32_t pairs_upto = pairs, keys_upto = keys;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const uint32_t o = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += o;
+    const uint32_t o = __shfl_up_sync(0xffffffffu, pairs_upto, off);
+    const uint32_t k = __shfl_up_sync(0xffffffffu, keys_upto, off);
+    if (lane >= off) pairs_upto += o, keys_upto += k;
   }
-  if (lane == 31) warp_sum[warp] = upto;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) warp_sum[warp] = make_uint3(pairs_upto, keys_upto, longest);
   __syncthreads();
-  uint32_t total = 0;
+  uint32_t all_pairs = 0, all_keys = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += warp_sum[w];
-    total += warp_sum[w];
+    const uint3 s = warp_sum[w];
+    if (w < warp) pairs_upto += s.x, keys_upto += s.y;
+    all_pairs += s.x;
+    all_keys += s.y;
+    longest = max(longest, s.z);
   }
-  // The units of a piece; piece c is [c per, (c + 1) per). One is not too few: four sequences of
-  // up to 777 keys take 12 us, with at least two 16.5, with four 19.5.
-  const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
+  if (!all_keys) return;
+  const uint32_t total = all_keys + kPair * all_pairs;
+  // The length of a piece; piece c is [c per, (c + 1) per). As few as give every block one, but the
+  // last block to finish a pair reads all its pieces, so the longest is not cut in more than about
+  // kCut times the root of its blocks: one sequence of 60000 keys on one kv head takes 45 us so,
+  // 53 with twice as many pieces at most and 55 with half as many.
+  const uint32_t least = static_cast<uint32_t>(sqrtf(static_cast<float>(longest)) / kCut);
+  const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, least);
   if (static_cast<uint64_t>(c) * per >= total) return;
   uint32_t u = c * per;
-  const uint32_t u_end = min(total, u + per), before = upto - mine;
+  const uint32_t upto = keys_upto + kPair * pairs_upto;
+  const uint32_t before = upto - keys - kPair * pairs;
   if (u >= before && u < upto) {
     uint32_t at = before;
     for (int b = first_b; b < end_b; ++b) {
-      int slot;
-      const uint32_t units = blocks_in(a, length_of(a, b, &slot)) * per_block;
-      if (u < at + units) {
-        found_b = b;
-        found_before = at;
+      const Sequence s = sequence_of<MANY>(a, b);
+      const uint32_t next = at + s.pairs * (s.blocks.count + kPair);
+      if (u < next) {
+        plan.sequence = b;
+        plan.before = at;
+        plan.end = min(total, u + per);
+        plan.per = per;
+        plan.turn = 0;
         break;
       }
-      at += units;
+      at = next;
     }
   }
   __syncthreads();
-  int b = found_b;
-  uint32_t seq_before = found_before;
 
   char *ring = reinterpret_cast<char *>(smem4) + warp * R::warp;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
 
-  while (u < u_end) {
-    int slot;
-    const int length = length_of(a, b, &slot);
-    const Blocks blocks = pg::blocks_of(a, length - 1, length - 1, kKeys);
-    if (!blocks.count) {
-      ++b;
-      continue;
+  while (u < plan.end) {
+    int b = plan.sequence;
+    Sequence seq = sequence_of<MANY>(a, b);
+    while (!seq.pairs) seq = sequence_of<MANY>(a, ++b);
+    const Blocks &blocks = seq.blocks;
+    const uint32_t before = plan.before, per = plan.per;
+    const uint32_t units = blocks.count + kPair, pair = (u - before) / units;
+    const int head = pair / seq.row_groups, row0 = (pair % seq.row_groups) * kRows;
+    const int rows = min(kRows, seq.count * a.group - row0);
+    const uint32_t pair_first = before + pair * units;
+    const uint32_t stop = min(plan.end, pair_first + units);
+    const int block0 = max(0, static_cast<int>(u - pair_first) - kPair);
+    const int block1 = static_cast<int>(stop - pair_first) - kPair;
+    if (block1 <= 0) break;  // the piece ends before the pair's first block
+    __syncthreads();
+    if (tid == 0) {
+      const bool ends = stop == before + seq.pairs * units;  // the sequence's last pair
+      plan.sequence = b + ends;
+      if (ends) plan.before = stop;
     }
-    const uint32_t pair = (u - seq_before) / blocks.count;
-    const int head = pair / row_groups, row0 = (pair % row_groups) * kRows;
-    const int rows = min(kRows, a.group - row0);
-    const uint32_t pair_first = seq_before + pair * blocks.count;
-    const int block0 = u - pair_first;
-    const uint32_t stop = min(u_end, pair_first + blocks.count);
-    const int block1 = stop - pair_first;
-    const int *pages = a.table + slot * a.table_row;
-    const int pos = length - 1;
+    u = stop;
+    const int *pages = a.table + seq.slot * a.table_row;
+    // the positions of the queries: of all, and of this thread's rows g and g + 8
+    const int lo = seq.length - seq.count, hi = seq.length - 1;
+    if (tid == 0)
+      sh = Pair{seq.query, row0, rows, head, lo, hi, block0, block1, pair_first,
+                (pair_first + kPair) / per, (pair_first + units - 1) / per, blocks, pages, 0};
+    const auto query_of = [&](int r) { return MANY ? (row0 + r) / a.group : 0; };
+    const auto head_of = [&](int r) {
+      return head * a.group + (MANY ? (row0 + r) % a.group : row0 + r);
+    };
+    const int pos[2] = {lo + query_of(g), lo + query_of(g + 8)};
+    int *const odd = odds + plan.turn;
 
     // the queries' fragments: rows g and g + 8, columns 2 t and 2 t + 8 of each 16
     uint32_t q[DIM / 16][4];
 #pragma unroll
-    for (int k = 0; k < DIM / 16; ++k)
+    for (int h = 0; h < 2; ++h) {
+      const int r = g + 8 * h;
+      const char *from =
+          a.q + (seq.query + query_of(r)) * a.q_token + head_of(r) * a.q_head + 4 * t4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = g + 8 * (i & 1), col = 16 * k + 2 * t4 + 8 * (i >> 1);
-        q[k][i] = r < rows && col < a.dim
-                      ? *reinterpret_cast<const uint32_t *>(
-                            a.q + b * a.q_token + (head * a.group + row0 + r) * a.q_head + col * 2)
-                      : 0u;
-      }
+      for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          q[k][h + 2 * i] = r < rows && 16 * k + 8 * i < a.dim
+                                ? *reinterpret_cast<const uint32_t *>(from + 32 * k + 16 * i)
+                                : 0u;
+    }
     float o[DIM / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < DIM / 8; ++n)
@@ -226,14 +452,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(Attention a) {
       return blocks.key_block(block0 + i) * kKeys + kStep * warp;
     };
     const auto all_seen = [&](int key) {
-      return key + kStep - 1 <= pos &&
-             (!a.window || key > pos - a.window || key + kStep <= a.sinks);
+      return key + kStep - 1 <= lo &&
+             (!a.window || key > hi - a.window || key + kStep <= a.sinks);
+    };
+    const auto some_see = [&](int key) {
+      return key <= hi && (!a.window || key > lo - a.window || key < a.sinks);
     };
     const auto page_for = [&](int i) {  // as the table names it; -1: not seen
       if (i >= steps) return -1;
       const int key = first_key(i);
       if (whole_pages && all_seen(key)) return pages[key / a.page_size];
-      return pg::sees(a, pos, key + (lane & 15)) ? pages[(key + (lane & 15)) / a.page_size] : -1;
+      return some_see(key + (lane & 15)) ? pages[(key + (lane & 15)) / a.page_size] : -1;
     };
     const int sub = lane / R::chunks, chunk = lane % R::chunks;
     const bool column = chunk * 8 < a.dim;
@@ -263,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(Attention a) {
           }
         } else {
           const int mine_key = key + (lane & 15);
-          if (pg::sees(a, pos, mine_key) && (page < 0 || page >= a.pages)) {
+          if (some_see(mine_key) && (page < 0 || page >= a.pages)) {
             atomicOr(a.status, PG_CACHE_BAD_PAGE);
             page = -1;
           }
@@ -282,16 +511,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(Attention a) {
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int next = page_for(0);
+    // pages are asked for two steps before their rows are
+    int next = page_for(0), after = page_for(1);
 #pragma unroll
     for (int i = 0; i < R::stages - 1; ++i) {
       const int page = next;
-      next = page_for(i + 1);
+      next = after;
+      after = page_for(i + 2);
       issue(i, page);
     }
     for (int i = 0; i < steps; ++i) {
       const int page = next;
-      next = page_for(i + R::stages);
+      next = after;
+      after = page_for(i + R::stages + 1);
       issue(i + R::stages - 1, page);
       asm volatile("cp.async.wait_group %0;" ::"n"(R::stages - 1) : "memory");
       __syncwarp();
@@ -308,13 +540,22 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(Attention a) {
         }
       const int key = first_key(i);
       const bool masked = !all_seen(key);
+      if (MANY && masked) {
+        bool any = false;
+        for (int j = lane; j < kStep * R::chunks; j += 32)
+          any |= pg::clean<Mma<T>::exponent>(reinterpret_cast<uint4 *>(
+              ring + (i % R::stages) * R::stage + R::tile + j * 16));
+        if (any) *const_cast<volatile int *>(odd) = 1;
+        __syncwarp();
+      }
       float top[2] = {m[0], m[1]};
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[n][e] *= a.scale_log2;
-          if (masked && !pg::sees(a, pos, key + 2 * t4 + 8 * n + (e & 1))) s[n][e] = -INFINITY;
+          if (masked && !pg::sees(a, pos[e >> 1], key + 2 * t4 + 8 * n + (e & 1)))
+            s[n][e] = -INFINITY;
           top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
         }
 #pragma unroll
@@ -381,105 +622,39 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(Attention a) {
     }
     __syncthreads();
 
-    const uint32_t c0 = pair_first / per, c1 = (pair_first + blocks.count - 1) / per;
-    const bool alone = c0 == c1;
-    constexpr int kPartial = kRows * (DIM + 2);
-    // a block has at most two pairs that others share: one that its piece starts with, and one
-    // it leaves in the middle of
-    const auto slot_of = [&](uint32_t piece) {
-      return a.partial + (2ll * piece + (pair_first > piece * per)) * kPartial;
-    };
-    // thread's columns: four of row `warp`, `warp + 4`, ...
-    const int lanes = DIM / 4;
-    for (int i = tid; i < kRows * lanes; i += kThreads) {
-      const int r = i / lanes, col = 4 * (i % lanes);
-      float top = -INFINITY, sum = 0.0f;
-      float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        top = fmaxf(top, reinterpret_cast<float *>(smem4)[w * (R::warp / 4) + kRows * DIM + r]);
-      const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float *from = reinterpret_cast<float *>(smem4) + w * (R::warp / 4);
-        const float f = pg::factor(from[kRows * DIM + r], base);
-        const float4 x = *reinterpret_cast<const float4 *>(from + r * DIM + col);
-        sum += f * from[kRows * DIM + kRows + r];
-        acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y);
-        acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
-      }
-      if (alone) {
-        if (r < rows && col < a.dim) {
-          const float inv = 1.0f / sum;
-          *reinterpret_cast<uint2 *>(a.out + b * a.out_token +
-                                     (head * a.group + row0 + r) * a.out_head + col * 2) =
-              make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv),
-                         Mma<T>::pack(acc.z * inv, acc.w * inv));
-        }
-      } else {
-        float *to = slot_of(c);
-        *reinterpret_cast<float4 *>(to + r * DIM + col) = acc;
-        if (col == 0) {
-          to[kRows * DIM + r] = top;
-          to[kRows * DIM + kRows + r] = sum;
-        }
-      }
-    }
-    if (!alone) {
-      __threadfence();
-      __syncthreads();
-      // the counter of the piece that the pair starts in: no other pair's
-      if (tid == 0) last = atomicInc(a.arrived + c0, c1 - c0) == c1 - c0;
-      __syncthreads();
-      if (last) {
-        __threadfence();
-        for (int i = tid; i < rows * lanes; i += kThreads) {
-          const int r = i / lanes, col = 4 * (i % lanes);
-          float top = -INFINITY, sum = 0.0f;
-          float4 acc = make_float4(0, 0, 0, 0);
-          for (uint32_t p = c0; p <= c1; ++p) top = fmaxf(top, __ldcg(slot_of(p) + kRows * DIM + r));
-          const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-          for (uint32_t p = c0; p <= c1; ++p) {
-            const float *from = slot_of(p);
-            const float f = pg::factor(__ldcg(from + kRows * DIM + r), base);
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + r * DIM + col));
-            sum += f * __ldcg(from + kRows * DIM + kRows + r);
-            acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y);
-            acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
-          }
-          if (col < a.dim) {
-            const float inv = 1.0f / sum;
-            *reinterpret_cast<uint2 *>(a.out + b * a.out_token +
-                                       (head * a.group + row0 + r) * a.out_head + col * 2) =
-                make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv),
-                           Mma<T>::pack(acc.z * inv, acc.w * inv));
-          }
-        }
-      }
-    }
+    finish_pair<T, DIM, MANY>(a, sh, plan.per, odds[plan.turn]);
     __syncthreads();  // the rings are free again
-    u = stop;
-    if (u == seq_before + blocks.count * per_block) {
-      seq_before = u;
-      ++b;
+    if (tid == 0) {
+      odds[plan.turn] = 0;  // for the turn after the next
+      plan.turn = plan.turn ^ 1;
     }
+    __syncthreads();
   }
 }
 
 template <class T, int DIM>
 int launch_decode(const Attention &a, int sms, cudaStream_t stream) {
-  return pg::launch<decode_kernel<T, DIM>>("decode_kernel", dim3(kPerSm * sms), kThreads,
-                                           Ring<DIM>::bytes, stream, a);
+  const dim3 grid(kPerSm * sms);
+  if (a.starts)
+    return pg::launch<decode_kernel<T, DIM, true>>("decode_kernel", grid, kThreads,
+                                                   Ring<DIM>::bytes, stream, a);
+  return pg::launch<decode_kernel<T, DIM, false>>("decode_kernel", grid, kThreads,
+                                                  Ring<DIM>::bytes, stream, a);
 }
 
 }  // namespace
 
 namespace pg {
 
-bool decode_fits(const Attention &a, int max_len) {
-  const int64_t pairs = static_cast<int64_t>(a.batch) * a.heads * ((a.group + kRows - 1) / kRows);
-  return pairs * (max_len / kKeys + 2ll) < INT32_MAX;
+// Whether this kernel takes a batch and not the large tiles of attention_prompt.cu: at up to 32
+// rows a sequence on average, which these fill badly. Seven sequences of up to 20000 keys on 4 kv
+// heads: 16 rows 57 us against 84, 32 rows 65 against 84, 48 rows 89 against 93, 64 rows 108
+// against 93; 32 sequences of up to 8000 on 8 kv heads, 48 rows: 264 against 159.
+bool decode_takes(const Attention &a, int max_len) {
+  const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
+  if (a.starts && rows > 32ll * a.batch) return false;
+  // its blocks of keys count in 31 bits
+  return (rows / kRows + a.batch) * a.heads * (max_len / kKeys + 2ll + kPair) < INT32_MAX;
 }
 
 int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream) {

@@ -274,22 +274,6 @@ struct Head {  // what the roles share
   unsigned last;
 };
 
-// Zeroes the numbers of 16 bytes of values that are not finite; whether there were any.
-template <class T>
-__device__ __forceinline__ bool clean(uint4 *at) {
-  const uint4 x = *at;
-  uint32_t u[4] = {x.x, x.y, x.z, x.w};
-  constexpr uint32_t e = Type<T>::exponent;
-  bool any = false;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if ((u[k] & e) == e) u[k] &= 0xffff0000u, any = true;
-    if ((u[k] >> 16 & e) == e) u[k] &= 0x0000ffffu, any = true;
-  }
-  if (any) *at = make_uint4(u[0], u[1], u[2], u[3]);
-  return any;
-}
-
 // Without TMA the maps and `boxes` are empty.
 template <class T, int DIM, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -426,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!both.all(key0)) {
             bool odd = false;
             for (int i = w; i < kKeys / kPer; i += kCopyWarps) {  // the pieces it has copied
-              odd |= clean<T>(reinterpret_cast<uint4 *>(smem + P::ring + s * P::tile +
+              odd |= pg::clean<Type<T>::exponent>(reinterpret_cast<uint4 *>(smem + P::ring + s * P::tile +
                                                         P::at(i * kPer + sub, piece)));
             }
             if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
@@ -591,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int piece = 0; piece < DIM / 8; ++piece) {
             uint4 *at16 = reinterpret_cast<uint4 *>(values + P::at(r, piece));
             if (key0 + r >= t.length) *at16 = make_uint4(0, 0, 0, 0);
-            else odd |= clean<T>(at16);
+            else odd |= pg::clean<Type<T>::exponent>(at16);
           }
           if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
           fence_async();

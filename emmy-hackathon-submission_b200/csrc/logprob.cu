@@ -527,7 +527,8 @@ int run_grad(uint64_t logits, int64_t row_stride, uint64_t tokens, int token_byt
   constexpr int span = Vec<T>::n * kThreads * kBatch;
   // a row may start in the middle of its first vector
   const int per_row = (vocab + Vec<T>::n - 2) / span + 1;
-  return pg::launch<logprobs_grad_kernel<T>>("logprobs_grad_kernel", dim3(static_cast<unsigned>(rows) * per_row), kThreads, 0, stream,
+  return pg::launch<logprobs_grad_kernel<T>>(
+      "logprobs_grad_kernel", dim3(static_cast<unsigned>(rows) * per_row), kThreads, 0, stream,
                     reinterpret_cast<const T *>(logits), row_stride,
                     reinterpret_cast<const void *>(tokens), token_bytes, rows, vocab,
                     reinterpret_cast<const float2 *>(norm), reinterpret_cast<const float *>(entropy),

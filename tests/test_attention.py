@@ -166,6 +166,27 @@ def test_prompt_ragged(ws, heads, group, dim, page, dtype) -> None:
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,dim,page", HEADS)
+def test_prompt_few_tokens(ws, heads, group, dim, page, dtype) -> None:
+    """A few drafted tokens a sequence, none of some, more than there are of others."""
+    lens = [1, 40, 0, 130, 300, 301, 2, 129, 64, 1000]
+    news = [1, 4, 2, 3, 0, 5, 4, 1, 2, 6]
+    b = Batch(lens, news, heads, group, dim, page, dtype, fused=True)
+    b.check(b.run(ws), b.definition())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (2, 1), (16, 0), (100, 4), (64, 70), (257, 5),
+                                          (5000, 3)])
+def test_prompt_few_tokens_window_and_sinks(ws, window, sinks, dtype) -> None:
+    lens, news = [700, 3, 1400, 91, 5000], [5, 3, 1, 4, 7]
+    b = Batch(lens, news, 2, 3, 64, 16, dtype, seed=window)
+    b.check(b.run(ws, window=window, sinks=sinks), b.definition(window, sinks))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 0), (100, 4), (128, 130), (257, 5),
                                           (5000, 3)])
 def test_prompt_window_and_sinks(ws, window, sinks, dtype) -> None:
@@ -218,6 +239,32 @@ def test_what_lies_in_masked_places_does_not_matter(ws, junk, dim, dtype) -> Non
     got = b.run(ws, window=window, sinks=2)
     assert torch.equal(torch.isnan(got).any(-1).any(-1)[:200], hit)
     assert not torch.isnan(got[200:]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 5)])
+def test_masked_places_of_a_few_tokens(ws, dim, page, dtype) -> None:
+    """Drafted tokens of which the first must not see the last one's key and value, nor the last
+    what has left its window."""
+    import torch
+
+    lens, news, window = [90, 333, 64], [4, 3, 4], 20
+    b = Batch(lens, news, 2, 2, dim, page, dtype, junk=float("nan"))
+    clean = b.run(ws, window=window, sinks=1)
+    b.check(clean, b.definition(window, 1))
+    # a key that token 0 of sequence 0 sees and its later ones have left; one that only the last
+    # of sequence 1 sees; and sequence 2's whole last token
+    for s, place in ((0, 67), (1, 332), (2, 63)):
+        at, row = int(b.table[s, place // page]), place % page
+        b.v[at, :, row, 7] = float("inf")
+        b.values[s][:, place, 7] = float("inf")
+    got, want = b.run(ws, window=window, sinks=1), b.definition(window, 1)
+    hit = torch.zeros(got.shape, dtype=torch.bool, device="cuda")
+    hit[[0, 6, 10], :, 7] = True
+    assert torch.equal(torch.isfinite(want), ~hit)
+    assert torch.equal(torch.isfinite(got), ~hit) and (got[hit] == float("inf")).all()
+    assert torch.equal(got[~hit], clean[~hit])
 
 
 @pytest.mark.gpu
