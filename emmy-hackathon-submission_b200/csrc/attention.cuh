@@ -14,6 +14,8 @@
 
 #include "common.cuh"
 
+#include <cmath>
+
 namespace pg {
 
 struct Attention {
@@ -180,6 +182,9 @@ inline int choose_parts(const Attention &a, int tiles, int rows_per_tile, int co
   int64_t parts = blocks / pairs;
   const int64_t steps = (seen + 4ll * keys - 1) / (4ll * keys);
   parts = steps < parts ? steps : parts;
+  // the last part to finish reads all: no more than about twice the root of the steps
+  const int64_t most = 2 * static_cast<int64_t>(std::sqrt(static_cast<double>(seen / keys + 1)));
+  parts = most < parts ? most : parts;
   const int64_t each = pairs * rows_per_tile * (columns + 2) * 4ll;
   parts = partial_bytes / each < parts ? partial_bytes / each : parts;
   return static_cast<int>(parts < 1 ? 1 : parts);

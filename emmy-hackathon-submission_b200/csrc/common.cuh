@@ -103,6 +103,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // Two 32-bit numbers that one instruction multiplies and adds.
 struct Two {
   uint64_t v;
+  Two() = default;
   __device__ Two(uint64_t x) : v(x) {}
   __device__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
   __device__ void get(float &x, float &y) const {
