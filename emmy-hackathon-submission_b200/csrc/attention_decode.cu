@@ -4,8 +4,9 @@
 // HBM bounds it: every key and value is read once and used for the query heads of its group
 // only. So the work is cut evenly by keys, not by sequences: the blocks of 64 keys of all
 // (sequence, kv head) pairs form one line, each pair with a few more for what it costs by itself,
-// and block c takes the c-th of as many equal pieces of it as there are blocks. A pair whose keys lie in several pieces is joined by the last block that finishes one, in
-// the pieces' order.
+// and block c takes the c-th of as many equal pieces of it as there are blocks. A pair whose keys
+// lie in several pieces is joined by the last block that finishes one, in the pieces' order. 48
+// sequences of up to 32768 keys, 64 heads on 8 of 128 in bf16, take 355 us (6.0 TB/s).
 //
 // Within a block each of four warps takes every fourth 16 keys by itself: it copies their rows
 // into its own ring in shared memory (cp.async, 16 bytes a lane, rows of whole heads, swizzled so
@@ -30,8 +31,8 @@ constexpr int kStep = 16;             // keys a warp takes at a time
 constexpr int kKeys = kStep * kWarps; // keys of a block's step
 constexpr int kRows = 16;
 constexpr int kPerSm = 2;             // blocks an SM holds
-// What a pair costs by itself, in blocks of keys (64 sequences of up to 8000 keys: 160 us with 8,
-// 190 with 4, 220 with 0).
+// What a pair costs by itself, in blocks of keys (64 sequences of up to 8000 keys on 8 kv heads:
+// 126 us with 8 or 4, 159 with 0).
 constexpr int kPair = 8;
 constexpr float kCut = 2.0f;
 
@@ -646,13 +647,15 @@ int launch_decode(const Attention &a, int sms, cudaStream_t stream) {
 
 namespace pg {
 
-// Whether this kernel takes a batch and not the large tiles of attention_prompt.cu: at up to 32
-// rows a sequence on average, which these fill badly. Seven sequences of up to 20000 keys on 4 kv
-// heads: 16 rows 57 us against 84, 32 rows 65 against 84, 48 rows 89 against 93, 64 rows 108
-// against 93; 32 sequences of up to 8000 on 8 kv heads, 48 rows: 264 against 159.
+// Whether this kernel takes a batch and not the large tiles of attention_prompt.cu: at up to 48
+// rows a sequence on average, which those fill badly. By rows a sequence, this against those, in
+// microseconds at head size 128: 7 sequences of up to 20000 keys on 4 kv heads, 16 rows 43 and 83,
+// 32 rows 56 and 84, 48 rows 60 and 84, 64 rows 70 and 96; 32 of up to 8000 on 8, 16 rows 74 and
+// 157, 32 rows 119 and 158, 48 rows 155 and 160, 64 rows 191 and 160; 100 of up to 500 on 4, 48
+// rows 51 and 49, 64 rows 63 and 50.
 bool decode_takes(const Attention &a, int max_len) {
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
-  if (a.starts && rows > 32ll * a.batch) return false;
+  if (a.starts && rows > 48ll * a.batch) return false;
   // its blocks of keys count in 31 bits
   return (rows / kRows + a.batch) * a.heads * (max_len / kKeys + 2ll + kPair) < INT32_MAX;
 }

@@ -13,15 +13,17 @@
 //                   they mix, and both tiles then wait for both
 //   warps 9, 10     bring keys and values, page by page, into a ring in shared memory
 //
-// Where pages are whole groups of eight keys, two warps bring them with TMA (a box is the run of
-// keys that a page and a block of 128 always share, 128-byte swizzled as the products read it).
-// Pages of other sizes come in 16-byte pieces through cp.async, whose arithmetic then
-// bounds the kernel: 4096 new tokens of up to 8192 with 32 heads take 1370 us that way, 579 with TMA.
+// Where pages are whole groups of eight keys, two warps bring them with TMA, a box eight keys by
+// 64 columns, 128-byte swizzled as the products read it. Pages of other sizes come in 16-byte
+// pieces through cp.async, whose arithmetic then bounds the kernel: two sequences of 4096 new
+// tokens and up to 8192 keys, 32 heads on 8 of 128 in bf16, take 1814 us that way, 498 with TMA
+// (885 TFLOP/s of the products that count).
 //
-// Exponentials bound it beside the products: 128 x 128 of them take the 16 lanes an SM has
-// for them 1024 cycles, the two products of DIM = 128 the same. O is rescaled only when a row's
-// running maximum has grown by more than 2^8 since the last time, so that a weight is at most
-// 2^8 and rescaling is rare; the sum l goes by the same maximum, so the result is the same.
+// The rows' threads bound it beside the products: 128 x 128 exponentials take the 16 lanes an SM
+// has for them 1024 cycles, the two products of DIM = 128 the same, and where a tile's weights
+// wait for its scores neither is at work. O is rescaled only when a row's running maximum has
+// grown by more than 2^8 since the last time, so that a weight is at most 2^8 and rescaling is
+// rare; the sum l goes by the same maximum, so the result is the same.
 //
 // Rounding: weights go into the second product in the values' type (2^-9 or 2^-12 of each, at
 // random), as the tensor cores take both operands in one type; S, m, l and O are in 32 bits.
@@ -95,13 +97,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap *map,
                "r"(w), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ void tma_load_5d(uint32_t to, const CUtensorMap *map, int z, int w,
-                                            uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-               "[%0], [%1, {%2, %2, %2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(0), "r"(z),
-               "r"(w), "r"(bar)
-               : "memory");
-}
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile("{\n.reg .pred p;\n"
@@ -116,7 +111,8 @@ __device__ __forceinline__ unsigned long long now_ns() {
   return t;
 }
 // Waits for a phase of a barrier; false once a wait of this block has run out of time.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed, unsigned *status) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *failed,
+                                         unsigned *status) {
   if (bar_try(bar, parity)) return true;
   const unsigned long long begin = now_ns();
   while (!bar_try(bar, parity)) {
@@ -260,14 +256,6 @@ struct Seen {
   }
 };
 
-// How the tensor maps name a page's rows of a kv head: by five coordinates with heads and pages
-// in one (`per_page` of it a page), so that one box is eight rows by all columns by the rest of
-// the run, or (per_page 0) by four, a box eight rows of 64 columns.
-struct Boxes {
-  int keys;  // the keys that a page and a block always share
-  int k_per_page, v_per_page;
-};
-
 struct Head {  // what the roles share
   uint32_t tmem;
   int failed, odd;
@@ -278,7 +266,7 @@ struct Head {  // what the roles share
 template <class T, int DIM, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(Attention a, const __grid_constant__ CUtensorMap k_map,
-                  const __grid_constant__ CUtensorMap v_map, Boxes boxes) {
+                  const __grid_constant__ CUtensorMap v_map, int run) {
   using P = Plan<DIM>;
   extern __shared__ char smem_raw[];
   __shared__ Head sh;
@@ -339,10 +327,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (TMA && (warp == 9 || warp == 10)) {
       // --- copies: one warp the keys of each block, one the values; lane i the i-th page run ----
-      const int half = warp - 9, runs = kKeys / boxes.keys;
+      const int half = warp - 9, runs = kKeys / run;
       const CUtensorMap *map = half ? &v_map : &k_map;
-      const int per_page = half ? boxes.v_per_page : boxes.k_per_page;
-      const auto key_of = [&](int j) { return blocks.key_block(b0 + j) * kKeys + lane * boxes.keys; };
+      const auto key_of = [&](int j) { return blocks.key_block(b0 + j) * kKeys + lane * run; };
       const auto page_for = [&](int j) {  // -1: the run lies past the length
         if (j >= steps || lane >= runs || key_of(j) >= t.length) return -1;
         return t.pages[key_of(j) / a.page_size];
@@ -362,20 +349,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n >= P::stages) ok = bar_wait(empty(s), (n / P::stages - 1) & 1, failed, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) bar_expect(full(s), held * boxes.keys * 128 * P::chunks);
+        if (lane == 0) bar_expect(full(s), held * run * 128 * P::chunks);
         __syncwarp();
         if (real) {
-          const uint32_t to = smem_at + P::ring + s * P::tile + lane * (boxes.keys / 8) * P::group;
-          if (per_page) {
-            // an index past the map's last head and page too where the page is not one
-            tma_load_5d(to, map, row / 8, page * per_page + head, full(s));
-          } else {
-            for (int g = 0; g < boxes.keys / 8; ++g)
+          const uint32_t to = smem_at + P::ring + s * P::tile + lane * (run / 8) * P::group;
+          // a box is eight rows of 64 columns
+          for (int g = 0; g < run / 8; ++g)
 #pragma unroll
-              for (int k = 0; k < P::chunks; ++k)
-                tma_load_4d(to + g * P::group + k * P::atom, map, 64 * k, row + 8 * g, head, page,
-                            full(s));
-          }
+            for (int k = 0; k < P::chunks; ++k)
+              tma_load_4d(to + g * P::group + k * P::atom, map, 64 * k, row + 8 * g, head, page,
+                          full(s));
         }
       }
       // no copy is in flight when the block's shared memory goes
@@ -766,29 +749,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The tensor map of the keys or values (see Boxes). One box a run of keys, where head size and
-// strides allow, takes half the copies: 4096 new tokens of up to 8192 @FOLD@
-int encode(CUtensorMap *map, int *per_page, const Attention &a, const char *base, int64_t head,
-           int64_t page, int dim, int keys) {
-  const uint64_t row = 2ull * a.dim, at = reinterpret_cast<uintptr_t>(base);
-  const int64_t unit = a.heads > 1 ? head : page;
-  if (a.dim == dim && unit > 0 && page % unit == 0 &&
-      (a.pages + 1ll) * (page / unit) < INT32_MAX) {
-    *per_page = static_cast<int>(page / unit);
-    const uint64_t dims[5] = {64, 8, static_cast<uint64_t>(dim / 64),
-                              static_cast<uint64_t>(a.page_size / 8),
-                              static_cast<uint64_t>(a.pages - 1) * *per_page + a.heads};
-    const uint64_t strides[4] = {row, 128, 8 * row, static_cast<uint64_t>(unit)};
-    const uint32_t box[5] = {64, 8, static_cast<uint32_t>(dim / 64),
-                             static_cast<uint32_t>(keys / 8), 1};
-    return pg_detail_tensormap(map, 5, at, dims, strides, box);
-  }
-  *per_page = 0;
+// The tensor map of the keys or values: columns, a page's rows, heads and pages. (Heads and pages
+// as one coordinate leave a fifth for the groups of eight rows and so one box for a whole run of
+// keys, but the many small boxes cost nothing: 500 us each for 4096 new tokens of up to 8192.)
+int encode(CUtensorMap *map, const Attention &a, const char *base, int64_t head, int64_t page) {
   const uint64_t dims[4] = {static_cast<uint64_t>(a.dim), static_cast<uint64_t>(a.page_size),
                             static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.pages)};
-  const uint64_t strides[3] = {row, static_cast<uint64_t>(head), static_cast<uint64_t>(page)};
+  const uint64_t strides[3] = {2ull * a.dim, static_cast<uint64_t>(head),
+                               static_cast<uint64_t>(page)};
   const uint32_t box[4] = {64, 8, 1, 1};
-  return pg_detail_tensormap(map, 4, at, dims, strides, box);
+  return pg_detail_tensormap(map, 4, reinterpret_cast<uintptr_t>(base), dims, strides, box);
 }
 
 template <class T, int DIM>
@@ -802,16 +772,15 @@ int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cuda
   CUtensorMap k_map = {}, v_map = {};
   // a kv head's tiles of the latest queries, which see the most keys, go first
   const dim3 grid(a.heads, tiles, a.parts);
-  const int keys = std::gcd(a.page_size, kKeys);
-  if (keys < 8)
+  const int run = std::gcd(a.page_size, kKeys);  // the keys that a page and a block always share
+  if (run < 8)
     return pg::launch<prompt_kernel<T, DIM, false>>("prompt_kernel", grid, kThreads,
-                      Plan<DIM>::bytes, stream, a, k_map, v_map, Boxes{});
-  Boxes boxes{keys, 0, 0};
-  int rc = encode(&k_map, &boxes.k_per_page, a, a.k, a.k_head, a.k_page, DIM, keys);
-  if (!rc) rc = encode(&v_map, &boxes.v_per_page, a, a.v, a.v_head, a.v_page, DIM, keys);
+                      Plan<DIM>::bytes, stream, a, k_map, v_map, run);
+  int rc = encode(&k_map, a, a.k, a.k_head, a.k_page);
+  if (!rc) rc = encode(&v_map, a, a.v, a.v_head, a.v_page);
   if (rc) return rc;
   return pg::launch<prompt_kernel<T, DIM, true>>("prompt_kernel", grid, kThreads,
-                    Plan<DIM>::bytes, stream, a, k_map, v_map, boxes);
+                    Plan<DIM>::bytes, stream, a, k_map, v_map, run);
 }
 
 }  // namespace

@@ -16,7 +16,12 @@ namespace {
 
 constexpr int kPlan = 1024;   // threads of a planning block
 constexpr int kCopy = 256;    // threads of a copying block
-constexpr int kCopyPerSm = 8; // copying blocks an SM holds at once (2048 threads)
+// Copying blocks an SM gets at most, eight times what it holds: a block that ends makes room for
+// the next, which spreads the copies better than blocks that stay and loop in step. With 8, 64 and
+// 512: half the pages of 96 sequences of up to 900 tokens moved in 16 layers 210, 193, 207 us; 250
+// children of 24 layers forked 127, 120, 122; 48 sequences of up to 4096 tokens written 143, 131,
+// 130 (with their extend and free).
+constexpr int kCopyPerSm = 64;
 constexpr int kUnroll = 4;    // 16-byte loads a copying thread has in flight
 
 // Scratch words (int32): [0] whether the plan went through, [1] its number of pages, then
@@ -102,7 +107,8 @@ __device__ int claim(int *len) {
 
 // --- extend: room for the new tokens of each slot ----------------------------------------------
 // One block: the pages it hands out are found by a scan of the counts that stops at the last one
-// needed, and 4096 counts are 16 KB, so the latency of a few dependent loads bounds it.
+// needed, and 4096 counts are 16 KB, so the latency of a few dependent loads bounds it: 5 us for a
+// few slots, 13 us for 48 slots and 6000 pages.
 
 __global__ void __launch_bounds__(kPlan) cache_extend(pg_cache c, const int *slots_in,
                                                       const int *starts, int n) {
@@ -166,7 +172,9 @@ __global__ void __launch_bounds__(kPlan) cache_extend(pg_cache c, const int *slo
 
 // --- write: new rows of one layer into the slots' pages ----------------------------------------
 // A warp takes one token: its slot and page are the same for all lanes, and its heads' rows of
-// keys and values are 16-byte pieces that the lanes load together before they store any.
+// keys and values are 16-byte pieces that the lanes load together before they store any. HBM
+// bounds it, each piece read and written once: 5.9 TB/s with 48 sequences of up to 4096 tokens of
+// 8 heads of 128 in bf16, their extend counted in.
 
 __device__ __forceinline__ int find_sequence(const int *starts, int n, int token) {
   int lo = 0, hi = n;
@@ -226,7 +234,7 @@ __global__ void __launch_bounds__(kCopy) cache_write(pg_cache c, int layer, cons
   }
 }
 
-// --- free: a slot lets go of its pages -------------------------------------------------------------
+// --- free: a slot lets go of its pages ---------------------------------------------------------
 
 __global__ void __launch_bounds__(kCopy) cache_free(pg_cache c, const int *slots_in, int n) {
   __shared__ int held;
@@ -252,9 +260,10 @@ __global__ void __launch_bounds__(kCopy) cache_free(pg_cache c, const int *slots
   }
 }
 
-// --- copying rows of pages -------------------------------------------------------------------------
+// --- copying rows of pages ---------------------------------------------------------------------
 // Copies the first `rows` rows of every head of page `from` to page `to` in one layer's keys or
-// values. HBM bounds it: each piece is read and written once, 16 bytes a lane.
+// values. HBM bounds it: each piece is read and written once, 16 bytes a lane, and 6.2 TB/s to 6.8
+// are reached by the forks and moves named above.
 
 __device__ void copy_rows(const pg_cache &c, char *base, int layer, int from, int to, int rows) {
   const int per_head = rows * (c.row_bytes / 16), all = c.heads * per_head;
@@ -292,7 +301,7 @@ __global__ void __launch_bounds__(kCopy) cache_copy(pg_cache c, const int *from,
   }
 }
 
-// --- fork: children that share their parents' full pages --------------------------------------------
+// --- fork: children that share their parents' full pages ---------------------------------------
 
 __global__ void __launch_bounds__(kPlan) cache_fork_plan(pg_cache c, const int *parents,
                                                          const int *children, int n) {
@@ -385,7 +394,7 @@ __global__ void __launch_bounds__(kCopy) cache_fork_copy(pg_cache c, const int *
   }
 }
 
-// --- compact: the live pages move to the front -------------------------------------------------------
+// --- compact: the live pages move to the front -------------------------------------------------
 // With L live pages, the k-th free page below L takes the k-th live page at or above L, both
 // ascending: the fewest moves, and no page is both read and written.
 
@@ -441,7 +450,7 @@ __global__ void __launch_bounds__(kCopy) cache_compact_move(pg_cache c) {
   }
 }
 
-// --- host side -----------------------------------------------------------------------------------------
+// --- host side ---------------------------------------------------------------------------------
 
 int check(const char *what, const pg_cache *c) {
   if (!c) return pg::argument_fail("%s: null cache", what);
@@ -488,7 +497,7 @@ int check_rows(const char *what, const pg_rows *r) {
   return PG_OK;
 }
 
-// Blocks for `tasks` tasks: one each, at most what the GPU holds at once (they loop).
+// Blocks for `tasks` tasks: one each, up to the most, which loop.
 int copy_grid(int64_t tasks, int *grid) {
   int sms;
   int rc = pg::sm_count(&sms);
