@@ -74,7 +74,7 @@ def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any
                              f"with a head's rows of one page one after another, got {t.dtype} "
                              f"{tuple(t.shape)} {t.stride()} on {t.device}")
     pages, heads, page_size, _ = shape
-    if hq % heads:
+    if not heads or hq % heads:
         raise ValueError(f"{hq} query heads are no multiple of {heads} kv heads")
     if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1 or \
             table.device != dev:
