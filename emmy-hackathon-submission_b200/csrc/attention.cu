@@ -423,10 +423,10 @@ extern "C" int pg_attention(const pg_attention_args *p, uint64_t stream) {
   const int max_len = static_cast<int>(p->max_len && p->max_len < most ? p->max_len : most);
   const int64_t partial_bytes = p->workspace_bytes - 256 - pg::kCounters * 4ll;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
-  if (dtype != PG_DT_F32 && a.dim <= 128) {
-    if (pg::decode_takes(a, static_cast<int>(most)))
-      return pg::decode_16bit(a, dtype == PG_DT_BF16, sms, s);
-    if (a.starts) return pg::prompt_16bit(a, dtype == PG_DT_BF16, max_len, partial_bytes, sms, s);
+  if (a.dim <= 128) {
+    if (pg::decode_takes(a, static_cast<int>(most))) return pg::decode(a, dtype, sms, s);
+    if (a.starts && dtype != PG_DT_F32)
+      return pg::prompt_16bit(a, dtype == PG_DT_BF16, max_len, partial_bytes, sms, s);
   }
   if (dtype == PG_DT_F32) return run<float>(a, max_len, partial_bytes, sms, s);
   if (dtype == PG_DT_BF16) return run<__nv_bfloat16>(a, max_len, partial_bytes, sms, s);

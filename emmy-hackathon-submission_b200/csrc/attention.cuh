@@ -139,6 +139,18 @@ __device__ __forceinline__ bool clean(uint4 *at) {
   return any;
 }
 
+// ... the f32 numbers.
+__device__ __forceinline__ bool clean32(uint4 *at) {
+  const uint4 x = *at;
+  uint32_t u[4] = {x.x, x.y, x.z, x.w};
+  bool any = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if ((u[k] & 0x7f800000u) == 0x7f800000u) u[k] = 0, any = true;
+  if (any) *at = make_uint4(u[0], u[1], u[2], u[3]);
+  return any;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -150,10 +162,10 @@ __device__ __forceinline__ float factor(float a, float b) {
   return a == -INFINITY ? 0.0f : exp2_fast(a - b);
 }
 
-// Kernels for the 16-bit types at head sizes of up to 128: few rows a sequence
-// (attention_decode.cu), and many (attention_prompt.cu).
+// Kernels for head sizes of up to 128: few rows a sequence (attention_decode.cu), and many in the
+// 16-bit types (attention_prompt.cu).
 bool decode_takes(const Attention &a, int max_len);
-int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream);
+int decode(const Attention &a, int dtype, int sms, cudaStream_t stream);
 int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                  cudaStream_t stream);
 

@@ -27,8 +27,6 @@ using pg::Attention;
 using pg::Blocks;
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kStep = 16;             // keys a warp takes at a time
-constexpr int kKeys = kStep * kWarps; // keys of a block's step
 constexpr int kRows = 16;
 constexpr int kPerSm = 2;             // blocks an SM holds
 // What a pair costs by itself, in blocks of keys (64 sequences of up to 8000 keys on 8 kv heads:
@@ -86,6 +84,20 @@ template <> struct Mma<__half> {
   }
 };
 
+template <> struct Mma<float> {
+  __device__ static void run(float *d, const uint32_t *a, const uint32_t *b) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, "
+                 "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  }
+  // the 11 leading bits of a number, and the next 11
+  __device__ static void split(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+  }
+};
+
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool real) {
   const int bytes = real ? 16 : 0;  // 0: the 16 bytes are zeroed and nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes)
@@ -100,10 +112,13 @@ __device__ __forceinline__ void load_matrices_t(uint32_t at, uint32_t *r) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
-template <int DIM>
+template <class T, int DIM>
 struct Ring {
-  static constexpr int row = DIM * 2, chunks = DIM / 8;
-  static constexpr int tile = kStep * row;        // 16 keys, or 16 values
+  static constexpr int size = sizeof(T);
+  static constexpr int row = DIM * size, chunks = row / 16;
+  static constexpr int step = 32 / size;          // keys a warp takes at a time
+  static constexpr int keys = step * kWarps;      // keys of a block's step
+  static constexpr int tile = step * row;         // a warp's keys, or values
   static constexpr int stage = 2 * tile;
   static constexpr int stages = 384 / DIM;
   static constexpr int warp = stages * stage;
@@ -120,7 +135,7 @@ struct Sequence {
   uint32_t pairs;
 };
 
-template <bool MANY>
+template <bool MANY, int KEYS>
 __device__ __forceinline__ Sequence sequence_of(const Attention &a, int b) {
   Sequence s;
   s.slot = a.slots ? a.slots[b] : b;
@@ -142,7 +157,7 @@ __device__ __forceinline__ Sequence sequence_of(const Attention &a, int b) {
     }
   }
   s.row_groups = (s.count * a.group + kRows - 1) / kRows;
-  s.blocks = pg::blocks_of(a, s.length - s.count, s.length - 1, kKeys);
+  s.blocks = pg::blocks_of(a, s.length - s.count, s.length - 1, KEYS);
   s.pairs = s.blocks.count ? a.heads * s.row_groups : 0;
   return s;
 }
@@ -156,11 +171,42 @@ struct Pair {
   const int *pages;
   unsigned last;
   // whether all rows see all of a step's keys
+  template <int STEP>
   __device__ bool all_see(const Attention &a, int key) const {
-    return key + kStep - 1 <= lo &&
-           (!a.window || key > hi - a.window || key + kStep <= a.sinks);
+    return key + STEP - 1 <= lo &&
+           (!a.window || key > hi - a.window || key + STEP <= a.sinks);
   }
 };
+
+// Four numbers of T at an address, or to it.
+template <class T>
+__device__ __forceinline__ float4 load4(const char *at) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4 *>(at);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2 *>(at);
+    return make_float4(Mma<T>::low(w.x), Mma<T>::high(w.x), Mma<T>::low(w.y), Mma<T>::high(w.y));
+  }
+}
+template <class T>
+__device__ __forceinline__ void store4(char *at, float4 x) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4 *>(at) = x;
+  else
+    *reinterpret_cast<uint2 *>(at) = make_uint2(Mma<T>::pack(x.x, x.y), Mma<T>::pack(x.z, x.w));
+}
+
+// q . k with k a row of a stage, one product after another.
+template <class R>
+__device__ __noinline__ float plain_product(const char *q, const char *stage, int row, int dim) {
+  float sum = 0.0f;
+  for (int c = 0; c < dim / 4; ++c) {
+    const float4 x = *reinterpret_cast<const float4 *>(q + 16 * c);
+    const float4 y = *reinterpret_cast<const float4 *>(stage + R::at(row, c));
+    sum = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sum))));
+  }
+  return sum;
+}
 
 // What the warps of a block have of a pair, from their rings' places: joined, and written as the
 // result, or left for the block that finishes the pair last, which joins all. A function of its own
@@ -168,7 +214,7 @@ struct Pair {
 // keys, whose loads of operands then wait for one another (a tenth of the whole).
 template <class T, int DIM, bool MANY>
 __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t per, int odd) {
-  using R = Ring<DIM>;
+  using R = Ring<T, DIM>;
   extern __shared__ float4 smem4[];
   const Pair p = sh;
   const int tid = threadIdx.x;
@@ -188,10 +234,10 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
     // a query before the sequence's start sees no key: zeros
     const float inv = 1.0f / sum;
     const bool none = p.lo + query_of(r) < 0;
-    *reinterpret_cast<uint2 *>(a.out + (p.query + query_of(r)) * a.out_token +
-                               head_of(r) * a.out_head + col * 2) =
-        none ? make_uint2(0, 0)
-             : make_uint2(Mma<T>::pack(x.x * inv, x.y * inv), Mma<T>::pack(x.z * inv, x.w * inv));
+    store4<T>(a.out + (p.query + query_of(r)) * a.out_token + head_of(r) * a.out_head +
+                  col * R::size,
+              none ? make_float4(0, 0, 0, 0)
+                   : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
   };
   // thread's columns: four of row `warp`, `warp + 4`, ...
   constexpr int lanes = DIM / 4;
@@ -212,22 +258,22 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
       acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y);
       acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
     }
-    if (MANY && odd && col < a.dim)
+    if ((MANY || sizeof(T) == 4) && odd && col < a.dim)
       for (int i = 0; i < p.block1 - p.block0; ++i)
-        for (int j = 0; j < kKeys; ++j) {
-          const int key = p.blocks.key_block(p.block0 + i) * kKeys + j;
-          if (p.all_see(a, key / kStep * kStep) || !pg::sees(a, p.lo + query_of(r), key)) continue;
+        for (int j = 0; j < R::keys; ++j) {
+          const int key = p.blocks.key_block(p.block0 + i) * R::keys + j;
+          if (!pg::sees(a, p.lo + query_of(r), key) ||
+              (sizeof(T) != 4 && p.all_see<R::step>(a, key / R::step * R::step)))
+            continue;
           const int page = p.pages[key / a.page_size];
           if (page < 0 || page >= a.pages) continue;
-          const uint2 w = *reinterpret_cast<const uint2 *>(
-              a.v + page * a.v_page + p.head * a.v_head +
-              static_cast<int64_t>(key % a.page_size) * a.dim * 2 + col * 2);
-          const float x[4] = {Mma<T>::low(w.x), Mma<T>::high(w.x), Mma<T>::low(w.y),
-                              Mma<T>::high(w.y)};
-          if (!(fabsf(x[0]) < INFINITY)) acc.x += x[0];
-          if (!(fabsf(x[1]) < INFINITY)) acc.y += x[1];
-          if (!(fabsf(x[2]) < INFINITY)) acc.z += x[2];
-          if (!(fabsf(x[3]) < INFINITY)) acc.w += x[3];
+          const float4 x = load4<T>(a.v + page * a.v_page + p.head * a.v_head +
+                                    static_cast<int64_t>(key % a.page_size) * a.dim * R::size +
+                                    col * R::size);
+          if (!(fabsf(x.x) < INFINITY)) acc.x += x.x;
+          if (!(fabsf(x.y) < INFINITY)) acc.y += x.y;
+          if (!(fabsf(x.z) < INFINITY)) acc.z += x.z;
+          if (!(fabsf(x.w) < INFINITY)) acc.w += x.w;
         }
     if (alone) {
       write(r, col, acc, sum);
@@ -307,7 +353,7 @@ struct Plan {
 // MANY: sequences have any number of queries, not one each.
 template <class T, int DIM, bool MANY>
 __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_constant__ Attention a) {
-  using R = Ring<DIM>;
+  using R = Ring<T, DIM>;
   extern __shared__ float4 smem4[];
   __shared__ uint3 warp_sum[kWarps];
   __shared__ Pair sh;
@@ -326,13 +372,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
   const int first_b = min(tid * run, a.batch), end_b = min(first_b + run, a.batch);
   uint32_t pairs = 0, keys = 0, longest = 0;
   for (int b = first_b; b < end_b; ++b) {
-    const Sequence s = sequence_of<MANY>(a, b);
+    const Sequence s = sequence_of<MANY, R::keys>(a, b);
     pairs += s.pairs;
     keys += s.pairs * s.blocks.count;
     longest = max(longest, static_cast<uint32_t>(s.blocks.count));
     if (!s.length && b % gridDim.x == c)  // no key: zeros
       for (int i = 0; i < s.count * a.heads * a.group; ++i)
-        for (int j = 0; j < a.dim / 8; ++j)
+        for (int j = 0; j < a.dim * R::size / 16; ++j)
           *reinterpret_cast<uint4 *>(a.out + (s.query + i / (a.heads * a.group)) * a.out_token +
                                      i % (a.heads * a.group) * a.out_head + j * 16) =
               make_uint4(0, 0, 0, 0);
@@ -371,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
   if (u >= before && u < upto) {
     uint32_t at = before;
     for (int b = first_b; b < end_b; ++b) {
-      const Sequence s = sequence_of<MANY>(a, b);
+      const Sequence s = sequence_of<MANY, R::keys>(a, b);
       const uint32_t next = at + s.pairs * (s.blocks.count + kPair);
       if (u < next) {
         plan.sequence = b;
@@ -391,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
 
   while (u < plan.end) {
     int b = plan.sequence;
-    Sequence seq = sequence_of<MANY>(a, b);
-    while (!seq.pairs) seq = sequence_of<MANY>(a, ++b);
+    Sequence seq = sequence_of<MANY, R::keys>(a, b);
+    while (!seq.pairs) seq = sequence_of<MANY, R::keys>(a, ++b);
     const Blocks &blocks = seq.blocks;
     const uint32_t before = plan.before, per = plan.per;
     const uint32_t units = blocks.count + kPair, pair = (u - before) / units;
@@ -423,18 +469,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
     const int pos[2] = {lo + query_of(g), lo + query_of(g + 8)};
     int *const odd = odds + plan.turn;
 
-    // the queries' fragments: rows g and g + 8, columns 2 t and 2 t + 8 of each 16
-    uint32_t q[DIM / 16][4];
+    // the queries' fragments: rows g and g + 8, columns 2 t and 2 t + 8 of each 16 (f32: t and t + 4
+    // of each 8)
+    uint32_t q[R::row / 32][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = g + 8 * h;
       const char *from =
           a.q + (seq.query + query_of(r)) * a.q_token + head_of(r) * a.q_head + 4 * t4;
 #pragma unroll
-      for (int k = 0; k < DIM / 16; ++k)
+      for (int k = 0; k < R::row / 32; ++k)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          q[k][h + 2 * i] = r < rows && 16 * k + 8 * i < a.dim
+          q[k][h + 2 * i] = r < rows && 32 * k + 16 * i < a.dim * R::size
                                 ? *reinterpret_cast<const uint32_t *>(from + 32 * k + 16 * i)
                                 : 0u;
     }
@@ -444,17 +491,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
 
-    // The warp's steps are the blocks' 16 keys at 16 warp. A step whose keys all are seen and lie
-    // in one page, as they do where pages are whole groups of 16, needs one look at the table and
-    // one address; else lane r < 16 knows key r's page and row.
+    // The warp's steps are the blocks' 16 keys at 16 warp (f32: 8 at 8 warp). A step whose keys all are seen and lie
+    // in one page, as they do where pages are whole groups of so many, needs one look at the table and
+    // one address; else lane r knows key r's page and row.
     const int steps = block1 - block0;
-    const bool whole_pages = a.page_size % kStep == 0;
+    const bool whole_pages = a.page_size % R::step == 0;
     const auto first_key = [&](int i) {
-      return blocks.key_block(block0 + i) * kKeys + kStep * warp;
+      return blocks.key_block(block0 + i) * R::keys + R::step * warp;
     };
     const auto all_seen = [&](int key) {
-      return key + kStep - 1 <= lo &&
-             (!a.window || key > hi - a.window || key + kStep <= a.sinks);
+      return key + R::step - 1 <= lo &&
+             (!a.window || key > hi - a.window || key + R::step <= a.sinks);
     };
     const auto some_see = [&](int key) {
       return key <= hi && (!a.window || key > lo - a.window || key < a.sinks);
@@ -463,14 +510,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
       if (i >= steps) return -1;
       const int key = first_key(i);
       if (whole_pages && all_seen(key)) return pages[key / a.page_size];
-      return some_see(key + (lane & 15)) ? pages[(key + (lane & 15)) / a.page_size] : -1;
+      return some_see(key + (lane & (R::step - 1))) ? pages[(key + (lane & (R::step - 1))) / a.page_size] : -1;
     };
     const int sub = lane / R::chunks, chunk = lane % R::chunks;
-    const bool column = chunk * 8 < a.dim;
-    const int64_t row_bytes = 2ll * a.dim;
+    const bool column = chunk * 16 < a.dim * R::size;
+    const int64_t row_bytes = static_cast<int64_t>(R::size) * a.dim;
     const char *const k_head = a.k + head * a.k_head + chunk * 16;
     const char *const v_head = a.v + head * a.v_head + chunk * 16;
-    constexpr int kCopies = kStep * R::chunks / 32, kRowsEach = 32 / R::chunks;
+    constexpr int kCopies = R::step * R::chunks / 32, kRowsEach = 32 / R::chunks;
     const auto issue = [&](int i, int page) {
       if (i < steps) {
         const uint32_t to = ring_at + (i % R::stages) * R::stage;
@@ -492,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
             v += kRowsEach * row_bytes;
           }
         } else {
-          const int mine_key = key + (lane & 15);
+          const int mine_key = key + (lane & (R::step - 1));
           if (some_see(mine_key) && (page < 0 || page >= a.pages)) {
             atomicOr(a.status, PG_CACHE_BAD_PAGE);
             page = -1;
@@ -529,29 +576,71 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
       asm volatile("cp.async.wait_group %0;" ::"n"(R::stages - 1) : "memory");
       __syncwarp();
       const uint32_t ks = ring_at + (i % R::stages) * R::stage, vs = ks + R::tile;
-      float s[2][4] = {};
+      constexpr int kN = R::step / 8;
+      float s[kN][4] = {};
+      if constexpr (sizeof(T) == 4) {
+        // even and odd columns, and hi by hi and the rest, by themselves: four short chains of sums
+        float part[4][4] = {};
 #pragma unroll
-      for (int k = 0; k < DIM / 32; ++k)
+        for (int k = 0; k < DIM / 16; ++k) {
+          uint32_t x[4];  // 8 keys by columns 16 k.., four 8 x 4 matrices along the columns
+          load_matrices(ks + R::at(lane & 7, 4 * k + (lane >> 3)), x);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          uint32_t x[4];  // keys 8 n.. by columns 32 k.., four 8 x 8 matrices along the columns
-          load_matrices(ks + R::at(8 * n + (lane & 7), 4 * k + (lane >> 3)), x);
-          Mma<T>::run(s[n], q[2 * k], x[0], x[1]);
-          Mma<T>::run(s[n], q[2 * k + 1], x[2], x[3]);
+          for (int j = 0; j < 2; ++j) {
+            uint32_t q_hi[4], q_lo[4], hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              Mma<T>::split(__uint_as_float(q[2 * k + j][e]), q_hi[e], q_lo[e]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) Mma<T>::split(__uint_as_float(x[2 * j + e]), hi[e], lo[e]);
+            Mma<T>::run(part[j], q_hi, hi);
+            Mma<T>::run(part[2 + j], q_hi, lo);
+            Mma<T>::run(part[2 + j], q_lo, hi);
+          }
         }
+        bool none = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[0][e] = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
+          none |= s[0][e] != s[0][e];
+        }
+        // a factor that is not finite has no two parts: such products are made anew, as they stand
+        if (__any_sync(0xffffffffu, none))
+          for (int e = 0; e < 4; ++e) {
+            const int r = g + 8 * (e >> 1);
+            if (r < rows)
+              s[0][e] = plain_product<R>(
+                  a.q + (seq.query + query_of(r)) * a.q_token + head_of(r) * a.q_head,
+                  ring + (i % R::stages) * R::stage, 2 * t4 + (e & 1), a.dim);
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < DIM / 32; ++k)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            uint32_t x[4];  // keys 8 n.. by columns 32 k.., four 8 x 8 matrices along the columns
+            load_matrices(ks + R::at(8 * n + (lane & 7), 4 * k + (lane >> 3)), x);
+            Mma<T>::run(s[n], q[2 * k], x[0], x[1]);
+            Mma<T>::run(s[n], q[2 * k + 1], x[2], x[3]);
+          }
+      }
       const int key = first_key(i);
       const bool masked = !all_seen(key);
-      if (MANY && masked) {
+      if (sizeof(T) == 4 || (MANY && masked)) {
         bool any = false;
-        for (int j = lane; j < kStep * R::chunks; j += 32)
-          any |= pg::clean<Mma<T>::exponent>(reinterpret_cast<uint4 *>(
-              ring + (i % R::stages) * R::stage + R::tile + j * 16));
+#pragma unroll
+        for (int j = lane; j < R::step * R::chunks; j += 32) {
+          uint4 *const at =
+              reinterpret_cast<uint4 *>(ring + (i % R::stages) * R::stage + R::tile + j * 16);
+          if constexpr (sizeof(T) == 4) any |= pg::clean32(at);
+          else any |= pg::clean<Mma<T>::exponent>(at);
+        }
         if (any) *const_cast<volatile int *>(odd) = 1;
         __syncwarp();
       }
       float top[2] = {m[0], m[1]};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[n][e] *= a.scale_log2;
@@ -580,22 +669,43 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
       const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
       uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float x = pg::exp2_fast(s[n][2 * h] - base[h]);
           const float y = pg::exp2_fast(s[n][2 * h + 1] - base[h]);
           l[h] += x + y;
-          Mma<T>::split(x, y, hi[2 * n + h], lo[2 * n + h]);
+          if constexpr (sizeof(T) == 4) {
+            Mma<T>::split(x, hi[h], lo[h]);  // the product's keys are 0, 2, 4, 6, 1, 3, 5, 7
+            Mma<T>::split(y, hi[2 + h], lo[2 + h]);
+          } else {
+            Mma<T>::split(x, y, hi[2 * n + h], lo[2 * n + h]);
+          }
         }
+      if constexpr (sizeof(T) == 4) {
+        const char *const v = ring + (i % R::stages) * R::stage + R::tile + 4 * (g & 3);
 #pragma unroll
-      for (int n = 0; n < DIM / 16; ++n) {
-        uint32_t x[4];  // keys 0.. and 8.. by columns 16 n.. and 16 n + 8.., transposed
-        load_matrices_t(vs + R::at(lane & 15, 2 * n + (lane >> 4)), x);
-        Mma<T>::run(o[2 * n], hi, x[0], x[1]);
-        Mma<T>::run(o[2 * n], lo, x[0], x[1]);
-        Mma<T>::run(o[2 * n + 1], hi, x[2], x[3]);
-        Mma<T>::run(o[2 * n + 1], lo, x[2], x[3]);
+        for (int n = 0; n < DIM / 8; ++n) {
+          uint32_t v_hi[2], v_lo[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            Mma<T>::split(
+                *reinterpret_cast<const float *>(v + R::at(2 * t4 + e, 2 * n + (g >> 2))),
+                v_hi[e], v_lo[e]);
+          Mma<T>::run(o[n], hi, v_hi);
+          Mma<T>::run(o[n], hi, v_lo);
+          Mma<T>::run(o[n], lo, v_hi);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < DIM / 16; ++n) {
+          uint32_t x[4];  // keys 0.. and 8.. by columns 16 n.. and 16 n + 8.., transposed
+          load_matrices_t(vs + R::at(lane & 15, 2 * n + (lane >> 4)), x);
+          Mma<T>::run(o[2 * n], hi, x[0], x[1]);
+          Mma<T>::run(o[2 * n], lo, x[0], x[1]);
+          Mma<T>::run(o[2 * n + 1], hi, x[2], x[3]);
+          Mma<T>::run(o[2 * n + 1], lo, x[2], x[3]);
+        }
       }
       __syncwarp();  // the stage may be filled again
     }
@@ -638,9 +748,9 @@ int launch_decode(const Attention &a, int sms, cudaStream_t stream) {
   const dim3 grid(kPerSm * sms);
   if (a.starts)
     return pg::launch<decode_kernel<T, DIM, true>>("decode_kernel", grid, kThreads,
-                                                   Ring<DIM>::bytes, stream, a);
+                                                   Ring<T, DIM>::bytes, stream, a);
   return pg::launch<decode_kernel<T, DIM, false>>("decode_kernel", grid, kThreads,
-                                                  Ring<DIM>::bytes, stream, a);
+                                                  Ring<T, DIM>::bytes, stream, a);
 }
 
 }  // namespace
@@ -656,12 +766,15 @@ namespace pg {
 bool decode_takes(const Attention &a, int max_len) {
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
   if (a.starts && rows > 48ll * a.batch) return false;
-  // its blocks of keys count in 31 bits
-  return (rows / kRows + a.batch) * a.heads * (max_len / kKeys + 2ll + kPair) < INT32_MAX;
+  // its blocks of 32 keys or more count in 31 bits
+  return (rows / kRows + a.batch) * a.heads * (max_len / 32 + 2ll + kPair) < INT32_MAX;
 }
 
-int decode_16bit(const Attention &a, bool bf16, int sms, cudaStream_t stream) {
-  if (bf16)
+int decode(const Attention &a, int dtype, int sms, cudaStream_t stream) {
+  if (dtype == PG_DT_F32)
+    return a.dim <= 64 ? launch_decode<float, 64>(a, sms, stream)
+                       : launch_decode<float, 128>(a, sms, stream);
+  if (dtype == PG_DT_BF16)
     return a.dim <= 64 ? launch_decode<__nv_bfloat16, 64>(a, sms, stream)
                        : launch_decode<__nv_bfloat16, 128>(a, sms, stream);
   return a.dim <= 64 ? launch_decode<__half, 64>(a, sms, stream)
