@@ -120,9 +120,11 @@ struct Ring {
   static constexpr int keys = step * kWarps;      // keys of a block's step
   static constexpr int tile = step * row;         // a warp's keys, or values
   static constexpr int stage = 2 * tile;
-  static constexpr int stages = 384 / DIM;
+  static constexpr int stages = (size == 4 ? 256 : 384) / DIM;
   static constexpr int warp = stages * stage;
-  static constexpr int bytes = kWarps * warp;
+  // f32: the queries' fragments in their two parts, of which registers have no room for one
+  static constexpr int q = kWarps * warp, q_part = size == 4 ? 16 * row : 0;
+  static constexpr int bytes = q + 2 * q_part;
   static_assert(warp >= kRows * (DIM + 2) * 4, "a warp's result takes its ring's place");
   __device__ static int at(int r, int chunk) { return r * row + ((chunk ^ (r & 7)) << 4); }
 };
@@ -471,19 +473,33 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
 
     // the queries' fragments: rows g and g + 8, columns 2 t and 2 t + 8 of each 16 (f32: t and t + 4
     // of each 8)
-    uint32_t q[R::row / 32][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    uint32_t q[sizeof(T) == 4 ? 1 : DIM / 16][4];
+    const auto q_word = [&](int k, int h, int i) {
       const int r = g + 8 * h;
-      const char *from =
-          a.q + (seq.query + query_of(r)) * a.q_token + head_of(r) * a.q_head + 4 * t4;
+      return r < rows && 32 * k + 16 * i < a.dim * R::size
+                 ? *reinterpret_cast<const uint32_t *>(a.q + (seq.query + query_of(r)) * a.q_token +
+                                                       head_of(r) * a.q_head + 32 * k + 16 * i +
+                                                       4 * t4)
+                 : 0u;
+    };
+    uint4 *const q_hi = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(smem4) + R::q) + lane;
+    uint4 *const q_lo = q_hi + R::q_part / 16;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int k = 0; k < R::row / 32; ++k)
+      for (int k = warp; k < DIM / 8; k += kWarps) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          q[k][h + 2 * i] = r < rows && 32 * k + 16 * i < a.dim * R::size
-                                ? *reinterpret_cast<const uint32_t *>(from + 32 * k + 16 * i)
-                                : 0u;
+        for (int e = 0; e < 4; ++e)
+          Mma<T>::split(__uint_as_float(q_word(k, e & 1, e >> 1)), hi[e], lo[e]);
+        q_hi[32 * k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        q_lo[32 * k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[k][e] = q_word(k, e & 1, e >> 1);
     }
     float o[DIM / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -587,15 +603,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
           load_matrices(ks + R::at(lane & 7, 4 * k + (lane >> 3)), x);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            uint32_t q_hi[4], q_lo[4], hi[2], lo[2];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              Mma<T>::split(__uint_as_float(q[2 * k + j][e]), q_hi[e], q_lo[e]);
+            const uint4 a_hi = q_hi[32 * (2 * k + j)], a_lo = q_lo[32 * (2 * k + j)];
+            uint32_t hi[2], lo[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) Mma<T>::split(__uint_as_float(x[2 * j + e]), hi[e], lo[e]);
-            Mma<T>::run(part[j], q_hi, hi);
-            Mma<T>::run(part[2 + j], q_hi, lo);
-            Mma<T>::run(part[2 + j], q_lo, hi);
+            Mma<T>::run(part[j], &a_hi.x, hi);
+            Mma<T>::run(part[2 + j], &a_hi.x, lo);
+            Mma<T>::run(part[2 + j], &a_lo.x, hi);
           }
         }
         bool none = false;
