@@ -344,9 +344,10 @@ int run(Attention a, int max_len, int64_t partial_bytes, int sms, cudaStream_t s
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
   const int size = rows <= 16ll * a.batch ? 16 : 64;
   const int tiles = pg::tile_bound(a, size);
-  // few rows read the keys at the memory's speed at best, and four parts a block that an SM holds
-  // even out ragged lengths: 32 sequences of up to 8000 f32 keys take 730 us so, 1550 in one part
-  a.parts = pg::choose_parts(a, tiles, size, a.dim, kKeys, max_len, (size == 16 ? 8 : 2) * sms,
+  // few rows read the keys at the memory's speed at best, and eight parts a block that an SM holds
+  // even out ragged lengths: 32 sequences of up to 8000 keys with f32 heads of 256 take 1540 us so,
+  // 1665 with four and 2470 in one part
+  a.parts = pg::choose_parts(a, tiles, size, a.dim, kKeys, max_len, (size == 16 ? 16 : 2) * sms,
                              partial_bytes);
   return size == 16 ? launch_dim<T, 16>(a, tiles, stream) : launch_dim<T, 64>(a, tiles, stream);
 }
@@ -424,7 +425,8 @@ extern "C" int pg_attention(const pg_attention_args *p, uint64_t stream) {
   const int64_t partial_bytes = p->workspace_bytes - 256 - pg::kCounters * 4ll;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
   if (a.dim <= 128) {
-    if (pg::decode_takes(a, static_cast<int>(most))) return pg::decode(a, dtype, sms, s);
+    if (pg::decode_takes(a, dtype == PG_DT_F32, static_cast<int>(most), max_len))
+      return pg::decode(a, dtype, sms, s);
     if (a.starts && dtype != PG_DT_F32)
       return pg::prompt_16bit(a, dtype == PG_DT_BF16, max_len, partial_bytes, sms, s);
   }

@@ -164,7 +164,7 @@ __device__ __forceinline__ float factor(float a, float b) {
 
 // Kernels for head sizes of up to 128: few rows a sequence (attention_decode.cu), and many in the
 // 16-bit types (attention_prompt.cu).
-bool decode_takes(const Attention &a, int max_len);
+bool decode_takes(const Attention &a, bool f32, int most, int max_len);
 int decode(const Attention &a, int dtype, int sms, cudaStream_t stream);
 int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                  cudaStream_t stream);

@@ -1,5 +1,4 @@
-// Attention of one new token a sequence, or a few, for the 16-bit types at head sizes of up to
-// 128 (pg_attention).
+// Attention of one new token a sequence, or a few, at head sizes of up to 128 (pg_attention).
 //
 // HBM bounds it: every key and value is read once and used for the query heads of its group
 // only. So the work is cut evenly by keys, not by sequences: the blocks of 64 keys of all
@@ -15,6 +14,14 @@
 // each key the memory is slower by far). A weight goes into the second product as the sum of two
 // numbers of the values' type, the rounded weight and what the rounding left, so that the
 // result is rounded once; that doubles the second product, which the memory hides.
+//
+// f32 goes the same way by eights of keys (m16n8k8, TF32). A factor x of either product is taken as
+// hi, its 11 leading bits, and lo, the next 11, and hi hi' + hi lo' + lo hi' is summed: what is left
+// out is 2^-20 of a product at most, and less on average; f32 sums of 128 products may be off by
+// 2^-17 of them. A factor that is not finite has no such parts: scores that come out as NaN are made
+// anew by plain products, and values are looked through at every step. 32 sequences of up to 8000 keys, 64 heads on 8 of 128,
+// take 222 us (4.1 TB/s), bound by the instructions' latency at two warps a scheduler; 32-bit FMA
+// from shared memory took 735.
 //
 // Several queries' heads make more rows, 16 to a pair of their own, so each of their groups of 16
 // reads the keys again, from L2. What some row of a step must not see has weight 0 there; values
@@ -640,9 +647,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
       }
       const int key = first_key(i);
       const bool masked = !all_seen(key);
-      if (sizeof(T) == 4 || (MANY && masked)) {
-        bool any = false;
+      bool look = MANY && masked;
+      if constexpr (sizeof(T) == 4) {
+        // 0 times a number that is not finite is NaN
+        pg::Two none(0.0f, 0.0f);
+        const pg::Two zero(0.0f, 0.0f);
 #pragma unroll
+        for (int j = lane; j < R::step * R::chunks; j += 32) {
+          const float4 x = *reinterpret_cast<const float4 *>(
+              ring + (i % R::stages) * R::stage + R::tile + j * 16);
+          none = fma(pg::Two(x.x, x.y), zero, none);
+          none = fma(pg::Two(x.z, x.w), zero, none);
+        }
+        float x, y;
+        none.get(x, y);
+        look = __any_sync(0xffffffffu, x + y != 0.0f);
+      }
+      if (look) {
+        bool any = false;
         for (int j = lane; j < R::step * R::chunks; j += 32) {
           uint4 *const at =
               reinterpret_cast<uint4 *>(ring + (i % R::stages) * R::stage + R::tile + j * 16);
@@ -777,11 +799,17 @@ namespace pg {
 // 32 rows 56 and 84, 48 rows 60 and 84, 64 rows 70 and 96; 32 of up to 8000 on 8, 16 rows 74 and
 // 157, 32 rows 119 and 158, 48 rows 155 and 160, 64 rows 191 and 160; 100 of up to 500 on 4, 48
 // rows 51 and 49, 64 rows 63 and 50.
-bool decode_takes(const Attention &a, int max_len) {
+// f32 has no such tiles, so it is taken at up to 256 rows, and at up to 1024 where most keys are
+// seen by all of a sequence's queries, since a group of 16 rows goes through all that any sees. This
+// against attention.cu: 8 sequences on 4 kv heads of 128, up to 4056 keys, 64 rows 72 and 164, 256
+// rows 207 and 390, 1024 rows 760 and 1270; of no other keys than the queries, 256 rows 12 and 17,
+// 512 rows 25 and 17; with a window of 100 and heads of 64, 256 rows 27 and 32, 512 rows 45 and 34.
+bool decode_takes(const Attention &a, bool f32, int most, int max_len) {
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
-  if (a.starts && rows > 48ll * a.batch) return false;
+  const bool early = !a.window && max_len / 8ll * a.batch >= a.queries;
+  if (a.starts && rows > (f32 ? early ? 1024ll : 256ll : 48ll) * a.batch) return false;
   // its blocks of 32 keys or more count in 31 bits
-  return (rows / kRows + a.batch) * a.heads * (max_len / 32 + 2ll + kPair) < INT32_MAX;
+  return (rows / kRows + a.batch) * a.heads * (most / 32 + 2ll + kPair) < INT32_MAX;
 }
 
 int decode(const Attention &a, int dtype, int sms, cudaStream_t stream) {
