@@ -19,10 +19,12 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-// Four small blocks an SM, not two large ones: one's sums and selection meet the others' loads
-// (4096 x 50257 in bf16: 85 us against 110).
-constexpr int kThreads = 256, kPerSm = 4;
-constexpr int kWarps = kThreads / 32;
+// Small blocks, not a few large ones: one's sums and selection meet the others' loads (four of 256
+// threads an SM against two of 512, 4096 x 50257 in bf16: 85 us against 110).
+constexpr int kOnSm = 1024;          // threads of the forward kernel that an SM holds
+// Threads of the gradient's blocks: short rows leave less of a small one idle (forward and gradient
+// of 3682 x 1718 in f16: 20.5 us with 128, 25.7 with 256; 4096 x 50257 in bf16: 207 and 209).
+constexpr int kThreads = 128;
 constexpr int kBatch = 4;            // 16-byte loads a thread has in flight
 constexpr int kTopMax = PG_LOGPROB_TOP;
 constexpr int kParts = 8;            // blocks a row is cut in at most (a portable cluster)
@@ -176,7 +178,7 @@ __device__ __forceinline__ uint64_t entry_of(float x, int column) {
 }
 
 // One block's part of a row, columns [first, last): thread i takes the 16-byte vectors i, i +
-// kThreads, ... of the part that are aligned, counted from the aligned address at or below its
+// THREADS, ... of the part that are aligned, counted from the aligned address at or below its
 // start; columns outside the part read as -inf.
 template <class T>
 struct Part {
@@ -204,15 +206,16 @@ struct Part {
   }
 };
 
+template <int THREADS>
 struct Shared {
-  Sums warp[kWarps];
+  Sums warp[THREADS / 32];
   Sums row;                          // the part's sums
   Sums part[kParts];                 // the parts' sums
-  uint32_t chosen[kThreads];         // the threads whose strips are looked at again
+  uint32_t chosen[THREADS];         // the threads whose strips are looked at again
   uint64_t found[kCandidates];
   uint64_t top[kTopMax];             // the part's top entries, best first; 0 where there is none
   uint64_t best;
-  uint64_t warp_best[kWarps];
+  uint64_t warp_best[THREADS / 32];
   int chosen_n, found_n;
 };
 
@@ -222,8 +225,9 @@ struct Shared {
 // L2, a warp to a strip, one load a lane where a strip is short), and what reaches T is ranked by
 // counting. Where more than kCandidates reach it (many equal logits), the entries are taken one
 // at a time instead, each the largest below the last.
-template <class T>
-__device__ void select_top(const Part<T> &part, float mine, bool any, int k, Shared &sh) {
+template <class T, int THREADS>
+__device__ void select_top(const Part<T> &part, float mine, bool any, int k,
+                           Shared<THREADS> &sh) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t key = any ? key_of(mine) : 0;
   if (tid == 0) sh.chosen_n = sh.found_n = 0;
@@ -240,8 +244,8 @@ __device__ void select_top(const Part<T> &part, float mine, bool any, int k, Sha
   if (any && key >= t) sh.chosen[atomicAdd(&sh.chosen_n, 1)] = tid;
   __syncthreads();
   const int strips = sh.chosen_n;
-  for (int c = warp; c < strips; c += kWarps)
-    for (int v = sh.chosen[c] + lane * kThreads; v < part.vectors; v += 32 * kThreads) {
+  for (int c = warp; c < strips; c += THREADS / 32)
+    for (int v = sh.chosen[c] + lane * THREADS; v < part.vectors; v += 32 * THREADS) {
       float x[Vec<T>::n];
       part.load(v, x);
       const int at = part.base + v * Vec<T>::n;
@@ -255,7 +259,7 @@ __device__ void select_top(const Part<T> &part, float mine, bool any, int k, Sha
   __syncthreads();
   const int n = sh.found_n;
   if (n <= kCandidates) {
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid; i < n; i += THREADS) {
       const uint64_t e = sh.found[i];
       int rank = 0;
       for (int j = 0; j < n; ++j) rank += sh.found[j] > e;
@@ -267,7 +271,7 @@ __device__ void select_top(const Part<T> &part, float mine, bool any, int k, Sha
   uint64_t below = ~0ull;
   for (int r = 0; r < k; ++r) {
     uint64_t best = 0;
-    for (int v = tid; v < part.vectors; v += kThreads) {
+    for (int v = tid; v < part.vectors; v += THREADS) {
       float x[Vec<T>::n];
       part.load(v, x);
       const int at = part.base + v * Vec<T>::n;
@@ -285,7 +289,7 @@ __device__ void select_top(const Part<T> &part, float mine, bool any, int k, Sha
     if (lane == 0) sh.warp_best[warp] = best;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 1; w < kWarps; ++w) best = sh.warp_best[w] > best ? sh.warp_best[w] : best;
+      for (int w = 1; w < THREADS / 32; ++w) best = sh.warp_best[w] > best ? sh.warp_best[w] : best;
       sh.best = sh.top[r] = best;
     }
     __syncthreads();
@@ -296,15 +300,15 @@ __device__ void select_top(const Part<T> &part, float mine, bool any, int k, Sha
 }
 
 // One cluster of blocks a row; block r of it takes the r-th part. At many rows the instructions a
-// logit costs bound it, close to HBM's time for reading each once: 4096 x 50257 in bf16 take 85 us
-// (4.8 TB/s), 1000 x 128256 with the top 20 68 us (3.8 TB/s). At few rows the parts keep all SMs
+// logit costs bound it, close to HBM's time for reading each once: 4096 x 50257 in bf16 take 80 us
+// (5.1 TB/s), 1000 x 128256 with the top 20 68 us (3.8 TB/s). At few rows the parts keep all SMs
 // reading and latency bounds it: 4 x 32001 in f32 with the top 5 take 8 us.
-template <class T>
-__global__ void __launch_bounds__(kThreads, kPerSm)
+template <class T, int THREADS>
+__global__ void __launch_bounds__(THREADS, kOnSm / THREADS)
     logprobs_kernel(const T *logits, int64_t row_stride, const void *tokens, int token_bytes,
                     int vocab, int top, float *logp, float *entropy, float2 *norm,
                     float *top_logp, int32_t *top_ids) {
-  __shared__ Shared sh;
+  __shared__ Shared<THREADS> sh;
   pg::wait_for_earlier_kernels();
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), rank = cluster.block_rank();
@@ -317,28 +321,28 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   int v = tid;
   // whole batches, the next one's loads on their way while one is added up
   const auto batch_here = [&](int at) {
-    return at + (kBatch - 1) * kThreads < part.vectors && part.whole(at) &&
-           part.whole(at + (kBatch - 1) * kThreads);
+    return at + (kBatch - 1) * THREADS < part.vectors && part.whole(at) &&
+           part.whole(at + (kBatch - 1) * THREADS);
   };
   const T *const vectors = part.row + part.base;
   if (v < part.vectors && !part.whole(v)) {  // the first vector may start before the part
     float x[Vec<T>::n];
     part.load(v, x);
     add<Vec<T>::n>(mine, x);
-    v += kThreads;
+    v += THREADS;
   }
   if (batch_here(v)) {
     uint4 raw[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
-      raw[u] = pg::load16(vectors + static_cast<int64_t>(v + u * kThreads) * Vec<T>::n);
+      raw[u] = pg::load16(vectors + static_cast<int64_t>(v + u * THREADS) * Vec<T>::n);
     for (bool more = true; more;) {
-      v += kBatch * kThreads;
+      v += kBatch * THREADS;
       more = batch_here(v);
       uint4 next[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (more) next[u] = pg::load16(vectors + static_cast<int64_t>(v + u * kThreads) * Vec<T>::n);
+        if (more) next[u] = pg::load16(vectors + static_cast<int64_t>(v + u * THREADS) * Vec<T>::n);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         float x[Vec<T>::n];
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       }
     }
   }
-  for (; v < part.vectors; v += kThreads) {
+  for (; v < part.vectors; v += THREADS) {
     float x[Vec<T>::n];
     part.load(v, x);
     add<Vec<T>::n>(mine, x);
@@ -368,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
   if (lane == 0) sh.warp[warp] = all;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) all = join(all, sh.warp[w]);
+    for (int w = 1; w < THREADS / 32; ++w) all = join(all, sh.warp[w]);
     sh.row = all;
   }
   if (top) select_top(part, largest, any, top, sh);
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     cluster.sync();
     if (rank == 0) {
       if (tid < parts) sh.part[tid] = cluster.map_shared_rank(&sh, tid)->row;
-      for (int i = tid; i < parts * top; i += kThreads)
+      for (int i = tid; i < parts * top; i += THREADS)
         sh.found[i] = cluster.map_shared_rank(&sh, i / top)->top[i % top];
     }
     cluster.sync();
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     entropy[row] = none ? NAN : log_s - kLn2 * (r.t / r.s);
     norm[row] = make_float2(r.m, log_s);
   }
-  for (int i = tid; i < parts * top; i += kThreads) {
+  for (int i = tid; i < parts * top; i += THREADS) {
     const uint64_t e = sh.found[i];
     int place = 0;
     for (int j = 0; j < parts * top; ++j) place += sh.found[j] > e;
@@ -491,21 +495,18 @@ __global__ void __launch_bounds__(kThreads)
     if (at >= 0 && at < vocab) grad_one(at);
 }
 
-template <class T>
-int run_logprobs(uint64_t logits, int64_t row_stride, uint64_t tokens, int token_bytes, int rows,
-                 int vocab, int top, uint64_t logp, uint64_t entropy, uint64_t norm,
-                 uint64_t top_logp, uint64_t top_ids, cudaStream_t stream) {
-  int sms;
-  int rc = pg::sm_count(&sms);
-  if (rc) return rc;
+template <class T, int THREADS>
+int launch_logprobs(uint64_t logits, int64_t row_stride, uint64_t tokens, int token_bytes,
+                    int rows, int vocab, int top, int sms, uint64_t logp, uint64_t entropy,
+                    uint64_t norm, uint64_t top_logp, uint64_t top_ids, cudaStream_t stream) {
   // blocks a row: as many as the SMs hold at once, up to a portable cluster, and no part
   // shorter than one batch of a block's loads
   int parts = 1;
-  const int least = kThreads * Vec<T>::n;
-  while (parts < kParts && rows * 2ll * parts <= kPerSm * sms && vocab / (2 * parts) >= least) parts *= 2;
+  const int least = THREADS * Vec<T>::n, most = kOnSm / THREADS * sms;
+  while (parts < kParts && rows * 2ll * parts <= most && vocab / (2 * parts) >= least) parts *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -515,12 +516,30 @@ int run_logprobs(uint64_t logits, int64_t row_stride, uint64_t tokens, int token
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   cudaError_t e = cudaLaunchKernelEx(
-      &cfg, logprobs_kernel<T>, reinterpret_cast<const T *>(logits), row_stride,
+      &cfg, logprobs_kernel<T, THREADS>, reinterpret_cast<const T *>(logits), row_stride,
       reinterpret_cast<const void *>(tokens), token_bytes, vocab, top,
       reinterpret_cast<float *>(logp), reinterpret_cast<float *>(entropy),
       reinterpret_cast<float2 *>(norm), reinterpret_cast<float *>(top_logp),
       reinterpret_cast<int32_t *>(top_ids));
   return e == cudaSuccess ? PG_OK : pg::runtime_fail(e, "logprobs_kernel");
+}
+
+template <class T>
+int run_logprobs(uint64_t logits, int64_t row_stride, uint64_t tokens, int token_bytes, int rows,
+                 int vocab, int top, uint64_t logp, uint64_t entropy, uint64_t norm,
+                 uint64_t top_logp, uint64_t top_ids, cudaStream_t stream) {
+  int sms;
+  int rc = pg::sm_count(&sms);
+  if (rc) return rc;
+  // Blocks of 128 threads where they fill the GPU, since a row's sums are joined sooner, but not
+  // where the top entries of long rows are asked for: a thread's strip is read again for each it
+  // may hold. 128 against 256, in microseconds: 3682 x 1718 with the gradient 26 and 32, 4096 x 50257
+  // 207 and 213, 600 x 2000 9.2 and 8.8; with top entries 4000 x 25000 56 and 70, 3000 x 32000 62 and
+  // 72, 1500 x 64000 67 and 57, 300 x 8000 11.6 and 9.1.
+  const auto launch = rows > 8 * sms && (!top || vocab <= 32768) ? launch_logprobs<T, 128>
+                                                                 : launch_logprobs<T, 256>;
+  return launch(logits, row_stride, tokens, token_bytes, rows, vocab, top, sms, logp, entropy, norm,
+                top_logp, top_ids, stream);
 }
 
 template <class T>
