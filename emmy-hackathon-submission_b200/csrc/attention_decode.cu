@@ -16,9 +16,10 @@
 // result is rounded once; that doubles the second product, which the memory hides.
 //
 // f32 goes the same way by eights of keys (m16n8k8, TF32). A factor x of either product is taken as
-// hi, its 11 leading bits, and lo, the next 11, and hi hi' + hi lo' + lo hi' is summed: what is left
-// out is 2^-20 of a product at most, and less on average; f32 sums of 128 products may be off by
-// 2^-17 of them. A factor that is not finite has no such parts: scores that come out as NaN are made
+// hi, 11 bits of it, and lo, 11 bits of the rest, and hi hi' + hi lo' + lo hi' is summed. Left out
+// are lo lo' and the roundings of lo: up to 2^-22 and 2^-23 of a product, of either sign, since lo is
+// rounded and one factor's hi too (with both cut off, scores were off by 2^-23 of themselves all the
+// same way, and the result four times as far as by f32 sums). A factor that is not finite has no such parts: scores that come out as NaN are made
 // anew by plain products, and values are looked through at every step. 32 sequences of up to 8000 keys, 64 heads on 8 of 128,
 // take 222 us (4.1 TB/s), bound by the instructions' latency at two warps a scheduler; 32-bit FMA
 // from shared memory took 735.
@@ -98,10 +99,20 @@ template <> struct Mma<float> {
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
   }
-  // the 11 leading bits of a number, and the next 11
+  __device__ static uint32_t nearest(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+  }
+  // a key or value: the 11 leading bits, which the largest number has too, and what is left
   __device__ static void split(float x, uint32_t &hi, uint32_t &lo) {
     hi = __float_as_uint(x) & 0xffffe000u;
-    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+    lo = nearest(x - __uint_as_float(hi));
+  }
+  // a query's number or a weight: rounded, so that what is left has either sign
+  __device__ static void split_near(float x, uint32_t &hi, uint32_t &lo) {
+    hi = nearest(x);
+    lo = nearest(x - __uint_as_float(hi));
   }
 };
 
@@ -497,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          Mma<T>::split(__uint_as_float(q_word(k, e & 1, e >> 1)), hi[e], lo[e]);
+          Mma<T>::split_near(__uint_as_float(q_word(k, e & 1, e >> 1)), hi[e], lo[e]);
         q_hi[32 * k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         q_lo[32 * k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
@@ -712,8 +723,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
           const float y = pg::exp2_fast(s[n][2 * h + 1] - base[h]);
           l[h] += x + y;
           if constexpr (sizeof(T) == 4) {
-            Mma<T>::split(x, hi[h], lo[h]);  // the product's keys are 0, 2, 4, 6, 1, 3, 5, 7
-            Mma<T>::split(y, hi[2 + h], lo[2 + h]);
+            Mma<T>::split_near(x, hi[h], lo[h]);  // the product's keys are 0, 2, 4, 6, 1, 3, 5, 7
+            Mma<T>::split_near(y, hi[2 + h], lo[2 + h]);
           } else {
             Mma<T>::split(x, y, hi[2 * n + h], lo[2 * n + h]);
           }
