@@ -18,10 +18,12 @@
 // f32 goes the same way by eights of keys (m16n8k8, TF32). A factor x of either product is taken as
 // hi, 11 bits of it, and lo, 11 bits of the rest, and hi hi' + hi lo' + lo hi' is summed. Left out
 // are lo lo' and the roundings of lo: up to 2^-22 and 2^-23 of a product, of either sign, since lo is
-// rounded and one factor's hi too (with both cut off, scores were off by 2^-23 of themselves all the
-// same way, and the result four times as far as by f32 sums). A factor that is not finite has no such parts: scores that come out as NaN are made
-// anew by plain products, and values are looked through at every step. 32 sequences of up to 8000 keys, 64 heads on 8 of 128,
-// take 222 us (4.1 TB/s), bound by the instructions' latency at two warps a scheduler; 32-bit FMA
+// rounded and one factor's hi too. A step's weighted values are summed apart and then added in f32:
+// the tensor cores do not round their sums to nearest, and over 1000s of steps that alone put
+// results 5e-6 off (24 sequences of up to 40000 keys; 3.3e-7 so, 4.2e-7 by f32 FMA). A factor that
+// is not finite has no two parts: scores that come out as NaN are made anew by plain products, and
+// values are looked through at every step. 32 sequences of up to 8000 keys, 64 heads on 8 of 128,
+// take 265 us (3.4 TB/s), bound by the instructions' latency at two warps a scheduler; 32-bit FMA
 // from shared memory took 735.
 //
 // Several queries' heads make more rows, 16 to a pair of their own, so each of their groups of 16
@@ -739,9 +741,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
             Mma<T>::split(
                 *reinterpret_cast<const float *>(v + R::at(2 * t4 + e, 2 * n + (g >> 2))),
                 v_hi[e], v_lo[e]);
-          Mma<T>::run(o[n], hi, v_hi);
-          Mma<T>::run(o[n], hi, v_lo);
-          Mma<T>::run(o[n], lo, v_hi);
+          // a step's products by themselves: the tensor cores do not round their sums to nearest, and
+          // thousands of steps would add those errors up
+          float sum[4] = {};
+          Mma<T>::run(sum, hi, v_lo);
+          Mma<T>::run(sum, lo, v_hi);
+          Mma<T>::run(sum, hi, v_hi);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][e] += sum[e];
         }
       } else {
 #pragma unroll
@@ -812,9 +819,9 @@ namespace pg {
 // rows 51 and 49, 64 rows 63 and 50.
 // f32 has no such tiles, so it is taken at up to 256 rows, and at up to 1024 where most keys are
 // seen by all of a sequence's queries, since a group of 16 rows goes through all that any sees. This
-// against attention.cu: 8 sequences on 4 kv heads of 128, up to 4056 keys, 64 rows 72 and 164, 256
-// rows 207 and 390, 1024 rows 760 and 1270; of no other keys than the queries, 256 rows 12 and 17,
-// 512 rows 25 and 17; with a window of 100 and heads of 64, 256 rows 27 and 32, 512 rows 45 and 34.
+// against attention.cu: 8 sequences on 4 kv heads of 128, up to 4056 keys, 64 rows 86 and 164, 256
+// rows 253 and 390, 1024 rows 947 and 1270; of no other keys than the queries, 256 rows 13 and 17,
+// 512 rows 25 and 17; with a window of 100 and heads of 64, 256 rows 28 and 32, 512 rows 45 and 34.
 bool decode_takes(const Attention &a, bool f32, int most, int max_len) {
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
   const bool early = !a.window && max_len / 8ll * a.batch >= a.queries;
