@@ -374,7 +374,8 @@ struct Plan {
 
 // MANY: sequences have any number of queries, not one each.
 template <class T, int DIM, bool MANY>
-__global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_constant__ Attention a) {
+__global__ void __launch_bounds__(kThreads, kPerSm)
+    decode_kernel(const __grid_constant__ Attention a) {
   using R = Ring<T, DIM>;
   extern __shared__ float4 smem4[];
   __shared__ uint3 warp_sum[kWarps];
@@ -527,9 +528,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) decode_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
 
-    // The warp's steps are the blocks' 16 keys at 16 warp (f32: 8 at 8 warp). A step whose keys all are seen and lie
-    // in one page, as they do where pages are whole groups of so many, needs one look at the table and
-    // one address; else lane r knows key r's page and row.
+    // The warp's steps are the blocks' 16 keys at 16 warp (f32: 8 at 8 warp). A step whose keys all
+    // are seen and lie in one page, as they do where pages are whole groups of so many, needs one
+    // look at the table and one address; else lane r knows key r's page and row.
     const int steps = block1 - block0;
     const bool whole_pages = a.page_size % R::step == 0;
     const auto first_key = [&](int i) {
