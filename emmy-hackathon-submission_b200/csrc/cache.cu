@@ -7,7 +7,9 @@
 //
 // extend and fork are planned by one block (cache_extend, cache_fork_plan): it checks every
 // request before it changes anything, so a request that cannot be met (no pages, a bad or
-// repeated slot) sets a bit of the status word and leaves the cache as it was. The bulk of the
+// repeated slot) sets a bit of the status word and leaves the cache as it was. Its write is queued
+// all the same, and would go to the slots' older tokens: so extend marks each of its slots as
+// refused or not, and write leaves out the marked ones. The bulk of the
 // work (rows of keys and values, table rows, counts) is done by a second kernel over the whole
 // GPU that the plan's scratch array drives.
 #include "common.cuh"
@@ -92,6 +94,9 @@ __device__ __forceinline__ int *refs_of(const pg_cache &c) {
 __device__ __forceinline__ int *lens_of(const pg_cache &c) {
   return reinterpret_cast<int *>(c.lens);
 }
+__device__ __forceinline__ int *refused_of(const pg_cache &c) {
+  return reinterpret_cast<int *>(c.refused);
+}
 __device__ __forceinline__ int *row_of(const pg_cache &c, int slot) {
   return reinterpret_cast<int *>(c.table) + slot * c.table_stride;
 }
@@ -152,8 +157,11 @@ __global__ void __launch_bounds__(kPlan) cache_extend(pg_cache c, const int *slo
     __syncthreads();
   }
   if (bad) {
-    for (int i = threadIdx.x; i < n; i += kPlan)
-      if (length[i] >= 0) lens[slots_in[i]] = length[i];
+    for (int i = threadIdx.x; i < n; i += kPlan) {
+      const int slot = slots_in[i];
+      if (length[i] >= 0) lens[slot] = length[i];
+      if (slot >= 0 && slot < c.slots) refused_of(c)[slot] = 1;
+    }
     if (threadIdx.x == 0) set_status(c, bad);
     return;
   }
@@ -166,8 +174,10 @@ __global__ void __launch_bounds__(kPlan) cache_extend(pg_cache c, const int *slo
     row_of(c, slots_in[lo])[ceil_div(length[lo], c.page_size) + r - offset[lo]] = fresh[r];
     refs[fresh[r]] = 1;
   }
-  for (int i = threadIdx.x; i < n; i += kPlan)
+  for (int i = threadIdx.x; i < n; i += kPlan) {
     lens[slots_in[i]] = length[i] + starts[i + 1] - starts[i];
+    refused_of(c)[slots_in[i]] = 0;
+  }
 }
 
 // --- write: new rows of one layer into the slots' pages ----------------------------------------
@@ -198,6 +208,10 @@ __global__ void __launch_bounds__(kCopy) cache_write(pg_cache c, int layer, cons
     const int slot = slots_in[i];
     if (slot < 0 || slot >= c.slots) {
       if (lane == 0) set_status(c, PG_CACHE_BAD_SLOT);
+      continue;
+    }
+    if (refused_of(c)[slot]) {
+      if (lane == 0) set_status(c, PG_CACHE_REFUSED);
       continue;
     }
     const int pos = lens_of(c)[slot] - (starts[i + 1] - t);
@@ -246,7 +260,10 @@ __global__ void __launch_bounds__(kCopy) cache_free(pg_cache c, const int *slots
       continue;
     }
     // the exchange gives a slot listed twice to one block only
-    if (threadIdx.x == 0) held = atomicExch(lens_of(c) + slot, 0);
+    if (threadIdx.x == 0) {
+      held = atomicExch(lens_of(c) + slot, 0);
+      refused_of(c)[slot] = 0;
+    }
     __syncthreads();
     const int count = min(ceil_div(held, c.page_size), c.width);
     int *row = row_of(c, slot);
@@ -354,7 +371,10 @@ __global__ void __launch_bounds__(kPlan) cache_fork_plan(pg_cache c, const int *
     return;
   }
   for (int r = threadIdx.x; r < need; r += kPlan) refs[fresh[r]] = 1;
-  for (int i = threadIdx.x; i < n; i += kPlan) lens[children[i]] = lens[parents[i]];
+  for (int i = threadIdx.x; i < n; i += kPlan) {
+    lens[children[i]] = lens[parents[i]];
+    refused_of(c)[children[i]] = 0;
+  }
 }
 
 // Task i * (2 layers + 1) + j: child i's table row and counts (j = 0), or the rows in use of its
@@ -490,6 +510,15 @@ int check_list(const char *what, const pg_cache *c, uint64_t a, uint64_t b, int 
   return PG_OK;
 }
 
+// ... of slots, by the calls that set, read or clear their marks.
+int check_slots(const char *what, const pg_cache *c, uint64_t a, uint64_t b, int n) {
+  int rc = check_list(what, c, a, b, n, c ? c->slots : 0);
+  if (rc) return rc;
+  if (n && (!c->refused || c->refused & 3))
+    return pg::argument_fail("%s: the slots' marks are null or not 4-byte aligned", what);
+  return PG_OK;
+}
+
 int check_rows(const char *what, const pg_rows *r) {
   if (!r || !r->data) return pg::argument_fail("%s: null rows", what);
   if ((r->data | static_cast<uint64_t>(r->token_stride | r->head_stride)) & 15)
@@ -518,7 +547,7 @@ inline const int *ints(uint64_t p) {
 
 extern "C" int pg_cache_extend(const pg_cache *c, uint64_t slots, uint64_t starts, int32_t n,
                                uint64_t stream) {
-  int rc = check_list("pg_cache_extend", c, slots, starts, n, c ? c->slots : 0);
+  int rc = check_slots("pg_cache_extend", c, slots, starts, n);
   if (rc || !n) return rc;
   return pg::launch<cache_extend>("cache_extend", dim3(1), kPlan, 0, stream_of(stream), *c,
                     ints(slots), ints(starts), n);
@@ -527,7 +556,7 @@ extern "C" int pg_cache_extend(const pg_cache *c, uint64_t slots, uint64_t start
 extern "C" int pg_cache_write(const pg_cache *c, int32_t layer, uint64_t slots, uint64_t starts,
                               int32_t n, int32_t tokens, const pg_rows *k, const pg_rows *v,
                               uint64_t stream) {
-  int rc = check_list("pg_cache_write", c, slots, starts, n, c ? c->slots : 0);
+  int rc = check_slots("pg_cache_write", c, slots, starts, n);
   if (rc) return rc;
   if (layer < 0 || layer >= c->layers || tokens < 0)
     return pg::argument_fail("pg_cache_write: layer %d of %d, %d tokens", layer, c->layers,
@@ -541,7 +570,7 @@ extern "C" int pg_cache_write(const pg_cache *c, int32_t layer, uint64_t slots, 
 }
 
 extern "C" int pg_cache_free(const pg_cache *c, uint64_t slots, int32_t n, uint64_t stream) {
-  int rc = check_list("pg_cache_free", c, slots, slots, n, c ? c->slots : 0);
+  int rc = check_slots("pg_cache_free", c, slots, slots, n);
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(n, &grid))) return rc;
@@ -561,7 +590,7 @@ extern "C" int pg_cache_copy(const pg_cache *c, uint64_t from, uint64_t to, int3
 
 extern "C" int pg_cache_fork(const pg_cache *c, uint64_t parents, uint64_t children, int32_t n,
                              uint64_t stream) {
-  int rc = check_list("pg_cache_fork", c, parents, children, n, c ? c->slots : 0);
+  int rc = check_slots("pg_cache_fork", c, parents, children, n);
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(static_cast<int64_t>(n) * (2 * c->layers + 1), &grid))) return rc;

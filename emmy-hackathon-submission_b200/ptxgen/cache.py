@@ -15,7 +15,9 @@
 ``ptxgen.attention`` reads the cache's ``k``, ``v``, ``table`` and ``lens``. Slots, starts and page
 ids are int32 device tensors, and nothing here waits for the GPU but ``check``: what only the
 device can see (no page left, a slot listed twice) sets bits of ``status``, and an ``extend`` or
-``fork`` that cannot be met changes nothing. Calls run on the current stream, or on ``stream``
+``fork`` that cannot be met changes nothing. A ``write`` that was queued behind a refused ``extend``
+leaves out that call's slots, since their last tokens are older ones, until an ``extend`` of them is
+met (by no tokens, if need be) or they are freed. Calls run on the current stream, or on ``stream``
 (a ``cudaStream_t`` as an integer); a cache's calls belong on one stream at a time.
 """
 
@@ -29,12 +31,13 @@ import torch
 from .launch import call, int32_list
 from .runtime import Cache, LaunchError, Rows, library
 
-NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG, WAIT = 1, 2, 4, 8, 16
+NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG, WAIT, REFUSED = 1, 2, 4, 8, 16, 32
 _WHY = {NO_PAGES: "fewer free pages than a call needed",
         BAD_SLOT: "a slot out of range, listed twice, or a fork's child in use",
         BAD_PAGE: "a page id or count out of range",
         TOO_LONG: "more tokens than a table row has pages for",
-        WAIT: "a bounded wait inside an attention kernel gave up"}
+        WAIT: "a bounded wait inside an attention kernel gave up",
+        REFUSED: "rows of a slot whose last extend could not be met were not written"}
 
 
 class CacheError(LaunchError):
@@ -70,11 +73,12 @@ class PagedCache:
         words = 4 + 3 * pages + 2 * slots + 2
         self._scratch = torch.empty(words, dtype=torch.int32, device=k.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._refused = torch.zeros(slots, dtype=torch.int32, device=k.device)
         self._c = Cache(
             k.data_ptr(), v.data_ptr(), k.stride(0) * size, k.stride(1) * size,
             k.stride(2) * size, int32_list("refs", refs, k.device, pages), table.data_ptr(),
             int32_list("lens", lens, k.device, slots), self.status.data_ptr(),
-            self._scratch.data_ptr(), max(table.stride(0), width), words, layers, pages, heads,
+            self._scratch.data_ptr(), self._refused.data_ptr(), max(table.stride(0), width), words, layers, pages, heads,
             page_size, dim * size, slots, width)
         self._ref = ctypes.byref(self._c)
         self._lib = library()

@@ -44,7 +44,8 @@ class Cache(ctypes.Structure):
 
     _fields_ = [*((n, ctypes.c_uint64) for n in ("k", "v")),
                 *((n, ctypes.c_int64) for n in ("layer_stride", "page_stride", "head_stride")),
-                *((n, ctypes.c_uint64) for n in ("refs", "table", "lens", "status", "scratch")),
+                *((n, ctypes.c_uint64) for n in ("refs", "table", "lens", "status", "scratch",
+                                                 "refused")),
                 *((n, ctypes.c_int64) for n in ("table_stride", "scratch_words")),
                 *((n, ctypes.c_int32) for n in ("layers", "pages", "heads", "page_size",
                                                 "row_bytes", "slots", "width"))]

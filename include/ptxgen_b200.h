@@ -194,14 +194,18 @@ int pg_grid_sum_f32_noalloc(uint64_t x, uint64_t n, uint64_t out, uint32_t block
  * The calls are asynchronous on `stream` and never wait for the host. What only the device can
  * see (no page left, a slot listed twice, a page id out of range) sets PG_CACHE_* bits of the
  * status word, which the caller clears: extend and fork then change nothing, free, write and
- * copy skip the entry. All calls on one cache share its scratch words and so belong on one
- * stream at a time. */
+ * copy skip the entry. An extend that could not be met also marks its slots in `refused`, and write
+ * leaves out the rows of a marked slot (PG_CACHE_REFUSED): they have no place, and the slot's last
+ * positions hold older tokens, in pages that other slots may share. The slot's next extend that is
+ * met (by no tokens, if need be), a free of it or a fork into it clears the mark. All calls on one
+ * cache share its scratch words and so belong on one stream at a time. */
 typedef struct pg_cache {
   uint64_t k, v;                                    /* device addresses, 16-byte aligned */
   int64_t layer_stride, page_stride, head_stride;   /* bytes, multiples of 16 */
   uint64_t refs, table, lens;                       /* int32: [pages], [slots, width], [slots] */
   uint64_t status;                                  /* one uint32 */
   uint64_t scratch;                                 /* int32[scratch_words], any contents */
+  uint64_t refused;                                 /* int32[slots], zeroed once */
   int64_t table_stride, scratch_words;              /* words */
   int32_t layers, pages, heads, page_size;
   int32_t row_bytes;                                /* one token's keys of one head */
@@ -221,6 +225,7 @@ typedef struct pg_rows {
 #define PG_CACHE_BAD_SLOT 2u /* a slot out of range, listed twice, or a fork's child in use */
 #define PG_CACHE_BAD_PAGE 4u /* a page id or count that cannot be */
 #define PG_CACHE_TOO_LONG 8u /* more tokens than a table row has pages for */
+#define PG_CACHE_REFUSED 32u /* rows for a slot whose last extend could not be met: not written */
 
 /* Makes room for the new tokens of n sequences: slots[i] grows by starts[i + 1] - starts[i]
  * tokens (starts: n + 1 ascending int32 on the device), taking pages as needed. */
@@ -228,7 +233,8 @@ int pg_cache_extend(const pg_cache *cache, uint64_t slots, uint64_t starts, int3
                     uint64_t stream);
 
 /* Writes one layer's rows of the last tokens of n sequences: token t of the `tokens` rows, with
- * starts[i] <= t < starts[i + 1], lands at position lens[slots[i]] - starts[i + 1] + t. */
+ * starts[i] <= t < starts[i + 1], lands at position lens[slots[i]] - starts[i + 1] + t. Rows of a
+ * slot whose last extend could not be met are left out. */
 int pg_cache_write(const pg_cache *cache, int32_t layer, uint64_t slots, uint64_t starts,
                    int32_t n, int32_t tokens, const pg_rows *k, const pg_rows *v,
                    uint64_t stream);
