@@ -5,7 +5,7 @@
 // pages takes the lowest free ones, in the order of its slots, so results never depend on
 // timing. Everything happens on the device in stream order: no operation waits for the host.
 //
-// extend and fork are planned by one block (cache_extend, cache_fork_plan): it checks every
+// extend and fork are planned by one block (of cache_extend, cache_fork_plan): it checks every
 // request before it changes anything, so a request that cannot be met (no pages, a bad or
 // repeated slot) sets a bit of the status word and leaves the cache as it was. Its write is queued
 // all the same, and would go to the slots' older tokens: so extend marks each of its slots as
@@ -14,9 +14,16 @@
 // GPU that the plan's scratch array drives.
 #include "common.cuh"
 
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
 namespace {
 
 constexpr int kPlan = 1024;   // threads of a planning block
+// Blocks that look through the parents' table rows before a fork is planned (250 children of parents
+// of up to 700 tokens in 24 layers: 120 us with 8, 125 with 1; of up to 30000 in one layer: 39, 49).
+constexpr int kLook = 8;
 constexpr int kCopy = 256;    // threads of a copying block
 // Copying blocks an SM gets at most, eight times what it holds: a block that ends makes room for
 // the next, which spreads the copies better than blocks that stay and loop in step. With 8, 64 and
@@ -320,16 +327,44 @@ __global__ void __launch_bounds__(kCopy) cache_copy(pg_cache c, const int *from,
 
 // --- fork: children that share their parents' full pages ---------------------------------------
 
-__global__ void __launch_bounds__(kPlan) cache_fork_plan(pg_cache c, const int *parents,
-                                                         const int *children, int n) {
+// Whether a page id that a parent's row holds within its length is out of range; a warp takes a row.
+__device__ bool bad_rows(const pg_cache &c, const int *parents, int n, int warp, int warps) {
+  constexpr int kAhead = 4;  // entries a lane has in flight
+  const int lane = threadIdx.x & 31;
+  bool bad = false;
+  for (int i = warp; i < n; i += warps) {
+    const int parent = parents[i];
+    if (parent < 0 || parent >= c.slots) continue;
+    const int *row = row_of(c, parent);
+    const int count = min(ceil_div(lens_of(c)[parent], c.page_size), c.width);
+    for (int j = lane; j < count; j += 32 * kAhead) {
+      int page[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) page[u] = j + 32 * u < count ? row[j + 32 * u] : 0;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) bad |= page[u] < 0 || page[u] >= c.pages;
+    }
+  }
+  return bad;
+}
+
+// The cluster's blocks look through the rows, then the first one plans by itself.
+__global__ void __cluster_dims__(kLook, 1, 1) __launch_bounds__(kPlan)
+    cache_fork_plan(pg_cache c, const int *parents, const int *children, int n) {
   __shared__ int warp_slots[32];
   __shared__ unsigned bad;
   pg::wait_for_earlier_kernels();
+  cg::cluster_group cluster = cg::this_cluster();
   if (threadIdx.x == 0) bad = 0;
+  cluster.sync();
+  const int rank = cluster.block_rank();
+  if (bad_rows(c, parents, n, (rank * kPlan + threadIdx.x) >> 5, kLook * kPlan / 32))
+    atomicOr(cluster.map_shared_rank(&bad, 0), PG_CACHE_BAD_PAGE);
+  cluster.sync();
+  if (rank) return;
   int *lens = lens_of(c), *refs = refs_of(c);
   int *scratch = reinterpret_cast<int *>(c.scratch);
   int *fresh = scratch + kHeader, *offset = fresh + c.pages, *claimed = offset + c.slots + 1;
-  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kPlan) {
     const int child = children[i];
     claimed[i] = -1;
@@ -393,22 +428,15 @@ __global__ void __launch_bounds__(kCopy) cache_fork_copy(pg_cache c, const int *
     const int len = lens_of(c)[parents[i]], full = len / c.page_size, open = len % c.page_size;
     const int *from = row_of(c, parents[i]);
     if (part) {
-      if (!open) continue;
-      const int source = from[full];
-      if (source < 0 || source >= c.pages) {
-        if (threadIdx.x == 0) set_status(c, PG_CACHE_BAD_PAGE);
-        continue;
-      }
-      copy_rows(c, reinterpret_cast<char *>(part & 1 ? c.k : c.v), (part - 1) >> 1, source,
-                fresh[offset[i]], open);
+      if (open)
+        copy_rows(c, reinterpret_cast<char *>(part & 1 ? c.k : c.v), (part - 1) >> 1, from[full],
+                  fresh[offset[i]], open);
       continue;
     }
     int *row = row_of(c, children[i]);
     for (int j = threadIdx.x; j < full; j += kCopy) {
-      const int page = from[j];
-      row[j] = page;
-      if (page < 0 || page >= c.pages) set_status(c, PG_CACHE_BAD_PAGE);
-      else atomicAdd(refs_of(c) + page, 1);
+      row[j] = from[j];
+      atomicAdd(refs_of(c) + from[j], 1);
     }
     if (open && threadIdx.x == 0) row[full] = fresh[offset[i]];
   }
@@ -594,7 +622,7 @@ extern "C" int pg_cache_fork(const pg_cache *c, uint64_t parents, uint64_t child
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(static_cast<int64_t>(n) * (2 * c->layers + 1), &grid))) return rc;
-  rc = pg::launch<cache_fork_plan>("cache_fork_plan", dim3(1), kPlan, 0, stream_of(stream), *c,
+  rc = pg::launch<cache_fork_plan>("cache_fork_plan", dim3(kLook), kPlan, 0, stream_of(stream), *c,
                   ints(parents), ints(children), n);
   if (rc) return rc;
   return pg::launch<cache_fork_copy>("cache_fork_copy", dim3(grid), kCopy, 0, stream_of(stream),

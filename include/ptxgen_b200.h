@@ -192,9 +192,10 @@ int pg_grid_sum_f32_noalloc(uint64_t x, uint64_t n, uint64_t out, uint32_t block
  * and a call that takes pages takes the lowest free ones, in the order of its slots.
  *
  * The calls are asynchronous on `stream` and never wait for the host. What only the device can
- * see (no page left, a slot listed twice, a page id out of range) sets PG_CACHE_* bits of the
+ * see (no page left, a slot out of range, a page id out of range) sets PG_CACHE_* bits of the
  * status word, which the caller clears: extend and fork then change nothing, free, write and
- * copy skip the entry. An extend that could not be met also marks its slots in `refused`, and write
+ * copy skip the entry. A slot listed twice is such a thing for extend and for fork's children;
+ * free lets go of its pages once and sets no bit. An extend that could not be met also marks its slots in `refused`, and write
  * leaves out the rows of a marked slot (PG_CACHE_REFUSED): they have no place, and the slot's last
  * positions hold older tokens, in pages that other slots may share. The slot's next extend that is
  * met (by no tokens, if need be), a free of it or a fork into it clears the mark. All calls on one
@@ -222,7 +223,7 @@ typedef struct pg_rows {
 #define PG_CACHE_SCRATCH(pages, slots) (4 + 3 * (int64_t)(pages) + 2 * (int64_t)(slots) + 2)
 
 #define PG_CACHE_NO_PAGES 1u /* fewer free pages than a call needs */
-#define PG_CACHE_BAD_SLOT 2u /* a slot out of range, listed twice, or a fork's child in use */
+#define PG_CACHE_BAD_SLOT 2u /* a slot out of range or listed twice, or a fork's child in use */
 #define PG_CACHE_BAD_PAGE 4u /* a page id or count that cannot be */
 #define PG_CACHE_TOO_LONG 8u /* more tokens than a table row has pages for */
 #define PG_CACHE_REFUSED 32u /* rows for a slot whose last extend could not be met: not written */
