@@ -16,7 +16,9 @@ q, k and v have one dtype (f32, bf16 or f16) and a head size of up to 256 whose 
 multiple of 16 bytes; q may be a slice of a fused projection. Sums and the softmax are held in 32
 bits. Nothing waits for the GPU; where only the device can see that a slot, page id or length is
 out of range, nothing is read, that sequence's result is not defined, and bits are set that
-``Workspace.check`` raises as ``CacheError``. The kernels are ``csrc/attention*.cu``
+``Workspace.check`` raises as ``CacheError``. Calls run on the current stream, or on ``stream`` (a
+``cudaStream_t`` as an integer), whose memory a new result then comes from: other streams wait for
+it and call ``record_stream``, as for any tensor of another stream. The kernels are ``csrc/attention*.cu``
 (``pg_attention``).
 """
 
@@ -29,7 +31,7 @@ from typing import Any
 import torch
 
 from .cache import CacheError
-from .launch import call, dtype_code, int32_list
+from .launch import call, dtype_code, empty, int32_list
 from .runtime import AttentionArgs, library
 
 WORKSPACE_BYTES = 64 << 20  # PG_ATTENTION_WORKSPACE
@@ -96,7 +98,7 @@ def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any
     if workspace.device != dev:
         raise ValueError(f"the workspace is on {workspace.device}, q on {dev}")
     if out is None:
-        out = torch.empty((tokens, hq, dim), dtype=dtype, device=dev)
+        out = empty((tokens, hq, dim), dtype, dev, stream)
     elif out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(2) != 1:
         raise ValueError(f"out: want {dtype} {tuple(q.shape)} on {dev} with contiguous rows")
     os_ = out.stride()

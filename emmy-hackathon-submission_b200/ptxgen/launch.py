@@ -34,6 +34,18 @@ def int32_list(name: str, t: Any, device: torch.device, n: int | None = None) ->
     return t.data_ptr()
 
 
+def empty(shape: Any, dtype: torch.dtype, device: torch.device, stream: int | None) -> Any:
+    """A new tensor for a call on ``stream``, from that stream's memory: what the current stream
+    has let go of may still be read there, and what this tensor lets go of is not the current
+    stream's to write while the call runs."""
+    if stream is None or stream == torch._C._cuda_getCurrentRawStream(device.index):
+        return torch.empty(shape, dtype=dtype, device=device)
+    # a null handle is the default stream, of which ExternalStream would make a new one
+    of = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.stream(of):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def call(fn: Callable[..., int], device: torch.device, stream: int | None, *args: Any) -> None:
     """``fn(*args, stream)`` with ``device`` current, on its current stream where ``stream`` is
     None; raises ``LaunchError`` where it fails."""

@@ -12,7 +12,9 @@ probability 0. ``logprobs_grad`` is the gradient of ``logp`` and ``entropy`` wit
 logits, in their type; either incoming gradient may be None.
 
 The kernels are ``csrc/logprob.cu`` (``pg_logprobs``, ``pg_logprobs_grad``); calls run on the
-current stream, or on ``stream`` (a ``cudaStream_t`` as an integer).
+current stream, or on ``stream`` (a ``cudaStream_t`` as an integer), whose memory new results then
+come from: other streams wait for them and call ``record_stream``, as for any tensor of another
+stream.
 """
 
 from __future__ import annotations
@@ -21,7 +23,7 @@ from typing import Any
 
 import torch
 
-from .launch import call, dtype_code
+from .launch import call, dtype_code, empty
 from .runtime import library
 
 TOP_MAX = 32  # PG_LOGPROB_TOP
@@ -33,9 +35,9 @@ class LogProbs:
 
     __slots__ = ("_all", "_rows", "_top")
 
-    def __init__(self, device: torch.device, rows: int, top: int):
+    def __init__(self, device: torch.device, rows: int, top: int, stream: int | None = None):
         # norm, logp, entropy, top_logp, top_ids
-        self._all = torch.empty((4 + 2 * top) * rows, dtype=torch.float32, device=device)
+        self._all = empty((4 + 2 * top) * rows, torch.float32, device, stream)
         self._rows, self._top = rows, top
 
     @property
@@ -95,7 +97,7 @@ def logprobs(logits: Any, tokens: Any, top: int = 0, stream: int | None = None) 
     rows, vocab = logits.shape
     if not 0 <= top <= min(TOP_MAX, vocab):
         raise ValueError(f"top {top}: want 0 to {min(TOP_MAX, vocab)}")
-    result = LogProbs(logits.device, rows, top)
+    result = LogProbs(logits.device, rows, top, stream)
     at = result._all.data_ptr()
     call(library().pg_logprobs, logits.device, stream, *args, top, at + 8 * rows, at + 12 * rows,
          at, at + 16 * rows, at + (16 + 4 * top) * rows)
@@ -108,7 +110,7 @@ def logprobs_grad(logits: Any, tokens: Any, result: LogProbs, d_logp: Any, d_ent
     ``result`` = ``logprobs(logits, tokens)``; into ``out`` (which may be ``logits``) if given."""
     args = _inputs(logits, tokens)
     if out is None:
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        out = empty(logits.shape, logits.dtype, logits.device, stream)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \
             or (out.shape[1] > 1 and out.stride(1) != 1):
         raise ValueError(f"out: want {logits.dtype} {tuple(logits.shape)} on {logits.device} "
