@@ -31,7 +31,7 @@ from typing import Any
 import torch
 
 from .cache import CacheError
-from .launch import call, dtype_code, empty, int32_list
+from .launch import call, dtype_code, empty, int32_list, take_status
 from .runtime import AttentionArgs, library
 
 WORKSPACE_BYTES = 64 << 20  # PG_ATTENTION_WORKSPACE
@@ -51,11 +51,10 @@ class Workspace:
         self.buffer = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.int32, device=self.device)
 
     def check(self) -> None:
-        """Wait for the GPU and raise ``CacheError`` if an earlier call met a slot, page id or
-        starts out of range (the bits are cleared)."""
-        bits = int(self.buffer[0].item())
+        """Wait for the GPU, all its streams, and raise ``CacheError`` if an earlier call met a slot,
+        page id or starts out of range (the bits are cleared)."""
+        bits = take_status(self.buffer[:1])
         if bits:
-            self.buffer[0].zero_()
             raise CacheError(bits)
 
 

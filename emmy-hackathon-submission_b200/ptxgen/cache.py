@@ -28,7 +28,7 @@ from typing import Any
 
 import torch
 
-from .launch import call, int32_list
+from .launch import call, int32_list, take_status
 from .runtime import Cache, LaunchError, Rows, library
 
 NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG, WAIT, REFUSED = 1, 2, 4, 8, 16, 32
@@ -145,9 +145,8 @@ class PagedCache:
         call(self._lib.pg_cache_compact, self.device, stream, self._ref)
 
     def check(self) -> None:
-        """Wait for the GPU and raise ``CacheError`` if an earlier call could not be met (the
-        status word is cleared)."""
-        bits = int(self.status.item())
+        """Wait for the GPU, all its streams, and raise ``CacheError`` if an earlier call could not
+        be met (the status word is cleared)."""
+        bits = take_status(self.status)
         if bits:
-            self.status.zero_()
             raise CacheError(bits)

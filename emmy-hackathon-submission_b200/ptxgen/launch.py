@@ -46,6 +46,18 @@ def empty(shape: Any, dtype: torch.dtype, device: torch.device, stream: int | No
         return torch.empty(shape, dtype=dtype, device=device)
 
 
+def take_status(word: Any) -> int:
+    """The bits of a status word (a one-element int32 tensor), which is cleared. The calls that set
+    it may have been on any stream, so this waits for the whole device, before it reads the word and
+    until it is cleared."""
+    torch.cuda.synchronize(word.device)
+    bits = int(word.item())
+    if bits:
+        word.zero_()
+        torch.cuda.synchronize(word.device)
+    return bits
+
+
 def call(fn: Callable[..., int], device: torch.device, stream: int | None, *args: Any) -> None:
     """``fn(*args, stream)`` with ``device`` current, on its current stream where ``stream`` is
     None; raises ``LaunchError`` where it fails."""
