@@ -31,7 +31,7 @@ from typing import Any
 import torch
 
 from .cache import CacheError
-from .launch import call, dtype_code, empty, int32_list, take_status
+from .launch import call, dtype_code, empty, int32_list, take_status, wait_until_set
 from .runtime import AttentionArgs, library
 
 WORKSPACE_BYTES = 64 << 20  # PG_ATTENTION_WORKSPACE
@@ -43,12 +43,14 @@ assert _PACK.size == ctypes.sizeof(AttentionArgs)
 
 class Workspace:
     """The device memory in which attention leaves the parts of a long sequence's result until
-    they are joined. One per stream: calls that overlap on the GPU must not share it."""
+    they are joined. One per stream: calls that overlap on the GPU must not share it. It has to
+    live until the calls that were given it have run."""
 
     def __init__(self, device: Any = None):
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None \
             else torch.device(device)
         self.buffer = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.int32, device=self.device)
+        wait_until_set(self.device)
 
     def check(self) -> None:
         """Wait for the GPU, all its streams, and raise ``CacheError`` if an earlier call met a slot,

@@ -28,7 +28,7 @@ from typing import Any
 
 import torch
 
-from .launch import call, int32_list, take_status
+from .launch import call, int32_list, take_status, wait_until_set
 from .runtime import Cache, LaunchError, Rows, library
 
 NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG, WAIT, REFUSED = 1, 2, 4, 8, 16, 32
@@ -80,6 +80,7 @@ class PagedCache:
             int32_list("lens", lens, k.device, slots), self.status.data_ptr(),
             self._scratch.data_ptr(), self._refused.data_ptr(), max(table.stride(0), width), words, layers, pages, heads,
             page_size, dim * size, slots, width)
+        wait_until_set(self.device)
         self._ref = ctypes.byref(self._c)
         self._lib = library()
 

@@ -46,6 +46,13 @@ def empty(shape: Any, dtype: torch.dtype, device: torch.device, stream: int | No
         return torch.empty(shape, dtype=dtype, device=device)
 
 
+def wait_until_set(device: torch.device) -> None:
+    """Wait for the current stream, which has set what calls on any stream will read. Under capture
+    nothing runs yet, and the graph's own order holds."""
+    if not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(device).synchronize()
+
+
 def take_status(word: Any) -> int:
     """The bits of a status word (a one-element int32 tensor), which is cleared. The calls that set
     it may have been on any stream, so this waits for the whole device, before it reads the word and
