@@ -427,7 +427,8 @@ extern "C" int pg_attention(const pg_attention_args *p, uint64_t stream) {
   if (a.dim <= 128) {
     if (pg::decode_takes(a, dtype == PG_DT_F32, static_cast<int>(most), max_len))
       return pg::decode(a, dtype, sms, s);
-    if (a.starts && dtype != PG_DT_F32)
+    // which masks a score before it is scaled, and 0 times a masked one's -inf is NaN
+    if (a.starts && dtype != PG_DT_F32 && a.scale_log2 != 0.0f)
       return pg::prompt_16bit(a, dtype == PG_DT_BF16, max_len, partial_bytes, sms, s);
   }
   if (dtype == PG_DT_F32) return run<float>(a, max_len, partial_bytes, sms, s);
