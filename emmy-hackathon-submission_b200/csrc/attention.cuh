@@ -151,6 +151,13 @@ __device__ __forceinline__ bool clean32(uint4 *at) {
   return any;
 }
 
+// Adds a visible value that is not finite to its column's sum. Its products with the weights as they
+// were rounded may be NaN (0 times infinity), so the first such value takes the place of a sum that is
+// not finite, and only the others add to it.
+__device__ __forceinline__ void add_odd(float value, float &sum, bool first) {
+  sum = first && !(fabsf(sum) < INFINITY) ? value : sum + value;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -28,7 +28,9 @@
 //
 // Several queries' heads make more rows, 16 to a pair of their own, so each of their groups of 16
 // reads the keys again, from L2. What some row of a step must not see has weight 0 there; values
-// that are not finite are zeroed in such steps, and added again at the end for rows that see them.
+// that are not finite are zeroed in such steps, and added again at the end for rows that see them. In
+// the other steps they meet both parts of a weight, the second of which may be 0 or negative: a result
+// that is not finite has the visible values looked through and is made of those that are not.
 #include "attention.cuh"
 
 namespace {
@@ -253,8 +255,9 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
   };
   const auto write = [&](int r, int col, float4 x, float sum) {
     if (r >= p.rows || col >= a.dim) return;
-    // a query before the sequence's start sees no key: zeros
-    const float inv = 1.0f / sum;
+    // a query before the sequence's start sees no key: zeros. Any other sees itself, so a sum of 0
+    // means that all its scores are -inf: 0 / 0.
+    const float inv = sum == 0.0f ? NAN : 1.0f / sum;
     const bool none = p.lo + query_of(r) < 0;
     store4<T>(a.out + (p.query + query_of(r)) * a.out_token + head_of(r) * a.out_head +
                   col * R::size,
@@ -280,23 +283,33 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
       acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y);
       acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
     }
-    if ((MANY || sizeof(T) == 4) && odd && col < a.dim)
+    // a score that is NaN or +inf makes the sum NaN, and with it all the row's results
+    const bool lost = sum < INFINITY && !(fabsf(acc.x) < INFINITY && fabsf(acc.y) < INFINITY &&
+                                          fabsf(acc.z) < INFINITY && fabsf(acc.w) < INFINITY);
+    if ((odd || lost) && col < a.dim) {
+      bool first[4] = {true, true, true, true};
+      const auto add = [&](int k, float value, float &to) {
+        if (fabsf(value) < INFINITY) return;
+        pg::add_odd(value, to, first[k]);
+        first[k] = false;
+      };
       for (int i = 0; i < p.block1 - p.block0; ++i)
         for (int j = 0; j < R::keys; ++j) {
           const int key = p.blocks.key_block(p.block0 + i) * R::keys + j;
           if (!pg::sees(a, p.lo + query_of(r), key) ||
-              (sizeof(T) != 4 && p.all_see<R::step>(a, key / R::step * R::step)))
+              (sizeof(T) != 4 && !lost && p.all_see<R::step>(a, key / R::step * R::step)))
             continue;
           const int page = p.pages[key / a.page_size];
           if (page < 0 || page >= a.pages) continue;
           const float4 x = load4<T>(a.v + page * a.v_page + p.head * a.v_head +
                                     static_cast<int64_t>(key % a.page_size) * a.dim * R::size +
                                     col * R::size);
-          if (!(fabsf(x.x) < INFINITY)) acc.x += x.x;
-          if (!(fabsf(x.y) < INFINITY)) acc.y += x.y;
-          if (!(fabsf(x.z) < INFINITY)) acc.z += x.z;
-          if (!(fabsf(x.w) < INFINITY)) acc.w += x.w;
+          add(0, x.x, acc.x);
+          add(1, x.y, acc.y);
+          add(2, x.z, acc.z);
+          add(3, x.w, acc.w);
         }
+    }
     if (alone) {
       write(r, col, acc, sum);
     } else {

@@ -31,7 +31,8 @@
 // A masked place has weight 0, and 0 times a value that is not finite would be NaN. So the values
 // of each block that some row must not see in full are looked through before they are used: what
 // is not finite is zeroed and a flag raised, and at the end a row adds the ones it does see again.
-// Rows past the sequence's length are zeroed.
+// Rows past the sequence's length are zeroed. In the other blocks a weight that was rounded to 0 may
+// have met an infinite value: a result that is not finite is made of the visible values that are not.
 //
 // Every wait is bounded: one that takes over two seconds sets PG_ATTENTION_WAIT in the status
 // word, and all roles leave their loops; the block then frees its tensor memory and returns.
@@ -640,11 +641,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_load(o_at + 32 * k, reinterpret_cast<uint32_t *>(x));
       wait_loads();
       tie(reinterpret_cast<uint32_t *>(x));
-      if (!*const_cast<volatile int *>(&sh.odd)) return;
-      // values that are not finite, in blocks that some row must not see in full
+      bool lost = false;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) lost |= !(fabsf(x[e]) < INFINITY);
+      // a score that is NaN or +inf makes l NaN, and with it all the row's results
+      if (pos < 0 || !(l < INFINITY) || !(lost || *const_cast<volatile int *>(&sh.odd))) return;
+      // values that are not finite: all, or those in blocks that some row must not see in full
+      uint32_t met = 0;
       for (int j = 0; j < steps; ++j) {
         const int key0 = blocks.key_block(b0 + j) * kKeys;
-        if (both.all(key0)) continue;
+        if (!lost && both.all(key0)) continue;
         for (int key = key0; key < min(key0 + kKeys, t.length); ++key) {
           if (!pg::sees(a, pos, key)) continue;
           const int page = pg::page_of(a, t, key);
@@ -659,8 +665,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float lo = Type<T>::low(w[e]), hi = Type<T>::high(w[e]);
-              if (!(fabsf(lo) < INFINITY)) x[8 * q + 2 * e] += lo;
-              if (!(fabsf(hi) < INFINITY)) x[8 * q + 2 * e + 1] += hi;
+              const int c0 = 8 * q + 2 * e;
+              if (!(fabsf(lo) < INFINITY)) {
+                pg::add_odd(lo, x[c0], !(met >> c0 & 1));
+                met |= 1u << c0;
+              }
+              if (!(fabsf(hi) < INFINITY)) {
+                pg::add_odd(hi, x[c0 + 1], !(met >> (c0 + 1) & 1));
+                met |= 2u << c0;
+              }
             }
           }
         }
@@ -679,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
     if (a.parts == 1) {
-      const float inv = 1.0f / l;
+      const float inv = l == 0.0f ? NAN : 1.0f / l;  // 0: all its scores are -inf, 0 / 0
 #pragma unroll 1
       for (int k = 0; k < DIM / 32; ++k) {
         float x[32];
@@ -720,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 ml = __ldcg(ml_of(all + p * size));
           total += ml.x == -INFINITY ? 0.0f : ml.y * pg::exp2_fast((ml.x - top) * c);
         }
-        const float inv = 1.0f / total;
+        const float inv = total == 0.0f ? NAN : 1.0f / total;
 #pragma unroll 1
         for (int k = 0; k < DIM / 32; ++k) {
           float x[32] = {};

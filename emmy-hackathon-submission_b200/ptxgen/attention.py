@@ -10,7 +10,8 @@
 cache: row b of q for ``decode``, rows ``starts[b]`` to ``starts[b + 1]`` for ``prompt``. A query
 at position p sees key j when j <= p and, with a ``window``, j > p - window or j < ``sinks``. A
 query that sees no key gives zeros; what lies past a sequence's length or in a masked place is
-never part of a result. Each group of heads / kv_heads query heads reads one kv head.
+never part of a result. A visible value that is not finite makes its column of the result so: an
+infinity, where all such values are that one (or NaN, where its weight is below 2^-126). Each group of heads / kv_heads query heads reads one kv head.
 
 q, k and v have one dtype (f32, bf16 or f16) and a head size of up to 256 whose rows are a
 multiple of 16 bytes; q may be a slice of a fused projection. Sums and the softmax are held in 32

@@ -287,7 +287,9 @@ int pg_logprobs_grad(uint64_t logits, int64_t row_stride, int32_t dtype, uint64_
  * position p sees key j when j <= p and (window == 0 or j > p - window or j < sinks);
  * out = softmax(scale q . k) v over the keys it sees. A query that sees none (a length of 0, or
  * fewer tokens than queries) gives zeros, and what lies in masked places, pages past the length
- * or unused rows of a page is never part of a result, whatever it is. Query head h reads kv head
+ * or unused rows of a page is never part of a result, whatever it is. A visible value that is not
+ * finite makes its column of the result so: an infinity, where all such values are that one (or NaN,
+ * where its weight is below 2^-126). Query head h reads kv head
  * h / group. q and out are [queries, heads * group, dim], k and v [pages, heads, page_size, dim]
  * with a head's rows of one page one after another; all of one dtype (PG_DT_F32, PG_DT_BF16 or
  * PG_DT_F16), with sums and softmax in 32 bits and one rounding of the result.
