@@ -418,9 +418,12 @@ extern "C" int pg_attention(const pg_attention_args *p, uint64_t stream) {
   a.table_row = p->table_stride;
   a.batch = p->batch, a.queries = p->queries, a.heads = p->heads, a.group = p->group;
   a.dim = p->dim, a.page_size = p->page_size, a.pages = p->pages, a.width = p->width;
-  a.slot_rows = p->slot_rows, a.window = p->window, a.sinks = p->sinks;
+  a.slot_rows = p->slot_rows, a.sinks = p->sinks;
   a.scale_log2 = p->scale * 1.4426950408889634f;
   const int64_t most = static_cast<int64_t>(p->width) * p->page_size;
+  // A window that the longest sequence fits in hides nothing. Positions less a smaller one stay in 32
+  // bits, those of queries before a sequence's start too.
+  a.window = p->window >= most ? 0 : p->window;
   const int max_len = static_cast<int>(p->max_len && p->max_len < most ? p->max_len : most);
   const int64_t partial_bytes = p->workspace_bytes - 256 - pg::kCounters * 4ll;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
