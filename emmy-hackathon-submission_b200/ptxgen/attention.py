@@ -48,9 +48,9 @@ class Workspace:
     live until the calls that were given it have run."""
 
     def __init__(self, device: Any = None):
-        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None \
-            else torch.device(device)
-        self.buffer = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.int32, device=self.device)
+        self.buffer = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.int32,
+                                  device="cuda" if device is None else device)
+        self.device = self.buffer.device  # with an index, as a call's tensors have it
         wait_until_set(self.device)
 
     def check(self) -> None:
