@@ -90,7 +90,11 @@ class Sample:
 def generate(model: Model, prompts: list[list[int]], samples: int = 4, steps: int = 24,
              page_size: int = 16, seed: int = 0) -> tuple[list[Sample], PagedCache]:
     """``samples`` continuations of each prompt by ``steps`` tokens; after half of them each
-    prompt's least likely sample is dropped and keeps what it has."""
+    prompt's least likely sample is dropped and keeps what it has. Every prompt has a token: the
+    samples begin from the hidden state of its last one."""
+    if not prompts or not all(prompts) or samples < 1 or steps < 1:
+        raise ValueError(f"prompts of {[len(p) for p in prompts]} tokens, {samples} samples, {steps} "
+                         "steps: want at least one of each")
     dev = model.embed.device
     g = torch.Generator(device=dev).manual_seed(seed)
 
