@@ -14,6 +14,11 @@ import torch
 
 from .runtime import _check
 
+# torch's own ways to the current device and to a device's current stream as an integer, which make no
+# stream object; the public ones where a torch has no such names
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                          lambda index: torch.cuda.current_stream(index).cuda_stream)
 _DTYPES = {torch.float16: 1, torch.bfloat16: 2, torch.float32: 3}  # PG_DT_*
 
 
@@ -38,7 +43,7 @@ def empty(shape: Any, dtype: torch.dtype, device: torch.device, stream: int | No
     """A new tensor for a call on ``stream``, from that stream's memory: what the current stream
     has let go of may still be read there, and what this tensor lets go of is not the current
     stream's to write while the call runs."""
-    if stream is None or stream == torch._C._cuda_getCurrentRawStream(device.index):
+    if stream is None or stream == _current_stream(device.index):
         return torch.empty(shape, dtype=dtype, device=device)
     # a null handle is the default stream, of which ExternalStream would make a new one
     of = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
@@ -69,9 +74,9 @@ def call(fn: Callable[..., int], device: torch.device, stream: int | None, *args
     """``fn(*args, stream)`` with ``device`` current, on its current stream where ``stream`` is
     None; raises ``LaunchError`` where it fails."""
     index = device.index
-    if torch._C._cuda_getDevice() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
             return call(fn, device, stream, *args)
-    rc = fn(*args, torch._C._cuda_getCurrentRawStream(index) if stream is None else stream)
+    rc = fn(*args, _current_stream(index) if stream is None else stream)
     if rc:
         _check(rc, fn.__name__)
