@@ -55,6 +55,7 @@ __device__ __forceinline__ float exp2_small(float x) {
 template <class T> struct Vec;  // 16 bytes of T as f32
 template <> struct Vec<float> {
   static constexpr int n = 4;
+  static constexpr bool small = true;  // holds numbers near 2^-126
   __device__ static void get(const uint4 &v, float *x) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y);
     x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
@@ -66,6 +67,7 @@ template <> struct Vec<float> {
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int n = 8;
+  static constexpr bool small = true;
   __device__ static void get(const uint4 &v, float *x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -86,6 +88,7 @@ template <> struct Vec<__nv_bfloat16> {
 };
 template <> struct Vec<__half> {
   static constexpr int n = 8;
+  static constexpr bool small = false;
   __device__ static void get(const uint4 &v, float *x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -442,14 +445,14 @@ __global__ void __launch_bounds__(kThreads)
   const float b = d_entropy ? d_entropy[row] : 0.0f;
   const float c = fmaf(b, h, a);
   // -p (a + b (log p + H)) of two columns; the token's a is added after. Probabilities below
-  // 2^-126 become 0 but for f32 results, which can hold such numbers times a large factor.
+  // 2^-126 become 0 but for f32 and bf16 results, which can hold such numbers times a large factor.
   const pg::Two m(-l.x, -l.x), log_s(-l.y, -l.y), scale(kLog2e, kLog2e), b2(-b, -b), c2(-c, -c);
   const auto grad = [&](float &x, float &y) {
     add(add(pg::Two(x, y), m), log_s).get(x, y);
     const pg::Two lp(max_nan(x, kCut), max_nan(y, kCut));
     mul(lp, scale).get(x, y);
-    const pg::Two p = sizeof(T) == 4 ? pg::Two(exp2_small(x), exp2_small(y))
-                                     : pg::Two(exp2_fast(x), exp2_fast(y));
+    const pg::Two p = Vec<T>::small ? pg::Two(exp2_small(x), exp2_small(y))
+                                    : pg::Two(exp2_fast(x), exp2_fast(y));
     mul(p, fma(b2, lp, c2)).get(x, y);
   };
   const auto grad_one = [&](int column) {
