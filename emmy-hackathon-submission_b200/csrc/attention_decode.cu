@@ -13,7 +13,8 @@
 // m16n8k16: with at most 16 rows of queries a larger tile would be empty, and at one use of
 // each key the memory is slower by far). A weight goes into the second product as the sum of two
 // numbers of the values' type, the rounded weight and what the rounding left, so that the
-// result is rounded once; that doubles the second product, which the memory hides.
+// result is rounded once; that doubles the second product, which the memory hides. In f16, which has
+// nothing below 2^-24, weights and their sum are 2^15 of what they are.
 //
 // f32 goes the same way by eights of keys (m16n8k8, TF32). A factor x of either product is taken as
 // hi, 11 bits of it, and lo, 11 bits of the rest, and hi hi' + hi lo' + lo hi' is summed. Left out
@@ -48,6 +49,7 @@ constexpr float kCut = 2.0f;
 
 template <class T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
+  static constexpr float shift = 0.0f;  // weights go in as 2^shift of what they are
   __device__ static void run(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, "
                  "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -71,6 +73,7 @@ template <> struct Mma<__nv_bfloat16> {
   }
 };
 template <> struct Mma<__half> {
+  static constexpr float shift = 15.0f;  // at most 2^15 of 65504
   static constexpr uint32_t exponent = 0x7c00;
   __device__ static float low(uint32_t w) {
     return __low2float(*reinterpret_cast<const __half2 *>(&w));
@@ -97,6 +100,7 @@ template <> struct Mma<__half> {
 };
 
 template <> struct Mma<float> {
+  static constexpr float shift = 0.0f;
   __device__ static void run(float *d, const uint32_t *a, const uint32_t *b) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, "
                  "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -735,8 +739,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float x = pg::exp2_fast(s[n][2 * h] - base[h]);
-          const float y = pg::exp2_fast(s[n][2 * h + 1] - base[h]);
+          float x = s[n][2 * h] - base[h], y = s[n][2 * h + 1] - base[h];
+          if constexpr (Mma<T>::shift != 0.0f) x += Mma<T>::shift, y += Mma<T>::shift;
+          x = pg::exp2_fast(x);
+          y = pg::exp2_fast(y);
           l[h] += x + y;
           if constexpr (sizeof(T) == 4) {
             Mma<T>::split_near(x, hi[h], lo[h]);  // the product's keys are 0, 2, 4, 6, 1, 3, 5, 7

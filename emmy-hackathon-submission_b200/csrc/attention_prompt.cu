@@ -25,8 +25,9 @@
 // grown by more than 2^8 since the last time, so that a weight is at most 2^8 and rescaling is
 // rare; the sum l goes by the same maximum, so the result is the same.
 //
-// Rounding: weights go into the second product in the values' type (2^-9 or 2^-12 of each, at
-// random), as the tensor cores take both operands in one type; S, m, l and O are in 32 bits.
+// Rounding: weights go into the second product in the values' type (up to 2^-8 or 2^-11 of each, at
+// random), as the tensor cores take both operands in one type; S, m, l and O are in 32 bits. In f16,
+// which rounds coarsely below 2^-14, weights and their sum are 2^7 of what they are.
 //
 // A masked place has weight 0, and 0 times a value that is not finite would be NaN. So the values
 // of each block that some row must not see in full are looked through before they are used: what
@@ -210,6 +211,7 @@ __device__ __forceinline__ float largest(const float *s, float m) {
 
 template <class T> struct Type;
 template <> struct Type<__nv_bfloat16> {
+  static constexpr float shift = 0.0f;  // weights go in as 2^shift of what they are
   static constexpr uint32_t format = 1, exponent = 0x7f80;
   __device__ static uint32_t pack(float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
@@ -219,6 +221,7 @@ template <> struct Type<__nv_bfloat16> {
   __device__ static float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 };
 template <> struct Type<__half> {
+  static constexpr float shift = 15.0f - kGrow;  // at most 2^15 of 65504
   static constexpr uint32_t format = 0, exponent = 0x7c00;
   __device__ static uint32_t pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -600,7 +603,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // an infinite maximum gives NaN, as the formula does, in every weight
-      const float base = m == -INFINITY ? 0.0f : m == INFINITY ? NAN : -m * c;
+      const float base =
+          m == -INFINITY ? 0.0f : m == INFINITY ? NAN : Type<T>::shift - m * c;
       Two sum[2] = {Two(l, 0.0f), Two(0.0f, 0.0f)};
       const Two c2(c, c), base2(base, base);
 #pragma unroll
