@@ -209,6 +209,8 @@ __global__ void __launch_bounds__(kCopy) cache_write(pg_cache c, int layer, cons
   const int lane = threadIdx.x & 31;
   const int warps = gridDim.x * (kCopy / 32);
   const int pieces = c.row_bytes / 16, all = c.heads * pieces;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && (starts[0] < 0 || starts[n] > tokens))
+    set_status(c, PG_CACHE_TOO_LONG);  // tokens that have no rows
   for (int t = (blockIdx.x * kCopy + threadIdx.x) >> 5; t < tokens; t += warps) {
     if (t < starts[0] || t >= starts[n]) continue;
     const int i = find_sequence(starts, n, t);

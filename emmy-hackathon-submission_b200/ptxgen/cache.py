@@ -35,7 +35,7 @@ NO_PAGES, BAD_SLOT, BAD_PAGE, TOO_LONG, WAIT, REFUSED = 1, 2, 4, 8, 16, 32
 _WHY = {NO_PAGES: "fewer free pages than a call needed",
         BAD_SLOT: "a slot out of range, listed twice, or a fork's child in use",
         BAD_PAGE: "a page id or count out of range",
-        TOO_LONG: "more tokens than a table row has pages for",
+        TOO_LONG: "more tokens than a table row has pages for, or than there are rows",
         WAIT: "a bounded wait inside an attention kernel gave up",
         REFUSED: "rows of a slot whose last extend could not be met were not written"}
 
@@ -114,7 +114,8 @@ class PagedCache:
     def write(self, layer: int, slots: Any, starts: Any, k: Any, v: Any,
               stream: int | None = None) -> None:
         """Write one layer's ``k`` and ``v`` [tokens, heads, dim] of the slots' last tokens:
-        rows ``starts[i]`` to ``starts[i + 1]`` are the last ones of ``slots[i]``."""
+        rows ``starts[i]`` to ``starts[i + 1]`` are the last ones of ``slots[i]``. Rows past the last
+        of ``starts`` belong to none."""
         n, dev = slots.shape[0], self.device
         if k.shape[0] != v.shape[0]:
             raise ValueError(f"k has {k.shape[0]} tokens, v has {v.shape[0]}")

@@ -225,7 +225,7 @@ typedef struct pg_rows {
 #define PG_CACHE_NO_PAGES 1u /* fewer free pages than a call needs */
 #define PG_CACHE_BAD_SLOT 2u /* a slot out of range or listed twice, or a fork's child in use */
 #define PG_CACHE_BAD_PAGE 4u /* a page id or count that cannot be */
-#define PG_CACHE_TOO_LONG 8u /* more tokens than a table row has pages for */
+#define PG_CACHE_TOO_LONG 8u /* more tokens than a table row has pages for, or than there are rows */
 #define PG_CACHE_REFUSED 32u /* rows for a slot whose last extend could not be met: not written */
 
 /* Makes room for the new tokens of n sequences: slots[i] grows by starts[i + 1] - starts[i]
@@ -235,7 +235,8 @@ int pg_cache_extend(const pg_cache *cache, uint64_t slots, uint64_t starts, int3
 
 /* Writes one layer's rows of the last tokens of n sequences: token t of the `tokens` rows, with
  * starts[i] <= t < starts[i + 1], lands at position lens[slots[i]] - starts[i + 1] + t. Rows of a
- * slot whose last extend could not be met are left out. */
+ * slot whose last extend could not be met are left out, as are rows of no sequence; tokens that have
+ * no row (starts[n] > tokens) set PG_CACHE_TOO_LONG. */
 int pg_cache_write(const pg_cache *cache, int32_t layer, uint64_t slots, uint64_t starts,
                    int32_t n, int32_t tokens, const pg_rows *k, const pg_rows *v,
                    uint64_t stream);
