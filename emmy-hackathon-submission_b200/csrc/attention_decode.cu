@@ -10,10 +10,10 @@
 // Within a block each of four warps takes every fourth 16 keys by itself: it copies their rows
 // into its own ring in shared memory (cp.async, 16 bytes a lane, rows of whole heads, swizzled so
 // that the matrix loads meet no bank twice), and multiplies on the tensor cores (mma.sync
-// m16n8k16: with at most 16 rows of queries a larger tile would be empty, and at one use of
-// each key the memory is slower by far). A weight goes into the second product as the sum of two
-// numbers of the values' type, the rounded weight and what the rounding left, so that the
-// result is rounded once; that doubles the second product, which the memory hides. In f16, which has
+// m16n8k16: with at most 16 rows of queries a larger tile would be empty, and at one use of each
+// key the memory is slower by far). A weight goes into the second product as the sum of two
+// numbers of the values' type, the rounded weight and what the rounding left, so that the result
+// is rounded once; that doubles the second product, which the memory hides. In f16, which has
 // nothing below 2^-24, weights and their sum are 2^15 of what they are.
 //
 // f32 goes the same way by eights of keys (m16n8k8, TF32). A factor x of either product is taken as
@@ -832,11 +832,14 @@ int launch_decode(const Attention &a, int sms, cudaStream_t stream) {
 namespace pg {
 
 // Whether this kernel takes a batch and not the large tiles of attention_prompt.cu: at up to 48
-// rows a sequence on average, which those fill badly. By rows a sequence, this against those, in
-// microseconds at head size 128: 7 sequences of up to 20000 keys on 4 kv heads, 16 rows 43 and 83,
-// 32 rows 56 and 84, 48 rows 60 and 84, 64 rows 70 and 96; 32 of up to 8000 on 8, 16 rows 74 and
-// 157, 32 rows 119 and 158, 48 rows 155 and 160, 64 rows 191 and 160; 100 of up to 500 on 4, 48
-// rows 51 and 49, 64 rows 63 and 50.
+// rows a sequence on average, which those fill badly. The average says little of an uneven batch:
+// 100 single tokens and one chunk of 1024, 4000 keys each and 4 heads on each of 8, come here and
+// take 997 us, where the chunk alone takes 126 there and the tokens 289 here; 63 and one of 2048
+// go there and take 387, alone 176 and 195. Even batches, by rows a sequence, this against those,
+// in microseconds at head size 128: 7 sequences of up to 20000 keys on 4 kv heads, 16 rows 43 and
+// 83, 32 rows 56 and 84, 48 rows 60 and 84, 64 rows 70 and 96; 32 of up to 8000 on 8, 16 rows 74
+// and 157, 32 rows 119 and 158, 48 rows 155 and 160, 64 rows 191 and 160; 100 of up to 500 on 4,
+// 48 rows 51 and 49, 64 rows 63 and 50.
 // f32 has no such tiles, so it is taken at up to 256 rows, and at up to 1024 where most keys are
 // seen by all of a sequence's queries, since a group of 16 rows goes through all that any sees. This
 // against attention.cu: 8 sequences on 4 kv heads of 128, up to 4056 keys, 64 rows 86 and 164, 256

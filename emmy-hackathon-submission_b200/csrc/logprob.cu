@@ -302,9 +302,10 @@ __device__ void select_top(const Part<T> &part, float mine, bool any, int k,
   __syncthreads();
 }
 
-// One cluster of blocks a row; block r of it takes the r-th part. At many rows the instructions a
-// logit costs bound it, close to HBM's time for reading each once: 4096 x 50257 in bf16 take 80 us
-// (5.1 TB/s), 1000 x 128256 with the top 20 68 us (3.8 TB/s). At few rows the parts keep all SMs
+// One cluster of blocks a row; block r of it takes the r-th part. 4096 x 50257 in bf16 take 78 us (5.3
+// TB/s); 1000 x 128256 with the top 20 68 us (3.8 TB/s), with issue at 56 %, special functions at 47 %
+// and DRAM at 53 % of what they can: 1000 blocks are 1.7 waves of what the SMs hold, and rows that have
+// left L2 are read again for their top entries. At few rows the parts keep all SMs
 // reading and latency bounds it: 4 x 32001 in f32 with the top 5 take 8 us.
 template <class T, int THREADS>
 __global__ void __launch_bounds__(THREADS, kOnSm / THREADS)
@@ -421,8 +422,8 @@ __global__ void __launch_bounds__(THREADS, kOnSm / THREADS)
   }
 }
 
-// Reads each logit once and writes its gradient; HBM bounds it: 4096 x 50257 in bf16 take 128 us
-// (6.4 TB/s). Rows go last to first, so that those a forward pass over the same logits read last
+// Reads each logit once and writes its gradient; HBM bounds it: 4096 x 50257 in bf16 take 127 us
+// (6.5 TB/s). Rows go last to first, so that those a forward pass over the same logits read last
 // are still in L2.
 template <class T>
 __global__ void __launch_bounds__(kThreads)
@@ -503,7 +504,7 @@ int launch_logprobs(uint64_t logits, int64_t row_stride, uint64_t tokens, int to
                     int rows, int vocab, int top, int sms, uint64_t logp, uint64_t entropy,
                     uint64_t norm, uint64_t top_logp, uint64_t top_ids, cudaStream_t stream) {
   // blocks a row: as many as the SMs hold at once, up to a portable cluster, and no part
-  // shorter than one batch of a block's loads
+  // shorter than one load of each thread
   int parts = 1;
   const int least = THREADS * Vec<T>::n, most = kOnSm / THREADS * sms;
   while (parts < kParts && rows * 2ll * parts <= most && vocab / (2 * parts) >= least) parts *= 2;

@@ -14,8 +14,10 @@ never part of a result. A visible value that is not finite makes its column of t
 infinity, where all such values are that one (or NaN, where its weight is below 2^-126). Each group of heads / kv_heads query heads reads one kv head.
 
 q, k and v have one dtype (f32, bf16 or f16) and a head size of up to 256 whose rows are a
-multiple of 16 bytes; q may be a slice of a fused projection. Sums and the softmax are held in 32
-bits. Nothing waits for the GPU; where only the device can see that a slot, page id or length is
+multiple of 16 bytes; q may be a slice of a fused projection. Scores, maxima and sums are held in 32
+bits. bf16 and f16 results are rounded to their type; prompts of more than 48 rows (tokens times heads
+/ kv_heads) a sequence on average with heads of up to 128 round each weight to it as well, before its
+product with a value. Rows of q that no sequence has leave theirs of the result as they are. Nothing waits for the GPU; where only the device can see that a slot, page id or length is
 out of range, nothing is read, that sequence's result is not defined, and bits are set that
 ``Workspace.check`` raises as ``CacheError``. Calls run on the current stream, or on ``stream`` (a
 ``cudaStream_t`` as an integer), whose memory a new result then comes from: other streams wait for

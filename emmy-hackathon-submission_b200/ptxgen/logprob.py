@@ -5,8 +5,8 @@
 
 For a row x of ``logits`` [rows, vocab] (f32, bf16 or f16; rows may lie apart) and p =
 softmax(x): ``logp`` = log p[token], ``entropy`` = -sum p log p, ``norm`` = (max x, log sum
-exp(x - max x)), and the ``top`` largest log probabilities with their columns, ties to the lowest column. All are f32 from
-32-bit sums. Token -1 means there is none: its ``logp`` is 0 and has no gradient. A token outside
+exp(x - max x)), and the ``top`` largest log probabilities with their columns, ties to the lowest
+column. All are f32 from 32-bit sums. Token -1 means there is none: its ``logp`` is 0 and has no gradient. A token outside
 [-1, vocab) gives NaN, as does a row with a NaN, a +inf or nothing but -inf; a column of -inf has
 probability 0. ``logprobs_grad`` is the gradient of ``logp`` and ``entropy`` with respect to the
 logits, in their type; either incoming gradient may be None.

@@ -191,15 +191,16 @@ int pg_grid_sum_f32_noalloc(uint64_t x, uint64_t n, uint64_t out, uint32_t block
  * page_size]. refs[p] counts the table rows that name page p; a page whose count is 0 is free,
  * and a call that takes pages takes the lowest free ones, in the order of its slots.
  *
- * The calls are asynchronous on `stream` and never wait for the host. What only the device can
- * see (no page left, a slot out of range, a page id out of range) sets PG_CACHE_* bits of the
- * status word, which the caller clears: extend and fork then change nothing, free, write and
- * copy skip the entry. A slot listed twice is such a thing for extend and for fork's children;
- * free lets go of its pages once and sets no bit. An extend that could not be met also marks its slots in `refused`, and write
- * leaves out the rows of a marked slot (PG_CACHE_REFUSED): they have no place, and the slot's last
- * positions hold older tokens, in pages that other slots may share. The slot's next extend that is
- * met (by no tokens, if need be), a free of it or a fork into it clears the mark. All calls on one
- * cache share its scratch words and so belong on one stream at a time. */
+ * The calls are asynchronous on `stream` and never wait for the host. What only the device can see
+ * (no page left, a slot out of range, a page id out of range) sets PG_CACHE_* bits of the status
+ * word, which the caller clears: extend and fork then change nothing, free, write and copy skip
+ * the entry. A slot listed twice is such a thing for extend and for fork's children; free lets go
+ * of its pages once and sets no bit. An extend that could not be met also marks its slots in
+ * `refused`, and write leaves out the rows of a marked slot (PG_CACHE_REFUSED): they have no
+ * place, and the slot's last positions hold older tokens, in pages that other slots may share. The
+ * slot's next extend that is met (by no tokens, if need be), a free of it or a fork into it clears
+ * the mark. All calls on one cache share its scratch words and so belong on one stream at a
+ * time. */
 typedef struct pg_cache {
   uint64_t k, v;                                    /* device addresses, 16-byte aligned */
   int64_t layer_stride, page_stride, head_stride;   /* bytes, multiples of 16 */
@@ -225,7 +226,7 @@ typedef struct pg_rows {
 #define PG_CACHE_NO_PAGES 1u /* fewer free pages than a call needs */
 #define PG_CACHE_BAD_SLOT 2u /* a slot out of range or listed twice, or a fork's child in use */
 #define PG_CACHE_BAD_PAGE 4u /* a page id or count that cannot be */
-#define PG_CACHE_TOO_LONG 8u /* more tokens than a table row has pages for, or than there are rows */
+#define PG_CACHE_TOO_LONG 8u /* more tokens than a table row has pages for, or than rows */
 #define PG_CACHE_REFUSED 32u /* rows for a slot whose last extend could not be met: not written */
 
 /* Makes room for the new tokens of n sequences: slots[i] grows by starts[i + 1] - starts[i]
@@ -260,16 +261,16 @@ int pg_cache_compact(const pg_cache *cache, uint64_t stream);
 /* --- log probabilities ------------------------------------------------------------------------
  *
  * No counterpart in the reference. For each row x of `rows` rows of `vocab` logits (dtype
- * PG_DT_F32, PG_DT_BF16 or PG_DT_F16; rows row_stride elements apart) and p = softmax(x):
- * logp[i] = log p[tokens[i]], entropy[i] = -sum p log p, norm[i] = (m, log sum exp(x - m)) with m
- * = max x, and the `top` (at most PG_LOGPROB_TOP) largest log probabilities with their columns in top_logp and
- * top_ids [rows, top], ties to the lowest column. Tokens are int32 or int64 (token_bytes 4 or
+ * PG_DT_F32, PG_DT_BF16 or PG_DT_F16; rows row_stride elements apart) and p = softmax(x): logp[i]
+ * = log p[tokens[i]], entropy[i] = -sum p log p, norm[i] = (m, log sum exp(x - m)) with m = max x,
+ * and the `top` (at most PG_LOGPROB_TOP) largest log probabilities with their columns in top_logp
+ * and top_ids [rows, top], ties to the lowest column. Tokens are int32 or int64 (token_bytes 4 or
  * 8); token -1 means there is none: logp 0. A token outside [-1, vocab) gives NaN, as does a row
  * with a NaN, a +inf or nothing but -inf. Outputs are f32, top_ids int32. Asynchronous. */
 #define PG_LOGPROB_TOP 32
 int pg_logprobs(uint64_t logits, int64_t row_stride, int32_t dtype, uint64_t tokens,
                 int32_t token_bytes, int32_t rows, int32_t vocab, int32_t top, uint64_t logp,
-                uint64_t entropy, uint64_t lse, uint64_t top_logp, uint64_t top_ids,
+                uint64_t entropy, uint64_t norm, uint64_t top_logp, uint64_t top_ids,
                 uint64_t stream);
 
 /* The gradient of sum_i d_logp[i] logp[i] + d_entropy[i] entropy[i] with respect to the logits,
@@ -283,17 +284,19 @@ int pg_logprobs_grad(uint64_t logits, int64_t row_stride, int32_t dtype, uint64_
 /* --- attention over a paged cache -------------------------------------------------------------
  *
  * No counterpart in the reference. Sequence b of the batch is table row s = slots[b] (b where
- * slots is 0) with lens[s] tokens. Its queries are its last tokens: rows starts[b] to
- * starts[b + 1] of q, or row b alone where starts is 0 (one new token a sequence). The query at
- * position p sees key j when j <= p and (window == 0 or j > p - window or j < sinks);
- * out = softmax(scale q . k) v over the keys it sees. A query that sees none (a length of 0, or
- * fewer tokens than queries) gives zeros, and what lies in masked places, pages past the length
- * or unused rows of a page is never part of a result, whatever it is. A visible value that is not
- * finite makes its column of the result so: an infinity, where all such values are that one (or NaN,
- * where its weight is below 2^-126). Query head h reads kv head
- * h / group. q and out are [queries, heads * group, dim], k and v [pages, heads, page_size, dim]
- * with a head's rows of one page one after another; all of one dtype (PG_DT_F32, PG_DT_BF16 or
- * PG_DT_F16), with sums and softmax in 32 bits and one rounding of the result.
+ * slots is 0) with lens[s] tokens. Its queries are its last tokens: rows starts[b] to starts[b +
+ * 1] of q, or row b alone where starts is 0 (one new token a sequence). The query at position p
+ * sees key j when j <= p and (window == 0 or j > p - window or j < sinks); out = softmax(scale q .
+ * k) v over the keys it sees. A query that sees none (a length of 0, or fewer tokens than queries)
+ * gives zeros, and what lies in masked places, pages past the length or unused rows of a page is
+ * never part of a result, whatever it is. A visible value that is not finite makes its column of
+ * the result so: an infinity, where all such values are that one (or NaN, where its weight is
+ * below 2^-126). Query head h reads kv head h / group. q and out are [queries, heads * group,
+ * dim], k and v [pages, heads, page_size, dim] with a head's rows of one page one after another;
+ * all of one dtype (PG_DT_F32, PG_DT_BF16 or PG_DT_F16), with scores, maxima and sums in 32 bits.
+ * bf16 and f16 round the result to their type; where a batch has more than 48 rows (queries times
+ * group) a sequence on average and heads of up to 128, they round each weight to it as well,
+ * before its product with a value. Rows of q that no sequence has leave theirs of out as they are.
  *
  * max_len, if not 0, is at least the longest length; it only shapes the launch. The workspace
  * must be zeroed once, belongs to one stream at a time and is left as a next call needs it. Its
