@@ -13,13 +13,13 @@
     cache.check()                                # raises CacheError if a call could not be met
 
 ``ptxgen.attention`` reads the cache's ``k``, ``v``, ``table`` and ``lens``. Slots, starts and page
-ids are int32 device tensors, and nothing here waits for the GPU but ``check``: what only the
-device can see (no page left, a slot listed twice) sets bits of ``status``, and an ``extend`` or
+ids are int32 device tensors, and nothing here waits for the GPU but ``check`` and the making of a
+cache: what only the device can see (no page left, a slot listed twice) sets bits of ``status``, and an ``extend`` or
 ``fork`` that cannot be met changes nothing. A ``write`` that was queued behind a refused ``extend``
 leaves out that call's slots, since their last tokens are older ones, until an ``extend`` of them is
 met (by no tokens, if need be) or they are freed. Calls run on the current stream, or on ``stream``
-(a ``cudaStream_t`` as an integer); a cache's calls belong on one stream at a time, and the cache has to
-live until they have run.
+(a ``cudaStream_t`` as an integer); a cache's calls belong on one stream at a time, and the cache
+has to live until they have run.
 """
 
 from __future__ import annotations
