@@ -58,6 +58,17 @@ class Rows(ctypes.Structure):
                 ("head_stride", ctypes.c_int64)]
 
 
+class SampleArgs(ctypes.Structure):
+    """``pg_sample_args``: drawing a token of each row (``ptxgen.sampling``)."""
+
+    _fields_ = [*((n, ctypes.c_uint64) for n in ("logits", "uniform", "temperature", "top_k",
+                                                 "top_p", "min_p", "tokens", "logp")),
+                ("row_stride", ctypes.c_int64),
+                *((n, ctypes.c_int32) for n in ("dtype", "rows", "vocab", "top_k_all")),
+                *((n, ctypes.c_float) for n in ("temperature_all", "top_p_all", "min_p_all")),
+                ("reserved", ctypes.c_int32)]
+
+
 class AttentionArgs(ctypes.Structure):
     """``pg_attention_args``: attention over a paged cache (``ptxgen.attention``)."""
 
@@ -121,6 +132,7 @@ def library() -> ctypes.CDLL:
                 "pg_cache_fork": [ctypes.POINTER(Cache), u64, u64, i32, u64],
                 "pg_cache_compact": [ctypes.POINTER(Cache), u64],
                 "pg_attention": [ctypes.POINTER(AttentionArgs), u64],
+                "pg_sample": [ctypes.POINTER(SampleArgs), u64],
                 "pg_logprobs": [u64, ctypes.c_int64, i32, u64, i32, i32, i32, i32, u64, u64, u64,
                                 u64, u64, u64],
                 "pg_logprobs_grad": [u64, ctypes.c_int64, i32, u64, i32, i32, i32, u64, u64, u64,

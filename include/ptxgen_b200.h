@@ -281,6 +281,31 @@ int pg_logprobs_grad(uint64_t logits, int64_t row_stride, int32_t dtype, uint64_
                      uint64_t entropy, uint64_t d_logp, uint64_t d_entropy, uint64_t out,
                      int64_t out_stride, uint64_t stream);
 
+/* --- drawing tokens ---------------------------------------------------------------------------
+ *
+ * No counterpart in the reference. For each row x of `rows` rows of `vocab` logits (as for
+ * pg_logprobs), with m = max x and w = exp((x - m) / T): the kept tokens are a prefix of the tokens
+ * ordered by logit, the largest first and ties by the lowest column, the shortest of the first
+ * top_k (0: all), the fewest whose w reach top_p of the sum of the top_k ones' (1: all) and those
+ * with w >= min_p; one at least. tokens[i] is the lowest kept column up to which the kept w add up to
+ * more than uniform[i] of their sum, logp[i] the log of its share. T = 0 takes the first of the
+ * largest. Weights and sums are 64-bit. A column of -inf is never drawn. A row with a NaN, a +inf or
+ * nothing but -inf, or one whose uniform, temperature, top_p or min_p is NaN, temperature negative or
+ * min_p above 1, gives token -1 and NaN; uniform is below 1, and 1 and more take the last kept column.
+ * Each setting has a value a row (an address, of float32 or for top_k int32) or, where that is 0, one
+ * for all. Asynchronous. */
+typedef struct pg_sample_args {
+  uint64_t logits, uniform;                     /* uniform: float32 [rows] */
+  uint64_t temperature, top_k, top_p, min_p;    /* [rows] each, or 0 */
+  uint64_t tokens, logp;                        /* int64, float32 [rows] */
+  int64_t row_stride;                           /* elements */
+  int32_t dtype, rows, vocab, top_k_all;
+  float temperature_all, top_p_all, min_p_all;
+  int32_t reserved;                             /* 0 */
+} pg_sample_args;
+
+int pg_sample(const pg_sample_args *args, uint64_t stream);
+
 /* --- attention over a paged cache -------------------------------------------------------------
  *
  * No counterpart in the reference. Sequence b of the batch is table row s = slots[b] (b where
