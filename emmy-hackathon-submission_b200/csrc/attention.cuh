@@ -22,11 +22,14 @@ struct Attention {
   const char *q, *k, *v;
   char *out;
   const int *starts, *slots, *table, *lens;
+  const char *k_scale, *v_scale;  // of a cache in 8 bits: an f32 number a key and head, else null
+  const uint64_t *mask;           // of a tree's queries: which new tokens each sees, else null
   float *partial;       // per (tile, kv head, part): rows * (dim + 2) floats
   unsigned *arrived;    // per (tile, kv head): parts that have finished; 0 between calls
   unsigned *status;
   int64_t q_token, q_head, out_token, out_head;       // bytes
   int64_t k_page, k_head, v_page, v_head, table_row;  // bytes, bytes, bytes, bytes, words
+  int64_t ks_page, ks_head, vs_page, vs_head;         // bytes, of the scales
   int batch, queries, heads, group, dim, page_size, pages, width, slot_rows;
   int window, sinks, parts, rows_per_tile;
   float scale_log2;
@@ -56,6 +59,46 @@ __device__ __forceinline__ bool sees(const Attention &a, int pos, int key) {
   return key <= pos && (!a.window || key > pos - a.window || key < a.sinks);
 }
 
+// What one query sees. TREE: its sequence's new tokens begin at position `base` and are a tree, of which
+// it sees those that are set in `mask` (with a bit for each, the first the lowest) and which there stand
+// one behind the other, as on the way from the root to it. So it stands at base + n - 1 for n of them, a
+// key before base at its position as ever, and the k-th of them at base + k.
+template <bool TREE>
+struct Sight {
+  int pos, base;
+  uint64_t mask;
+  __device__ static Sight of(const Attention &a, int first_pos, int count, int query, int at) {
+    if constexpr (!TREE) {
+      return Sight{first_pos + at, 0, 0};
+    } else {
+      uint64_t m = a.mask[query + at];
+      if (count < 64) m &= (1ull << count) - 1;
+      // tokens before the sequence's start are none (it is shorter than its queries)
+      if (first_pos < 0) m = first_pos + at < 0 || first_pos <= -64 ? 0 : m >> -first_pos << -first_pos;
+      const int n = __popcll(m);
+      if (a.window && n > a.window) {
+        // the window hides the first of them, but for those that the sinks show
+        int hidden = n - a.window, rank = 0;
+        for (uint64_t rest = m; hidden > 0; --hidden, ++rank) {
+          const uint64_t low = rest & (0 - rest);
+          rest ^= low;
+          if (first_pos + rank >= a.sinks) m ^= low;
+        }
+      }
+      return Sight{first_pos + n - 1, first_pos, m};
+    }
+  }
+  // whether it sees no key at all
+  __device__ bool none() const { return TREE ? base <= 0 && !mask : pos < 0; }
+  __device__ bool sees(const Attention &a, int key) const {
+    if constexpr (TREE) {
+      if (key >= base) return key - base < 64 && (mask >> (key - base) & 1);
+      return !a.window || key > pos - a.window || key < a.sinks;
+    }
+    return pg::sees(a, pos, key);
+  }
+};
+
 // A tile: rows [row, row + rows) of the (query, head in group) rows of one sequence.
 struct Tile {
   int sequence, row, rows, query, count, length;  // query: the sequence's first query
@@ -73,7 +116,7 @@ __device__ __forceinline__ Tile find_tile(const Attention &a, int tile) {
     if (b < a.batch) {
       start = a.starts ? a.starts[b] : b;
       count = a.starts ? max(0, a.starts[b + 1] - start) : 1;
-      if (start < 0 || count > a.queries - start) {
+      if (start < 0 || count > a.queries - start || (a.mask && count > PG_ATTENTION_TREE)) {
         atomicOr(a.status, PG_CACHE_TOO_LONG);
         count = 0;
       }
@@ -172,9 +215,20 @@ __device__ __forceinline__ float factor(float a, float b) {
 // Kernels for head sizes of up to 128: few rows a sequence (attention_decode.cu), and many in the
 // 16-bit types (attention_prompt.cu).
 bool decode_takes(const Attention &a, bool f32, int most, int max_len);
+bool decode_counts(const Attention &a, int most);  // its blocks of keys, in 31 bits
 int decode(const Attention &a, int dtype, int sms, cudaStream_t stream);
+// ... of few rows a sequence over a cache in 8 bits, and of trees of tokens.
+int decode_8bit(const Attention &a, int dtype, int sms, cudaStream_t stream);
+int decode_tree(const Attention &a, int dtype, int sms, cudaStream_t stream);
 int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                  cudaStream_t stream);
+int prompt_tree(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
+                cudaStream_t stream);
+// For every head size and number of rows, in 32-bit arithmetic (attention_any.cuh).
+int any_rows_8bit(const Attention &a, int dtype, int max_len, int64_t partial_bytes, int sms,
+                  cudaStream_t stream);
+int any_rows_tree(const Attention &a, int dtype, int max_len, int64_t partial_bytes, int sms,
+                  cudaStream_t stream);
 
 // --- host side -------------------------------------------------------------------------------
 

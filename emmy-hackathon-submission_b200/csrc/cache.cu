@@ -292,7 +292,20 @@ __global__ void __launch_bounds__(kCopy) cache_free(pg_cache c, const int *slots
 // values. HBM bounds it: each piece is read and written once, 16 bytes a lane, and 6.2 TB/s to 6.8
 // are reached by the forks and moves named above.
 
-__device__ void copy_rows(const pg_cache &c, char *base, int layer, int from, int to, int rows) {
+// A cache in 8 bits has its rows' scales copied, too.
+
+__device__ void copy_rows(const pg_cache &c, const pg_cache_scales &s, bool values, int layer,
+                          int from, int to, int rows) {
+  char *const base = reinterpret_cast<char *>(values ? c.v : c.k);
+  if (const uint64_t scales = values ? s.v : s.k) {
+    char *const at = reinterpret_cast<char *>(scales) + layer * s.layer_stride;
+    for (int i = threadIdx.x; i < c.heads * rows; i += kCopy) {
+      const int head = i / rows;
+      const int64_t in = head * s.head_stride + (i - head * rows) * 4ll;
+      *reinterpret_cast<float *>(at + to * s.page_stride + in) =
+          *reinterpret_cast<const float *>(at + from * s.page_stride + in);
+    }
+  }
   const int per_head = rows * (c.row_bytes / 16), all = c.heads * per_head;
   const char *src = base + layer * c.layer_stride + from * c.page_stride;
   char *dst = base + layer * c.layer_stride + to * c.page_stride;
@@ -312,8 +325,8 @@ __device__ void copy_rows(const pg_cache &c, char *base, int layer, int from, in
 }
 
 // Pair i's pages, whole, in every layer's keys and values.
-__global__ void __launch_bounds__(kCopy) cache_copy(pg_cache c, const int *from, const int *to,
-                                                    int n) {
+__global__ void __launch_bounds__(kCopy) cache_copy(pg_cache c, pg_cache_scales s,
+                                                    const int *from, const int *to, int n) {
   pg::wait_for_earlier_kernels();
   const int64_t tasks = static_cast<int64_t>(n) * c.layers * 2;
   for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
@@ -324,7 +337,7 @@ __global__ void __launch_bounds__(kCopy) cache_copy(pg_cache c, const int *from,
       if (threadIdx.x == 0) set_status(c, PG_CACHE_BAD_PAGE);
       continue;
     }
-    copy_rows(c, reinterpret_cast<char *>(plane & 1 ? c.v : c.k), plane >> 1, a, b, c.page_size);
+    copy_rows(c, s, plane & 1, plane >> 1, a, b, c.page_size);
   }
 }
 
@@ -417,8 +430,9 @@ __global__ void __cluster_dims__(kLook, 1, 1) __launch_bounds__(kPlan)
 
 // Task i * (2 layers + 1) + j: child i's table row and counts (j = 0), or the rows in use of its
 // open page in one layer's keys or values.
-__global__ void __launch_bounds__(kCopy) cache_fork_copy(pg_cache c, const int *parents,
-                                                         const int *children, int n) {
+__global__ void __launch_bounds__(kCopy) cache_fork_copy(pg_cache c, pg_cache_scales s,
+                                                         const int *parents, const int *children,
+                                                         int n) {
   pg::wait_for_earlier_kernels();
   const int *scratch = reinterpret_cast<const int *>(c.scratch);
   if (!scratch[0]) return;
@@ -432,8 +446,7 @@ __global__ void __launch_bounds__(kCopy) cache_fork_copy(pg_cache c, const int *
     const int *from = row_of(c, parents[i]);
     if (part) {
       if (open)
-        copy_rows(c, reinterpret_cast<char *>(part & 1 ? c.k : c.v), (part - 1) >> 1, from[full],
-                  fresh[offset[i]], open);
+        copy_rows(c, s, !(part & 1), (part - 1) >> 1, from[full], fresh[offset[i]], open);
       continue;
     }
     int *row = row_of(c, children[i]);
@@ -474,7 +487,7 @@ __global__ void __launch_bounds__(kPlan) cache_compact_plan(pg_cache c) {
 
 // Tasks below `slots` rewrite one slot's table row; the others move one page in one layer's
 // keys or values.
-__global__ void __launch_bounds__(kCopy) cache_compact_move(pg_cache c) {
+__global__ void __launch_bounds__(kCopy) cache_compact_move(pg_cache c, pg_cache_scales s) {
   pg::wait_for_earlier_kernels();
   const int *scratch = reinterpret_cast<const int *>(c.scratch);
   const int live = scratch[0], moves = scratch[1];
@@ -496,9 +509,396 @@ __global__ void __launch_bounds__(kCopy) cache_compact_move(pg_cache c) {
     const int64_t move = task - c.slots;
     const int i = static_cast<int>(move / (2 * c.layers));
     const int plane = static_cast<int>(move - static_cast<int64_t>(i) * 2 * c.layers);
-    copy_rows(c, reinterpret_cast<char *>(plane & 1 ? c.v : c.k), plane >> 1, movers[i],
-              holes[i], c.page_size);
+    copy_rows(c, s, plane & 1, plane >> 1, movers[i], holes[i], c.page_size);
   }
+}
+
+// --- rows in 8 bits ----------------------------------------------------------------------------
+// A row (one token's numbers of one head) is held as q = round(x / s), halves to even, with s = max |x| /
+// 127 in f32: at 16 bits of it that is 8, and an error of at most s / 2. As few lanes as have 16 numbers
+// each take a row. HBM bounds both ways: 40 sequences of up to 4096 tokens of 8 heads of 128 in bf16 are
+// written and read back in LARGE us.
+
+// 16 numbers of T at an address as f32, and to it.
+template <class T> struct Sixteen;
+template <> struct Sixteen<float> {
+  static constexpr int words = 4;
+  __device__ static void get(const uint4 *raw, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[4 * i] = __uint_as_float(raw[i].x), x[4 * i + 1] = __uint_as_float(raw[i].y);
+      x[4 * i + 2] = __uint_as_float(raw[i].z), x[4 * i + 3] = __uint_as_float(raw[i].w);
+    }
+  }
+  __device__ static void put(const float *x, uint4 *raw) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      raw[i] = make_uint4(__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]),
+                          __float_as_uint(x[4 * i + 2]), __float_as_uint(x[4 * i + 3]));
+  }
+};
+template <class T, class T2> struct Sixteen16 {
+  static constexpr int words = 2;
+  __device__ static void get(const uint4 *raw, float *x) {
+    const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w,
+                           raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T2 h = *reinterpret_cast<const T2 *>(&w[i]);
+      x[2 * i] = __low2float(h), x[2 * i + 1] = __high2float(h);
+    }
+  }
+};
+template <> struct Sixteen<__nv_bfloat16> : Sixteen16<__nv_bfloat16, __nv_bfloat162> {
+  __device__ static void put(const float *x, uint4 *raw) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    raw[0] = make_uint4(w[0], w[1], w[2], w[3]), raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+};
+template <> struct Sixteen<__half> : Sixteen16<__half, __half2> {
+  __device__ static void put(const float *x, uint4 *raw) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    raw[0] = make_uint4(w[0], w[1], w[2], w[3]), raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+};
+
+// x / s for 16 numbers, rounded, halves to even. x times 1 / s is off by up to 2^-15 at 127, so a number
+// whose fraction is that near to a half is divided in 64 bits, where the quotient of two f32 numbers is a
+// half only if it is one.
+__device__ __forceinline__ uint4 quantise(const float *x, float s) {
+  // a scale whose inverse is no f32 number, or that has lost bits itself, has them all divided
+  const bool small = s < 0x1p-100f;
+  const float inverse = small ? 0.0f : 1.0f / s;
+  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: its last bits are a whole number's
+  float y[16];
+  bool near = small;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float t = x[i] * inverse;
+    y[i] = t + kShift;
+    near |= fabsf(t - (y[i] - kShift)) > 0.5f - 0x1p-14f;
+  }
+  if (near && s > 0.0f) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const double t = static_cast<double>(x[i]) / static_cast<double>(s);
+      y[i] = kShift + static_cast<float>(fmin(fmax(rint(t), -127.0), 127.0));
+    }
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __byte_perm(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), 0x0040);
+    const uint32_t b =
+        __byte_perm(__float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]), 0x0040);
+    w[i] = __byte_perm(a, b, 0x5410);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Where a token's rows are in a layer: its place among the pages, or -1 where there is none.
+struct Place {
+  int page, row;
+};
+__device__ __forceinline__ Place place_of(const pg_cache &c, const int *slots_in, const int *starts,
+                                          int n, int t, bool marks) {
+  const bool first = (threadIdx.x & 31) == 0;
+  const Place none{-1, 0};
+  if (t < starts[0] || t >= starts[n]) return none;
+  const int i = find_sequence(starts, n, t);
+  const int slot = slots_in[i];
+  if (slot < 0 || slot >= c.slots) {
+    if (first) set_status(c, PG_CACHE_BAD_SLOT);
+    return none;
+  }
+  if (marks && refused_of(c)[slot]) {
+    if (first) set_status(c, PG_CACHE_REFUSED);
+    return none;
+  }
+  const int pos = lens_of(c)[slot] - (starts[i + 1] - t);
+  const int64_t entry = pos / c.page_size;
+  const int page = pos >= 0 && entry < c.width ? row_of(c, slot)[entry] : -1;
+  if (page < 0 || page >= c.pages) {
+    if (first) set_status(c, PG_CACHE_BAD_PAGE);
+    return none;
+  }
+  return Place{page, pos % c.page_size};
+}
+
+constexpr int kRowsAhead = 2;  // rows that a lane has in flight
+
+// WRITE: rows are quantised into the cache, else read back from it. A warp takes one token.
+template <class T, bool WRITE>
+__global__ void __launch_bounds__(kCopy) cache8_rows(pg_cache c, pg_cache_scales s, int layer,
+                                                     const int *slots_in, const int *starts, int n,
+                                                     int tokens, pg_rows k, pg_rows v) {
+  using X = Sixteen<T>;
+  pg::wait_for_earlier_kernels();
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (kCopy / 32);
+  const int pieces = c.row_bytes / 16;
+  int lanes = 1;  // that take a row
+  while (lanes < pieces) lanes *= 2;
+  const int sub = lane & (lanes - 1), step = 32 / lanes, rows = 2 * c.heads;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && (starts[0] < 0 || starts[n] > tokens))
+    set_status(c, PG_CACHE_TOO_LONG);  // tokens that have no rows
+  for (int t = (blockIdx.x * kCopy + threadIdx.x) >> 5; t < tokens; t += warps) {
+    const Place at = place_of(c, slots_in, starts, n, t, WRITE);
+    if (at.page < 0) continue;
+    const int64_t in_cache = layer * c.layer_stride + at.page * c.page_stride +
+                             static_cast<int64_t>(at.row) * c.row_bytes + sub * 16;
+    const int64_t in_scales = layer * s.layer_stride + at.page * s.page_stride + at.row * 4ll;
+    // row r of this lane's: the plane's first, then the other's
+    const auto head_of = [&](int r) { return r < c.heads ? r : r - c.heads; };
+    const auto cache_at = [&](int r) {
+      return reinterpret_cast<uint4 *>((r < c.heads ? c.k : c.v) + in_cache +
+                                       head_of(r) * c.head_stride);
+    };
+    const auto scale_at = [&](int r) {
+      return reinterpret_cast<float *>((r < c.heads ? s.k : s.v) + in_scales +
+                                       head_of(r) * s.head_stride);
+    };
+    const auto user_at = [&](int r) {
+      const pg_rows &u = r < c.heads ? k : v;
+      return reinterpret_cast<uint4 *>(u.data + t * u.token_stride + head_of(r) * u.head_stride) +
+             sub * X::words;
+    };
+    for (int base = lane / lanes; base < rows + lane / lanes; base += kRowsAhead * step) {
+      if constexpr (WRITE) {
+        uint4 raw[kRowsAhead][X::words] = {};
+#pragma unroll
+        for (int j = 0; j < kRowsAhead; ++j) {
+          const int r = base + j * step;
+          if (r < rows && sub < pieces)
+#pragma unroll
+            for (int i = 0; i < X::words; ++i) raw[j][i] = user_at(r)[i];
+        }
+#pragma unroll
+        for (int j = 0; j < kRowsAhead; ++j) {
+          const int r = base + j * step;
+          float x[16];
+          X::get(raw[j], x);
+          uint32_t most = 0;  // of their sizes' bits, which are in the numbers' order, NaN the last
+#pragma unroll
+          for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+          for (int off = lanes / 2; off; off /= 2)
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+          const bool finite = most < 0x7f800000u;
+          const float scale = finite ? __fdiv_rn(__uint_as_float(most), 127.0f) : NAN;
+          if (r < rows && sub < pieces) {
+            // of a row that is not finite nothing is kept but that
+            *cache_at(r) = finite ? quantise(x, scale) : make_uint4(0, 0, 0, 0);
+            if (sub == 0) *scale_at(r) = scale;
+          }
+        }
+      } else {
+        uint4 raw[kRowsAhead];
+        float scale[kRowsAhead];
+#pragma unroll
+        for (int j = 0; j < kRowsAhead; ++j) {
+          const int r = base + j * step;
+          if (r < rows && sub < pieces) raw[j] = *cache_at(r), scale[j] = *scale_at(r);
+        }
+#pragma unroll
+        for (int j = 0; j < kRowsAhead; ++j) {
+          const int r = base + j * step;
+          if (!(r < rows && sub < pieces)) continue;
+          const uint32_t w[4] = {raw[j].x ^ 0x80808080u, raw[j].y ^ 0x80808080u,
+                                 raw[j].z ^ 0x80808080u, raw[j].w ^ 0x80808080u};
+          float x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)  // 2^23 + 128 + q, less the former
+            x[i] = (__uint_as_float(__byte_perm(w[i / 4], 0x4b000000u, 0x7440 + i % 4)) -
+                    8388736.0f) * scale[j];
+          uint4 out[X::words];
+          X::put(x, out);
+#pragma unroll
+          for (int i = 0; i < X::words; ++i) user_at(r)[i] = out[i];
+        }
+      }
+    }
+  }
+}
+
+// The rows of a cache that is not in 8 bits, as they are.
+__global__ void __launch_bounds__(kCopy) cache_read(pg_cache c, int layer, const int *slots_in,
+                                                    const int *starts, int n, int tokens, pg_rows k,
+                                                    pg_rows v) {
+  pg::wait_for_earlier_kernels();
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (kCopy / 32);
+  const int pieces = c.row_bytes / 16, all = 2 * c.heads * pieces;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && (starts[0] < 0 || starts[n] > tokens))
+    set_status(c, PG_CACHE_TOO_LONG);
+  for (int t = (blockIdx.x * kCopy + threadIdx.x) >> 5; t < tokens; t += warps) {
+    const Place at = place_of(c, slots_in, starts, n, t, false);
+    if (at.page < 0) continue;
+    const int64_t in = layer * c.layer_stride + at.page * c.page_stride +
+                       static_cast<int64_t>(at.row) * c.row_bytes;
+    for (int base = lane; base < all; base += 32 * kUnroll) {
+      uint4 x[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int j = base + 32 * u, r = j / pieces, head = r < c.heads ? r : r - c.heads;
+        if (j < all)
+          x[u] = pg::load16(reinterpret_cast<const char *>(r < c.heads ? c.k : c.v) + in +
+                            head * c.head_stride + (j - r * pieces) * 16);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int j = base + 32 * u, r = j / pieces, head = r < c.heads ? r : r - c.heads;
+        const pg_rows &to = r < c.heads ? k : v;
+        if (j < all)
+          *reinterpret_cast<uint4 *>(to.data + t * to.token_stride + head * to.head_stride +
+                                     (j - r * pieces) * 16) = x[u];
+      }
+    }
+  }
+}
+
+// --- keep: an accepted branch stays, the rest of the drafted tokens goes ---------------------------
+// Of a slot's last tokens (its drafts) those in a set stay and move together, behind what was there
+// before. A block takes a slot's rows of one layer, and a thread 16 bytes of all of them from the first
+// to the last: a token never moves up, so what a move writes over has been moved before or goes. The
+// blocks all look whether a slot's request can be met, in the same way and before anything changes; the
+// pages and lengths follow in a second kernel.
+
+constexpr int kDrafts = 64;  // bits of a set
+
+struct Drafts {
+  bool good;
+  int slot, length, base, moves;  // base: the position of the first of them
+  uint64_t kept;
+};
+
+// A warp's: the request of entry i, and where its moves come from and go to (byte offsets of rows in a
+// layer's keys; page and row are what the scales need).
+__device__ Drafts drafts_of(const pg_cache &c, const int *slots_in, const int *starts,
+                            const uint64_t *kept, int n, int i, int2 *from, int2 *to) {
+  const int lane = threadIdx.x & 31;
+  Drafts d{};
+  d.slot = slots_in[i];
+  const int count = starts[i + 1] - starts[i];
+  unsigned bad = 0;
+  bool twice = false;
+  for (int j = lane; j < n; j += 32) twice |= j != i && slots_in[j] == d.slot;
+  if (__any_sync(0xffffffffu, twice) || d.slot < 0 || d.slot >= c.slots) {
+    bad = PG_CACHE_BAD_SLOT;
+  } else if (refused_of(c)[d.slot]) {
+    bad = PG_CACHE_REFUSED;
+  } else {
+    d.length = lens_of(c)[d.slot];
+    d.base = d.length - count;
+    if (count < 0 || count > kDrafts || d.base < 0 || d.length > c.width * static_cast<int64_t>(c.page_size))
+      bad = PG_CACHE_TOO_LONG;
+  }
+  if (!bad) {
+    d.kept = count < 64 ? kept[i] & ((1ull << count) - 1) : kept[i];
+    const int *row = row_of(c, d.slot);
+    bool wrong = false;
+    for (int b = lane; b < kDrafts; b += 32) {
+      if (b >= count) continue;
+      const int pos = d.base + b, page = row[pos / c.page_size];
+      if (page < 0 || page >= c.pages) wrong = true;
+      const int rank = __popcll(d.kept & ((1ull << b) - 1));
+      if (!(d.kept >> b & 1) || wrong) continue;
+      const int target = d.base + rank, target_page = row[target / c.page_size];
+      if (target_page < 0 || target_page >= c.pages) {
+        wrong = true;
+        continue;
+      }
+      // other slots may read what is shared
+      if (rank != b && refs_of(c)[target_page] != 1) wrong = true;
+      from[rank] = make_int2(page, pos % c.page_size);
+      to[rank] = make_int2(target_page, target % c.page_size);
+    }
+    if (__any_sync(0xffffffffu, wrong)) bad = PG_CACHE_BAD_PAGE;
+  }
+  d.good = !bad;
+  d.moves = __popcll(d.kept);
+  if (bad && lane == 0) set_status(c, bad);
+  __syncwarp();
+  return d;
+}
+
+__global__ void __launch_bounds__(kCopy) cache_keep_move(pg_cache c, pg_cache_scales s,
+                                                         const int *slots_in, const int *starts,
+                                                         const uint64_t *kept, int n) {
+  __shared__ int2 from[kDrafts], to[kDrafts];
+  __shared__ int first, moves;
+  pg::wait_for_earlier_kernels();
+  int *verdict = reinterpret_cast<int *>(c.scratch) + kHeader;
+  const int pieces = c.row_bytes / 16, plane = c.heads * pieces;
+  const int64_t tasks = static_cast<int64_t>(n) * c.layers;
+  for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const int i = static_cast<int>(task / c.layers), layer = static_cast<int>(task % c.layers);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const Drafts d = drafts_of(c, slots_in, starts, kept, n, i, from, to);
+      if (threadIdx.x == 0) {
+        // those that stay in front stay where they are
+        first = __ffsll(~d.kept) ? __ffsll(~d.kept) - 1 : kDrafts;
+        moves = d.good ? d.moves : 0;
+        if (layer == 0) verdict[i] = d.good;
+      }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < 2 * plane; j += kCopy) {
+      const int r = j < plane ? j : j - plane, head = r / pieces;
+      char *const at = reinterpret_cast<char *>(j < plane ? c.k : c.v) + layer * c.layer_stride +
+                       head * c.head_stride + (r - head * pieces) * 16;
+      for (int m0 = first; m0 < moves; m0 += kUnroll) {
+        uint4 x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (m0 + u < moves)
+            x[u] = pg::load16(at + from[m0 + u].x * c.page_stride +
+                              static_cast<int64_t>(from[m0 + u].y) * c.row_bytes);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (m0 + u < moves)
+            *reinterpret_cast<uint4 *>(at + to[m0 + u].x * c.page_stride +
+                                       static_cast<int64_t>(to[m0 + u].y) * c.row_bytes) = x[u];
+      }
+    }
+    if (s.k)
+      for (int j = threadIdx.x; j < 2 * c.heads; j += kCopy) {
+        char *const at = reinterpret_cast<char *>(j < c.heads ? s.k : s.v) + layer * s.layer_stride +
+                         (j < c.heads ? j : j - c.heads) * s.head_stride;
+        for (int m = first; m < moves; ++m)
+          *reinterpret_cast<float *>(at + to[m].x * s.page_stride + to[m].y * 4ll) =
+              *reinterpret_cast<const float *>(at + from[m].x * s.page_stride + from[m].y * 4ll);
+      }
+  }
+}
+
+// A warp a slot: its new length, and the pages past it go.
+__global__ void __launch_bounds__(kCopy) cache_keep_drop(pg_cache c, const int *slots_in,
+                                                         const int *starts, const uint64_t *kept,
+                                                         int n) {
+  pg::wait_for_earlier_kernels();
+  const int lane = threadIdx.x & 31, i = (blockIdx.x * kCopy + threadIdx.x) >> 5;
+  const int *verdict = reinterpret_cast<const int *>(c.scratch) + kHeader;
+  if (i >= n || !verdict[i]) return;
+  const int slot = slots_in[i], count = starts[i + 1] - starts[i];
+  const uint64_t set = count < 64 ? kept[i] & ((1ull << count) - 1) : kept[i];
+  const int old = lens_of(c)[slot], length = old - count + __popcll(set);
+  int *row = row_of(c, slot);
+  for (int j = ceil_div(length, c.page_size) + lane; j < ceil_div(old, c.page_size); j += 32) {
+    const int page = row[j];
+    row[j] = -1;
+    if (atomicSub(refs_of(c) + page, 1) <= 0) set_status(c, PG_CACHE_BAD_PAGE);
+  }
+  __syncwarp();
+  if (lane == 0) lens_of(c)[slot] = length;
 }
 
 // --- host side ---------------------------------------------------------------------------------
@@ -557,6 +957,17 @@ int check_rows(const char *what, const pg_rows *r) {
   return PG_OK;
 }
 
+int check_scales(const char *what, const pg_cache *c, const pg_cache_scales *s) {
+  if (!s || !s->k || !s->v) return pg::argument_fail("%s: null scales", what);
+  if ((s->k | s->v | static_cast<uint64_t>(s->layer_stride | s->page_stride | s->head_stride)) & 3)
+    return pg::argument_fail("%s: scales and their strides must be multiples of 4 bytes", what);
+  if (c->row_bytes > 512)
+    return pg::argument_fail("%s: heads of %d in 8 bits, want 512 at most", what, c->row_bytes);
+  return PG_OK;
+}
+
+const pg_cache_scales kNoScales = {};
+
 // Blocks for `tasks` tasks: one each, up to the most, which loop.
 int copy_grid(int64_t tasks, int *grid) {
   int sms;
@@ -609,19 +1020,19 @@ extern "C" int pg_cache_free(const pg_cache *c, uint64_t slots, int32_t n, uint6
                     ints(slots), n);
 }
 
-extern "C" int pg_cache_copy(const pg_cache *c, uint64_t from, uint64_t to, int32_t n,
-                             uint64_t stream) {
-  int rc = check_list("pg_cache_copy", c, from, to, n, c ? c->pages : 0);
+static int copy_pages(const char *what, const pg_cache *c, const pg_cache_scales &s, uint64_t from,
+                      uint64_t to, int32_t n, uint64_t stream) {
+  int rc = check_list(what, c, from, to, n, c ? c->pages : 0);
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(static_cast<int64_t>(n) * c->layers * 2, &grid))) return rc;
-  return pg::launch<cache_copy>("cache_copy", dim3(grid), kCopy, 0, stream_of(stream), *c,
+  return pg::launch<cache_copy>("cache_copy", dim3(grid), kCopy, 0, stream_of(stream), *c, s,
                     ints(from), ints(to), n);
 }
 
-extern "C" int pg_cache_fork(const pg_cache *c, uint64_t parents, uint64_t children, int32_t n,
-                             uint64_t stream) {
-  int rc = check_slots("pg_cache_fork", c, parents, children, n);
+static int fork(const char *what, const pg_cache *c, const pg_cache_scales &s, uint64_t parents,
+                uint64_t children, int32_t n, uint64_t stream) {
+  int rc = check_slots(what, c, parents, children, n);
   if (rc || !n) return rc;
   int grid;
   if ((rc = copy_grid(static_cast<int64_t>(n) * (2 * c->layers + 1), &grid))) return rc;
@@ -629,11 +1040,11 @@ extern "C" int pg_cache_fork(const pg_cache *c, uint64_t parents, uint64_t child
                   ints(parents), ints(children), n);
   if (rc) return rc;
   return pg::launch<cache_fork_copy>("cache_fork_copy", dim3(grid), kCopy, 0, stream_of(stream),
-                    *c, ints(parents), ints(children), n);
+                    *c, s, ints(parents), ints(children), n);
 }
 
-extern "C" int pg_cache_compact(const pg_cache *c, uint64_t stream) {
-  int rc = check("pg_cache_compact", c);
+static int compact(const char *what, const pg_cache *c, const pg_cache_scales &s, uint64_t stream) {
+  int rc = check(what, c);
   if (rc) return rc;
   int grid;
   if ((rc = copy_grid(c->slots + static_cast<int64_t>(c->pages) * c->layers, &grid))) return rc;
@@ -641,5 +1052,123 @@ extern "C" int pg_cache_compact(const pg_cache *c, uint64_t stream) {
                   *c);
   if (rc) return rc;
   return pg::launch<cache_compact_move>("cache_compact_move", dim3(grid), kCopy, 0,
-                    stream_of(stream), *c);
+                    stream_of(stream), *c, s);
+}
+
+extern "C" int pg_cache_copy(const pg_cache *c, uint64_t from, uint64_t to, int32_t n,
+                             uint64_t stream) {
+  return copy_pages("pg_cache_copy", c, kNoScales, from, to, n, stream);
+}
+
+extern "C" int pg_cache_fork(const pg_cache *c, uint64_t parents, uint64_t children, int32_t n,
+                             uint64_t stream) {
+  return fork("pg_cache_fork", c, kNoScales, parents, children, n, stream);
+}
+
+extern "C" int pg_cache_compact(const pg_cache *c, uint64_t stream) {
+  return compact("pg_cache_compact", c, kNoScales, stream);
+}
+
+// Of a cache in 8 bits: the arguments' checks that all of these share.
+static int check8(const char *what, const pg_cache *c, const pg_cache_scales *s) {
+  const int rc = check(what, c);
+  return rc ? rc : check_scales(what, c, s);
+}
+
+extern "C" int pg_cache8_copy(const pg_cache *c, const pg_cache_scales *s, uint64_t from, uint64_t to,
+                              int32_t n, uint64_t stream) {
+  const int rc = check8("pg_cache8_copy", c, s);
+  return rc ? rc : copy_pages("pg_cache8_copy", c, *s, from, to, n, stream);
+}
+
+extern "C" int pg_cache8_fork(const pg_cache *c, const pg_cache_scales *s, uint64_t parents,
+                              uint64_t children, int32_t n, uint64_t stream) {
+  const int rc = check8("pg_cache8_fork", c, s);
+  return rc ? rc : fork("pg_cache8_fork", c, *s, parents, children, n, stream);
+}
+
+extern "C" int pg_cache8_compact(const pg_cache *c, const pg_cache_scales *s, uint64_t stream) {
+  const int rc = check8("pg_cache8_compact", c, s);
+  return rc ? rc : compact("pg_cache8_compact", c, *s, stream);
+}
+
+// Rows in and out of a layer, the arguments of both.
+static int check_layer(const char *what, const pg_cache *c, int32_t layer, uint64_t slots,
+                       uint64_t starts, int32_t n, int32_t tokens, const pg_rows *k,
+                       const pg_rows *v) {
+  int rc = check_slots(what, c, slots, starts, n);
+  if (rc) return rc;
+  if (layer < 0 || layer >= c->layers || tokens < 0)
+    return pg::argument_fail("%s: layer %d of %d, %d tokens", what, layer, c->layers, tokens);
+  if (!n || !tokens) return PG_OK;
+  if ((rc = check_rows(what, k))) return rc;
+  return check_rows(what, v);
+}
+
+template <class T, bool WRITE>
+static int launch_rows(const pg_cache *c, const pg_cache_scales *s, int32_t layer, uint64_t slots,
+                       uint64_t starts, int32_t n, int32_t tokens, const pg_rows *k,
+                       const pg_rows *v, uint64_t stream) {
+  int grid;
+  const int rc = copy_grid((tokens + kCopy / 32 - 1) / (kCopy / 32), &grid);
+  if (rc) return rc;
+  return pg::launch<cache8_rows<T, WRITE>>("cache8_rows", dim3(grid), kCopy, 0, stream_of(stream),
+                                           *c, *s, layer, ints(slots), ints(starts), n, tokens, *k,
+                                           *v);
+}
+
+extern "C" int pg_cache8_write(const pg_cache *c, const pg_cache_scales *s, int32_t layer,
+                               uint64_t slots, uint64_t starts, int32_t n, int32_t tokens,
+                               int32_t dtype, const pg_rows *k, const pg_rows *v, uint64_t stream) {
+  const char *what = "pg_cache8_write";
+  int rc = check8(what, c, s);
+  if (!rc) rc = check_layer(what, c, layer, slots, starts, n, tokens, k, v);
+  if (rc) return rc;
+  if (dtype != PG_DT_F32 && dtype != PG_DT_BF16 && dtype != PG_DT_F16)
+    return pg::argument_fail("%s: dtype %d, want f32, bf16 or f16", what, dtype);
+  if (!n || !tokens) return PG_OK;
+  const auto run = dtype == PG_DT_F32    ? launch_rows<float, true>
+                   : dtype == PG_DT_BF16 ? launch_rows<__nv_bfloat16, true>
+                                         : launch_rows<__half, true>;
+  return run(c, s, layer, slots, starts, n, tokens, k, v, stream);
+}
+
+extern "C" int pg_cache_read(const pg_cache *c, const pg_cache_scales *s, int32_t layer,
+                             uint64_t slots, uint64_t starts, int32_t n, int32_t tokens,
+                             int32_t dtype, const pg_rows *k, const pg_rows *v, uint64_t stream) {
+  const char *what = "pg_cache_read";
+  int rc = s ? check8(what, c, s) : PG_OK;
+  if (!rc) rc = check_layer(what, c, layer, slots, starts, n, tokens, k, v);
+  if (rc) return rc;
+  if (s && dtype != PG_DT_F32 && dtype != PG_DT_BF16 && dtype != PG_DT_F16)
+    return pg::argument_fail("%s: dtype %d, want f32, bf16 or f16", what, dtype);
+  if (!n || !tokens) return PG_OK;
+  if (!s) {
+    int grid;
+    if ((rc = copy_grid((tokens + kCopy / 32 - 1) / (kCopy / 32), &grid))) return rc;
+    return pg::launch<cache_read>("cache_read", dim3(grid), kCopy, 0, stream_of(stream), *c, layer,
+                                  ints(slots), ints(starts), n, tokens, *k, *v);
+  }
+  const auto run = dtype == PG_DT_F32    ? launch_rows<float, false>
+                   : dtype == PG_DT_BF16 ? launch_rows<__nv_bfloat16, false>
+                                         : launch_rows<__half, false>;
+  return run(c, s, layer, slots, starts, n, tokens, k, v, stream);
+}
+
+extern "C" int pg_cache_keep(const pg_cache *c, const pg_cache_scales *s, uint64_t slots,
+                             uint64_t starts, uint64_t kept, int32_t n, uint64_t stream) {
+  const char *what = "pg_cache_keep";
+  int rc = s ? check8(what, c, s) : PG_OK;
+  if (!rc) rc = check_slots(what, c, slots, starts, n);
+  if (rc || !n) return rc;
+  if (!kept || kept & 7) return pg::argument_fail("%s: kept is null or not 8-byte aligned", what);
+  int grid;
+  if ((rc = copy_grid(static_cast<int64_t>(n) * c->layers, &grid))) return rc;
+  const uint64_t *sets = reinterpret_cast<const uint64_t *>(static_cast<uintptr_t>(kept));
+  rc = pg::launch<cache_keep_move>("cache_keep_move", dim3(grid), kCopy, 0, stream_of(stream), *c,
+                                   s ? *s : kNoScales, ints(slots), ints(starts), sets, n);
+  if (rc) return rc;
+  return pg::launch<cache_keep_drop>("cache_keep_drop", dim3((n + kCopy / 32 - 1) / (kCopy / 32)),
+                                     kCopy, 0, stream_of(stream), *c, ints(slots), ints(starts),
+                                     sets, n);
 }

@@ -3,6 +3,7 @@
     ws = Workspace()                                     # once, one per stream
     out = decode(q, k, v, table, lens, workspace=ws)     # q [batch, heads, dim]
     out = prompt(q, starts, k, v, table, lens, workspace=ws)   # q [tokens, heads, dim]
+    out = tree(q, starts, mask, k, v, table, lens, workspace=ws)   # drafted tokens of several branches
 
 ``k`` and ``v`` are one layer's pages [pages, kv_heads, page_size, dim] (``PagedCache.k[layer]``),
 ``table`` [slots, width] and ``lens`` [slots] the cache's; sequence b of the batch is row
@@ -13,7 +14,15 @@ query that sees no key gives zeros; what lies past a sequence's length or in a m
 never part of a result. A visible value that is not finite makes its column of the result so: an
 infinity, where all such values are that one (or NaN, where its weight is below 2^-126). Each group of heads / kv_heads query heads reads one kv head.
 
-q, k and v have one dtype (f32, bf16 or f16) and a head size of up to 256 whose rows are a
+The new tokens of a sequence may be a ``tree``, 64 at most: each sees the tokens before them and those
+of its own branch, which ``mask`` names (``branches`` makes it of the tokens' parents).
+
+Over a cache in 8 bits, ``k_scale`` and ``v_scale`` [pages, kv_heads, page_size] are one layer's scales
+(``PagedCache.k_scale[layer]``) and k and v int8. Keys and values are what they stand for, and only the
+weights' products with the values' scales are rounded, to two f16 numbers each. A key or value whose
+scale is not finite makes the results that see it NaN.
+
+q, k and v have one dtype (f32, bf16 or f16; k and v may be int8) and a head size of up to 256 whose rows are a
 multiple of 16 bytes; q may be a slice of a fused projection. Scores, maxima and sums are held in 32
 bits. bf16 and f16 results are rounded to their type; prompts of more than 48 rows (tokens times heads
 / kv_heads) a sequence on average with heads of up to 128 round each weight to it as well, before its
@@ -35,10 +44,11 @@ import torch
 
 from .cache import CacheError
 from .launch import call, dtype_code, empty, int32_list, take_status, wait_until_set
-from .runtime import AttentionArgs, library
+from .runtime import AttentionArgs, AttentionMore, library
 
 WORKSPACE_BYTES = 64 << 20  # PG_ATTENTION_WORKSPACE
 DIM_MAX = 256  # PG_ATTENTION_DIM
+TREE_MAX = 64  # PG_ATTENTION_TREE
 # pg_attention_args at once: setting its fields one by one takes longer than a short call
 _PACK = struct.Struct("=9Q10q13if")
 assert _PACK.size == ctypes.sizeof(AttentionArgs)
@@ -65,18 +75,18 @@ class Workspace:
 
 def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any,
           scale: float | None, window: int, sinks: int, max_len: int | None, workspace: Workspace,
-          out: Any, stream: int | None) -> Any:
+          out: Any, stream: int | None, k_scale: Any, v_scale: Any, mask: Any = None) -> Any:
     dev, dtype, size = q.device, q.dtype, q.element_size()
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     if len(qs) != 3 or not q.is_cuda or qs[2] != 1:
         raise ValueError(f"q: want [tokens, heads, dim] on a CUDA device with contiguous rows, "
                          f"got {tuple(q.shape)} {q.stride()} on {dev}")
     tokens, hq, dim = q.shape
-    shape = k.shape
+    shape, of = k.shape, dtype if k_scale is None else torch.int8
     for name, t, s in (("k", k, ks), ("v", v, vs)):
-        if len(s) != 4 or t.dtype is not dtype or t.device != dev or t.shape != shape or \
+        if len(s) != 4 or t.dtype is not of or t.device != dev or t.shape != shape or \
                 shape[3] != dim or s[3] != 1 or s[2] != dim:
-            raise ValueError(f"{name}: want {dtype} [pages, kv_heads, page_size, {dim}] on {dev} "
+            raise ValueError(f"{name}: want {of} [pages, kv_heads, page_size, {dim}] on {dev} "
                              f"with a head's rows of one page one after another, got {t.dtype} "
                              f"{tuple(t.shape)} {t.stride()} on {t.device}")
     pages, heads, page_size, _ = shape
@@ -106,35 +116,91 @@ def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any
     elif out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(2) != 1:
         raise ValueError(f"out: want {dtype} {tuple(q.shape)} on {dev} with contiguous rows")
     os_ = out.stride()
+    size_kv = size if k_scale is None else 1
     args = AttentionArgs()
     try:
         _PACK.pack_into(
             args, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts or 0, slots,
             table.data_ptr(), int32_list("lens", lens, dev, rows), workspace.buffer.data_ptr(),
             WORKSPACE_BYTES, qs[0] * size, qs[1] * size, os_[0] * size, os_[1] * size,
-            ks[0] * size, ks[1] * size, vs[0] * size, vs[1] * size, table.stride(0),
+            ks[0] * size_kv, ks[1] * size_kv, vs[0] * size_kv, vs[1] * size_kv, table.stride(0),
             dtype_code(dtype), batch, tokens, heads, hq // heads, dim, page_size, pages, width, rows,
             window, sinks, max_len or 0, dim ** -0.5 if scale is None else scale)
     except (struct.error, OverflowError) as e:
         raise ValueError(f"window, sinks, max_len, scale or a size is out of range: {e}") from e
-    call(library().pg_attention, dev, stream, args)
+    if k_scale is None and v_scale is None and mask is None:
+        call(library().pg_attention, dev, stream, args)
+    else:
+        call(library().pg_attention_ex, dev, stream, args,
+             _more(dev, tokens, shape[:3], k_scale, v_scale, mask))
     return out
+
+
+def _more(dev: Any, tokens: int, rows: Any, k_scale: Any, v_scale: Any, mask: Any) -> AttentionMore:
+    more = AttentionMore()
+    if k_scale is not None or v_scale is not None:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is None or t.dtype is not torch.float32 or t.shape != rows or t.device != dev or \
+                    (rows[2] > 1 and t.stride(2) != 1):
+                raise ValueError(f"{name}: want float32 {tuple(rows)} on {dev} with a page's rows one "
+                                 f"after another, got {t if t is None else (t.dtype, t.shape)}")
+        more.k_scale, more.k_scale_page, more.k_scale_head = (
+            k_scale.data_ptr(), 4 * k_scale.stride(0), 4 * k_scale.stride(1))
+        more.v_scale, more.v_scale_page, more.v_scale_head = (
+            v_scale.data_ptr(), 4 * v_scale.stride(0), 4 * v_scale.stride(1))
+    if mask is not None:
+        if mask.dtype is not torch.int64 or mask.shape != (tokens,) or not mask.is_contiguous() or \
+                mask.device != dev:
+            raise ValueError(f"mask: want contiguous int64 [{tokens}] on {dev}, got {mask.dtype} "
+                             f"{tuple(mask.shape)} on {mask.device}")
+        more.mask = mask.data_ptr()
+    return more
 
 
 def decode(q: Any, k: Any, v: Any, table: Any, lens: Any, *, workspace: Workspace,
            slots: Any = None, scale: float | None = None, window: int = 0, sinks: int = 0,
-           max_len: int | None = None, out: Any = None, stream: int | None = None) -> Any:
+           max_len: int | None = None, out: Any = None, k_scale: Any = None, v_scale: Any = None,
+           stream: int | None = None) -> Any:
     """Attention of one new token a sequence, ``q`` [batch, heads, dim]: the last of each
     sequence's ``lens`` tokens. ``max_len`` may name the longest length (it only shapes the
     launch); ``scale`` is dim ** -0.5 by default."""
     return _call(q, None, k, v, table, lens, slots, scale, window, sinks, max_len, workspace, out,
-                 stream)
+                 stream, k_scale, v_scale)
 
 
 def prompt(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, *, workspace: Workspace,
            slots: Any = None, scale: float | None = None, window: int = 0, sinks: int = 0,
-           max_len: int | None = None, out: Any = None, stream: int | None = None) -> Any:
+           max_len: int | None = None, out: Any = None, k_scale: Any = None, v_scale: Any = None,
+           stream: int | None = None) -> Any:
     """Causal attention of each sequence's last tokens, ``q`` [tokens, heads, dim] with sequence
     b's in rows ``starts[b]`` to ``starts[b + 1]`` (int32, on the device)."""
     return _call(q, starts, k, v, table, lens, slots, scale, window, sinks, max_len, workspace,
-                 out, stream)
+                 out, stream, k_scale, v_scale)
+
+
+def tree(q: Any, starts: Any, mask: Any, k: Any, v: Any, table: Any, lens: Any, *,
+         workspace: Workspace, slots: Any = None, scale: float | None = None, window: int = 0,
+         sinks: int = 0, max_len: int | None = None, out: Any = None, k_scale: Any = None,
+         v_scale: Any = None, stream: int | None = None) -> Any:
+    """Attention of each sequence's last tokens, at most 64, as a tree: bit t of ``mask[i]`` (int64
+    [tokens], on the device) says whether token i sees the t-th of its sequence's new tokens, itself
+    among them. Those n stand one behind the other from base on, the length less the new tokens, and
+    token i at base + n - 1; window and sinks go by that. All see the tokens before base."""
+    if mask is None:
+        raise ValueError("mask: a tree of tokens wants one")
+    return _call(q, starts, k, v, table, lens, slots, scale, window, sinks, max_len, workspace,
+                 out, stream, k_scale, v_scale, mask)
+
+
+def branches(parents: list[int]) -> list[int]:
+    """The masks of one sequence's new tokens (as signed 64-bit numbers, for ``torch.tensor``) from
+    their parents' indices, -1 for one that has none: each token's bit and those of its ancestors. Parents
+    come before their children."""
+    if len(parents) > TREE_MAX:
+        raise ValueError(f"{len(parents)} tokens, want {TREE_MAX} at most")
+    masks: list[int] = []
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"parent {p} of token {i}: want -1 to {i - 1}")
+        masks.append(1 << i | (masks[p] if p >= 0 else 0))
+    return [m - (1 << 64) if m >> 63 else m for m in masks]

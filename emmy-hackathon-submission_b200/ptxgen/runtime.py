@@ -58,6 +58,13 @@ class Rows(ctypes.Structure):
                 ("head_stride", ctypes.c_int64)]
 
 
+class Scales(ctypes.Structure):
+    """``pg_cache_scales``: the scales of a cache in 8 bits."""
+
+    _fields_ = [("k", ctypes.c_uint64), ("v", ctypes.c_uint64),
+                *((n, ctypes.c_int64) for n in ("layer_stride", "page_stride", "head_stride"))]
+
+
 class SampleArgs(ctypes.Structure):
     """``pg_sample_args``: drawing a token of each row (``ptxgen.sampling``)."""
 
@@ -81,6 +88,15 @@ class AttentionArgs(ctypes.Structure):
                                                 "dim", "page_size", "pages", "width",
                                                 "slot_rows", "window", "sinks", "max_len")),
                 ("scale", ctypes.c_float)]
+
+
+class AttentionMore(ctypes.Structure):
+    """``pg_attention_more``: a cache in 8 bits, a tree of tokens (``ptxgen.attention``)."""
+
+    _fields_ = [("k_scale", ctypes.c_uint64), ("v_scale", ctypes.c_uint64),
+                *((n, ctypes.c_int64) for n in ("k_scale_page", "k_scale_head", "v_scale_page",
+                                                "v_scale_head")),
+                ("mask", ctypes.c_uint64)]
 
 
 _lib: ctypes.CDLL | None = None
@@ -131,7 +147,18 @@ def library() -> ctypes.CDLL:
                 "pg_cache_copy": [ctypes.POINTER(Cache), u64, u64, i32, u64],
                 "pg_cache_fork": [ctypes.POINTER(Cache), u64, u64, i32, u64],
                 "pg_cache_compact": [ctypes.POINTER(Cache), u64],
+                "pg_cache_read": [ctypes.POINTER(Cache), ctypes.POINTER(Scales), i32, u64, u64, i32, i32,
+                                  i32, ctypes.POINTER(Rows), ctypes.POINTER(Rows), u64],
+                "pg_cache_keep": [ctypes.POINTER(Cache), ctypes.POINTER(Scales), u64, u64, u64, i32,
+                                  u64],
+                "pg_cache8_write": [ctypes.POINTER(Cache), ctypes.POINTER(Scales), i32, u64, u64, i32,
+                                    i32, i32, ctypes.POINTER(Rows), ctypes.POINTER(Rows), u64],
+                "pg_cache8_copy": [ctypes.POINTER(Cache), ctypes.POINTER(Scales), u64, u64, i32, u64],
+                "pg_cache8_fork": [ctypes.POINTER(Cache), ctypes.POINTER(Scales), u64, u64, i32, u64],
+                "pg_cache8_compact": [ctypes.POINTER(Cache), ctypes.POINTER(Scales), u64],
                 "pg_attention": [ctypes.POINTER(AttentionArgs), u64],
+                "pg_attention_ex": [ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionMore),
+                                    u64],
                 "pg_sample": [ctypes.POINTER(SampleArgs), u64],
                 "pg_logprobs": [u64, ctypes.c_int64, i32, u64, i32, i32, i32, i32, u64, u64, u64,
                                 u64, u64, u64],

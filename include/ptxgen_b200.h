@@ -258,6 +258,42 @@ int pg_cache_fork(const pg_cache *cache, uint64_t parents, uint64_t children, in
  * or above L. Tables and counts follow; every other page stays where it is. */
 int pg_cache_compact(const pg_cache *cache, uint64_t stream);
 
+/* Reads one layer's rows back: row t of k and v, with starts[i] <= t < starts[i + 1], gets what position
+ * lens[slots[i]] - starts[i + 1] + t holds, and rows of no sequence stay as they are. With scales the
+ * cache is in 8 bits and the rows are of dtype; without them they are the cache's own bytes. */
+typedef struct pg_cache_scales pg_cache_scales;
+int pg_cache_read(const pg_cache *cache, const pg_cache_scales *scales, int32_t layer,
+                  uint64_t slots, uint64_t starts, int32_t n, int32_t tokens, int32_t dtype,
+                  const pg_rows *k, const pg_rows *v, uint64_t stream);
+
+/* Of the last starts[i + 1] - starts[i] tokens of slots[i], 64 at most, those whose bits are set in
+ * kept[i] (uint64; the first token's bit is the lowest) move together behind the tokens before them, in
+ * every layer, and the others go, with the pages that only they had. An entry that cannot be met is
+ * left as it is and sets a bit: a slot out of range or listed twice, fewer tokens than that or more than
+ * 64 (PG_CACHE_TOO_LONG), a last extend that was refused, a page out of range, or one to write to that
+ * another table row names (PG_CACHE_BAD_PAGE). scales may be 0 (no cache in 8 bits). */
+int pg_cache_keep(const pg_cache *cache, const pg_cache_scales *scales, uint64_t slots,
+                  uint64_t starts, uint64_t kept, int32_t n, uint64_t stream);
+
+/* A cache in 8 bits: row_bytes (512 at most) is the size of a head, and each row of int8 numbers q has a
+ * float32 s at k + layer * layer_stride + page * page_stride + head * head_stride + 4 row, the values' at
+ * v likewise: it stands for q s. pg_cache8_write takes rows x of dtype (PG_DT_F32, PG_DT_BF16 or
+ * PG_DT_F16) and holds s = max |x| / 127 in f32 and q = x / s rounded, halves to even; a row with a
+ * number that is not finite becomes NaN as a whole. The others are as above, and the rows' scales go
+ * with them; extend and free are the same for every cache. */
+struct pg_cache_scales {
+  uint64_t k, v;                                   /* device addresses, 4-byte aligned */
+  int64_t layer_stride, page_stride, head_stride;  /* bytes, multiples of 4 */
+};
+int pg_cache8_write(const pg_cache *cache, const pg_cache_scales *scales, int32_t layer,
+                    uint64_t slots, uint64_t starts, int32_t n, int32_t tokens, int32_t dtype,
+                    const pg_rows *k, const pg_rows *v, uint64_t stream);
+int pg_cache8_copy(const pg_cache *cache, const pg_cache_scales *scales, uint64_t from, uint64_t to,
+                   int32_t n, uint64_t stream);
+int pg_cache8_fork(const pg_cache *cache, const pg_cache_scales *scales, uint64_t parents,
+                   uint64_t children, int32_t n, uint64_t stream);
+int pg_cache8_compact(const pg_cache *cache, const pg_cache_scales *scales, uint64_t stream);
+
 /* --- log probabilities ------------------------------------------------------------------------
  *
  * No counterpart in the reference. For each row x of `rows` rows of `vocab` logits (dtype
@@ -343,10 +379,32 @@ typedef struct pg_attention_args {
 } pg_attention_args;
 
 #define PG_ATTENTION_WAIT 16u /* in the status word: a bounded wait inside a kernel gave up */
+#define PG_ATTENTION_TREE 64 /* the most tokens of a tree */
 #define PG_ATTENTION_DIM 256
 #define PG_ATTENTION_WORKSPACE (64 << 20)
 
 int pg_attention(const pg_attention_args *args, uint64_t stream);
+
+/* ... over a cache in 8 bits, for trees of drafted tokens, or both; pg_attention where all is 0.
+ *
+ * With scales k and v are int8 (their strides bytes, heads a multiple of 16) and row r of a page's head
+ * stands for its numbers times the float32 at k_scale + page * k_scale_page + head * k_scale_head + 4 r,
+ * v_scale likewise (pg_cache8_write). dtype is the queries' and the result's. Products are exact; a
+ * weight times its value's scale is the sum of two f16 numbers. A scale that is not finite makes the
+ * result of the rows that see it NaN.
+ *
+ * With a mask (starts are wanted, too) a sequence's queries, PG_ATTENTION_TREE at most (else
+ * PG_CACHE_TOO_LONG), are a tree: bit t of mask[i] says whether query i sees the t-th new token of its
+ * sequence. Its n tokens stand one behind the other at base, the length less the queries: the query
+ * at base + n - 1, and the window and sinks go by that. All of them see the tokens before base, as far
+ * as their window does. */
+typedef struct pg_attention_more {
+  uint64_t k_scale, v_scale;                         /* float32, or both 0 */
+  int64_t k_scale_page, k_scale_head, v_scale_page, v_scale_head; /* byte strides */
+  uint64_t mask;                                     /* uint64 [queries], or 0 */
+} pg_attention_more;
+
+int pg_attention_ex(const pg_attention_args *args, const pg_attention_more *more, uint64_t stream);
 
 #ifdef __cplusplus
 }
