@@ -87,6 +87,10 @@ int attend(const char *what, const pg_attention_args *p, const pg_attention_more
   a.dim = p->dim, a.page_size = p->page_size, a.pages = p->pages, a.width = p->width;
   a.slot_rows = p->slot_rows, a.sinks = p->sinks;
   a.scale_log2 = p->scale * 1.4426950408889634f;
+  // 2^32 (2^l / d - 1) rounded up, with the smallest l that makes 2^l d or more: exact below 2^31
+  while (1ll << a.page_shift < a.page_size) ++a.page_shift;
+  a.page_mul = static_cast<uint32_t>(
+      ((1ull << 32) * ((1ull << a.page_shift) - a.page_size)) / a.page_size + 1);
   if (m) {
     a.k_scale = ptr(m->k_scale), a.v_scale = ptr(m->v_scale);
     a.ks_page = m->k_scale_page, a.ks_head = m->k_scale_head;

@@ -48,7 +48,6 @@ enum Mode { kOne, kMany, kTree };  // one query a sequence, any number, or a tre
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kRows = 16;
-constexpr int kPerSm = 2;             // blocks an SM holds
 // What a pair costs by itself, in blocks of keys (64 sequences of up to 8000 keys on 8 kv heads:
 // 126 us with 8 or 4, 159 with 0).
 constexpr int kPair = 8;
@@ -141,6 +140,10 @@ __device__ __forceinline__ void copy4(uint32_t to, const void *from, bool real) 
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes)
                : "memory");
 }
+// Keys go into their product with 16-bit queries by their bytes plus 128, which are f16 numbers below the
+// normal ones as they stand; the sums begin at what that adds, -128 times the sum of a query's numbers,
+// and lose two bits to it, which f32 queries keep. Values, whose sums run over all keys, go in as they
+// are.
 // Four 8-bit numbers as two pairs of f16, of the bytes that the selectors name: 0x6400 and a byte are
 // 1024 and the byte's value, and 1024 + 128 is taken off what the byte is with its sign turned.
 __device__ __forceinline__ void from_8(uint32_t x, uint32_t select0, uint32_t select1, uint32_t &a,
@@ -153,6 +156,12 @@ __device__ __forceinline__ void from_8(uint32_t x, uint32_t select0, uint32_t se
   a = *reinterpret_cast<const uint32_t *>(&y);
   b = *reinterpret_cast<const uint32_t *>(&z);
 }
+// ... as they are plus 128, times 2^-24: a byte and no exponent.
+__device__ __forceinline__ void from_8_small(uint32_t x, uint32_t &a, uint32_t &b) {
+  x ^= 0x80808080u;
+  a = __byte_perm(x, 0, 0x4140);
+  b = __byte_perm(x, 0, 0x4342);
+}
 __device__ __forceinline__ void load_matrices(uint32_t at, uint32_t *r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -161,6 +170,10 @@ __device__ __forceinline__ void load_matrices_t(uint32_t at, uint32_t *r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
+
+template <int N> struct Constant {};
+template <int N> __device__ constexpr int to_bytes(Constant<N>) { return N; }
+__device__ __forceinline__ int64_t to_bytes(int64_t n) { return n; }
 
 // K: the keys' and values' type
 template <class K, int DIM>
@@ -172,7 +185,8 @@ struct Ring {
   static constexpr int tile = step * row;         // a warp's keys, or values
   static constexpr int scales = size == 1 ? step * 4 : 0;  // ... and their scales
   static constexpr int stage = 2 * tile + 2 * scales;
-  static constexpr int stages = (size == 4 ? 256 : 384) / DIM;
+  static constexpr int stages = (size == 4 || size == 1 ? 256 : 384) / DIM;
+  static constexpr int per_sm = size == 1 ? 3 : 2;  // blocks an SM holds
   static constexpr int warp = stages * stage;
   // f32: the queries' fragments in their two parts, of which registers have no room for one
   static constexpr int q = kWarps * warp;
@@ -431,10 +445,15 @@ struct Plan {
 
 // T: the queries' and the result's type, K: the keys' and values' (T, or int8_t)
 template <class T, class K, int DIM, Mode MODE>
-__global__ void __launch_bounds__(kThreads, kPerSm)
+__global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
     decode_kernel(const __grid_constant__ Attention a) {
   using R = Ring<K, DIM>;
   constexpr bool MANY = MODE != kOne, TREE = MODE == kTree, k8 = sizeof(K) == 1;
+  // Weights for bf16 results over 8 bits go in as one f16 number, 2^-12 of themselves off at random,
+  // where the result's own rounding is 2^-9.
+  constexpr bool kOnePart = k8 && std::is_same<T, __nv_bfloat16>::value;
+  // Keys for 16-bit queries go in as 2^-24 of 128 more than what they are.
+  constexpr bool kSmall = k8 && sizeof(T) == 2;
   using M = Mma<typename std::conditional<k8, __half, T>::type>;  // what the products are made in
   extern __shared__ float4 smem4[];
   __shared__ uint3 warp_sum[kWarps];
@@ -559,8 +578,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
 
     // the queries' fragments: rows g and g + 8, columns 2 t and 2 t + 8 of each 16 (f32: t and t + 4
     // of each 8; over keys in 8 bits: 4 t.. + 1 and 4 t + 2.. of each 16)
-    uint32_t q[sizeof(T) == 4 ? 1 : DIM / 16][4];
-    float q_scale[2] = {a.scale_log2, a.scale_log2};
+    uint32_t q[sizeof(T) == 4 || k8 ? 1 : DIM / 16][4];
+    float q_scale[2] = {fabsf(a.scale_log2), fabsf(a.scale_log2)};
+    float start[2] = {0.0f, 0.0f};  // of a score's sum
     uint4 *const q_hi = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(smem4) + R::q) + lane;
     uint4 *const q_lo = q_hi + R::q_part / 16;
     if constexpr (k8) {
@@ -588,8 +608,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
         const int e = min(max(static_cast<int>(__float_as_uint(top[h]) >> 23) - 127, -110), 127);
         const bool some = top[h] > 0.0f && top[h] < INFINITY;
         up[h] = some ? __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23) : 1.0f;
-        if (some) q_scale[h] *= __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+        // the scale's sign, or a scale of 0, is the queries'
+        if (a.scale_log2 <= 0.0f) up[h] = a.scale_log2 < 0.0f ? -up[h] : 0.0f;
+        if (a.scale_log2 == 0.0f) q_scale[h] = 1.0f;
+        else if (some) q_scale[h] *= __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+        if (kSmall) q_scale[h] *= 0x1p24f;
       }
+      float q_sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < DIM / 16; ++k) {
         uint32_t hi[4], lo4[4];
@@ -598,18 +623,20 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
           const float4 x = four(k, h);
           M::split(x.x * up[h], x.y * up[h], hi[h], lo4[h]);
           M::split(x.z * up[h], x.w * up[h], hi[2 + h], lo4[2 + h]);
+          q_sum[h] += (M::low(hi[h]) + M::high(hi[h])) + (M::low(hi[2 + h]) + M::high(hi[2 + h]));
         }
-        if constexpr (sizeof(T) == 4) {
-          if (k % kWarps == warp) {
-            q_hi[32 * k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            q_lo[32 * k] = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q[k][e] = hi[e];
+        if (k % kWarps == warp) {
+          q_hi[32 * k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (sizeof(T) == 4) q_lo[32 * k] = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
         }
       }
-      if (sizeof(T) == 4) __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        q_sum[h] += __shfl_xor_sync(0xffffffffu, q_sum[h], 1);
+        q_sum[h] += __shfl_xor_sync(0xffffffffu, q_sum[h], 2);
+        if (kSmall) start[h] = -128.0f * 0x1p-24f * q_sum[h];
+      }
+      __syncthreads();
     } else {
     const auto q_word = [&](int k, int h, int i) {
       const int r = g + 8 * h;
@@ -667,8 +694,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       if (i >= steps) return -1;
       const int key = first_key(i);
       if (whole_pages && all_seen(key))
-        return pages[(k8 ? key + (lane & 16) : key) / a.page_size];
-      return some_see(key + (lane & (R::step - 1))) ? pages[(key + (lane & (R::step - 1))) / a.page_size] : -1;
+        return pages[k8 ? pg::page_index(a, key + (lane & 16)) : key / a.page_size];
+      const int mine = key + (lane & (R::step - 1));
+      return some_see(mine) ? pages[k8 ? pg::page_index(a, mine) : mine / a.page_size] : -1;
     };
     const int sub = lane / R::chunks, chunk = lane % R::chunks;
     const bool column = chunk * 16 < a.dim * R::size;
@@ -692,22 +720,28 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
             atomicOr(a.status, PG_CACHE_BAD_PAGE);
             page = -1;
           }
-          issue_scales(to + 2 * R::tile, page, (key + lane) % a.page_size);
+          // a lane's half of the keys: where their first row is in its page
+          const int mine_key = key + (lane & 16);
+          const int mine_row = mine_key - pg::page_index(a, mine_key) * a.page_size;
+          issue_scales(to + 2 * R::tile, page, mine_row + (lane & 15));
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int at_page = __shfl_sync(0xffffffffu, page, 16 * half);
+            const int row = __shfl_sync(0xffffffffu, mine_row, 16 * half) + sub;
             const bool real = at_page >= 0 && column;
-            const int64_t in = ((key + 16 * half) % a.page_size + sub) * row_bytes;
-            const char *k = k_head + (real ? at_page : 0) * a.k_page + (real ? in : 0);
-            const char *v = v_head + (real ? at_page : 0) * a.v_page + (real ? in : 0);
+            const int64_t in = static_cast<int64_t>(row) * row_bytes, pg = real ? at_page : 0;
+            const char *const k = k_head + pg * a.k_page + in, *const v = v_head + pg * a.v_page + in;
+            const auto rows = [&](auto bytes) {
 #pragma unroll
-            for (int j = 0; j < kCopies / 2; ++j) {
-              const uint32_t at = to + R::at((half * kCopies / 2 + j) * kRowsEach + sub, chunk);
-              copy16(at, k, real);
-              copy16(at + R::tile, v, real);
-              k += kRowsEach * row_bytes;
-              v += kRowsEach * row_bytes;
-            }
+              for (int j = 0; j < kCopies / 2; ++j) {
+                const uint32_t at = to + R::at((half * kCopies / 2 + j) * kRowsEach + sub, chunk);
+                copy16(at, k + j * kRowsEach * to_bytes(bytes), real);
+                copy16(at + R::tile, v + j * kRowsEach * to_bytes(bytes), real);
+              }
+            };
+            // whole heads: distances that the instructions hold
+            if (a.dim == DIM) rows(Constant<R::row>());
+            else rows(row_bytes);
           }
         } else if (whole_pages && all_seen(key)) {
           bool real = column;
@@ -731,7 +765,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
             atomicOr(a.status, PG_CACHE_BAD_PAGE);
             page = -1;
           }
-          const int mine_row = mine_key % a.page_size;
+          const int mine_row =
+              k8 ? mine_key - pg::page_index(a, mine_key) * a.page_size : mine_key % a.page_size;
           if (k8) issue_scales(to + 2 * R::tile, page, mine_row);
 #pragma unroll
           for (int j = 0; j < kCopies; ++j) {
@@ -765,31 +800,35 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       __syncwarp();
       const uint32_t ks = ring_at + (i % R::stages) * R::stage, vs = ks + R::tile;
       constexpr int kN = R::step / 8;
-      float s[kN][4] = {};
+      float s[kN][4];
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = start[e >> 1];
       if constexpr (k8) {
 #pragma unroll
         for (int k = 0; k < DIM / 64; ++k) {
-          uint4 hi[4], low[4];
-          if constexpr (sizeof(T) == 4) {
+          uint4 hi[4], low[sizeof(T) == 4 ? 4 : 1];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) hi[j] = q_hi[32 * (4 * k + j)], low[j] = q_lo[32 * (4 * k + j)];
+          for (int j = 0; j < 4; ++j) {
+            hi[j] = q_hi[32 * (4 * k + j)];
+            if constexpr (sizeof(T) == 4) low[j] = q_lo[32 * (4 * k + j)];
           }
+          uint32_t x[4][4];  // keys 8 n.. by columns 64 k.., four 8 x 16 matrices along the columns
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint32_t x[4];  // keys 8 n.. by columns 64 k.., four 8 x 16 matrices along the columns
-            load_matrices(ks + R::at(8 * n + (lane & 7), 4 * k + (lane >> 3)), x);
+          for (int n = 0; n < 4; ++n)
+            load_matrices(ks + R::at(8 * n + (lane & 7), 4 * k + (lane >> 3)), x[n]);
+          // four sums in turn, so that none waits for its own last product
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
               uint32_t b0, b1;
-              from_8(x[j], 0x4140, 0x4342, b0, b1);
-              if constexpr (sizeof(T) == 4) {
-                M::run(s[n], &hi[j].x, b0, b1);
-                M::run(s[n], &low[j].x, b0, b1);
-              } else {
-                M::run(s[n], q[4 * k + j], b0, b1);
-              }
+              if constexpr (kSmall) from_8_small(x[n][j], b0, b1);
+              else from_8(x[n][j], 0x4140, 0x4342, b0, b1);
+              M::run(s[n], &hi[j].x, b0, b1);
+              if constexpr (sizeof(T) == 4) M::run(s[n], &low[j].x, b0, b1);
             }
-          }
         }
         const char *const scales = ring + (i % R::stages) * R::stage + 2 * R::tile;
 #pragma unroll
@@ -875,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[n][e] *= k8 ? q_scale[e >> 1] : a.scale_log2;
+          if constexpr (!k8) s[n][e] *= a.scale_log2;
           if (masked && !sight[e >> 1].sees(a, key + 2 * t4 + 8 * n + (e & 1)))
             s[n][e] = -INFINITY;
           top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
@@ -888,7 +927,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
       if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float f = pg::factor(m[h], top[h] == -INFINITY ? 0.0f : top[h]);
+          const float f = k8 ? m[h] == -INFINITY ? 0.0f : pg::exp2_fast((m[h] - top[h]) * q_scale[h])
+                             : pg::factor(m[h], top[h] == -INFINITY ? 0.0f : top[h]);
           m[h] = top[h];
           l[h] *= f;
 #pragma unroll
@@ -915,26 +955,43 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
             for (int e = 0; e < 4; ++e) o[n][e] *= f;
         }
       }
-      const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+      // (8 bits: of the exponent, less what the weights go in above what they are; a maximum that is
+      // infinite gives NaN, as the formula does)
+      const float base[2] = {k8 ? m[0] == -INFINITY ? 0.0f : M::shift - m[0] * q_scale[0]
+                                : m[0] == -INFINITY ? 0.0f : m[0],
+                             k8 ? m[1] == -INFINITY ? 0.0f : M::shift - m[1] * q_scale[1]
+                                : m[1] == -INFINITY ? 0.0f : m[1]};
       constexpr int kWords = kN == 1 ? 4 : 2 * kN;
       uint32_t hi[kWords], lo[kWords];
       const float v_part = __uint_as_float(0x7f000000u - __float_as_uint(v_scale));  // 1 / v_scale
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
+      for (int n = 0; n < kN; ++n) {
+        float2 of = make_float2(0.0f, 0.0f);  // 8 bits: what the values' scales are of v_scale
+        if constexpr (k8) {
+          of = *reinterpret_cast<const float2 *>(
+              ring + (i % R::stages) * R::stage + 2 * R::tile + R::scales + 4 * (8 * n + 2 * t4));
+          of.x *= v_part, of.y *= v_part;
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float x = s[n][2 * h] - base[h], y = s[n][2 * h + 1] - base[h];
-          if constexpr (M::shift != 0.0f) x += M::shift, y += M::shift;
+          if constexpr (k8) {
+            x = fmaf(s[n][2 * h], q_scale[h], base[h]);
+            y = fmaf(s[n][2 * h + 1], q_scale[h], base[h]);
+          } else if constexpr (M::shift != 0.0f) {
+            x += M::shift, y += M::shift;
+          }
           x = pg::exp2_fast(x);
           y = pg::exp2_fast(y);
           l[h] += x + y;
           if constexpr (k8) {
-            const float2 of = *reinterpret_cast<const float2 *>(
-                ring + (i % R::stages) * R::stage + 2 * R::tile + R::scales + 4 * (8 * n + 2 * t4));
-            // what is not seen may have any scale
-            x = masked && s[n][2 * h] == -INFINITY ? 0.0f : x * (of.x * v_part);
-            y = masked && s[n][2 * h + 1] == -INFINITY ? 0.0f : y * (of.y * v_part);
-            M::split(x, y, hi[2 * n + h], lo[2 * n + h]);
+            x *= of.x, y *= of.y;
+            if (masked) {  // what is not seen may have any scale
+              if (s[n][2 * h] == -INFINITY) x = 0.0f;
+              if (s[n][2 * h + 1] == -INFINITY) y = 0.0f;
+            }
+            if constexpr (kOnePart) hi[2 * n + h] = M::pack(x, y);
+            else M::split(x, y, hi[2 * n + h], lo[2 * n + h]);
           } else if constexpr (sizeof(T) == 4) {
             M::split_near(x, hi[h], lo[h]);  // the product's keys are 0, 2, 4, 6, 1, 3, 5, 7
             M::split_near(y, hi[2 + h], lo[2 + h]);
@@ -942,20 +999,33 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
             M::split(x, y, hi[2 * n + h], lo[2 * n + h]);
           }
         }
+      }
       if constexpr (k8) {
 #pragma unroll
-        for (int n = 0; n < DIM / 16; ++n) {
-          uint32_t x[4];  // keys 0.., 8.., 16.. and 24.. by columns 16 n.., pairs of columns transposed
-          load_matrices_t(vs + R::at(lane, n), x);
-          uint32_t even[4], uneven[4];
+        for (int n0 = 0; n0 < DIM / 16; n0 += 2) {
+          uint32_t x[2][4];  // keys 0.., 8.., 16.. and 24.. by columns 16 n.., pairs of them transposed
 #pragma unroll
-          for (int j = 0; j < 4; ++j) from_8(x[j], 0x4240, 0x4341, even[j], uneven[j]);
+          for (int n = 0; n < 2; ++n) load_matrices_t(vs + R::at(lane, n0 + n), x[n]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            M::run(o[2 * n], hi + 4 * j, even[2 * j], even[2 * j + 1]);
-            M::run(o[2 * n], lo + 4 * j, even[2 * j], even[2 * j + 1]);
-            M::run(o[2 * n + 1], hi + 4 * j, uneven[2 * j], uneven[2 * j + 1]);
-            M::run(o[2 * n + 1], lo + 4 * j, uneven[2 * j], uneven[2 * j + 1]);
+            uint32_t even[2][2], uneven[2][2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                from_8(x[n][2 * j + e], 0x4240, 0x4341, even[n][e], uneven[n][e]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              M::run(o[2 * (n0 + n)], hi + 4 * j, even[n][0], even[n][1]);
+              M::run(o[2 * (n0 + n) + 1], hi + 4 * j, uneven[n][0], uneven[n][1]);
+            }
+            if constexpr (!kOnePart) {
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                M::run(o[2 * (n0 + n)], lo + 4 * j, even[n][0], even[n][1]);
+                M::run(o[2 * (n0 + n) + 1], lo + 4 * j, uneven[n][0], uneven[n][1]);
+              }
+            }
           }
         }
       } else if constexpr (sizeof(T) == 4) {
@@ -1019,7 +1089,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
               make_float2(o[n][2 * h], o[n][2 * h + 1]);
       }
       if (t4 == 0) {
-        res[kRows * DIM + r] = m[h];
+        res[kRows * DIM + r] = k8 && m[h] != -INFINITY ? m[h] * q_scale[h] : m[h];
         res[kRows * DIM + kRows + r] = l[h];
       }
     }
@@ -1037,7 +1107,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
 
 template <class T, class K, int DIM, Mode MODE>
 int launch_mode(const Attention &a, int sms, cudaStream_t stream) {
-  return pg::launch<decode_kernel<T, K, DIM, MODE>>("decode_kernel", dim3(kPerSm * sms), kThreads,
+  return pg::launch<decode_kernel<T, K, DIM, MODE>>("decode_kernel", dim3(Ring<K, DIM>::per_sm * sms), kThreads,
                                                     Ring<K, DIM>::bytes, stream, a);
 }
 template <class T, class K, Mode MODE>

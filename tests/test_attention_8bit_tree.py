@@ -5,11 +5,14 @@ bf16, 2^-11 f16, 2^-24 f32):
 
 * a score is a sum of products in 32 bits, under 1e-5 off at these sizes, so a weight is 1e-5 of itself
   off and the result 2e-5 A; the queries of an 8-bit cache lose no more than 2^-22 of their largest
-  on the way to f16 (f32 ones, in two parts);
+  on the way to f16 (f32 ones, in two parts); the keys for 16-bit ones go in with 128 added, so their sums
+  pass numbers up to four times as large, and the result is 8e-5 A off there;
 * a weight goes into its product as two numbers, 2^-16 of itself off (bf16) or 2^-22 (f16, and all over 8
   bits; there its product with the value's scale loses what is below 2^-39 of the largest scale, with
   |q| up to 127 and n keys of no more weight than 1 each against a sum of at least 1: 2^-32 n of it),
   and the result is rounded once: e |o| + 4e-5 A + 2^-32 n s, with 2^-24 for what f16 cannot hold;
+* a bf16 result over 8 bits has its weights as one f16 number each, 2^-12 of itself off, independently:
+  six times the root of that variance, 3.5 2^-12 S, more;
 * tiles of many rows round each weight once, independently: six times the root of that variance more,
   3.5 e S, is met by one in 10^9 results.
 
@@ -155,6 +158,10 @@ class Batch:
                 bound = e * o.abs() + 4e-5 * a + 2.0 ** -24 * (self.dtype != torch.float32)
                 if self.bits8:
                     bound = bound + 2.0 ** -32 * n * float(v.abs().max()) / 127
+                if self.bits8 and self.dtype != torch.float32:
+                    bound = bound + 4e-5 * a
+                if self.bits8 and self.dtype is torch.bfloat16:
+                    bound = bound + 3.5 * 2.0 ** -12 * m
                 if tiles:
                     bound = bound + 3.5 * e * m
                 bad = ~((y - o).abs() <= bound)
