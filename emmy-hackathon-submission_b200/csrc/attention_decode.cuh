@@ -47,7 +47,7 @@ using pg::Sight;
 enum Mode { kOne, kMany, kTree };  // one query a sequence, any number, or a tree of them
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kRows = 16;
+constexpr int kRows = 16;  // of a pair at most
 // What a pair costs by itself, in blocks of keys (64 sequences of up to 8000 keys on 8 kv heads:
 // 126 us with 8 or 4, 159 with 0).
 constexpr int kPair = 8;
@@ -162,6 +162,12 @@ __device__ __forceinline__ void from_8_small(uint32_t x, uint32_t &a, uint32_t &
   a = __byte_perm(x, 0, 0x4140);
   b = __byte_perm(x, 0, 0x4342);
 }
+// An 8 x 8 matrix of 16-bit numbers over a warp, two to a thread, turned over.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
 __device__ __forceinline__ void load_matrices(uint32_t at, uint32_t *r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -176,8 +182,9 @@ template <int N> __device__ constexpr int to_bytes(Constant<N>) { return N; }
 __device__ __forceinline__ int64_t to_bytes(int64_t n) { return n; }
 
 // K: the keys' and values' type
-template <class K, int DIM>
+template <class K, int DIM, int ROWS>
 struct Ring {
+  static constexpr int rows = ROWS;               // of a pair
   static constexpr int size = sizeof(K);
   static constexpr int row = DIM * size, chunks = row / 16;
   static constexpr int step = 32 / size;          // keys a warp takes at a time
@@ -190,9 +197,9 @@ struct Ring {
   static constexpr int warp = stages * stage;
   // f32: the queries' fragments in their two parts, of which registers have no room for one
   static constexpr int q = kWarps * warp;
-  static constexpr int q_part = size == 4 ? 16 * row : size == 1 ? 32 * row : 0;
+  static constexpr int q_part = size == 4 ? 16 * row : size == 1 ? 2 * ROWS * row : 0;
   static constexpr int bytes = q + 2 * q_part;
-  static_assert(warp >= kRows * (DIM + 2) * 4, "a warp's result takes its ring's place");
+  static_assert(warp >= ROWS * (DIM + 2) * 4, "a warp's result takes its ring's place");
   __device__ static int at(int r, int chunk) {
     // rows of 64 bytes: two to a line of all banks
     return r * row + ((chunk ^ (chunks == 4 ? r >> 1 & 3 : r & 7)) << 4);
@@ -207,7 +214,7 @@ struct Sequence {
   uint32_t pairs;
 };
 
-template <Mode MODE, int KEYS>
+template <Mode MODE, int KEYS, int ROWS>
 __device__ __forceinline__ Sequence sequence_of(const Attention &a, int b) {
   constexpr bool MANY = MODE != kOne;
   Sequence s;
@@ -230,7 +237,7 @@ __device__ __forceinline__ Sequence sequence_of(const Attention &a, int b) {
       s.length = s.length < 0 ? 0 : most;
     }
   }
-  s.row_groups = (s.count * a.group + kRows - 1) / kRows;
+  s.row_groups = (s.count * a.group + ROWS - 1) / ROWS;
   s.blocks = pg::blocks_of(a, s.length - s.count - (MODE == kTree), s.length - 1, KEYS);
   s.pairs = s.blocks.count ? a.heads * s.row_groups : 0;
   return s;
@@ -288,9 +295,9 @@ __device__ __noinline__ float plain_product(const char *q, const char *stage, in
 // result, or left for the block that finishes the pair last, which joins all. A function of its own
 // for the registers: what is needed here only would otherwise be held through the loop over the
 // keys, whose loads of operands then wait for one another (a tenth of the whole).
-template <class T, class K, int DIM, Mode MODE>
+template <class T, class K, int DIM, Mode MODE, int ROWS>
 __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t per, int odd) {
-  using R = Ring<K, DIM>;
+  using R = Ring<K, DIM, ROWS>;
   constexpr bool MANY = MODE != kOne, TREE = MODE == kTree;
   extern __shared__ float4 smem4[];
   const Pair p = sh;
@@ -300,7 +307,7 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
     return p.head * a.group + (MANY ? (p.row0 + r) % a.group : p.row0 + r);
   };
   const bool alone = p.c0 == p.c1;
-  constexpr int kPartial = kRows * (DIM + 2);
+  constexpr int kPartial = ROWS * (DIM + 2);
   // a block has at most two pairs that others share: one that its piece starts with, and one
   // it leaves in the middle of
   const auto slot_of = [&](uint32_t piece) {
@@ -328,14 +335,14 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
     float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
-      top = fmaxf(top, reinterpret_cast<float *>(smem4)[w * (R::warp / 4) + kRows * DIM + r]);
+      top = fmaxf(top, reinterpret_cast<float *>(smem4)[w * (R::warp / 4) + ROWS * DIM + r]);
     const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float *from = reinterpret_cast<float *>(smem4) + w * (R::warp / 4);
-      const float f = pg::factor(from[kRows * DIM + r], base);
+      const float f = pg::factor(from[ROWS * DIM + r], base);
       const float4 x = *reinterpret_cast<const float4 *>(from + r * DIM + col);
-      sum += f * from[kRows * DIM + kRows + r];
+      sum += f * from[ROWS * DIM + ROWS + r];
       acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y);
       acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
     }
@@ -374,8 +381,8 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
       float *to = slot_of(blockIdx.x);
       *reinterpret_cast<float4 *>(to + r * DIM + col) = acc;
       if (col == 0) {
-        to[kRows * DIM + r] = top;
-        to[kRows * DIM + kRows + r] = sum;
+        to[ROWS * DIM + r] = top;
+        to[ROWS * DIM + ROWS + r] = sum;
       }
     }
   }
@@ -389,7 +396,7 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
       __threadfence();
       // as many pieces as the rings have room for at a time, all their loads in flight together
       constexpr int kBatch = R::bytes / (kPartial * 4), kPieces16 = kPartial / 4;
-      constexpr int kEach = kThreads / lanes, kMine = kRows / kEach;
+      constexpr int kEach = kThreads / lanes, kMine = ROWS / kEach;
       const int col = 4 * (tid % lanes), first_r = tid / lanes;
       const int used = p.rows * lanes;  // 16-byte pieces of the rows there are
       float *const stage = reinterpret_cast<float *>(smem4);
@@ -406,8 +413,8 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
         __syncthreads();
         for (int i = 0; i < here; ++i) {
           const float *from = slot_of(at + i);
-          for (int j = tid; j < used + kRows / 2; j += kThreads) {
-            const int piece = j < used ? j : j - used + kRows * lanes;  // rows, then m and l
+          for (int j = tid; j < used + ROWS / 2; j += kThreads) {
+            const int piece = j < used ? j : j - used + ROWS * lanes;  // rows, then m and l
             copy16(stage_at + (i * kPieces16 + piece) * 16, from + 4 * piece, true);
           }
         }
@@ -419,12 +426,12 @@ __device__ __noinline__ void finish_pair(const Attention &a, Pair &sh, uint32_t 
           for (int k = 0; k < kMine; ++k) {
             const int r = first_r + k * kEach;
             if (r >= p.rows) continue;
-            const float m_here = from[kRows * DIM + r], most = fmaxf(top[k], m_here);
+            const float m_here = from[ROWS * DIM + r], most = fmaxf(top[k], m_here);
             const float base = most == -INFINITY ? 0.0f : most;
             const float f = pg::factor(m_here, base), old = pg::factor(top[k], base);
             const float4 x = *reinterpret_cast<const float4 *>(from + r * DIM + col);
             top[k] = most;
-            sum[k] = fmaf(f, from[kRows * DIM + kRows + r], old * sum[k]);
+            sum[k] = fmaf(f, from[ROWS * DIM + ROWS + r], old * sum[k]);
             acc[k].x = fmaf(f, x.x, old * acc[k].x), acc[k].y = fmaf(f, x.y, old * acc[k].y);
             acc[k].z = fmaf(f, x.z, old * acc[k].z), acc[k].w = fmaf(f, x.w, old * acc[k].w);
           }
@@ -444,10 +451,10 @@ struct Plan {
 };
 
 // T: the queries' and the result's type, K: the keys' and values' (T, or int8_t)
-template <class T, class K, int DIM, Mode MODE>
-__global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
+template <class T, class K, int DIM, Mode MODE, int ROWS>
+__global__ void __launch_bounds__(kThreads, Ring<K, DIM, ROWS>::per_sm)
     decode_kernel(const __grid_constant__ Attention a) {
-  using R = Ring<K, DIM>;
+  using R = Ring<K, DIM, ROWS>;
   constexpr bool MANY = MODE != kOne, TREE = MODE == kTree, k8 = sizeof(K) == 1;
   // Weights for bf16 results over 8 bits go in as one f16 number, 2^-12 of themselves off at random,
   // where the result's own rounding is 2^-9.
@@ -473,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
   const int first_b = min(tid * run, a.batch), end_b = min(first_b + run, a.batch);
   uint32_t pairs = 0, keys = 0, longest = 0;
   for (int b = first_b; b < end_b; ++b) {
-    const Sequence s = sequence_of<MODE, R::keys>(a, b);
+    const Sequence s = sequence_of<MODE, R::keys, ROWS>(a, b);
     pairs += s.pairs;
     keys += s.pairs * s.blocks.count;
     longest = max(longest, static_cast<uint32_t>(s.blocks.count));
@@ -518,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
   if (u >= before && u < upto) {
     uint32_t at = before;
     for (int b = first_b; b < end_b; ++b) {
-      const Sequence s = sequence_of<MODE, R::keys>(a, b);
+      const Sequence s = sequence_of<MODE, R::keys, ROWS>(a, b);
       const uint32_t next = at + s.pairs * (s.blocks.count + kPair);
       if (u < next) {
         plan.sequence = b;
@@ -538,13 +545,13 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
 
   while (u < plan.end) {
     int b = plan.sequence;
-    Sequence seq = sequence_of<MODE, R::keys>(a, b);
-    while (!seq.pairs) seq = sequence_of<MODE, R::keys>(a, ++b);
+    Sequence seq = sequence_of<MODE, R::keys, ROWS>(a, b);
+    while (!seq.pairs) seq = sequence_of<MODE, R::keys, ROWS>(a, ++b);
     const Blocks &blocks = seq.blocks;
     const uint32_t before = plan.before, per = plan.per;
     const uint32_t units = blocks.count + kPair, pair = (u - before) / units;
-    const int head = pair / seq.row_groups, row0 = (pair % seq.row_groups) * kRows;
-    const int rows = min(kRows, seq.count * a.group - row0);
+    const int head = pair / seq.row_groups, row0 = (pair % seq.row_groups) * ROWS;
+    const int rows = min(ROWS, seq.count * a.group - row0);
     const uint32_t pair_first = before + pair * units;
     const uint32_t stop = min(plan.end, pair_first + units);
     const int block0 = max(0, static_cast<int>(u - pair_first) - kPair);
@@ -569,110 +576,6 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
     const auto head_of = [&](int r) {
       return head * a.group + (MANY ? (row0 + r) % a.group : row0 + r);
     };
-    Sight<TREE> sight[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      sight[h] = Sight<TREE>::of(a, first_pos, seq.count, seq.query,
-                                 TREE && g + 8 * h >= rows ? 0 : query_of(g + 8 * h));
-    int *const odd = odds + plan.turn;
-
-    // the queries' fragments: rows g and g + 8, columns 2 t and 2 t + 8 of each 16 (f32: t and t + 4
-    // of each 8; over keys in 8 bits: 4 t.. + 1 and 4 t + 2.. of each 16)
-    uint32_t q[sizeof(T) == 4 || k8 ? 1 : DIM / 16][4];
-    float q_scale[2] = {fabsf(a.scale_log2), fabsf(a.scale_log2)};
-    float start[2] = {0.0f, 0.0f};  // of a score's sum
-    uint4 *const q_hi = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(smem4) + R::q) + lane;
-    uint4 *const q_lo = q_hi + R::q_part / 16;
-    if constexpr (k8) {
-      // As f16, each row 2^n of what it is, so that its largest is 2^14 or more: that is exact for
-      // 16-bit queries but for what is 2^-38 of the largest; an f32 number goes in as two parts.
-      float top[2] = {0.0f, 0.0f}, up[2];
-      const auto four = [&](int k, int h) {
-        const int r = g + 8 * h, column = 16 * k + 4 * t4;
-        if (r >= rows || column >= a.dim) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        return load4<T>(a.q + (seq.query + query_of(r)) * a.q_token + head_of(r) * a.q_head +
-                        column * static_cast<int>(sizeof(T)));
-      };
-#pragma unroll
-      for (int k = 0; k < DIM / 16; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 x = four(k, h);
-          top[h] = fmaxf(top[h], fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        // 2^(14 - e) and 2^(e - 14) for the largest's exponent e, both finite; none for 0 and infinity
-        const int e = min(max(static_cast<int>(__float_as_uint(top[h]) >> 23) - 127, -110), 127);
-        const bool some = top[h] > 0.0f && top[h] < INFINITY;
-        up[h] = some ? __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23) : 1.0f;
-        // the scale's sign, or a scale of 0, is the queries'
-        if (a.scale_log2 <= 0.0f) up[h] = a.scale_log2 < 0.0f ? -up[h] : 0.0f;
-        if (a.scale_log2 == 0.0f) q_scale[h] = 1.0f;
-        else if (some) q_scale[h] *= __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
-        if (kSmall) q_scale[h] *= 0x1p24f;
-      }
-      float q_sum[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < DIM / 16; ++k) {
-        uint32_t hi[4], lo4[4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 x = four(k, h);
-          M::split(x.x * up[h], x.y * up[h], hi[h], lo4[h]);
-          M::split(x.z * up[h], x.w * up[h], hi[2 + h], lo4[2 + h]);
-          q_sum[h] += (M::low(hi[h]) + M::high(hi[h])) + (M::low(hi[2 + h]) + M::high(hi[2 + h]));
-        }
-        if (k % kWarps == warp) {
-          q_hi[32 * k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (sizeof(T) == 4) q_lo[32 * k] = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        q_sum[h] += __shfl_xor_sync(0xffffffffu, q_sum[h], 1);
-        q_sum[h] += __shfl_xor_sync(0xffffffffu, q_sum[h], 2);
-        if (kSmall) start[h] = -128.0f * 0x1p-24f * q_sum[h];
-      }
-      __syncthreads();
-    } else {
-    const auto q_word = [&](int k, int h, int i) {
-      const int r = g + 8 * h;
-      return r < rows && 32 * k + 16 * i < a.dim * R::size
-                 ? *reinterpret_cast<const uint32_t *>(a.q + (seq.query + query_of(r)) * a.q_token +
-                                                       head_of(r) * a.q_head + 32 * k + 16 * i +
-                                                       4 * t4)
-                 : 0u;
-    };
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int k = warp; k < DIM / 8; k += kWarps) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          M::split_near(__uint_as_float(q_word(k, e & 1, e >> 1)), hi[e], lo[e]);
-        q_hi[32 * k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        q_lo[32 * k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      __syncthreads();
-    } else {
-#pragma unroll
-      for (int k = 0; k < DIM / 16; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[k][e] = q_word(k, e & 1, e >> 1);
-    }
-    }
-    // in 8 bits: values go in as vs / v_scale of what they are, a power of two that is no smaller than
-    // any scale so far
-    float v_scale = 0x1p-100f;
-    float o[DIM / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int n = 0; n < DIM / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
-
     // The warp's steps are the blocks' 16 keys at 16 warp (f32: 8 at 8 warp). A step whose keys all
     // are seen and lie in one page, as they do where pages are whole groups of so many, needs one
     // look at the table and one address; else lane r knows key r's page and row.
@@ -782,6 +685,316 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    if constexpr (k8) {
+      // Queries are the products' columns here: S^T = K Q^T for keys 16 j + g, + 8 (rows) and queries 2 t
+      // and 2 t + 1 of each eight (columns), then O^T += V^T P^T for columns 2 g and 2 g + 1 of each 16 of
+      // the heads, so eight rows of queries leave nothing empty.
+      constexpr int NT = ROWS / 8, kChunks = DIM / 16;
+      constexpr bool kHeld = NT == 1 && sizeof(T) == 2;  // whether registers hold the queries
+      float q_scale[NT][2], start[NT][2];  // of the queries of this thread's columns; of a score's sum
+      Sight<TREE> sight[NT][2];
+      uint32_t q_held[kHeld ? kChunks : 1][2];
+      uint2 *const q_hi = reinterpret_cast<uint2 *>(reinterpret_cast<char *>(smem4) + R::q) + lane;
+      uint2 *const q_lo = q_hi + R::q_part / 8;
+      // As f16, each query 2^n of what it is, so that its largest is 2^14 or more: that is exact for 16-bit
+      // ones but for what is 2^-38 of the largest; an f32 number goes in as two parts. A thread has query
+      // g's columns 4 t.. of each 16: its keys' fragments have those bytes together.
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const int r = 8 * u + g;
+        const auto four = [&](int k) {
+          const int column = 16 * k + 4 * t4;
+          if (r >= rows || column >= a.dim) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          return load4<T>(a.q + (seq.query + query_of(r)) * a.q_token + head_of(r) * a.q_head +
+                          column * static_cast<int>(sizeof(T)));
+        };
+        float top = 0.0f, sum = 0.0f, scale = fabsf(a.scale_log2);
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+          const float4 x = four(k);
+          top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^(14 - e) and 2^(e - 14) for the largest's exponent e, both finite; none for 0 and infinity
+        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -110), 127);
+        const bool some = top > 0.0f && top < INFINITY;
+        float up = some ? __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23) : 1.0f;
+        // the scale's sign, or a scale of 0, is the queries'
+        if (a.scale_log2 <= 0.0f) up = a.scale_log2 < 0.0f ? -up : 0.0f;
+        if (a.scale_log2 == 0.0f) scale = 1.0f;
+        else if (some) scale *= __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+        if (kSmall) scale *= 0x1p24f;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+          const float4 x = four(k);
+          uint32_t hi[2], low[2];
+          M::split(x.x * up, x.y * up, hi[0], low[0]);
+          M::split(x.z * up, x.w * up, hi[1], low[1]);
+          sum += (M::low(hi[0]) + M::high(hi[0])) + (M::low(hi[1]) + M::high(hi[1]));
+          if constexpr (kHeld) {
+            q_held[k][0] = hi[0], q_held[k][1] = hi[1];
+          } else if (k % kWarps == warp) {
+            q_hi[32 * (u * kChunks + k)] = make_uint2(hi[0], hi[1]);
+            if (sizeof(T) == 4) q_lo[32 * (u * kChunks + k)] = make_uint2(low[0], low[1]);
+          }
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // query 2 t + c's, which lanes 4 (2 t + c).. have
+          q_scale[u][c] = __shfl_sync(0xffffffffu, scale, 8 * t4 + 4 * c);
+          const float of = __shfl_sync(0xffffffffu, sum, 8 * t4 + 4 * c);
+          start[u][c] = kSmall ? -128.0f * 0x1p-24f * of : 0.0f;
+          const int row = 8 * u + 2 * t4 + c;
+          sight[u][c] = Sight<TREE>::of(a, first_pos, seq.count, seq.query,
+                                        row < rows ? query_of(row) : 0);
+        }
+      }
+      if (!kHeld) __syncthreads();
+      float o[kChunks][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][u][e] = 0.0f;
+        m[u][0] = m[u][1] = -INFINITY, l[u][0] = l[u][1] = 0.0f;
+      }
+      // values go in as vs / v_scale of what they are, a power of two that is no smaller than any scale so
+      // far
+      float v_scale = 0x1p-100f;
+      // pages are asked for two steps before their rows are
+      int next = page_for(0), after = page_for(1);
+#pragma unroll
+      for (int i = 0; i < R::stages - 1; ++i) {
+        const int page = next;
+        next = after;
+        after = page_for(i + 2);
+        issue(i, page);
+      }
+      for (int i = 0; i < steps; ++i) {
+        const int page = next;
+        next = after;
+        after = page_for(i + R::stages + 1);
+        issue(i + R::stages - 1, page);
+        asm volatile("cp.async.wait_group %0;" ::"n"(R::stages - 1) : "memory");
+        __syncwarp();
+        const uint32_t ks = ring_at + (i % R::stages) * R::stage, vs = ks + R::tile;
+        const char *const stage = ring + (i % R::stages) * R::stage + 2 * R::tile;
+        float s[2][NT][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][u][e] = start[u][e & 1];
+#pragma unroll
+        for (int k = 0; k < kChunks; k += 2) {
+          uint32_t x[2][4];  // keys 16 j.. and 16 j + 8.. by columns 16 k.., then by 16 k + 16..
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            load_matrices(ks + R::at(16 * j + (lane & 15), k + (lane >> 4)), x[j]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint2 hi[NT], low[NT];
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+              if constexpr (kHeld) hi[u] = make_uint2(q_held[k + c][0], q_held[k + c][1]);
+              else hi[u] = q_hi[32 * (u * kChunks + k + c)];
+              if constexpr (sizeof(T) == 4) low[u] = q_lo[32 * (u * kChunks + k + c)];
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t of[4];
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if constexpr (kSmall) from_8_small(x[j][2 * c + h], of[h], of[2 + h]);
+                else from_8(x[j][2 * c + h], 0x4140, 0x4342, of[h], of[2 + h]);
+#pragma unroll
+              for (int u = 0; u < NT; ++u) {
+                M::run(s[j][u], of, hi[u].x, hi[u].y);
+                if constexpr (sizeof(T) == 4) M::run(s[j][u], of, low[u].x, low[u].y);
+              }
+            }
+          }
+        }
+        const int key = first_key(i);
+        const bool masked = !all_seen(key);
+        // the scales of keys g, 8 + g, 16 + g and 24 + g
+        float k_of[4], v_of[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          k_of[j] = *reinterpret_cast<const float *>(stage + 4 * (8 * j + g));
+          v_of[j] = *reinterpret_cast<const float *>(stage + R::scales + 4 * (8 * j + g));
+        }
+        float top[NT][2];
+        bool grown = false;
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            top[u][c] = m[u][c];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float &x = s[j >> 1][u][2 * (j & 1) + c];
+              x *= k_of[j];
+              if (masked && !sight[u][c].sees(a, key + 8 * j + g)) x = -INFINITY;
+              top[u][c] = fmaxf(top[u][c], x);
+            }
+#pragma unroll
+            for (int off = 4; off < 32; off *= 2)
+              top[u][c] = fmaxf(top[u][c], __shfl_xor_sync(0xffffffffu, top[u][c], off));
+            grown |= top[u][c] > m[u][c];
+          }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float f = m[u][c] == -INFINITY
+                                  ? 0.0f
+                                  : pg::exp2_fast((m[u][c] - top[u][c]) * q_scale[u][c]);
+              m[u][c] = top[u][c];
+              l[u][c] *= f;
+#pragma unroll
+              for (int n = 0; n < kChunks; ++n) o[n][u][c] *= f, o[n][u][2 + c] *= f;
+            }
+        }
+        {
+          // the largest scale of those that some row sees; one that is not finite counts as none here
+          float of = *reinterpret_cast<const float *>(stage + R::scales + 4 * lane);
+          of = fabsf(of) < 0x1p125f && (!masked || some_see(key + lane)) ? fabsf(of) : 0.0f;
+          const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(of));
+          if (__uint_as_float(largest) > v_scale) {
+            const float next = __uint_as_float((largest & 0x7f800000u) + 0x00800000u);
+            const float f = v_scale / next;
+            v_scale = next;
+#pragma unroll
+            for (int n = 0; n < kChunks; ++n)
+#pragma unroll
+              for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][u][e] *= f;
+          }
+        }
+        const float v_part = __uint_as_float(0x7f000000u - __float_as_uint(v_scale));  // 1 / v_scale
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v_of[j] *= v_part;
+        // the weights, times their values' scales; turned over so that a thread has keys 2 t and 2 t + 1 of
+        // each eight and query g
+        uint32_t hi[NT][4], lo[NT][kOnePart ? 1 : 4];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          // (a maximum that is infinite gives NaN, as the formula does)
+          float from[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            from[c] = m[u][c] == -INFINITY ? 0.0f : M::shift - m[u][c] * q_scale[u][c];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float w[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float x = s[j >> 1][u][2 * (j & 1) + c];
+              const float p = pg::exp2_fast(fmaf(x, q_scale[u][c], from[c]));
+              l[u][c] += p;
+              w[c] = p * v_of[j];
+              if (masked && x == -INFINITY) w[c] = 0.0f;  // what is not seen may have any scale
+            }
+            if constexpr (kOnePart) {
+              hi[u][j] = turned(M::pack(w[0], w[1]));
+            } else {
+              M::split(w[0], w[1], hi[u][j], lo[u][j]);
+              hi[u][j] = turned(hi[u][j]), lo[u][j] = turned(lo[u][j]);
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n) {
+          uint32_t x[4];  // keys 0.., 8.., 16.. and 24.. by columns 16 n.., pairs of columns transposed
+          load_matrices_t(vs + R::at(lane, n), x);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t of[4];
+            from_8(x[2 * j], 0x4240, 0x4341, of[0], of[1]);
+            from_8(x[2 * j + 1], 0x4240, 0x4341, of[2], of[3]);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+              M::run(o[n][u], of, hi[u][2 * j], hi[u][2 * j + 1]);
+              if constexpr (!kOnePart) M::run(o[n][u], of, lo[u][2 * j], lo[u][2 * j + 1]);
+            }
+          }
+        }
+        __syncwarp();  // the stage may be filled again
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+
+      // the warps' results, in their rings' places: rows of DIM numbers, then m and l of each row
+      float *res = reinterpret_cast<float *>(ring);
+      constexpr float down = 1.0f / (1 << static_cast<int>(M::shift));
+      const float f = v_scale * down;
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int r = 8 * u + 2 * t4 + c;
+#pragma unroll
+          for (int off = 4; off < 32; off *= 2)
+            l[u][c] += __shfl_xor_sync(0xffffffffu, l[u][c], off);
+#pragma unroll
+          for (int n = 0; n < kChunks; ++n)
+            *reinterpret_cast<float2 *>(res + r * DIM + 16 * n + 2 * g) =
+                make_float2(o[n][u][c] * f, o[n][u][2 + c] * f);
+          if (g == 0) {
+            res[ROWS * DIM + r] = m[u][c] == -INFINITY ? m[u][c] : m[u][c] * q_scale[u][c];
+            res[ROWS * DIM + ROWS + r] = l[u][c] * down;
+          }
+        }
+    } else {
+    Sight<TREE> sight[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      sight[h] = Sight<TREE>::of(a, first_pos, seq.count, seq.query,
+                                 TREE && g + 8 * h >= rows ? 0 : query_of(g + 8 * h));
+    int *const odd = odds + plan.turn;
+
+    // the queries' fragments: rows g and g + 8, columns 2 t and 2 t + 8 of each 16 (f32: t and t + 4 of each 8)
+    uint32_t q[sizeof(T) == 4 ? 1 : DIM / 16][4];
+    uint4 *const q_hi = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(smem4) + R::q) + lane;
+    uint4 *const q_lo = q_hi + R::q_part / 16;
+    const auto q_word = [&](int k, int h, int i) {
+      const int r = g + 8 * h;
+      return r < rows && 32 * k + 16 * i < a.dim * R::size
+                 ? *reinterpret_cast<const uint32_t *>(a.q + (seq.query + query_of(r)) * a.q_token +
+                                                       head_of(r) * a.q_head + 32 * k + 16 * i +
+                                                       4 * t4)
+                 : 0u;
+    };
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = warp; k < DIM / 8; k += kWarps) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          M::split_near(__uint_as_float(q_word(k, e & 1, e >> 1)), hi[e], lo[e]);
+        q_hi[32 * k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        q_lo[32 * k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[k][e] = q_word(k, e & 1, e >> 1);
+    }
+    float o[DIM / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < DIM / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+
     // pages are asked for two steps before their rows are
     int next = page_for(0), after = page_for(1);
 #pragma unroll
@@ -800,43 +1013,8 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
       __syncwarp();
       const uint32_t ks = ring_at + (i % R::stages) * R::stage, vs = ks + R::tile;
       constexpr int kN = R::step / 8;
-      float s[kN][4];
-#pragma unroll
-      for (int n = 0; n < kN; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = start[e >> 1];
-      if constexpr (k8) {
-#pragma unroll
-        for (int k = 0; k < DIM / 64; ++k) {
-          uint4 hi[4], low[sizeof(T) == 4 ? 4 : 1];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            hi[j] = q_hi[32 * (4 * k + j)];
-            if constexpr (sizeof(T) == 4) low[j] = q_lo[32 * (4 * k + j)];
-          }
-          uint32_t x[4][4];  // keys 8 n.. by columns 64 k.., four 8 x 16 matrices along the columns
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-            load_matrices(ks + R::at(8 * n + (lane & 7), 4 * k + (lane >> 3)), x[n]);
-          // four sums in turn, so that none waits for its own last product
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              uint32_t b0, b1;
-              if constexpr (kSmall) from_8_small(x[n][j], b0, b1);
-              else from_8(x[n][j], 0x4140, 0x4342, b0, b1);
-              M::run(s[n], &hi[j].x, b0, b1);
-              if constexpr (sizeof(T) == 4) M::run(s[n], &low[j].x, b0, b1);
-            }
-        }
-        const char *const scales = ring + (i % R::stages) * R::stage + 2 * R::tile;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float2 of = *reinterpret_cast<const float2 *>(scales + 4 * (8 * n + 2 * t4));
-          s[n][0] *= of.x, s[n][1] *= of.y, s[n][2] *= of.x, s[n][3] *= of.y;
-        }
-      } else if constexpr (sizeof(T) == 4) {
+      float s[kN][4] = {};
+      if constexpr (sizeof(T) == 4) {
         // even and odd columns, and hi by hi and the rest, by themselves: four short chains of sums
         float part[4][4] = {};
 #pragma unroll
@@ -883,7 +1061,7 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
       const int key = first_key(i);
       const bool masked = !all_seen(key);
       bool look = MANY && masked;
-      if constexpr (sizeof(T) == 4 && !k8) {
+      if constexpr (sizeof(T) == 4) {
         // 0 times a number that is not finite is NaN
         pg::Two none(0.0f, 0.0f);
         const pg::Two zero(0.0f, 0.0f);
@@ -898,7 +1076,7 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
         none.get(x, y);
         look = __any_sync(0xffffffffu, x + y != 0.0f);
       }
-      if (!k8 && look) {
+      if (look) {
         bool any = false;
         for (int j = lane; j < R::step * R::chunks; j += 32) {
           uint4 *const at =
@@ -914,7 +1092,7 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
       for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (!k8) s[n][e] *= a.scale_log2;
+          s[n][e] *= a.scale_log2;
           if (masked && !sight[e >> 1].sees(a, key + 2 * t4 + 8 * n + (e & 1)))
             s[n][e] = -INFINITY;
           top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
@@ -927,8 +1105,7 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
       if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float f = k8 ? m[h] == -INFINITY ? 0.0f : pg::exp2_fast((m[h] - top[h]) * q_scale[h])
-                             : pg::factor(m[h], top[h] == -INFINITY ? 0.0f : top[h]);
+          const float f = pg::factor(m[h], top[h] == -INFINITY ? 0.0f : top[h]);
           m[h] = top[h];
           l[h] *= f;
 #pragma unroll
@@ -938,97 +1115,25 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
           }
         }
       }
-      if constexpr (k8) {
-        // the largest scale of those that some row sees; one that is not finite counts as none here
-        const char *const scales =
-            ring + (i % R::stages) * R::stage + 2 * R::tile + R::scales;
-        float of = *reinterpret_cast<const float *>(scales + 4 * lane);
-        of = fabsf(of) < 0x1p125f && (!masked || some_see(key + lane)) ? fabsf(of) : 0.0f;
-        const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(of));
-        if (__uint_as_float(largest) > v_scale) {
-          const float next = __uint_as_float((largest & 0x7f800000u) + 0x00800000u);
-          const float f = v_scale / next;
-          v_scale = next;
+      const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+      uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int n = 0; n < DIM / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] *= f;
-        }
-      }
-      // (8 bits: of the exponent, less what the weights go in above what they are; a maximum that is
-      // infinite gives NaN, as the formula does)
-      const float base[2] = {k8 ? m[0] == -INFINITY ? 0.0f : M::shift - m[0] * q_scale[0]
-                                : m[0] == -INFINITY ? 0.0f : m[0],
-                             k8 ? m[1] == -INFINITY ? 0.0f : M::shift - m[1] * q_scale[1]
-                                : m[1] == -INFINITY ? 0.0f : m[1]};
-      constexpr int kWords = kN == 1 ? 4 : 2 * kN;
-      uint32_t hi[kWords], lo[kWords];
-      const float v_part = __uint_as_float(0x7f000000u - __float_as_uint(v_scale));  // 1 / v_scale
-#pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        float2 of = make_float2(0.0f, 0.0f);  // 8 bits: what the values' scales are of v_scale
-        if constexpr (k8) {
-          of = *reinterpret_cast<const float2 *>(
-              ring + (i % R::stages) * R::stage + 2 * R::tile + R::scales + 4 * (8 * n + 2 * t4));
-          of.x *= v_part, of.y *= v_part;
-        }
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float x = s[n][2 * h] - base[h], y = s[n][2 * h + 1] - base[h];
-          if constexpr (k8) {
-            x = fmaf(s[n][2 * h], q_scale[h], base[h]);
-            y = fmaf(s[n][2 * h + 1], q_scale[h], base[h]);
-          } else if constexpr (M::shift != 0.0f) {
-            x += M::shift, y += M::shift;
-          }
+          if constexpr (M::shift != 0.0f) x += M::shift, y += M::shift;
           x = pg::exp2_fast(x);
           y = pg::exp2_fast(y);
           l[h] += x + y;
-          if constexpr (k8) {
-            x *= of.x, y *= of.y;
-            if (masked) {  // what is not seen may have any scale
-              if (s[n][2 * h] == -INFINITY) x = 0.0f;
-              if (s[n][2 * h + 1] == -INFINITY) y = 0.0f;
-            }
-            if constexpr (kOnePart) hi[2 * n + h] = M::pack(x, y);
-            else M::split(x, y, hi[2 * n + h], lo[2 * n + h]);
-          } else if constexpr (sizeof(T) == 4) {
+          if constexpr (sizeof(T) == 4) {
             M::split_near(x, hi[h], lo[h]);  // the product's keys are 0, 2, 4, 6, 1, 3, 5, 7
             M::split_near(y, hi[2 + h], lo[2 + h]);
           } else {
             M::split(x, y, hi[2 * n + h], lo[2 * n + h]);
           }
         }
-      }
-      if constexpr (k8) {
-#pragma unroll
-        for (int n0 = 0; n0 < DIM / 16; n0 += 2) {
-          uint32_t x[2][4];  // keys 0.., 8.., 16.. and 24.. by columns 16 n.., pairs of them transposed
-#pragma unroll
-          for (int n = 0; n < 2; ++n) load_matrices_t(vs + R::at(lane, n0 + n), x[n]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t even[2][2], uneven[2][2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                from_8(x[n][2 * j + e], 0x4240, 0x4341, even[n][e], uneven[n][e]);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              M::run(o[2 * (n0 + n)], hi + 4 * j, even[n][0], even[n][1]);
-              M::run(o[2 * (n0 + n) + 1], hi + 4 * j, uneven[n][0], uneven[n][1]);
-            }
-            if constexpr (!kOnePart) {
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                M::run(o[2 * (n0 + n)], lo + 4 * j, even[n][0], even[n][1]);
-                M::run(o[2 * (n0 + n) + 1], lo + 4 * j, uneven[n][0], uneven[n][1]);
-              }
-            }
-          }
-        }
-      } else if constexpr (sizeof(T) == 4) {
+      if constexpr (sizeof(T) == 4) {
         const char *const v = ring + (i % R::stages) * R::stage + R::tile + 4 * (g & 3);
 #pragma unroll
         for (int n = 0; n < DIM / 8; ++n) {
@@ -1073,29 +1178,19 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = g + 8 * h;
-      if constexpr (k8) {  // columns 4 t, 4 t + 2 and 4 t + 1, 4 t + 3 of each 16
-        constexpr float down = 1.0f / (1 << static_cast<int>(M::shift));
-        const float f = v_scale * down;
 #pragma unroll
-        for (int n = 0; n < DIM / 16; ++n)
-          *reinterpret_cast<float4 *>(res + r * DIM + 16 * n + 4 * t4) =
-              make_float4(o[2 * n][2 * h] * f, o[2 * n + 1][2 * h] * f, o[2 * n][2 * h + 1] * f,
-                          o[2 * n + 1][2 * h + 1] * f);
-        l[h] *= down;
-      } else {
-#pragma unroll
-        for (int n = 0; n < DIM / 8; ++n)
-          *reinterpret_cast<float2 *>(res + r * DIM + 8 * n + 2 * t4) =
-              make_float2(o[n][2 * h], o[n][2 * h + 1]);
-      }
+      for (int n = 0; n < DIM / 8; ++n)
+        *reinterpret_cast<float2 *>(res + r * DIM + 8 * n + 2 * t4) =
+            make_float2(o[n][2 * h], o[n][2 * h + 1]);
       if (t4 == 0) {
-        res[kRows * DIM + r] = k8 && m[h] != -INFINITY ? m[h] * q_scale[h] : m[h];
+        res[kRows * DIM + r] = m[h];
         res[kRows * DIM + kRows + r] = l[h];
       }
     }
+    }
     __syncthreads();
 
-    finish_pair<T, K, DIM, MODE>(a, sh, plan.per, odds[plan.turn]);
+    finish_pair<T, K, DIM, MODE, ROWS>(a, sh, plan.per, odds[plan.turn]);
     __syncthreads();  // the rings are free again
     if (tid == 0) {
       odds[plan.turn] = 0;  // for the turn after the next
@@ -1105,10 +1200,18 @@ __global__ void __launch_bounds__(kThreads, Ring<K, DIM>::per_sm)
   }
 }
 
+template <class T, class K, int DIM, Mode MODE, int ROWS>
+int launch_rows(const Attention &a, int sms, cudaStream_t stream) {
+  using R = Ring<K, DIM, ROWS>;
+  return pg::launch<decode_kernel<T, K, DIM, MODE, ROWS>>("decode_kernel", dim3(R::per_sm * sms),
+                                                          kThreads, R::bytes, stream, a);
+}
 template <class T, class K, int DIM, Mode MODE>
 int launch_mode(const Attention &a, int sms, cudaStream_t stream) {
-  return pg::launch<decode_kernel<T, K, DIM, MODE>>("decode_kernel", dim3(Ring<K, DIM>::per_sm * sms), kThreads,
-                                                    Ring<K, DIM>::bytes, stream, a);
+  // over 8 bits a pair may have eight rows, which single tokens of up to eight heads fill
+  if constexpr (sizeof(K) == 1 && MODE == kOne)
+    if (a.group <= 8) return launch_rows<T, K, DIM, MODE, 8>(a, sms, stream);
+  return launch_rows<T, K, DIM, MODE, kRows>(a, sms, stream);
 }
 template <class T, class K, Mode MODE>
 int launch_dim(const Attention &a, int sms, cudaStream_t stream) {
