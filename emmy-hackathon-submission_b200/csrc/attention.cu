@@ -106,10 +106,12 @@ int attend(const char *what, const pg_attention_args *p, const pg_attention_more
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
   const bool f32 = dtype == PG_DT_F32, bf16 = dtype == PG_DT_BF16;
   const bool counts = a.dim <= 128 && pg::decode_counts(a, static_cast<int>(most));
+  // as in decode_takes: rows that tiles of 128 are worth while for
+  const bool tiles = a.starts && a.dim <= 128 && !f32 && a.scale_log2 != 0.0f &&
+                     static_cast<int64_t>(a.queries) * a.group > 48ll * a.batch;
+  if (a.k_scale && tiles) return pg::prompt_8bit(a, bf16, max_len, partial_bytes, sms, s);
   if (a.mask) {
-    const bool many = static_cast<int64_t>(a.queries) * a.group > 48ll * a.batch;
-    if (a.dim <= 128 && many && !f32 && !a.k_scale && a.scale_log2 != 0.0f)
-      return pg::prompt_tree(a, bf16, max_len, partial_bytes, sms, s);
+    if (tiles) return pg::prompt_tree(a, bf16, max_len, partial_bytes, sms, s);
     return counts ? pg::decode_tree(a, dtype, sms, s)
                   : pg::any_rows_tree(a, dtype, max_len, partial_bytes, sms, s);
   }

@@ -230,6 +230,8 @@ int decode_8bit(const Attention &a, int dtype, int sms, cudaStream_t stream);
 int decode_tree(const Attention &a, int dtype, int sms, cudaStream_t stream);
 int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                  cudaStream_t stream);
+int prompt_8bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
+                cudaStream_t stream);
 int prompt_tree(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                 cudaStream_t stream);
 // For every head size and number of rows, in 32-bit arithmetic (attention_any.cuh).

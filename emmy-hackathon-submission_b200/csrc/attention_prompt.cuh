@@ -62,16 +62,18 @@ constexpr int kKeys = 128, kRows = 256, kHalf = 128;
 constexpr int kThreads = 384;
 constexpr int kCopyWarps = 2, kCopyThreads = 32 * kCopyWarps;  // without TMA
 constexpr int kLag = 2;  // tiles whose cp.async copies are in flight before the oldest is waited for
+constexpr int kConvertWarps = 3;  // of a cache in 8 bits
 constexpr float kGrow = 8.0f;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
-template <int DIM>
+template <int DIM, bool K8>
 struct Plan {
   // 128 queries, keys or values: by eight rows, then by 64 columns, each such 1024 bytes swizzled
   static constexpr int atom = 1024, chunks = DIM / 64, group = chunks * atom;
   static constexpr int tile = 16 * group;
-  static constexpr int stages = DIM == 128 ? 5 : 8;
-  static constexpr int q = 0, ring = 2 * tile, bars = ring + stages * tile;
+  static constexpr int raw = K8 ? kKeys * DIM : 0;  // keys or values in 8 bits, on their way
+  static constexpr int stages = DIM == 128 ? K8 ? 4 : 5 : 8;
+  static constexpr int q = 0, ring = 2 * tile, raws = ring + stages * tile, bars = raws + 2 * raw;
   // over half an SM's shared memory, so that no other block that takes all its tensor memory
   // is resident beside this one
   static constexpr int bytes = 1024 + bars + 256;
@@ -222,8 +224,10 @@ template <> struct Type<__nv_bfloat16> {
   }
   __device__ static float low(uint32_t w) { return __uint_as_float(w << 16); }
   __device__ static float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+  static constexpr float largest = 3.3895e38f;  // none above is finite
 };
 template <> struct Type<__half> {
+  static constexpr float largest = 65504.0f;
   static constexpr float shift = 15.0f - kGrow;  // at most 2^15 of 65504
   static constexpr uint32_t format = 0, exponent = 0x7c00;
   __device__ static uint32_t pack(float x, float y) {
@@ -237,6 +241,26 @@ template <> struct Type<__half> {
     return __high2float(*reinterpret_cast<const __half2 *>(&w));
   }
 };
+
+// 16 numbers of 8 bits times their scale, rounded to T.
+template <class T>
+__device__ __forceinline__ void widen(const uint4 &raw, float scale, uint4 *to) {
+  const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u,
+                         raw.w ^ 0x80808080u};
+  const Two off(-8388736.0f, -8388736.0f), by(scale, scale);  // 2^23 + 128
+  uint32_t out[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t of = w[i / 2];
+    const Two x(__uint_as_float(__byte_perm(of, 0x4b000000u, i & 1 ? 0x7442 : 0x7440)),
+                __uint_as_float(__byte_perm(of, 0x4b000000u, i & 1 ? 0x7443 : 0x7441)));
+    float y, z;
+    mul(add(x, off), by).get(y, z);
+    out[i] = Type<T>::pack(y, z);
+  }
+  to[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  to[1] = make_uint4(out[4], out[5], out[6], out[7]);
+}
 
 // A shared-memory operand of 128-byte swizzled rows: `rows` is the distance of its groups of
 // eight, `columns` that of its 64-column chunks where columns are the product's N.
@@ -272,7 +296,7 @@ struct Head {  // what the roles share
 // Adds the values that are not finite and that the query at `pos` sees to 32 columns of its result: of
 // all blocks of keys, or of those that some row must not see in full. A function of its own for the
 // registers, as it is hardly ever called: in the kernel it made every step slower (508 us for 498).
-template <class T, bool TREE>
+template <class T, bool TREE, bool K8>
 __device__ __noinline__ void add_values(const Attention &a, const int *pages, int length, Blocks blocks,
                                         Seen both, int b0, int steps, int head, Sight<TREE> sight,
                                         int k, bool all, float *x) {
@@ -284,11 +308,23 @@ __device__ __noinline__ void add_values(const Attention &a, const int *pages, in
       if (!sight.sees(a, key)) continue;
       const int page = pages[key / a.page_size];
       if (page < 0 || page >= a.pages) continue;
+      constexpr int size = K8 ? 1 : 2;
+      const int row = key % a.page_size;
       const char *v = a.v + page * a.v_page + head * a.v_head +
-                      static_cast<int64_t>(key % a.page_size) * a.dim * 2 + 64 * k;
+                      static_cast<int64_t>(row) * a.dim * size + 32 * size * k;
+      float scale = 0.0f;
+      if constexpr (K8) {
+        scale = *reinterpret_cast<const float *>(a.v_scale + page * a.vs_page + head * a.vs_head +
+                                                 row * 4ll);
+        if (127.0f * fabsf(scale) < Type<T>::largest) continue;
+      }
       for (int c = 0; c < 32; c += 2) {
         if (32 * k + c >= a.dim) break;
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(v + 2 * c);
+        uint32_t w;
+        if constexpr (K8)
+          w = Type<T>::pack(scale * static_cast<int8_t>(v[c]), scale * static_cast<int8_t>(v[c + 1]));
+        else
+          w = *reinterpret_cast<const uint32_t *>(v + 2 * c);
         const float value[2] = {Type<T>::low(w), Type<T>::high(w)};
         for (int e = 0; e < 2; ++e)
           if (!(fabsf(value[e]) < INFINITY)) {
@@ -301,12 +337,13 @@ __device__ __noinline__ void add_values(const Attention &a, const int *pages, in
 }
 
 // Without TMA the maps and `boxes` are empty.
-// TREE: a sequence's new tokens are a tree.
-template <class T, int DIM, bool TMA, bool TREE>
+// TREE: a sequence's new tokens are a tree. K8: the cache is in 8 bits (and comes without TMA).
+template <class T, int DIM, bool TMA, bool TREE, bool K8>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ Attention a, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map, int run) {
-  using P = Plan<DIM>;
+  using P = Plan<DIM, K8>;
+  static_assert(!(TMA && K8), "keys in 8 bits come by cp.async");
   extern __shared__ char smem_raw[];
   __shared__ Head sh;
   char *smem = reinterpret_cast<char *>(
@@ -336,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t o_full = q_full + 40;
   if (tid == 0) {
     for (int s = 0; s < P::stages; ++s) {
-      bar_init(full(s), TMA ? 1 : kCopyThreads);
+      bar_init(full(s), TMA ? 1 : K8 ? 32 * kConvertWarps : kCopyThreads);
       bar_init(empty(s), 1);
     }
     bar_init(q_full, 2 * kHalf);
@@ -407,7 +444,99 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = 2 * k + half;
         if (n + P::stages >= 2 * j + half) bar_drain(full(n % P::stages), n / P::stages & 1, a.status);
       }
-    } else if (!TMA && (warp == 9 || warp == 10)) {
+    } else if (K8 && warp >= 9) {
+      // --- keys and values in 8 bits: copied 16 bytes at a time to where the same thread takes them up a
+      // step later, widens them to T times their row's scale, and hands them on in the products' layout --
+      const int w = warp - 9;
+      constexpr int kPieces = DIM / 16, kPer = 32 / kPieces;  // 16 bytes of a row; rows a warp takes at once
+      constexpr int kMine = (kKeys / kPer + kConvertWarps - 1) / kConvertWarps;
+      const int sub = lane / kPieces, piece = lane % kPieces;
+      const bool column = piece * 16 < a.dim;
+      const auto pages_of = [&](int j, int2 *p) {  // keys lane, lane + 32, ... of step j
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = make_int2(-1, 0);
+          const int key = blocks.key_block(b0 + j) * kKeys + lane + 32 * i;
+          if (j < steps && key < t.length) {
+            const int entry = pg::page_index(a, key);
+            p[i] = make_int2(t.pages[entry], key - entry * a.page_size);
+            if (p[i].x < 0 || p[i].x >= a.pages) {
+              atomicOr(a.status, PG_CACHE_BAD_PAGE);
+              p[i].x = -1;
+            }
+          }
+        }
+      };
+      const auto place = [&](int half, int m) {  // a thread's m-th row's 16 bytes
+        return smem_at + P::raws + half * P::raw +
+               ((m * kConvertWarps + w) * kPer * kPieces + lane) * 16;
+      };
+      float scales[2][kMine];
+      const auto issue = [&](int half, const int2 *p) {
+        const char *from = (half ? a.v : a.k) + head * (half ? a.v_head : a.k_head) + piece * 16;
+        const char *of = (half ? a.v_scale : a.k_scale) + head * (half ? a.vs_head : a.ks_head);
+        const int64_t page_bytes = half ? a.v_page : a.k_page;
+        const int64_t of_bytes = half ? a.vs_page : a.ks_page;
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+          const int i = m * kConvertWarps + w, r = i * kPer + sub, run = (i * kPer) >> 5;
+          if (i >= kKeys / kPer) break;
+          const int2 mine = run == 0 ? p[0] : run == 1 ? p[1] : run == 2 ? p[2] : p[3];
+          const int page = __shfl_sync(0xffffffffu, mine.x, r & 31);
+          const int row = __shfl_sync(0xffffffffu, mine.y, r & 31);
+          const bool real = page >= 0;
+          scales[half][m] =
+              real ? *reinterpret_cast<const float *>(of + page * of_bytes + row * 4ll) : 0.0f;
+          const char *src = real && column ? from + page * page_bytes +
+                                                 static_cast<int64_t>(row) * a.dim
+                                           : from;
+          const int bytes = real && column ? 16 : 0;  // 0: zeroed, nothing read
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place(half, m)),
+                       "l"(src), "r"(bytes)
+                       : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      int2 p[4];
+      pages_of(0, p);
+      issue(0, p);
+      issue(1, p);
+      bool ok = true;
+      for (int j = 0; j < steps && ok; ++j) {
+        pages_of(j + 1, p);
+        const int key0 = blocks.key_block(b0 + j) * kKeys;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int n = 2 * j + half, s = n % P::stages;
+          if (n >= P::stages) ok = bar_wait(empty(s), (n / P::stages - 1) & 1, failed, a.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          char *const to = smem + P::ring + s * P::tile;
+          // values that some row must not see are looked over: what is not finite is zeroed here
+          const bool look = half && !both.all(key0);
+#pragma unroll
+          for (int m = 0; m < kMine; ++m) {
+            const int i = m * kConvertWarps + w, r = i * kPer + sub;
+            if (i >= kKeys / kPer) break;
+            const float scale = scales[half][m];
+            uint4 out[2];
+            widen<T>(*reinterpret_cast<const uint4 *>(smem + (place(half, m) - smem_at)), scale, out);
+            if (look && !(127.0f * fabsf(scale) < Type<T>::largest)) {
+              bool odd = pg::clean<Type<T>::exponent>(out);
+              odd |= pg::clean<Type<T>::exponent>(out + 1);
+              if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
+            }
+            *reinterpret_cast<uint4 *>(to + P::at(r, 2 * piece)) = out[0];
+            *reinterpret_cast<uint4 *>(to + P::at(r, 2 * piece + 1)) = out[1];
+          }
+          fence_async();
+          bar_arrive(full(s));
+          issue(half, p);
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else if (!TMA && !K8 && (warp == 9 || warp == 10)) {
       // --- copies: K and V of each block in turn ----------------------------------------------
       const int w = warp - 9;
       constexpr int kPieces = DIM / 8, kPer = 32 / kPieces;  // rows a warp copies at once
@@ -698,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float y[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e) y[e] = x[e];
-      add_values<T, TREE>(a, t.pages, t.length, blocks, both, b0, steps, head, sight, k, lost, y);
+      add_values<T, TREE, K8>(a, t.pages, t.length, blocks, both, b0, steps, head, sight, k, lost, y);
 #pragma unroll
       for (int e = 0; e < 32; ++e) x[e] = y[e];
     };
@@ -797,7 +926,7 @@ int encode(CUtensorMap *map, const Attention &a, const char *base, int64_t head,
   return pg_detail_tensormap(map, 4, reinterpret_cast<uintptr_t>(base), dims, strides, box);
 }
 
-template <class T, int DIM, bool TREE>
+template <class T, int DIM, bool TREE, bool K8>
 int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cudaStream_t stream) {
   a.rows_per_tile = kRows;
   const int tiles = pg::tile_bound(a, kRows);
@@ -809,25 +938,30 @@ int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cuda
   // a kv head's tiles of the latest queries, which see the most keys, go first
   const dim3 grid(a.heads, tiles, a.parts);
   const int run = std::gcd(a.page_size, kKeys);  // the keys that a page and a block always share
+  if constexpr (K8) {
+    return pg::launch<prompt_kernel<T, DIM, false, TREE, true>>("prompt_kernel", grid, kThreads,
+                      Plan<DIM, true>::bytes, stream, a, k_map, v_map, run);
+  } else {
   if (run < 8)
-    return pg::launch<prompt_kernel<T, DIM, false, TREE>>("prompt_kernel", grid, kThreads,
-                      Plan<DIM>::bytes, stream, a, k_map, v_map, run);
+    return pg::launch<prompt_kernel<T, DIM, false, TREE, false>>("prompt_kernel", grid, kThreads,
+                      Plan<DIM, false>::bytes, stream, a, k_map, v_map, run);
   int rc = encode(&k_map, a, a.k, a.k_head, a.k_page);
   if (!rc) rc = encode(&v_map, a, a.v, a.v_head, a.v_page);
   if (rc) return rc;
-  return pg::launch<prompt_kernel<T, DIM, true, TREE>>("prompt_kernel", grid, kThreads,
-                    Plan<DIM>::bytes, stream, a, k_map, v_map, run);
+  return pg::launch<prompt_kernel<T, DIM, true, TREE, false>>("prompt_kernel", grid, kThreads,
+                    Plan<DIM, false>::bytes, stream, a, k_map, v_map, run);
+  }
 }
 
-template <bool TREE>
+template <bool TREE, bool K8>
 int run_prompt(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                cudaStream_t stream) {
   if (bf16)
     return a.dim <= 64
-               ? launch_prompt<__nv_bfloat16, 64, TREE>(a, max_len, partial_bytes, sms, stream)
-               : launch_prompt<__nv_bfloat16, 128, TREE>(a, max_len, partial_bytes, sms, stream);
-  return a.dim <= 64 ? launch_prompt<__half, 64, TREE>(a, max_len, partial_bytes, sms, stream)
-                     : launch_prompt<__half, 128, TREE>(a, max_len, partial_bytes, sms, stream);
+               ? launch_prompt<__nv_bfloat16, 64, TREE, K8>(a, max_len, partial_bytes, sms, stream)
+               : launch_prompt<__nv_bfloat16, 128, TREE, K8>(a, max_len, partial_bytes, sms, stream);
+  return a.dim <= 64 ? launch_prompt<__half, 64, TREE, K8>(a, max_len, partial_bytes, sms, stream)
+                     : launch_prompt<__half, 128, TREE, K8>(a, max_len, partial_bytes, sms, stream);
 }
 
 }  // namespace
