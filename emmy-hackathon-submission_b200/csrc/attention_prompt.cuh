@@ -62,7 +62,7 @@ constexpr int kKeys = 128, kRows = 256, kHalf = 128;
 constexpr int kThreads = 384;
 constexpr int kCopyWarps = 2, kCopyThreads = 32 * kCopyWarps;  // without TMA
 constexpr int kLag = 2;  // tiles whose cp.async copies are in flight before the oldest is waited for
-constexpr int kConvertWarps = 3;  // of a cache in 8 bits
+constexpr int kThreads8 = 512, kConvertWarps = 7;  // of a cache in 8 bits
 constexpr float kGrow = 8.0f;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
@@ -339,7 +339,7 @@ __device__ __noinline__ void add_values(const Attention &a, const int *pages, in
 // Without TMA the maps and `boxes` are empty.
 // TREE: a sequence's new tokens are a tree. K8: the cache is in 8 bits (and comes without TMA).
 template <class T, int DIM, bool TMA, bool TREE, bool K8>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
     prompt_kernel(const __grid_constant__ Attention a, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map, int run) {
   using P = Plan<DIM, K8>;
@@ -399,9 +399,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // Registers: three groups of 128 threads start with 168 each; the rows' threads, which hold a
   // row of S and what is made of it, take what the third group can do without (2 x 232 + 40 or
-  // 2 x 200 + 104 = 3 x 168).
+  // 2 x 200 + 104 = 3 x 168). With keys in 8 bits there are four groups of 128 each: 2 x 200 + 2 x 56.
   if (warp >= 8) {
     if (TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    else if (K8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (TMA && (warp == 9 || warp == 10)) {
       // --- copies: one warp the keys of each block, one the values; lane i the i-th page run ----
@@ -452,59 +453,68 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kMine = (kKeys / kPer + kConvertWarps - 1) / kConvertWarps;
       const int sub = lane / kPieces, piece = lane % kPieces;
       const bool column = piece * 16 < a.dim;
-      const auto pages_of = [&](int j, int2 *p) {  // keys lane, lane + 32, ... of step j
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = make_int2(-1, 0);
-          const int key = blocks.key_block(b0 + j) * kKeys + lane + 32 * i;
-          if (j < steps && key < t.length) {
-            const int entry = pg::page_index(a, key);
-            p[i] = make_int2(t.pages[entry], key - entry * a.page_size);
-            if (p[i].x < 0 || p[i].x >= a.pages) {
-              atomicOr(a.status, PG_CACHE_BAD_PAGE);
-              p[i].x = -1;
-            }
-          }
-        }
+      // where a thread's m-th row of step j is, among the pages
+      const auto row_key = [&](int j, int m) {
+        return blocks.key_block(b0 + j) * kKeys + (m * kConvertWarps + w) * kPer + sub;
+      };
+      const auto page_for = [&](int j, int m) {  // as the table names it; -1: there is no such key
+        if (j >= steps || (m * kConvertWarps + w) * kPer >= kKeys) return -1;
+        const int key = row_key(j, m);
+        if (key >= t.length) return -1;
+        const int page = t.pages[pg::page_index(a, key)];
+        return page < 0 ? a.pages : page;
       };
       const auto place = [&](int half, int m) {  // a thread's m-th row's 16 bytes
         return smem_at + P::raws + half * P::raw +
                ((m * kConvertWarps + w) * kPer * kPieces + lane) * 16;
       };
       float scales[2][kMine];
-      const auto issue = [&](int half, const int2 *p) {
+      int pages[kMine];
+      const auto issue = [&](int half, int j) {
         const char *from = (half ? a.v : a.k) + head * (half ? a.v_head : a.k_head) + piece * 16;
         const char *of = (half ? a.v_scale : a.k_scale) + head * (half ? a.vs_head : a.ks_head);
         const int64_t page_bytes = half ? a.v_page : a.k_page;
         const int64_t of_bytes = half ? a.vs_page : a.ks_page;
 #pragma unroll
         for (int m = 0; m < kMine; ++m) {
-          const int i = m * kConvertWarps + w, r = i * kPer + sub, run = (i * kPer) >> 5;
-          if (i >= kKeys / kPer) break;
-          const int2 mine = run == 0 ? p[0] : run == 1 ? p[1] : run == 2 ? p[2] : p[3];
-          const int page = __shfl_sync(0xffffffffu, mine.x, r & 31);
-          const int row = __shfl_sync(0xffffffffu, mine.y, r & 31);
-          const bool real = page >= 0;
+          const bool real = pages[m] >= 0;
+          const int key = row_key(j, m), row = key - pg::page_index(a, key) * a.page_size;
           scales[half][m] =
-              real ? *reinterpret_cast<const float *>(of + page * of_bytes + row * 4ll) : 0.0f;
-          const char *src = real && column ? from + page * page_bytes +
+              real ? *reinterpret_cast<const float *>(of + pages[m] * of_bytes + row * 4ll) : 0.0f;
+          const char *src = real && column ? from + pages[m] * page_bytes +
                                                  static_cast<int64_t>(row) * a.dim
                                            : from;
           const int bytes = real && column ? 16 : 0;  // 0: zeroed, nothing read
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place(half, m)),
-                       "l"(src), "r"(bytes)
-                       : "memory");
+          if ((m * kConvertWarps + w) * kPer < kKeys)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place(half, m)),
+                         "l"(src), "r"(bytes)
+                         : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      int2 p[4];
-      pages_of(0, p);
-      issue(0, p);
-      issue(1, p);
+      const auto checked = [&](int page) {
+        if (page >= a.pages) {
+          atomicOr(a.status, PG_CACHE_BAD_PAGE);
+          return -1;
+        }
+        return page;
+      };
+      int next[kMine];
+#pragma unroll
+      for (int m = 0; m < kMine; ++m) {
+        pages[m] = checked(page_for(0, m));
+        next[m] = page_for(1, m);
+      }
+      issue(0, 0);
+      issue(1, 0);
       bool ok = true;
       for (int j = 0; j < steps && ok; ++j) {
-        pages_of(j + 1, p);
         const int key0 = blocks.key_block(b0 + j) * kKeys;
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+          pages[m] = checked(next[m]);
+          next[m] = page_for(j + 2, m);
+        }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int n = 2 * j + half, s = n % P::stages;
@@ -517,8 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool look = half && !both.all(key0);
 #pragma unroll
           for (int m = 0; m < kMine; ++m) {
-            const int i = m * kConvertWarps + w, r = i * kPer + sub;
-            if (i >= kKeys / kPer) break;
+            const int r = (m * kConvertWarps + w) * kPer + sub;
+            if (r - sub >= kKeys) break;
             const float scale = scales[half][m];
             uint4 out[2];
             widen<T>(*reinterpret_cast<const uint4 *>(smem + (place(half, m) - smem_at)), scale, out);
@@ -532,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_async();
           bar_arrive(full(s));
-          issue(half, p);
+          issue(half, j + 1);
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -939,7 +949,7 @@ int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cuda
   const dim3 grid(a.heads, tiles, a.parts);
   const int run = std::gcd(a.page_size, kKeys);  // the keys that a page and a block always share
   if constexpr (K8) {
-    return pg::launch<prompt_kernel<T, DIM, false, TREE, true>>("prompt_kernel", grid, kThreads,
+    return pg::launch<prompt_kernel<T, DIM, false, TREE, true>>("prompt_kernel", grid, kThreads8,
                       Plan<DIM, true>::bytes, stream, a, k_map, v_map, run);
   } else {
   if (run < 8)
