@@ -32,6 +32,7 @@ struct Attention {
   int64_t ks_page, ks_head, vs_page, vs_head;         // bytes, of the scales
   int batch, queries, heads, group, dim, page_size, pages, width, slot_rows;
   int window, sinks, parts, rows_per_tile;
+  int part_blocks;  // of keys that a part has at least, where tiles have as many parts as they are long
   uint32_t page_mul;  // for page_index
   int page_shift;
   float scale_log2;

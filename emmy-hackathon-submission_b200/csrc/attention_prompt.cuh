@@ -360,9 +360,12 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
   const int hi = TREE ? t.length - 1 : first_pos + (t.row + t.rows - 1) / a.group;
   const Blocks blocks = pg::blocks_of(a, lo, hi, kKeys);
   const Seen both(a, lo, hi, t.length);
-  const int b0 = static_cast<int>(static_cast<int64_t>(blocks.count) * part / a.parts);
+  const int parts =
+      TREE ? max(1, min(a.parts, (blocks.count + a.part_blocks - 1) / a.part_blocks)) : a.parts;
+  if (TREE && part >= parts) return;
+  const int b0 = static_cast<int>(static_cast<int64_t>(blocks.count) * part / parts);
   const int steps =
-      static_cast<int>(static_cast<int64_t>(blocks.count) * (part + 1) / a.parts) - b0;
+      static_cast<int>(static_cast<int64_t>(blocks.count) * (part + 1) / parts) - b0;
 
   const uint32_t smem_at = shared_at(smem), bars = smem_at + P::bars;
   const auto full = [&](int s) { return bars + 8 * s; };
@@ -853,7 +856,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
           *reinterpret_cast<uint4 *>(to + 16 * q) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     };
-    if (a.parts == 1) {
+    if (parts == 1) {
       const float inv = l == 0.0f ? NAN : 1.0f / l;  // 0: all its scores are -inf, 0 / 0
 #pragma unroll 1
       for (int k = 0; k < DIM / 32; ++k) {
@@ -885,13 +888,13 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
       *ml_of(to) = make_float2(m, l);
       __threadfence();
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (tid == 0) sh.last = atomicInc(a.arrived + pair, a.parts - 1) == a.parts - 1u;
+      if (tid == 0) sh.last = atomicInc(a.arrived + pair, parts - 1) == parts - 1u;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (sh.last) {
         __threadfence();
         float top = -INFINITY, total = 0.0f;
-        for (int p = 0; p < a.parts; ++p) top = fmaxf(top, __ldcg(ml_of(all + p * size)).x);
-        for (int p = 0; p < a.parts; ++p) {
+        for (int p = 0; p < parts; ++p) top = fmaxf(top, __ldcg(ml_of(all + p * size)).x);
+        for (int p = 0; p < parts; ++p) {
           const float2 ml = __ldcg(ml_of(all + p * size));
           total += ml.x == -INFINITY ? 0.0f : ml.y * pg::exp2_fast((ml.x - top) * c);
         }
@@ -899,7 +902,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
 #pragma unroll 1
         for (int k = 0; k < DIM / 32; ++k) {
           float x[32] = {};
-          for (int p = 0; p < a.parts; ++p) {
+          for (int p = 0; p < parts; ++p) {
             const float pm = __ldcg(ml_of(all + p * size)).x;
             const float f = pm == -INFINITY ? 0.0f : pg::exp2_fast((pm - top) * c);
 #pragma unroll
@@ -939,11 +942,30 @@ int encode(CUtensorMap *map, const Attention &a, const char *base, int64_t head,
 template <class T, int DIM, bool TREE, bool K8>
 int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cudaStream_t stream) {
   a.rows_per_tile = kRows;
-  const int tiles = pg::tile_bound(a, kRows);
+  int tiles = pg::tile_bound(a, kRows);
+  if (TREE) {
+    const int64_t most = a.batch * ((static_cast<int64_t>(PG_ATTENTION_TREE) * a.group + kRows - 1) / kRows);
+    tiles = static_cast<int>(most < tiles ? most : tiles);
+  }
   if (tiles > 65535)
     return pg::argument_fail("pg_attention: %d queries of %d heads: too many tiles", a.queries,
                              a.group);
   a.parts = pg::choose_parts(a, tiles, kRows, DIM, kKeys, max_len, sms, partial_bytes);
+  if (TREE) {
+    // A tree's few rows go over all of a context, so lengths of unlike size leave most SMs idle at the
+    // end: long ones are cut, in parts as long as a third or a fourth of the longest (16 trees of 64
+    // tokens on up to 16384 keys, 32 heads on 8 of 128: 277 us in one part, 149 so).
+    const int64_t pairs = static_cast<int64_t>(tiles) * a.heads, longest = max_len / kKeys + 1;
+    const int64_t each = pairs * kRows * (DIM + 2) * 4ll;
+    int64_t parts = a.parts;
+    if (parts == 1 && pairs <= pg::kCounters) {
+      parts = 4ll * sms / pairs;
+      parts = partial_bytes / each < parts ? partial_bytes / each : parts;
+      parts = longest / 4 < parts ? longest / 4 : parts;
+      a.parts = static_cast<int>(parts < 1 ? 1 : parts);
+    }
+    a.part_blocks = static_cast<int>((longest + a.parts - 1) / a.parts);
+  }
   CUtensorMap k_map = {}, v_map = {};
   // a kv head's tiles of the latest queries, which see the most keys, go first
   const dim3 grid(a.heads, tiles, a.parts);
