@@ -572,28 +572,22 @@ template <> struct Sixteen<__half> : Sixteen16<__half, __half2> {
   }
 };
 
-// x / s for 16 numbers, rounded, halves to even. x times 1 / s is off by up to 2^-15 at 127, so a number
-// whose fraction is that near to a half is divided in 64 bits, where the quotient of two f32 numbers is a
-// half only if it is one.
+// x / s for 16 numbers, rounded, halves to even. x times 1 / s is off by up to 2^-16 at 127, so what it
+// rounds to, q, may be one off where the quotient is next to a half. The remainder x - q s is exact in
+// f32 (a multiple of half the scale's last bit, no larger than about s / 2), and against s / 2 it tells.
+// bf16 rows have exact halves often: a number and the largest are whole numbers below 256 by powers of two.
+// For scales of 2^-100 and more.
 __device__ __forceinline__ uint4 quantise(const float *x, float s) {
-  // a scale whose inverse is no f32 number, or that has lost bits itself, has them all divided
-  const bool small = s < 0x1p-100f;
-  const float inverse = small ? 0.0f : 1.0f / s;
+  const float inverse = 1.0f / s;
+  // from where on a remainder is too large: s / 2 for an odd q, the number after it for an even one
+  const uint32_t even = __float_as_uint(0.5f * s) + 1;
   constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: its last bits are a whole number's
   float y[16];
-  bool near = small;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float t = x[i] * inverse;
-    y[i] = t + kShift;
-    near |= fabsf(t - (y[i] - kShift)) > 0.5f - 0x1p-14f;
-  }
-  if (near && s > 0.0f) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const double t = static_cast<double>(x[i]) / static_cast<double>(s);
-      y[i] = kShift + static_cast<float>(fmin(fmax(rint(t), -127.0), 127.0));
-    }
+    y[i] = fmaf(x[i], inverse, kShift);
+    const float r = fmaf(kShift - y[i], s, x[i]);
+    if (fabsf(r) >= __uint_as_float(even - (__float_as_uint(y[i]) & 1))) y[i] += copysignf(1.0f, r);
   }
   uint32_t w[4];
 #pragma unroll
@@ -603,6 +597,22 @@ __device__ __forceinline__ uint4 quantise(const float *x, float s) {
         __byte_perm(__float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]), 0x0040);
     w[i] = __byte_perm(a, b, 0x5410);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// ... of any other scale, whose inverse may be no f32 number, and which may have lost bits itself: by 64-bit
+// division, where the quotient of two f32 numbers is a half only if it is one.
+__device__ __noinline__ uint4 quantise_small(const uint4 *raw, int words, float s) {
+  uint32_t w[4] = {};
+  if (s > 0.0f)
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t bits = reinterpret_cast<const uint32_t *>(raw)[words == 4 ? i : i / 2];
+      // 16-bit rows with such scales are bf16: f16 has no numbers as small
+      const float x = __uint_as_float(words == 4 ? bits : i & 1 ? bits & 0xffff0000u : bits << 16);
+      const double q = rint(static_cast<double>(x) / static_cast<double>(s));
+      const int b = static_cast<int>(fmin(fmax(q, -127.0), 127.0)) & 255;
+      w[i / 4] |= b << 8 * (i % 4);
+    }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -635,14 +645,14 @@ __device__ __forceinline__ Place place_of(const pg_cache &c, const int *slots_in
   return Place{page, pos % c.page_size};
 }
 
-constexpr int kRowsAhead = 2;  // rows that a lane has in flight
 
 // WRITE: rows are quantised into the cache, else read back from it. A warp takes one token.
 template <class T, bool WRITE>
-__global__ void __launch_bounds__(kCopy) cache8_rows(pg_cache c, pg_cache_scales s, int layer,
+__global__ void __launch_bounds__(kCopy, 4) cache8_rows(pg_cache c, pg_cache_scales s, int layer,
                                                      const int *slots_in, const int *starts, int n,
                                                      int tokens, pg_rows k, pg_rows v) {
   using X = Sixteen<T>;
+  constexpr int kRowsAhead = WRITE ? 2 : 4;  // rows that a lane has in flight
   pg::wait_for_earlier_kernels();
   const int lane = threadIdx.x & 31, warps = gridDim.x * (kCopy / 32);
   const int pieces = c.row_bytes / 16;
@@ -687,16 +697,20 @@ __global__ void __launch_bounds__(kCopy) cache8_rows(pg_cache c, pg_cache_scales
           const int r = base + j * step;
           float x[16];
           X::get(raw[j], x);
-          uint32_t most = 0;  // of their sizes' bits, which are in the numbers' order, NaN the last
+          float most = 0.0f;  // NaN if one is
 #pragma unroll
-          for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-          for (int off = lanes / 2; off; off /= 2)
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-          const bool finite = most < 0x7f800000u;
-          const float scale = finite ? __fdiv_rn(__uint_as_float(most), 127.0f) : NAN;
+          for (int i = 0; i < 16; i += 2) most = pg::max3(most, fabsf(x[i]), fabsf(x[i + 1]));
+          for (int off = lanes / 2; off; off /= 2) {
+            const float o = __shfl_xor_sync(0xffffffffu, most, off);
+            most = pg::max3(most, o, o);
+          }
+          const bool finite = most < INFINITY;
+          const float scale = finite ? __fdiv_rn(most, 127.0f) : NAN;
           if (r < rows && sub < pieces) {
             // of a row that is not finite nothing is kept but that
-            *cache_at(r) = finite ? quantise(x, scale) : make_uint4(0, 0, 0, 0);
+            *cache_at(r) = !finite            ? make_uint4(0, 0, 0, 0)
+                           : scale < 0x1p-100f ? quantise_small(raw[j], X::words, scale)
+                                               : quantise(x, scale);
             if (sub == 0) *scale_at(r) = scale;
           }
         }
