@@ -52,16 +52,22 @@ TREE_MAX = 64  # PG_ATTENTION_TREE
 # pg_attention_args at once: setting its fields one by one takes longer than a short call
 _PACK = struct.Struct("=9Q10q13if")
 assert _PACK.size == ctypes.sizeof(AttentionArgs)
+_PACK_MORE = struct.Struct("=2Q4qQ")  # pg_attention_more
+assert _PACK_MORE.size == ctypes.sizeof(AttentionMore)
 
 
 class Workspace:
     """The device memory in which attention leaves the parts of a long sequence's result until
-    they are joined. One per stream: calls that overlap on the GPU must not share it. It has to
-    live until the calls that were given it have run."""
+    they are joined, and widens the keys and values of prompts over 8 bits. One per stream: calls that
+    overlap on the GPU must not share it. It has to live until the calls that were given it have run.
+    ``size`` in bytes may be more than the default: trees and long prompts over 8 bits make use of it."""
 
-    def __init__(self, device: Any = None):
-        self.buffer = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.int32,
+    def __init__(self, device: Any = None, size: int = WORKSPACE_BYTES):
+        if size < WORKSPACE_BYTES:
+            raise ValueError(f"size {size}: want {WORKSPACE_BYTES} bytes at least")
+        self.buffer = torch.zeros(size // 4, dtype=torch.int32,
                                   device="cuda" if device is None else device)
+        self.size = size // 4 * 4
         self.device = self.buffer.device  # with an index, as a call's tensors have it
         wait_until_set(self.device)
 
@@ -122,7 +128,7 @@ def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any
         _PACK.pack_into(
             args, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), starts or 0, slots,
             table.data_ptr(), int32_list("lens", lens, dev, rows), workspace.buffer.data_ptr(),
-            WORKSPACE_BYTES, qs[0] * size, qs[1] * size, os_[0] * size, os_[1] * size,
+            workspace.size, qs[0] * size, qs[1] * size, os_[0] * size, os_[1] * size,
             ks[0] * size_kv, ks[1] * size_kv, vs[0] * size_kv, vs[1] * size_kv, table.stride(0),
             dtype_code(dtype), batch, tokens, heads, hq // heads, dim, page_size, pages, width, rows,
             window, sinks, max_len or 0, dim ** -0.5 if scale is None else scale)
@@ -137,23 +143,23 @@ def _call(q: Any, starts: Any, k: Any, v: Any, table: Any, lens: Any, slots: Any
 
 
 def _more(dev: Any, tokens: int, rows: Any, k_scale: Any, v_scale: Any, mask: Any) -> AttentionMore:
-    more = AttentionMore()
+    scales, at = (0, 0, 0, 0, 0, 0), 0
     if k_scale is not None or v_scale is not None:
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
             if t is None or t.dtype is not torch.float32 or t.shape != rows or t.device != dev or \
                     (rows[2] > 1 and t.stride(2) != 1):
                 raise ValueError(f"{name}: want float32 {tuple(rows)} on {dev} with a page's rows one "
                                  f"after another, got {t if t is None else (t.dtype, t.shape)}")
-        more.k_scale, more.k_scale_page, more.k_scale_head = (
-            k_scale.data_ptr(), 4 * k_scale.stride(0), 4 * k_scale.stride(1))
-        more.v_scale, more.v_scale_page, more.v_scale_head = (
-            v_scale.data_ptr(), 4 * v_scale.stride(0), 4 * v_scale.stride(1))
+        ks, vs = k_scale.stride(), v_scale.stride()
+        scales = (k_scale.data_ptr(), v_scale.data_ptr(), 4 * ks[0], 4 * ks[1], 4 * vs[0], 4 * vs[1])
     if mask is not None:
         if mask.dtype is not torch.int64 or mask.shape != (tokens,) or not mask.is_contiguous() or \
                 mask.device != dev:
             raise ValueError(f"mask: want contiguous int64 [{tokens}] on {dev}, got {mask.dtype} "
                              f"{tuple(mask.shape)} on {mask.device}")
-        more.mask = mask.data_ptr()
+        at = mask.data_ptr()
+    more = AttentionMore()
+    _PACK_MORE.pack_into(more, 0, *scales, at)
     return more
 
 
