@@ -9,6 +9,12 @@ samples that share its full pages (``fork``), and the samples are continued toke
 (``attention.decode``), every token drawn from the distribution whose log probability, entropy and
 best alternatives ``logprobs`` gives. Halfway the worst sample of each prompt is dropped (``free``)
 and the cache compacted. Nothing in the loop waits for the GPU; the result comes back at the end.
+
+With ``--temperature``, ``--top-k``, ``--top-p`` or ``--min-p`` tokens are drawn by ``sampling.sample``, with
+``--bits8`` the cache is in 8 bits. ``--draft`` continues each prompt by drafted trees instead
+(``drafted``): a small tree of guesses a sequence goes through the model at once (``attention.tree``),
+a token is drawn at each of its nodes, and the branch that the draws follow stays in the cache
+(``PagedCache.keep``). The tokens have the distribution that one at a time would have.
 """
 
 from __future__ import annotations
@@ -24,7 +30,7 @@ if __package__ in (None, ""):
 
 import torch
 
-from ptxgen import attention
+from ptxgen import attention, sampling
 from ptxgen.cache import PagedCache
 from ptxgen.logprob import logprobs
 
@@ -59,9 +65,10 @@ class Model:
                     for _ in range(layers)], heads, kv_heads, dim, window, sinks)
 
     def forward(self, tokens: Any, slots: Any, starts: Any, cache: PagedCache, workspace: Any,
-                prompts: bool) -> Any:
+                prompts: bool, mask: Any = None) -> Any:
         """The hidden states [tokens, width] of each slot's new tokens, which get room in the
-        cache: rows ``starts[i]`` to ``starts[i + 1]``, or row i alone where not ``prompts``."""
+        cache: rows ``starts[i]`` to ``starts[i + 1]``, or row i alone where not ``prompts``. With a
+        ``mask`` (``attention.branches``) they are trees."""
         cache.extend(slots, starts)
         x = self.embed[tokens]
         for i, (qkv, out) in enumerate(self.layers):
@@ -69,7 +76,12 @@ class Model:
             q, k, v = y.split([self.heads, self.kv_heads, self.kv_heads], 1)
             cache.write(i, slots, starts, k, v)
             at = dict(slots=slots, window=self.window, sinks=self.sinks, workspace=workspace)
-            if prompts:
+            if cache.k_scale is not None:
+                at |= dict(k_scale=cache.k_scale[i], v_scale=cache.v_scale[i])
+            if mask is not None:
+                o = attention.tree(q, starts, mask, cache.k[i], cache.v[i], cache.table, cache.lens,
+                                   **at)
+            elif prompts:
                 o = attention.prompt(q, starts, cache.k[i], cache.v[i], cache.table, cache.lens,
                                      **at)
             else:
@@ -88,10 +100,12 @@ class Sample:
 
 
 def generate(model: Model, prompts: list[list[int]], samples: int = 4, steps: int = 24,
-             page_size: int = 16, seed: int = 0) -> tuple[list[Sample], PagedCache]:
+             page_size: int = 16, seed: int = 0, bits8: bool = False,
+             **limits: Any) -> tuple[list[Sample], PagedCache]:
     """``samples`` continuations of each prompt by ``steps`` tokens; after half of them each
     prompt's least likely sample is dropped and keeps what it has. Every prompt has a token: the
-    samples begin from the hidden state of its last one."""
+    samples begin from the hidden state of its last one. ``limits`` are ``sampling.sample``'s; the
+    scores are those of the whole distribution."""
     if not prompts or not all(prompts) or samples < 1 or steps < 1:
         raise ValueError(f"prompts of {[len(p) for p in prompts]} tokens, {samples} samples, {steps} "
                          "steps: want at least one of each")
@@ -106,7 +120,7 @@ def generate(model: Model, prompts: list[list[int]], samples: int = 4, steps: in
     width = -(-longest // page_size)
     cache = PagedCache.allocate(len(model.layers), count * (samples + 1) * width, model.kv_heads,
                                 page_size, model.dim, count * (samples + 1), width,
-                                dtype=model.embed.dtype, device=dev)
+                                dtype=torch.int8 if bits8 else model.embed.dtype, device=dev)
     workspace = attention.Workspace(dev)
 
     # the prompts, at once: slot i holds prompt i; the last hidden state of each begins its samples
@@ -125,8 +139,12 @@ def generate(model: Model, prompts: list[list[int]], samples: int = 4, steps: in
     likely = torch.zeros(count * samples, device=dev)
     for step in range(steps):
         logits = hidden @ model.unembed
-        noise = torch.rand(logits.shape, device=dev, generator=g).clamp_(1e-9)
-        drawn = (logits.float() - noise.log().neg_().log_()).argmax(-1)
+        if limits:
+            uniform = torch.rand(logits.shape[0], device=dev, generator=g)
+            drawn = sampling.sample(logits, uniform, **limits).tokens
+        else:
+            noise = torch.rand(logits.shape, device=dev, generator=g).clamp_(1e-9)
+            drawn = (logits.float() - noise.log().neg_().log_()).argmax(-1)
         r = logprobs(logits, drawn)
         made.append((live, drawn))
         scores.append((r.logp, r.entropy))
@@ -156,16 +174,95 @@ def generate(model: Model, prompts: list[list[int]], samples: int = 4, steps: in
     return out, cache
 
 
+# A tree of guesses: the last token, three that may follow it, and one that may follow each of them.
+_PARENTS = [-1, 0, 0, 0, 1, 2, 3]
+
+
+def drafted(model: Model, prompts: list[list[int]], rounds: int = 12, page_size: int = 16,
+            seed: int = 0, bits8: bool = False, **limits: Any) -> tuple[list[list[int]], PagedCache]:
+    """Each prompt continued by one to three tokens a round, as ``sampling.sample`` with ``limits`` draws
+    them. Guesses are what the embedding alone makes of a token."""
+    if not prompts or not all(prompts) or rounds < 1:
+        raise ValueError(f"prompts of {[len(p) for p in prompts]} tokens, {rounds} rounds: want at least "
+                         "one of each")
+    dev, nodes = model.embed.device, len(_PARENTS)
+    g = torch.Generator(device=dev).manual_seed(seed)
+
+    def ints(values: Any, dtype: torch.dtype = torch.int32) -> Any:
+        return torch.tensor(list(values), dtype=dtype, device=dev)
+
+    def draw(hidden: Any) -> Any:
+        uniform = torch.rand(hidden.shape[0], device=dev, generator=g)
+        return sampling.sample(hidden @ model.unembed, uniform, **limits).tokens
+
+    count = len(prompts)
+    width = -(-(max(map(len, prompts)) + 3 * rounds + nodes) // page_size)
+    cache = PagedCache.allocate(len(model.layers), count * width, model.kv_heads, page_size, model.dim,
+                                count, width, dtype=torch.int8 if bits8 else model.embed.dtype,
+                                device=dev)
+    workspace = attention.Workspace(dev)
+    slots = ints(range(count))
+    ends = torch.tensor([len(p) for p in prompts]).cumsum(0).tolist()
+    tokens = torch.tensor([t for p in prompts for t in p], device=dev)
+    hidden = model.forward(tokens, slots, ints([0, *ends]), cache, workspace, True)
+    last = draw(hidden[[e - 1 for e in ends]])
+    starts = ints(range(0, nodes * (count + 1), nodes))
+    branches = ints(attention.branches(_PARENTS), torch.int64)
+    mask = branches.repeat(count)
+    made = [(last, None, None)]
+    for _ in range(rounds):
+        likely = (model.embed[last] @ model.unembed).topk(3).indices
+        after = (model.embed[likely] @ model.unembed).argmax(-1)
+        tree = torch.cat([last[:, None], likely, after], 1)
+        hidden = model.forward(tree.reshape(-1), slots, starts, cache, workspace, True, mask)
+        drawn = draw(hidden).view(count, nodes)
+        # from the root to the guess that is what was drawn there, and on to the guess after it
+        hit = likely == drawn[:, :1]
+        at = torch.where(hit.any(1), hit.int().argmax(1) + 1, 0)
+        guess = after.gather(1, (at - 1).clamp(min=0)[:, None])
+        more = (at > 0) & (guess == drawn.gather(1, at[:, None]))[:, 0]
+        at = torch.where(more, at + 3, at)
+        cache.keep(slots, starts, branches[at])
+        last = drawn.gather(1, at[:, None])[:, 0]
+        made.append((last, tree, at))
+    cache.check()
+    workspace.check()
+    out: list[list[int]] = [[] for _ in prompts]
+    for drawn, tree, at in made:
+        for i, t in enumerate(drawn.tolist()):
+            if tree is not None:
+                path, node = [], int(at[i])
+                while node > 0:
+                    path.append(int(tree[i, node]))
+                    node = _PARENTS[node]
+                out[i] += reversed(path)
+            out[i].append(t)
+    return out, cache
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--samples", type=int, default=4)
     ap.add_argument("--steps", type=int, default=24)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--bits8", action="store_true", help="a cache in 8 bits")
+    ap.add_argument("--draft", action="store_true", help="drafted trees, --steps rounds of them")
+    for name, kind in (("temperature", float), ("top-k", int), ("top-p", float), ("min-p", float)):
+        ap.add_argument(f"--{name}", type=kind)
     args = ap.parse_args()
+    limits = {n: v for n in ("temperature", "top_k", "top_p", "min_p")
+              if (v := getattr(args, n)) is not None}
     model = Model.random(window=64, sinks=4)
     g = torch.Generator().manual_seed(args.seed)
     prompts = [torch.randint(0, 1000, (n,), generator=g).tolist() for n in (40, 133, 7)]
-    out, cache = generate(model, prompts, args.samples, args.steps, seed=args.seed)
+    if args.draft:
+        texts, cache = drafted(model, prompts, args.steps, seed=args.seed, bits8=args.bits8, **limits)
+        for i, t in enumerate(texts):
+            print(f"prompt {i}: {len(t)} tokens in {args.steps} rounds: "
+                  f"{' '.join(map(str, t[:8]))} ...")
+        return
+    out, cache = generate(model, prompts, args.samples, args.steps, seed=args.seed,
+                          bits8=args.bits8, **limits)
     for i, s in enumerate(out):
         mean = sum(s.entropies) / len(s.entropies)
         print(f"prompt {s.prompt} sample {i % args.samples}: log p {sum(s.logps):8.2f}, mean "
