@@ -210,6 +210,9 @@ __device__ __forceinline__ void add_odd(float value, float &sum, bool first) {
   sum = first && !(fabsf(sum) < INFINITY) ? value : sum + value;
 }
 
+// 2^n of -126..127
+__device__ __forceinline__ float power_of_2(int n) { return __int_as_float((n + 127) << 23); }
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -5,7 +5,7 @@ namespace pg {
 
 int prompt_16bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                  cudaStream_t stream) {
-  return run_prompt<false, false>(a, bf16, max_len, partial_bytes, sms, stream);
+  return run_prompt<false, kOfType>(a, bf16, max_len, partial_bytes, sms, stream);
 }
 
 }  // namespace pg

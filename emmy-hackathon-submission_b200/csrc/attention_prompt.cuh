@@ -19,6 +19,9 @@
 // tokens and up to 8192 keys, 32 heads on 8 of 128 in bf16, take 1814 us that way, 498 with TMA
 // (885 TFLOP/s of the products that count).
 //
+// Over a cache in 8 bits seven warps (9 to 15) widen what they have copied to f16, for both types, or the
+// keys and values were widened before (attention_prompt_8bit.cu, which says when).
+//
 // The rows' threads bound it beside the products: 128 x 128 exponentials take the 16 lanes an SM
 // has for them 1024 cycles, the two products of DIM = 128 the same, and where a tile's weights
 // wait for its scores neither is at work. O is rescaled only when a row's running maximum has
@@ -44,6 +47,7 @@
 #include <cuda.h>
 
 #include <numeric>
+#include <type_traits>
 
 // Encodes a tensor map of 2-byte elements, 128-byte swizzled (launcher.cpp).
 int pg_detail_tensormap(void *map, int rank, uint64_t base, const uint64_t *dims,
@@ -60,19 +64,23 @@ using pg::Two;
 
 constexpr int kKeys = 128, kRows = 256, kHalf = 128;
 constexpr int kThreads = 384;
+constexpr int kThreads8 = 512, kConvertWarps = 7;  // of a cache in 8 bits
 constexpr int kCopyWarps = 2, kCopyThreads = 32 * kCopyWarps;  // without TMA
 constexpr int kLag = 2;  // tiles whose cp.async copies are in flight before the oldest is waited for
-constexpr int kThreads8 = 512, kConvertWarps = 7;  // of a cache in 8 bits
 constexpr float kGrow = 8.0f;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
-template <int DIM, bool K8>
+// What a cache holds: numbers of the type T; f16 ones whatever T is, as 2^-k (keys) and 2^-v (values) of
+// what they are, with the ints k and v for each page, of kKeys keys, at k_scale; or ones of 8 bits.
+enum Held { kOfType, kShifted, kBytes };
+
+template <int DIM, Held HELD>
 struct Plan {
   // 128 queries, keys or values: by eight rows, then by 64 columns, each such 1024 bytes swizzled
   static constexpr int atom = 1024, chunks = DIM / 64, group = chunks * atom;
   static constexpr int tile = 16 * group;
-  static constexpr int raw = K8 ? kKeys * DIM : 0;  // keys or values in 8 bits, on their way
-  static constexpr int stages = DIM == 128 ? K8 ? 4 : 5 : 8;
+  static constexpr int raw = HELD == kBytes ? kKeys * DIM : 0;  // keys or values in 8 bits, on their way
+  static constexpr int stages = DIM == 128 ? HELD == kBytes ? 4 : 5 : 8;
   static constexpr int q = 0, ring = 2 * tile, raws = ring + stages * tile, bars = raws + 2 * raw;
   // over half an SM's shared memory, so that no other block that takes all its tensor memory
   // is resident beside this one
@@ -224,10 +232,8 @@ template <> struct Type<__nv_bfloat16> {
   }
   __device__ static float low(uint32_t w) { return __uint_as_float(w << 16); }
   __device__ static float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-  static constexpr float largest = 3.3895e38f;  // none above is finite
 };
 template <> struct Type<__half> {
-  static constexpr float largest = 65504.0f;
   static constexpr float shift = 15.0f - kGrow;  // at most 2^15 of 65504
   static constexpr uint32_t format = 0, exponent = 0x7c00;
   __device__ static uint32_t pack(float x, float y) {
@@ -242,8 +248,7 @@ template <> struct Type<__half> {
   }
 };
 
-// 16 numbers of 8 bits times their scale, rounded to T.
-template <class T>
+// 16 numbers of 8 bits times their scale, rounded to f16.
 __device__ __forceinline__ void widen(const uint4 &raw, float scale, uint4 *to) {
   const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u,
                          raw.w ^ 0x80808080u};
@@ -256,10 +261,22 @@ __device__ __forceinline__ void widen(const uint4 &raw, float scale, uint4 *to) 
                 __uint_as_float(__byte_perm(of, 0x4b000000u, i & 1 ? 0x7443 : 0x7441)));
     float y, z;
     mul(add(x, off), by).get(y, z);
-    out[i] = Type<T>::pack(y, z);
+    out[i] = Type<__half>::pack(y, z);
   }
   to[0] = make_uint4(out[0], out[1], out[2], out[3]);
   to[1] = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+// e, so that 2^-e brings scales of at most `top`, as bits, to 2^7..2^8, and numbers to 2^15. What falls below
+// f16's 2^-14 so is under 2^-28 of the largest. A row's weights are held times 2^e of its values, so for
+// those e is at least -60: the weights of values that are all 0 must not be lost beside others.
+__device__ __forceinline__ int shift_of(unsigned top, bool values) {
+  return max(static_cast<int>(top >> 23) - 134, values ? -60 : -126);
+}
+// A scale's magnitude as bits, 0 if it is not finite.
+__device__ __forceinline__ unsigned magnitude(const char *scale) {
+  const unsigned x = *reinterpret_cast<const unsigned *>(scale) & 0x7fffffffu;
+  return x < 0x7f800000u ? x : 0;
 }
 
 // A shared-memory operand of 128-byte swizzled rows: `rows` is the distance of its groups of
@@ -291,6 +308,7 @@ struct Head {  // what the roles share
   uint32_t tmem;
   int failed, odd;
   unsigned last;
+  unsigned k_top[kThreads8 / 32], v_top[kThreads8 / 32];  // kBytes: the largest scales a warp has seen
 };
 
 // Adds the values that are not finite and that the query at `pos` sees to 32 columns of its result: of
@@ -316,16 +334,17 @@ __device__ __noinline__ void add_values(const Attention &a, const int *pages, in
       if constexpr (K8) {
         scale = *reinterpret_cast<const float *>(a.v_scale + page * a.vs_page + head * a.vs_head +
                                                  row * 4ll);
-        if (127.0f * fabsf(scale) < Type<T>::largest) continue;
+        if (fabsf(scale) < INFINITY) continue;
       }
       for (int c = 0; c < 32; c += 2) {
         if (32 * k + c >= a.dim) break;
-        uint32_t w;
-        if constexpr (K8)
-          w = Type<T>::pack(scale * static_cast<int8_t>(v[c]), scale * static_cast<int8_t>(v[c + 1]));
-        else
-          w = *reinterpret_cast<const uint32_t *>(v + 2 * c);
-        const float value[2] = {Type<T>::low(w), Type<T>::high(w)};
+        float value[2];
+        if constexpr (K8) {
+          value[0] = scale * static_cast<int8_t>(v[c]), value[1] = scale * static_cast<int8_t>(v[c + 1]);
+        } else {
+          const uint32_t w = *reinterpret_cast<const uint32_t *>(v + 2 * c);
+          value[0] = Type<T>::low(w), value[1] = Type<T>::high(w);
+        }
         for (int e = 0; e < 2; ++e)
           if (!(fabsf(value[e]) < INFINITY)) {
             pg::add_odd(value[e], x[c + e], !(met >> (c + e) & 1));
@@ -337,12 +356,16 @@ __device__ __noinline__ void add_values(const Attention &a, const int *pages, in
 }
 
 // Without TMA the maps and `boxes` are empty.
-// TREE: a sequence's new tokens are a tree. K8: the cache is in 8 bits (and comes without TMA).
-template <class T, int DIM, bool TMA, bool TREE, bool K8>
-__global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
+// TREE: a sequence's new tokens are a tree. Where numbers are SHIFTED, queries are brought into f16 too, by
+// row; a row's scores are in powers of 2, with v added to them, so that its weights are what they are times
+// 2^v as its maximum is, and l takes them times 2^-v.
+template <class T, int DIM, bool TMA, bool TREE, Held HELD>
+__global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
     prompt_kernel(const __grid_constant__ Attention a, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map, int run) {
-  using P = Plan<DIM, K8>;
+  constexpr bool SHIFTED = HELD != kOfType, K8 = HELD == kBytes;
+  using P = Plan<DIM, HELD>;
+  using C = std::conditional_t<SHIFTED, __half, T>;  // what products are of
   static_assert(!(TMA && K8), "keys in 8 bits come by cp.async");
   extern __shared__ char smem_raw[];
   __shared__ Head sh;
@@ -394,9 +417,31 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if constexpr (K8) {  // one shift for all keys of the part, and one for its values
+    unsigned k_top = 0, v_top = 0;
+#pragma unroll 4
+    for (int n = tid; n < steps * kKeys; n += kThreads8) {
+      const int key = blocks.key_block(b0 + n / kKeys) * kKeys + n % kKeys;
+      if (key >= t.length) continue;
+      const int entry = pg::page_index(a, key), page = t.pages[entry];
+      if (page < 0 || page >= a.pages) continue;
+      const int64_t row = (key - entry * a.page_size) * 4ll;
+      k_top = max(k_top, magnitude(a.k_scale + page * a.ks_page + head * a.ks_head + row));
+      v_top = max(v_top, magnitude(a.v_scale + page * a.vs_page + head * a.vs_head + row));
+    }
+    sh.k_top[warp] = __reduce_max_sync(0xffffffffu, k_top);
+    sh.v_top[warp] = __reduce_max_sync(0xffffffffu, v_top);
+  }
   fence_before();
   __syncthreads();
   fence_after();
+  int2 shift = make_int2(0, 0);
+  if constexpr (K8) {
+    unsigned k_top = 0, v_top = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads8 / 32; ++w) k_top = max(k_top, sh.k_top[w]), v_top = max(v_top, sh.v_top[w]);
+    shift = make_int2(shift_of(k_top, false), shift_of(v_top, true));
+  }
   const uint32_t tmem = sh.tmem;  // S and P of tile i at 128 i, O at 256 + 128 i
   volatile int *failed = &sh.failed;
 
@@ -450,7 +495,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
       }
     } else if (K8 && warp >= 9) {
       // --- keys and values in 8 bits: copied 16 bytes at a time to where the same thread takes them up a
-      // step later, widens them to T times their row's scale, and hands them on in the products' layout --
+      // step later, widens them to f16, and hands them on in the products' layout --
       const int w = warp - 9;
       constexpr int kPieces = DIM / 16, kPer = 32 / kPieces;  // 16 bytes of a row; rows a warp takes at once
       constexpr int kMine = (kKeys / kPer + kConvertWarps - 1) / kConvertWarps;
@@ -471,6 +516,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
         return smem_at + P::raws + half * P::raw +
                ((m * kConvertWarps + w) * kPer * kPieces + lane) * 16;
       };
+      const float by[2] = {pg::power_of_2(-shift.x), pg::power_of_2(-shift.y)};
       float scales[2][kMine];
       int pages[kMine];
       const auto issue = [&](int half, int j) {
@@ -534,10 +580,10 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
             if (r - sub >= kKeys) break;
             const float scale = scales[half][m];
             uint4 out[2];
-            widen<T>(*reinterpret_cast<const uint4 *>(smem + (place(half, m) - smem_at)), scale, out);
-            if (look && !(127.0f * fabsf(scale) < Type<T>::largest)) {
-              bool odd = pg::clean<Type<T>::exponent>(out);
-              odd |= pg::clean<Type<T>::exponent>(out + 1);
+            widen(*reinterpret_cast<const uint4 *>(smem + (place(half, m) - smem_at)), scale * by[half], out);
+            if (look && !(fabsf(scale) < INFINITY)) {
+              bool odd = pg::clean<Type<C>::exponent>(out);
+              odd |= pg::clean<Type<C>::exponent>(out + 1);
               if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
             }
             *reinterpret_cast<uint4 *>(to + P::at(r, 2 * piece)) = out[0];
@@ -576,7 +622,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
           if (!both.all(key0)) {
             bool odd = false;
             for (int i = w; i < kKeys / kPer; i += kCopyWarps) {  // the pieces it has copied
-              odd |= pg::clean<Type<T>::exponent>(reinterpret_cast<uint4 *>(smem + P::ring + s * P::tile +
+              odd |= pg::clean<Type<C>::exponent>(reinterpret_cast<uint4 *>(smem + P::ring + s * P::tile +
                                                         P::at(i * kPer + sub, piece)));
             }
             if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
@@ -629,7 +675,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
     } else if (warp == 8 && steps) {
       // --- products --------------------------------------------------------------------------
       const uint32_t elected = lane == 0;
-      constexpr uint32_t s_desc = product<T>(kKeys, false), o_desc = product<T>(DIM, true);
+      constexpr uint32_t s_desc = product<C>(kKeys, false), o_desc = product<C>(DIM, true);
       const auto scores = [&](int i, int s) {  // S_i = Q_i K^T
         const uint32_t q_at = smem_at + P::q + i * P::tile, k_at = smem_at + P::ring + s * P::tile;
 #pragma unroll
@@ -688,15 +734,38 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
                                    : Sight<TREE>{-1, 0, 0};
     const int pos = sight.pos;
     const float c = fabsf(a.scale_log2);  // a negative scale turns the queries' signs instead
+    int q_shift = 0;                      // queries are 2^-q_shift of what they are
     {
       const char *from = a.q + (t.query + token) * a.q_token + h * a.q_head;
       const uint32_t flip = a.scale_log2 < 0 ? 0x80008000u : 0u;
+      constexpr bool to_f16 = !std::is_same_v<T, C>;
+      if (to_f16 && real) {  // the largest that is finite comes to 2^14..2^15
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int piece = 0; piece < a.dim / 8; ++piece) {
+          const uint4 x = pg::load16(from + piece * 16);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t y = w[e / 2] >> 16 * (e & 1) & 0x7fff;
+            if (y < Type<T>::exponent) top = max(top, y);
+          }
+        }
+        q_shift = max(static_cast<int>(top >> 7) - 141, -126);
+      }
+      const float by = pg::power_of_2(-q_shift);
 #pragma unroll
       for (int piece = 0; piece < DIM / 8; ++piece) {
         uint4 x = make_uint4(0, 0, 0, 0);
         if (real && piece * 8 < a.dim) {
           x = pg::load16(from + piece * 16);
           x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+          if constexpr (to_f16) {
+            uint32_t *const w = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = Type<C>::pack(Type<T>::low(w[e]) * by, Type<T>::high(w[e]) * by);
+          }
         }
         *reinterpret_cast<uint4 *>(smem + P::q + i * P::tile + P::at(r, piece)) = x;
       }
@@ -716,12 +785,25 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
     const int whole_end = both.high < 0 ? 0 : min(steps, both.high / kKeys + 1 - at_first);
     const unsigned wholes = max(0, whole_end - whole);
     float m = -INFINITY, l = 0.0f;
+    const auto shifts_of = [&](int j) {  // asked for a step before
+      if (HELD != kShifted || j >= steps) return shift;
+      return *reinterpret_cast<const int2 *>(a.k_scale + t.pages[blocks.key_block(b0 + j)] * a.ks_page +
+                                             head * a.ks_head);
+    };
+    int2 next = shifts_of(0);
+    const float m_to_2 = SHIFTED ? 1.0f : c;  // brings m into powers of 2
     const bool active = i < tiles;
     bool ok = true;
     for (int j = 0; j < steps && active; ++j) {
       ok = __all_sync(0xffffffffu, bar_wait(s_full(i), j & 1, failed, a.status));
       if (!ok) break;
       fence_after();
+      if constexpr (HELD == kShifted) {
+        shift = next;
+        next = shifts_of(j + 1);
+      }
+      const float to_2 = SHIFTED ? c * pg::power_of_2(min(max(q_shift + shift.x, -126), 127)) : c;
+      const float plus = static_cast<float>(shift.y);
       float s[kKeys];
       uint32_t *const s_bits = reinterpret_cast<uint32_t *>(s);
 #pragma unroll
@@ -743,7 +825,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
           for (int piece = 0; piece < DIM / 8; ++piece) {
             uint4 *at16 = reinterpret_cast<uint4 *>(values + P::at(r, piece));
             if (key0 + r >= t.length) *at16 = make_uint4(0, 0, 0, 0);
-            else odd |= pg::clean<Type<T>::exponent>(at16);
+            else odd |= pg::clean<Type<C>::exponent>(at16);
           }
           if (odd) *const_cast<volatile int *>(&sh.odd) = 1;
           fence_async();
@@ -770,12 +852,12 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
           }
         }
       }
-      const float most = largest(s, m);
+      const float most = SHIFTED ? fmaxf(m, fmaf(largest(s, -INFINITY), to_2, plus)) : largest(s, m);
       // the first block's maximum stands until a row's has grown by 2^8 (or is NaN)
       if (j == 0) {
         m = most;
-      } else if (__any_sync(0xffffffffu, !((most - m) * c <= kGrow))) {
-        const float f = m == -INFINITY ? 0.0f : pg::exp2_fast((m - most) * c);
+      } else if (__any_sync(0xffffffffu, !((most - m) * m_to_2 <= kGrow))) {
+        const float f = m == -INFINITY ? 0.0f : pg::exp2_fast((m - most) * m_to_2);
         m = most;
         l *= f;
 #pragma unroll
@@ -790,10 +872,12 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
         }
       }
       // an infinite maximum gives NaN, as the formula does, in every weight
-      const float base =
-          m == -INFINITY ? 0.0f : m == INFINITY ? NAN : Type<T>::shift - m * c;
-      Two sum[2] = {Two(l, 0.0f), Two(0.0f, 0.0f)};
-      const Two c2(c, c), base2(base, base);
+      const float base = m == -INFINITY ? 0.0f
+                         : m == INFINITY ? NAN
+                         : SHIFTED            ? plus + Type<C>::shift - m
+                                         : Type<C>::shift - m * c;
+      Two sum[2] = {Two(SHIFTED ? 0.0f : l, 0.0f), Two(0.0f, 0.0f)};
+      const Two c2(to_2, to_2), base2(base, base);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         uint32_t x[32];
@@ -804,14 +888,14 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
           y = pg::exp2_fast(y);
           z = pg::exp2_fast(z);
           sum[e & 1] = add(sum[e & 1], Two(y, z));
-          x[e] = Type<T>::pack(y, z);
+          x[e] = Type<C>::pack(y, z);
         }
         tmem_store(s_at + 32 * k, x);
       }
       {
         float y, z;
         add(sum[0], sum[1]).get(y, z);
-        l = y + z;
+        l = SHIFTED ? fmaf(y + z, pg::power_of_2(-shift.y), l) : y + z;
       }
       wait_stores();
       fence_before();
@@ -840,7 +924,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
       float y[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e) y[e] = x[e];
-      add_values<T, TREE, K8>(a, t.pages, t.length, blocks, both, b0, steps, head, sight, k, lost, y);
+      add_values<C, TREE, HELD == kBytes>(a, t.pages, t.length, blocks, both, b0, steps, head, sight, k, lost, y);
 #pragma unroll
       for (int e = 0; e < 32; ++e) x[e] = y[e];
     };
@@ -896,7 +980,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
         for (int p = 0; p < parts; ++p) top = fmaxf(top, __ldcg(ml_of(all + p * size)).x);
         for (int p = 0; p < parts; ++p) {
           const float2 ml = __ldcg(ml_of(all + p * size));
-          total += ml.x == -INFINITY ? 0.0f : ml.y * pg::exp2_fast((ml.x - top) * c);
+          total += ml.x == -INFINITY ? 0.0f : ml.y * pg::exp2_fast((ml.x - top) * m_to_2);
         }
         const float inv = total == 0.0f ? NAN : 1.0f / total;
 #pragma unroll 1
@@ -904,7 +988,7 @@ __global__ void __launch_bounds__(K8 ? kThreads8 : kThreads, 1)
           float x[32] = {};
           for (int p = 0; p < parts; ++p) {
             const float pm = __ldcg(ml_of(all + p * size)).x;
-            const float f = pm == -INFINITY ? 0.0f : pg::exp2_fast((pm - top) * c);
+            const float f = pm == -INFINITY ? 0.0f : pg::exp2_fast((pm - top) * m_to_2);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const float4 y = __ldcg(o_of(all + p * size, 8 * k + q));
@@ -939,7 +1023,7 @@ int encode(CUtensorMap *map, const Attention &a, const char *base, int64_t head,
   return pg_detail_tensormap(map, 4, reinterpret_cast<uintptr_t>(base), dims, strides, box);
 }
 
-template <class T, int DIM, bool TREE, bool K8>
+template <class T, int DIM, bool TREE, Held HELD>
 int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cudaStream_t stream) {
   a.rows_per_tile = kRows;
   int tiles = pg::tile_bound(a, kRows);
@@ -970,30 +1054,31 @@ int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cuda
   // a kv head's tiles of the latest queries, which see the most keys, go first
   const dim3 grid(a.heads, tiles, a.parts);
   const int run = std::gcd(a.page_size, kKeys);  // the keys that a page and a block always share
-  if constexpr (K8) {
-    return pg::launch<prompt_kernel<T, DIM, false, TREE, true>>("prompt_kernel", grid, kThreads8,
-                      Plan<DIM, true>::bytes, stream, a, k_map, v_map, run);
+  if constexpr (HELD == kBytes) {
+    return pg::launch<prompt_kernel<T, DIM, false, TREE, HELD>>("prompt_kernel", grid, kThreads8,
+                      Plan<DIM, HELD>::bytes, stream, a, k_map, v_map, run);
   } else {
-  if (run < 8)
-    return pg::launch<prompt_kernel<T, DIM, false, TREE, false>>("prompt_kernel", grid, kThreads,
-                      Plan<DIM, false>::bytes, stream, a, k_map, v_map, run);
-  int rc = encode(&k_map, a, a.k, a.k_head, a.k_page);
-  if (!rc) rc = encode(&v_map, a, a.v, a.v_head, a.v_page);
-  if (rc) return rc;
-  return pg::launch<prompt_kernel<T, DIM, true, TREE, false>>("prompt_kernel", grid, kThreads,
-                    Plan<DIM, false>::bytes, stream, a, k_map, v_map, run);
+    if constexpr (HELD == kOfType)
+      if (run < 8)
+        return pg::launch<prompt_kernel<T, DIM, false, TREE, HELD>>("prompt_kernel", grid, kThreads,
+                          Plan<DIM, HELD>::bytes, stream, a, k_map, v_map, run);
+    int rc = encode(&k_map, a, a.k, a.k_head, a.k_page);
+    if (!rc) rc = encode(&v_map, a, a.v, a.v_head, a.v_page);
+    if (rc) return rc;
+    return pg::launch<prompt_kernel<T, DIM, true, TREE, HELD>>("prompt_kernel", grid, kThreads,
+                      Plan<DIM, HELD>::bytes, stream, a, k_map, v_map, run);
   }
 }
 
-template <bool TREE, bool K8>
+template <bool TREE, Held HELD>
 int run_prompt(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                cudaStream_t stream) {
   if (bf16)
     return a.dim <= 64
-               ? launch_prompt<__nv_bfloat16, 64, TREE, K8>(a, max_len, partial_bytes, sms, stream)
-               : launch_prompt<__nv_bfloat16, 128, TREE, K8>(a, max_len, partial_bytes, sms, stream);
-  return a.dim <= 64 ? launch_prompt<__half, 64, TREE, K8>(a, max_len, partial_bytes, sms, stream)
-                     : launch_prompt<__half, 128, TREE, K8>(a, max_len, partial_bytes, sms, stream);
+               ? launch_prompt<__nv_bfloat16, 64, TREE, HELD>(a, max_len, partial_bytes, sms, stream)
+               : launch_prompt<__nv_bfloat16, 128, TREE, HELD>(a, max_len, partial_bytes, sms, stream);
+  return a.dim <= 64 ? launch_prompt<__half, 64, TREE, HELD>(a, max_len, partial_bytes, sms, stream)
+                     : launch_prompt<__half, 128, TREE, HELD>(a, max_len, partial_bytes, sms, stream);
 }
 
 }  // namespace

@@ -2,10 +2,16 @@
 //
 // Its blocks take 256 rows each, and those of one kv head widen the same keys over and over: seven warps
 // beside the products need 7000 cycles for what a step's exponentials and products need 4000 for. So
-// where a sequence has rows for several blocks, its keys and values are widened once, into the
-// workspace as a 16-bit cache with pages of 128 tokens, as many kv heads at a time as there is room for,
-// and the kernel runs over that. Both ways round a key or value to the type once, so the results are
-// the same.
+// where a sequence has rows for several blocks, its keys and values are widened once, into the workspace as
+// a 16-bit cache with pages of 128 tokens, as many kv heads at a time as there is room for, and the kernel
+// runs over that.
+//
+// Either way they are widened to f16 for both types of results, as 2^-e of what they are, with one e for
+// the keys, and one for the values, of a page of a head or of a block's part. bf16 would lose too much:
+// keys rounded to it change a score of 8 by a hundredth, and results by three times as much as all other
+// roundings together. (The whole numbers, with scores multiplied by each key's scale, lose nothing, but the
+// rows' threads took a third longer for it: two sequences of 2048 new tokens and up to 8192 keys, 32 heads
+// on 8 of 128 in bf16, 605 us so and 490 us in f16.)
 #include "attention_prompt.cuh"
 
 namespace {
@@ -22,10 +28,9 @@ constexpr int kFewRounds = 3;
 
 // Block (i, h): keys 128 i.. of the batch's sequences, each with `blocks` such blocks, of kv head first + h;
 // block (i, heads + h) the values. HBM bounds it: a byte read and two written.
-template <class T>
 __global__ void __launch_bounds__(kWiden)
-    widen_kernel(Attention a, int blocks, int first, int heads, char *k_to, char *v_to, int *table,
-                 int *lens) {
+    widen_kernel(Attention a, int blocks, int first, int heads, char *k_to, char *v_to, int2 *shifts,
+                 int *table, int *lens) {
   pg::wait_for_earlier_kernels();
   const int b = blockIdx.x / blocks, block = blockIdx.x - b * blocks;
   const int head = blockIdx.y < heads ? blockIdx.y : blockIdx.y - heads;
@@ -59,6 +64,22 @@ __global__ void __launch_bounds__(kWiden)
   const int64_t page_bytes = values ? a.v_page : a.k_page, of_bytes = values ? a.vs_page : a.ks_page;
   uint4 *const to = reinterpret_cast<uint4 *>(
       (values ? v_to : k_to) + (static_cast<int64_t>(blockIdx.x) * heads + head) * kKeys * a.dim * 2);
+  __shared__ unsigned top;  // the largest scale that is finite
+  if (!threadIdx.x) top = 0;
+  __syncthreads();
+  if (threadIdx.x < kKeys && key0 + static_cast<int>(threadIdx.x) < length) {
+    const int key = key0 + threadIdx.x, entry = pg::page_index(a, key), page = pages[entry];
+    if (page >= 0 && page < a.pages) {
+      atomicMax(&top, magnitude(of + page * of_bytes + (key - entry * a.page_size) * 4ll));
+    }
+  }
+  __syncthreads();
+  const int shift = shift_of(top, values);
+  const float by = pg::power_of_2(-shift);
+  if (!threadIdx.x) {
+    int2 *const to = shifts + static_cast<int64_t>(blockIdx.x) * heads + head;
+    (values ? to->y : to->x) = shift;
+  }
   constexpr int kAhead = 4;  // loads a thread has in flight
   for (int i0 = threadIdx.x; i0 < kKeys * pieces; i0 += kWiden * kAhead) {
     uint4 raw[kAhead];
@@ -83,39 +104,34 @@ __global__ void __launch_bounds__(kWiden)
       const int i = i0 + u * kWiden;
       if (i >= kKeys * pieces) continue;
       uint4 out[2];
-      widen<T>(raw[u], scale[u], out);
+      widen(raw[u], scale[u] * by, out);
       to[2 * i] = out[0], to[2 * i + 1] = out[1];
     }
   }
 }
 
-template <class T>
-int widen_first(Attention a, bool bf16, int max_len, int heads, int blocks, int64_t head_bytes, int sms,
-                cudaStream_t stream) {
-  const int64_t meta = (4ll * a.batch * (blocks + 1) + 255) / 256 * 256;
+int widen_first(Attention a, bool bf16, int max_len, int heads, int blocks, int sms, cudaStream_t stream) {
+  const int pages = a.batch * blocks;
   char *const scratch = reinterpret_cast<char *>(a.partial) + kPartsBytes;
-  int *const table = reinterpret_cast<int *>(scratch);
-  int *const lens = table + static_cast<int64_t>(a.batch) * blocks;
-  const int rounds = (a.heads + heads - 1) / heads;
-  for (int i = 0; i < rounds; ++i) {
-    // as even as they come
-    const int first = static_cast<int>(static_cast<int64_t>(a.heads) * i / rounds);
-    const int n = static_cast<int>(static_cast<int64_t>(a.heads) * (i + 1) / rounds) - first;
-    char *const k = scratch + meta, *const v = k + n * head_bytes;
-    int rc = pg::launch<widen_kernel<T>>("widen_kernel", dim3(a.batch * blocks, 2 * n), kWiden, 0,
-                                         stream, a, blocks, first, n, k, v, table, lens);
-    if (rc) return rc;
+  int *const table = reinterpret_cast<int *>(scratch), *const lens = table + pages;
+  char *const k = scratch + (4ll * (pages + a.batch) + 255) / 256 * 256;
+  for (int first = 0; first < a.heads; first += heads) {
+    const int n = a.heads - first < heads ? a.heads - first : heads;
     Attention b = a;
+    const int64_t head_bytes = static_cast<int64_t>(kKeys) * a.dim * 2;
+    char *const v = k + pages * n * head_bytes;
+    int2 *const shifts = reinterpret_cast<int2 *>(v + pages * n * head_bytes);
+    int rc = pg::launch<widen_kernel>("widen_kernel", dim3(pages, 2 * n), kWiden, 0, stream, a, blocks, first,
+                                      n, k, v, shifts, table, lens);
+    if (rc) return rc;
     b.q += first * a.group * a.q_head, b.out += first * a.group * a.out_head;
-    b.k = k, b.v = v, b.k_scale = b.v_scale = nullptr;
-    b.k_head = b.v_head = static_cast<int64_t>(kKeys) * a.dim * 2;
-    b.k_page = b.v_page = n * b.k_head;
+    b.k = k, b.v = v, b.k_scale = reinterpret_cast<char *>(shifts);
+    b.k_head = b.v_head = head_bytes, b.k_page = b.v_page = n * head_bytes;
+    b.ks_head = 8, b.ks_page = n * 8;
     b.table = table, b.table_row = blocks, b.lens = lens, b.slots = nullptr;
-    b.slot_rows = a.batch, b.heads = n, b.page_size = kKeys, b.width = blocks;
-    b.pages = a.batch * blocks;
-    b.page_mul = 1, b.page_shift = 7;
-    rc = a.mask ? pg::prompt_tree(b, bf16, max_len, kPartsBytes, sms, stream)
-                : pg::prompt_16bit(b, bf16, max_len, kPartsBytes, sms, stream);
+    b.slot_rows = a.batch, b.heads = n, b.page_size = kKeys, b.width = blocks, b.pages = pages;
+    rc = a.mask ? run_prompt<true, kShifted>(b, bf16, max_len, kPartsBytes, sms, stream)
+                : run_prompt<false, kShifted>(b, bf16, max_len, kPartsBytes, sms, stream);
     if (rc) return rc;
   }
   return PG_OK;
@@ -127,18 +143,20 @@ namespace pg {
 
 int prompt_8bit(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                 cudaStream_t stream) {
-  const int64_t blocks = (max_len + kKeys - 1ll) / kKeys;
-  const int64_t head_bytes = a.batch * blocks * kKeys * a.dim * 2;  // of its keys
-  const int64_t room = partial_bytes - kPartsBytes - 4 * a.batch * (blocks + 1) - 256;
-  const int64_t heads = room > 0 ? room / (2 * head_bytes) : 0;
+  const int64_t blocks = (max_len + kKeys - 1ll) / kKeys, pages = a.batch * blocks;
+  const int64_t room = partial_bytes - kPartsBytes - 4 * (pages + a.batch) - 256;
+  const int64_t each = pages * (kKeys * a.dim * 4ll + 8);  // of a kv head: keys, values and shifts
+  int64_t heads = room > 0 ? room / each : 0;
+  heads = heads < a.heads ? heads : a.heads;
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
-  if (heads >= 1 && a.batch * blocks <= INT32_MAX / 2 && rows >= kWidenRows * a.batch &&
-      (heads * kFewRounds >= a.heads || heads * rows >= static_cast<int64_t>(kRows) * sms))
-    return (bf16 ? widen_first<__nv_bfloat16> : widen_first<__half>)(
-        a, bf16, max_len, static_cast<int>(heads < a.heads ? heads : a.heads), static_cast<int>(blocks),
-        head_bytes, sms, stream);
-  return a.mask ? run_prompt<true, true>(a, bf16, max_len, partial_bytes, sms, stream)
-                : run_prompt<false, true>(a, bf16, max_len, partial_bytes, sms, stream);
+  if (heads >= 1 && pages <= INT32_MAX / 2 && rows >= kWidenRows * a.batch &&
+      (heads * kFewRounds >= a.heads || heads * rows >= static_cast<int64_t>(kRows) * sms)) {
+    const int64_t rounds = (a.heads + heads - 1) / heads;  // as even as they come
+    return widen_first(a, bf16, max_len, static_cast<int>((a.heads + rounds - 1) / rounds),
+                       static_cast<int>(blocks), sms, stream);
+  }
+  return a.mask ? run_prompt<true, kBytes>(a, bf16, max_len, partial_bytes, sms, stream)
+                : run_prompt<false, kBytes>(a, bf16, max_len, partial_bytes, sms, stream);
 }
 
 }  // namespace pg

@@ -18,9 +18,12 @@ The new tokens of a sequence may be a ``tree``, 64 at most: each sees the tokens
 of its own branch, which ``mask`` names (``branches`` makes it of the tokens' parents).
 
 Over a cache in 8 bits, ``k_scale`` and ``v_scale`` [pages, kv_heads, page_size] are one layer's scales
-(``PagedCache.k_scale[layer]``) and k and v int8. Keys and values are what they stand for, and only the
-weights' products with the values' scales are rounded, to two f16 numbers each. A key or value whose
-scale is not finite makes the results that see it NaN.
+(``PagedCache.k_scale[layer]``) and k and v int8. For few rows keys and values are what they stand for, and
+only the weights' products with the values' scales are rounded, to f16 numbers (one each for bf16 results,
+else two). Prompts of many rows, as below, have keys, values and weights rounded to f16 each. What is below
+2^-22 of the largest scale loses digits there. A key or value whose scale is not finite makes the results
+that see it NaN. ``max_len`` must not be below a length then: such a sequence is cut, and ``Workspace.check``
+raises for it.
 
 q, k and v have one dtype (f32, bf16 or f16; k and v may be int8) and a head size of up to 256 whose rows are a
 multiple of 16 bytes; q may be a slice of a fused projection. Scores, maxima and sums are held in 32

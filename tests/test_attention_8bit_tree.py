@@ -14,10 +14,10 @@ bf16, 2^-11 f16, 2^-24 f32):
 * a bf16 result over 8 bits has its weights as one f16 number each, 2^-12 of itself off, independently:
   six times the root of that variance, 3.5 2^-12 S, more;
 * tiles of many rows round each weight once, independently: six times the root of that variance more,
-  3.5 e S, is met by one in 10^9 results. Over 8 bits they round keys and values to the type, too: half a
-  step each, again at random, so the values add 1.75 e S, and a score has a variance of c^2, c = e / 12^(1/2)
-  times the scale and (sum q^2 k^2)^(1/2), the weights that much of themselves and the result 6 c (S + |o|)
-  with the largest c.
+  3.5 e S, is met by one in 10^9 results. Over 8 bits weights, keys and values are in f16 for both types,
+  e = 2^-11 for these: half a step each, again at random, so the values add 1.75 e S, and a score has a
+  variance of c^2, c = e / 12^(1/2) times the scale and (sum q^2 k^2)^(1/2), the weights that much of
+  themselves and the result 6 c (S + |o|) with the largest c.
 
 Heads above 128 are summed in f32 in order: n^(1/2) 2^-24 of the largest sum, within 4e-5 A at 4000."""
 
@@ -136,7 +136,7 @@ class Batch:
             out[r, sees] = True
         return torch.from_numpy(out).cuda()
 
-    def hold(self, got, window=0, sinks=0, tiles=False, scale=None) -> None:
+    def hold(self, got, window=0, sinks=0, tiles=False, scale=None, but=None) -> None:
         import torch
 
         scale = self.dim ** -0.5 if scale is None else scale
@@ -144,7 +144,7 @@ class Batch:
         for i, (n, new) in enumerate(zip(self.lens, self.news)):
             rows = slice(at, at + new)
             at += new
-            if not new:
+            if not new or i == but:
                 continue
             if not n:
                 assert (got[rows] == 0).all()
@@ -165,12 +165,15 @@ class Batch:
                     bound = bound + 4e-5 * a
                 if self.bits8 and self.dtype is torch.bfloat16:
                     bound = bound + 3.5 * 2.0 ** -12 * m
+                # the tiles' products over 8 bits are in f16 for both types
+                e = UNIT["float16"] if self.bits8 else e
                 if tiles:
                     bound = bound + 3.5 * e * m
                 if tiles and self.bits8:
                     c = torch.einsum("tgd,kd->tgk", q[:, h] ** 2, k ** 2).sqrt()
                     c = c.masked_fill(~seen[:, None], 0.0).amax(-1, keepdim=True) * abs(scale)
                     bound = bound + 1.75 * e * m + 6 * c * e / 12 ** 0.5 * (m + o.abs())
+                e = UNIT[str(self.dtype).split(".")[1]]
                 bad = ~((y - o).abs() <= bound)
                 assert not bad.any(), (i, h, float(((y - o).abs() / bound).nan_to_num(1e9).max()),
                                        bad.nonzero()[:4].tolist())
@@ -288,6 +291,149 @@ def test_out_strides_slots_and_streams_over_8_bits(ws) -> None:
         got = attention.decode(b.q, b.k, b.v, b.table, lens, workspace=ws, **b.scales)
     graph.replay()
     assert torch.equal(got, want)
+
+
+# (lens, news, max_len): prompts whose keys are widened block by block, and in the workspace first
+WAYS = [([900, 200], [70, 60], None), ([1500, 1000], [900, 700], None)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("spread", [0.0, 2.0])
+@pytest.mark.parametrize("lens,news,max_len", WAYS)
+def test_prompts_with_scales_of_unlike_size(ws, lens, news, max_len, spread, dtype) -> None:
+    """Values far apart, also from page to page; pages of zeros; a head of nothing else."""
+    b = Batch(lens, news, 2, 4, 128, 16, dtype, True, spread=spread)
+    b.scales["k_scale"].clamp_(max=0.05)
+    v = b.scales["v_scale"]
+    for i in range(len(lens)):
+        v[b.table[i, 2:60:7].long()] *= 2.0 ** -20
+        v[b.table[i, 5:60:7].long()] *= 2.0 ** 6
+        v[b.table[i, 0:8].long()] = 0.0  # all of the first 128 tokens
+        b.v[b.table[i, 24:33].long()] = 0  # ... and of others, by numbers that are 0
+        v[b.table[i].long().clamp(min=0), 1] = 0.0
+    b.hold(b.run(ws, max_len=max_len), tiles=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("size", [1e-6, 1e4])
+@pytest.mark.parametrize("lens,news,max_len", WAYS)
+def test_prompts_with_queries_of_any_size(ws, lens, news, max_len, size, dtype) -> None:
+    if dtype == "float16" and size > 1:
+        size = 1000.0
+    b = Batch(lens, news, 1, 4, 64, 16, dtype, True)
+    b.q = (b.q * size).to(b.dtype)
+    b.q[0, 1] = 0
+    b.q[1:3] = b.q[1:3] * 2.0 ** -10  # rows have their own
+    b.hold(b.run(ws, scale=-0.125 / size, max_len=max_len), scale=-0.125 / size, tiles=True)
+
+
+@pytest.mark.gpu
+def test_wide_tables_and_larger_workspaces(ws) -> None:
+    """A table for far more tokens than there are: nothing of the workspace goes by it."""
+    import torch
+
+    b = Batch([1500, 1000], [900, 700], 2, 4, 128, 16, "bfloat16", True)
+    want = b.run(ws, max_len=1500)
+    table = torch.full((2, 1 << 16), -1, dtype=torch.int32, device="cuda")
+    table[:, :b.table.shape[1]] = b.table
+    b.table, narrow = table, b.table
+    b.hold(b.run(ws), tiles=True)
+    b.table = narrow
+    large = attention.Workspace(size=200 << 20)
+    assert torch.equal(b.run(large, max_len=1500), want)
+    large.check()
+    with pytest.raises(ValueError, match="bytes at least"):
+        attention.Workspace(size=1 << 20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("news,masked", [([1, 1, 1], False), ([9, 9, 9], False), ([70, 60, 50], False),
+                                         ([900, 400, 800], False), ([5, 6, 7], True), ([64, 60, 50], True)])
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("bad", ["slot", "slot below", "page", "page below", "length", "length below"])
+def test_what_only_the_device_sees(cuda, bad, bits8, news, masked, dtype) -> None:
+    """The second sequence is refused; the others have their results, and the next call is sound."""
+    import torch
+
+    w = attention.Workspace()
+    masks = _trees(2, news) if masked else None
+    b = Batch([1100, 1000, 900], news, 1, 8, 64, 16, dtype, bits8, masks)
+    want = b.run(w)
+    w.check()
+    slots, table, lens = _ints([0, 1, 2]), b.table.clone(), _ints(b.lens)
+    bit = {"slot": cache_module.BAD_SLOT, "page": cache_module.BAD_PAGE,
+           "length": cache_module.TOO_LONG}[bad.split()[0]]
+    if bad.startswith("slot"):
+        slots[1] = -1 if "below" in bad else 3
+    elif bad.startswith("page"):
+        table[1, 60] = -1 if "below" in bad else b.k.shape[0]
+    else:
+        lens[1] = -1 if "below" in bad else table.shape[1] * 16 + 1
+    more = dict(workspace=w, slots=slots, **b.scales)
+    if masked:
+        got = attention.tree(b.q, b.starts, b.mask, b.k, b.v, table, lens, **more)
+    else:
+        got = attention.prompt(b.q, b.starts, b.k, b.v, table, lens, **more)
+    with pytest.raises(CacheError) as e:
+        w.check()
+    # a length that is cut to the table's width goes over entries that no page has been set to
+    assert e.value.bits in (bit, bit | (cache_module.BAD_PAGE if bad == "length" else 0))
+    b.hold(got, tiles=True, but=1)
+    assert torch.equal(b.run(w), want)
+    w.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("news,masked", [([5, 6], True), ([64, 60], True), ([70, 60], False),
+                                         ([900, 700], False)])
+def test_graphs_streams_and_slots(ws, news, masked, bits8) -> None:
+    """Captured once and replayed with other queries and lengths; on a second stream with a workspace
+    of its own at the same time; rows that no sequence has stay."""
+    import torch
+
+    masks = _trees(3, news) if masked else None
+    b = Batch([1500, 1000], news, 2, 4, 64, 16, "bfloat16", bits8, masks)
+    rows = sum(news)
+    q = torch.cat([b.q, b.q[:3]])
+    out = torch.full_like(q, 5.0)
+    lens, table = _ints(b.lens), b.table[[1, 0]].contiguous()
+    mask = torch.cat([b.mask, b.mask[:3]]) if masked else None
+    other, side = attention.Workspace(), torch.cuda.Stream()
+
+    def go(w, to, stream=None):
+        more = dict(workspace=w, slots=_ints([1, 0]) if stream is None else slots, out=to, stream=stream,
+                    **b.scales)
+        if masked:
+            attention.tree(q, b.starts, mask, b.k, b.v, table, lens[[1, 0]] if stream is None else turned,
+                           **more)
+        else:
+            attention.prompt(q, b.starts, b.k, b.v, table, lens[[1, 0]] if stream is None else turned,
+                             **more)
+
+    slots, turned = _ints([1, 0]), _ints(b.lens[::-1])
+    want = b.run(ws)
+    twice = torch.full_like(q, 5.0)
+    torch.cuda.synchronize()
+    go(other, twice, side.cuda_stream)
+    go(ws, out, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(out[:rows], want) and torch.equal(twice[:rows], want)
+    assert (out[rows:] == 5.0).all() and (twice[rows:] == 5.0).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go(ws, out, torch.cuda.current_stream().cuda_stream)
+    q.mul_(0.5)
+    turned -= 16
+    b.q, b.lens = q[:rows], [n - 16 for n in b.lens]
+    out.fill_(5.0)
+    graph.replay()
+    want = b.run(ws)
+    assert torch.equal(out[:rows], want) and (out[rows:] == 5.0).all()
+    other.check()
 
 
 # --- trees --------------------------------------------------------------------------------------
