@@ -9,7 +9,7 @@
 //
 // Which token that is hangs on sums of up to 100000s of weights next to a border, so sums in 32 bits
 // would give another token about once in a hundred rows of a flat distribution. Weights and sums are
-// 64-bit numbers here: any order of the sum gives the same token but for one draw in 10^9.
+// 64-bit numbers here, weights to 2^-38: any order of the sum gives the same token but for one draw in 10^9.
 //
 // A cluster of blocks takes a row, each a part of it, which stays in shared memory while it is gone
 // through: the largest logit; the sum of weights, where top_p is of all; then the last kept token is
@@ -21,6 +21,8 @@
 
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 namespace cg = cooperative_groups;
 
 namespace {
@@ -30,11 +32,15 @@ constexpr int kPerSm = 2;             // blocks an SM holds
 constexpr int kParts = 8;             // blocks a row is cut in at most (a portable cluster)
 constexpr int kBins = 1024;           // two a thread
 constexpr int kFew = 512;             // tokens that are ranked one against another
-constexpr int kTable = 256;           // 2^(i / 256)
+constexpr int kTable = 16;            // 2^(i / 16): one bank of shared memory each
 constexpr int kResident = 88 * 1024;  // bytes of a part that stay in shared memory
 // Each interval is one of 1024 of the last one and never all of it. Values that lie evenly take two or
 // three; ones of ever smaller size, ten binades at a time, 28.
 constexpr int kLevels = 64;
+// From so many rows on, those without limits take a block each and one pass over a row. With and without,
+// in microseconds, bf16: 32 rows of 32001 14 and 13, 64 of 128256 both 38, 128 of 128256 42 and 66, 128 of
+// 32001 11 and 22, 300 of 32001 22 and 49.
+constexpr int kDrawRows = 128;
 constexpr float kLargest = 3.402823466e38f;
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
@@ -132,20 +138,21 @@ struct Shared {
   int bin;
 };
 
-// 2^t for t <= 0, to about 2^-52: 2^(i/256) from a table, and with |r| <= 1/512 the powers of r ln 2
-// up to the fourth (the fifth is below 2^-54). Below 2^-1000 it stays there.
+// 2^t to about 2^-38, for t of -1000 to 1000: 2^(i/16) from a table, and e^x with |x| <= a = ln 2 / 32 by
+// the series up to x^4 and, in place of x^5 / 120, the cubic that is nearest to it there (Chebyshev's: it
+// leaves a^5 / 1920). 2^0 is 1.
 __device__ __forceinline__ double power_of_two(const double *power, double t) {
-  t = fmax(t, -1000.0);
-  constexpr double kShift = 6755399441055744.0 / kTable;  // 1.5 * 2^52 in steps of 1/256
+  constexpr double kShift = 6755399441055744.0 / kTable;  // 1.5 * 2^52 in steps of 1/16
+  constexpr double k2 = kLn2 * kLn2, kA2 = k2 / (4 * kTable * kTable);
   const double z = t + kShift;
-  const int n = __double2loint(z);  // t in 256ths, rounded
+  const int n = __double2loint(z);  // t in 16ths, rounded
   const double r = t - (z - kShift);
-  double p = fma(r, kLn2 * kLn2 * kLn2 * kLn2 / 24, kLn2 * kLn2 * kLn2 / 6);
-  p = fma(r, p, kLn2 * kLn2 / 2);
-  p = fma(r, p, kLn2) * r;
+  double p = fma(r, k2 * k2 / 24, k2 * kLn2 * (1.0 / 6 + 1.25 * kA2 / 120));
+  p = fma(r, p, k2 / 2);
+  p = fma(r, p, kLn2 * (1.0 - 0.3125 * kA2 * kA2 / 120)) * r;
   const double f = power[n & (kTable - 1)];
   const double y = fma(f, p, f);
-  return __hiloint2double(__double2hiint(y) + ((n >> 8) << 20), __double2loint(y));
+  return __hiloint2double(__double2hiint(y) + (n >> 4 << 20), __double2loint(y));
 }
 
 // A block's part of a row: columns [first, last). Warp w takes a run of its 16-byte vectors, so
@@ -230,7 +237,9 @@ struct Row {
   double scale;     // log2 e / T
 
   __device__ double weight(float x) const {
-    return power_of_two(sh.power, (static_cast<double>(x) - static_cast<double>(top)) * scale);
+    // below 2^-1000 it stays there
+    return power_of_two(sh.power,
+                        fmax((static_cast<double>(x) - static_cast<double>(top)) * scale, -1000.0));
   }
 
   // f(x, column)'s sum over the row, in an order of its own for each size of a row
@@ -576,18 +585,16 @@ struct Row {
   }
 };
 
+// A row by the definition, taken by a cluster.
 template <class T>
-__global__ void __launch_bounds__(kThreads, kPerSm) sample_kernel(const __grid_constant__ Arguments a) {
-  __shared__ Shared sh;
-  extern __shared__ uint4 held[];
-  pg::wait_for_earlier_kernels();
+__device__ __forceinline__ void sample_row(const Arguments &a, Shared &sh, int row, uint4 *held) {
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
-  const int row = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T *x_row = static_cast<const T *>(a.logits) + row * a.row_stride;
   const int64_t v64 = a.vocab;
   const Part<T> part(x_row, static_cast<int>(v64 * rank / blocks),
-                     static_cast<int>(v64 * (rank + 1) / blocks), a.resident ? held : nullptr);
+                     static_cast<int>(v64 * (rank + 1) / blocks), held);
   const float u = a.uniform[row];
   const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
   const float top_p = a.top_p ? a.top_p[row] : a.top_p_all;
@@ -598,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) sample_kernel(const __grid_c
   Extent e{-INFINITY, INFINITY};
   for (int v = part.begin + lane; v < part.end; v += 32) {
     const uint4 raw = part.fetch(v);
-    if (a.resident) held[v] = raw;
+    if (held) held[v] = raw;
     float x[Vec<T>::n];
     Vec<T>::get(raw, x);
 #pragma unroll
@@ -669,7 +676,197 @@ __global__ void __launch_bounds__(kThreads, kPerSm) sample_kernel(const __grid_c
 }
 
 template <class T>
+__global__ void __launch_bounds__(kThreads, kPerSm) sample_kernel(const __grid_constant__ Arguments a) {
+  __shared__ Shared sh;
+  extern __shared__ uint4 held[];
+  pg::wait_for_earlier_kernels();
+  sample_row<T>(a, sh, blockIdx.x / cg::this_cluster().num_blocks(), a.resident ? held : nullptr);
+}
+
+// ... by a block, for a row that a kernel hardly ever has.
+template <class T>
+__device__ __noinline__ void sample_rare_row(const Arguments &a, Shared &sh, int row) {
+  sample_row<T>(a, sh, row, nullptr);
+}
+
+// Rows without limits. A block takes a row and goes over it once, a run of it a warp, with each warp's weights
+// by the largest logit of the first that it has met (and by a larger one, its sum scaled, where later ones'
+// weights pass 2^500). Then all of the block goes over the run of the warp that has the token.
+//
+// Ten 64-bit instructions a token bound it, 20 cycles of a quarter of an SM for 32 tokens, and one in eight
+// of those for its conversion: 2000 rows of 50257 bf16 logits take 131 us, where these alone take 56 and
+// HBM 31. (By sample_kernel, which keeps a row in shared memory and waits for all of it twice, 315 us; with
+// the series in place of the table of 16 up to 2^-51, two instructions more, 166.) Tables of 256 numbers
+// lie in the same banks for eight of 32 lanes: with one both kernels wait for shared memory.
+constexpr int kBatch = 4;  // vectors a thread has in flight
+template <class T>
+__global__ void __launch_bounds__(kThreads, kPerSm) draw_kernel(const __grid_constant__ Arguments a) {
+  __shared__ Shared sh;
+  __shared__ float refs[kWarps];
+  __shared__ int odd, hit;
+  pg::wait_for_earlier_kernels();
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr unsigned kAll = 0xffffffffu;
+  constexpr int N = Vec<T>::n;
+  const T *x_row = static_cast<const T *>(a.logits) + row * a.row_stride;
+  const Part<T> part(x_row, 0, a.vocab, nullptr);
+  const float u = a.uniform[row];
+  const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
+  const double scale = kLog2e / temperature;
+  // What is none of an ordinary row goes by the definition: also u = 0, for which weights must be 0 that
+  // are 2^-1000 here, and any that is not finite.
+  if (!(u > 0.0f && u < 1.0f && scale > 1e-30 && scale < 1e30)) {
+    sample_rare_row<T>(a, sh, row);
+    return;
+  }
+  if (tid < kTable) sh.power[tid] = exp2(tid / static_cast<double>(kTable));
+  if (tid == 0) odd = 0, hit = -1;
+  __syncthreads();
+
+  const float scale_f = static_cast<float>(scale);
+  float ref = -INFINITY, floor = -INFINITY;  // of the warp
+  double sum = 0.0, off = 0.0;
+  const auto weigh = [&](float x) {
+    return power_of_two(sh.power, fma(static_cast<double>(fmaxf(x, floor)), scale, off));
+  };
+  const auto take = [&](const uint4 *raw, auto number) {
+    constexpr int n = decltype(number)::value;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      float x[N];
+      Vec<T>::get(raw[k], x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) top = max_nan(top, x[i]);
+    }
+    if (__any_sync(kAll, !((top - ref) * scale_f <= 500.0f))) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(kAll, top, o));
+      if (!(top < INFINITY)) odd = 1;
+      if (top == -INFINITY || odd) return;  // all of them are
+      sum = ref == -INFINITY ? 0.0 : sum * exp2(fmax((static_cast<double>(ref) - top) * scale, -2000.0));
+      ref = top;
+      off = -static_cast<double>(ref) * scale;
+      floor = fmaxf(-kLargest, __double2float_ru(ref - 1000.0 / scale));
+    }
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      float x[N];
+      Vec<T>::get(raw[k], x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum += weigh(x[i]);
+    }
+  };
+  const uint4 none = [] {
+    union {
+      uint4 raw;
+      T x[N];
+    } u;
+    for (int i = 0; i < N; ++i) u.x[i] = lowest<T>();
+    return u.raw;
+  }();
+  // the row's first and last vector may hold others' numbers: they come one number at a time
+  const int inner = max(part.begin, 1), outer = min(part.end, part.vectors - 1);
+  int v0 = inner;
+  for (; v0 + 32 * kBatch <= outer; v0 += 32 * kBatch) {
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) raw[k] = pg::load16(x_row + part.base + (v0 + 32 * k + lane) * N);
+    take(raw, std::integral_constant<int, kBatch>());
+  }
+  for (; v0 < outer; v0 += 32) {
+    const uint4 raw = v0 + lane < outer ? pg::load16(x_row + part.base + (v0 + lane) * N) : none;
+    take(&raw, std::integral_constant<int, 1>());
+  }
+  if (part.begin == 0 || part.end == part.vectors) {
+    uint4 raw = none;
+    const int last = part.vectors - 1;
+    const int v = lane == 0 && part.begin == 0 ? 0 : lane == 1 && last > 0 && part.begin <= last ? last : -1;
+    if (v >= 0 && v < part.end) raw = part.fetch(v);
+    take(&raw, std::integral_constant<int, 1>());
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) sh.warp_total[warp] = sum, refs[warp] = ref;
+  __syncthreads();
+  // all warps' sums by the largest reference, added up along the row
+  float top = lane < kWarps ? refs[lane] : -INFINITY;
+  const float mine = top;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+  if (odd || top == -INFINITY) {
+    __syncthreads();
+    sample_rare_row<T>(a, sh, row);
+    return;
+  }
+  const double by =
+      mine == -INFINITY ? 0.0 : exp2(fmax((static_cast<double>(mine) - top) * scale, -2000.0));
+  double upto = lane < kWarps ? sh.warp_total[lane] * by : 0.0;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const double other = __shfl_up_sync(kAll, upto, o);
+    if (lane >= o) upto += other;
+  }
+  const double all = __shfl_sync(kAll, upto, kWarps - 1), target = u * all;
+  const unsigned past = __ballot_sync(kAll, lane < kWarps && upto > target);
+  const int owner = past ? __ffs(past) - 1 : kWarps - 1;
+  double start = owner ? __shfl_sync(kAll, upto, owner - 1) : 0.0;
+  const double owner_by = __shfl_sync(kAll, by, owner);
+  ref = __shfl_sync(kAll, mine, owner);
+  off = -static_cast<double>(ref) * scale;
+  floor = fmaxf(-kLargest, __double2float_ru(ref - 1000.0 / scale));
+  const int each = (part.vectors + kThreads - 1) / kThreads * 32;
+  const int begin = min(owner * each, part.vectors), end = min(begin + each, part.vectors);
+  for (int v0 = begin; v0 < end; v0 += kThreads) {
+    const int v = v0 + tid;
+    float x[N];
+    double y[N], here = 0.0;
+    if (v < end) part.load(v, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      y[i] = v < end && x[i] > -INFINITY ? weigh(x[i]) * owner_by : 0.0;
+      here += y[i];
+    }
+    double sums = here;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double other = __shfl_up_sync(kAll, sums, o);
+      if (lane >= o) sums += other;
+    }
+    if (lane == 31) sh.warp_sum[warp] = sums;
+    __syncthreads();
+    double before = start;
+    for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
+    for (int w = 0; w < kWarps; ++w) start += sh.warp_sum[w];
+    // one thread's start is the end of the one before it, so that one at most has the target
+    const double left = __shfl_up_sync(kAll, sums, 1);
+    double c = lane ? before + left : before;
+    if (c <= target && before + sums > target) {
+      int best = 0;
+      double best_y = 0.0;
+      bool past = false;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        c += y[i];
+        if (y[i] > 0.0 && !past) {
+          best = part.base + v * N + i, best_y = y[i];
+          past = c > target;
+        }
+      }
+      hit = best;
+      a.tokens[row] = best;
+      a.logp[row] = static_cast<float>(log(best_y / all));
+    }
+    __syncthreads();
+    if (hit >= 0) return;
+  }
+  sample_rare_row<T>(a, sh, row);  // rounding has left no column
+}
+
+template <class T>
 int launch_sample(Arguments a, int rows, int sms, cudaStream_t stream) {
+  if (!a.top_k && !a.top_p && !a.min_p && (a.top_k_all == 0 || a.top_k_all >= a.vocab) &&
+      a.top_p_all >= 1.0f && a.min_p_all == 0.0f && rows >= kDrawRows)
+    return pg::launch<draw_kernel<T>>("draw_kernel", dim3(rows), kThreads, 0, stream, a);
   // Blocks a row: as many as let a part stay in shared memory, and more where that leaves SMs
   // without any, but no part shorter than one vector a thread.
   const auto part_bytes = [&](int blocks) {

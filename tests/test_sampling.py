@@ -116,6 +116,57 @@ def test_many_rows_with_one_setting(cuda, limit) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("vocab", [1, 2, 9, 63, 513, 4097, 8192, 50257, 150001])
+def test_many_rows_without_limits(cuda, vocab, dtype) -> None:
+    """One block a row; rows that are no ordinary ones among them."""
+    import torch
+
+    rng = np.random.default_rng(vocab)
+    rows = 160
+    x = (rng.standard_normal((rows, vocab)) * rng.choice([0.1, 1, 3], (rows, 1))).astype(np.float32)
+    x[3, rng.random(vocab) < 0.9] = -np.inf
+    x[4, :-1] = -np.inf
+    x[5, 1:] = -np.inf
+    x[6, vocab // 2] = np.nan
+    x[7, vocab - 1] = np.inf
+    x[8] = -np.inf
+    x[9] = np.linspace(0, 2000, vocab)  # later ones 2^500 times as large, and more
+    x[10] = x[9][::-1]
+    x[11, :vocab // 3] = -np.inf
+    x[12] = 7.0
+    x[13] = np.where(rng.random(vocab) < 0.5, 0.0, -0.0)
+    x[14] += 30000
+    x[15] *= 1e4
+    x[16, vocab // 2:] = 60000
+    u = rng.random(rows, dtype=np.float32)
+    u[20:30] = [0.0, -0.0, 1e-38, 2.0 ** -60, 1 - 2.0 ** -24, 1.0, 2.0, -1.0, np.nan, 0.5]
+    u[30:34], x[30:34, 0] = [0.0, 1e-38, 1e-30, 0.999], -np.inf
+    t = rng.choice([0.3, 0.7, 1.0, 1.0, 1.5, 20.0], rows).astype(np.float32)
+    t[40:50] = [0.0, 1e-38, 1e-45, 1e-6, 1e30, 3e38, np.inf, -1.0, np.nan, 1e6]
+    _check(x, u, getattr(torch, dtype), vocab + 11, 3, temperature=t)
+    _check(x, u, getattr(torch, dtype), temperature=0.9)
+
+
+@pytest.mark.gpu
+def test_a_captured_draw_without_limits(cuda) -> None:
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn((300, 9001), device="cuda", generator=g).half()
+    u = torch.rand(300, device="cuda", generator=g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sampling.sample(x, u)
+    for _ in range(2):
+        x.normal_(generator=g)
+        u.uniform_(generator=g)
+        graph.replay()
+        want = sampling.sample(x, u, top_k=torch.zeros(300, dtype=torch.int32, device="cuda"))
+        assert torch.equal(got.tokens, want.tokens) and torch.equal(got.logp, want.logp)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["equal", "few values", "masked", "lowest", "one finite", "far",
                                   "tiny", "zeros of both signs", "one above"])
 def test_rows_that_are_not_spread(cuda, kind) -> None:
