@@ -42,6 +42,7 @@ constexpr int kLevels = 64;
 // 32001 11 and 22, 300 of 32001 22 and 49.
 constexpr int kDrawRows = 128;
 constexpr float kLargest = 3.402823466e38f;
+constexpr double kSteep = 200.0 * (1 << 24);
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
 struct Arguments {
@@ -112,6 +113,11 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// Weights below about 2^-500 of that of `top` stay there.
+__device__ __forceinline__ float floor_of(float top, double scale) {
+  return fmaxf(-kLargest, __double2float_rd(top - 500.0 / scale));
+}
+
 // What a warp, and then a block, knows of its tokens.
 struct Extent {
   float top, low;  // the largest and the lowest that is more than -inf
@@ -138,15 +144,15 @@ struct Shared {
   int bin;
 };
 
-// 2^t to about 2^-38, for t of -1000 to 1000: 2^(i/16) from a table, and e^x with |x| <= a = ln 2 / 32 by
-// the series up to x^4 and, in place of x^5 / 120, the cubic that is nearest to it there (Chebyshev's: it
-// leaves a^5 / 1920). 2^0 is 1.
-__device__ __forceinline__ double power_of_two(const double *power, double t) {
+// 2^t to about 2^-38, for t = d scale of -1000 to 1000 (whose product is not rounded): 2^(i/16) from a
+// table, and e^x with |x| <= a = ln 2 / 32 by the series up to x^4 and, in place of x^5 / 120, the cubic
+// that is nearest to it there (Chebyshev's: it leaves a^5 / 1920). 2^0 is 1.
+__device__ __forceinline__ double power_of_two(const double *power, double d, double scale) {
   constexpr double kShift = 6755399441055744.0 / kTable;  // 1.5 * 2^52 in steps of 1/16
   constexpr double k2 = kLn2 * kLn2, kA2 = k2 / (4 * kTable * kTable);
-  const double z = t + kShift;
+  const double z = fma(d, scale, kShift);
   const int n = __double2loint(z);  // t in 16ths, rounded
-  const double r = t - (z - kShift);
+  const double r = fma(d, scale, kShift - z);
   double p = fma(r, k2 * k2 / 24, k2 * kLn2 * (1.0 / 6 + 1.25 * kA2 / 120));
   p = fma(r, p, k2 / 2);
   p = fma(r, p, kLn2 * (1.0 - 0.3125 * kA2 * kA2 / 120)) * r;
@@ -234,12 +240,12 @@ struct Row {
   cg::cluster_group cluster;
   int blocks, rank;
   float top, low;   // the row's largest and lowest finite logits
+  float mine;       // the thread's largest
   double scale;     // log2 e / T
+  float floor;      // what is below weighs as much, 2^-500 or less
 
   __device__ double weight(float x) const {
-    // below 2^-1000 it stays there
-    return power_of_two(sh.power,
-                        fmax((static_cast<double>(x) - static_cast<double>(top)) * scale, -1000.0));
+    return power_of_two(sh.power, static_cast<double>(fmaxf(x, floor)) - static_cast<double>(top), scale);
   }
 
   // f(x, column)'s sum over the row, in an order of its own for each size of a row
@@ -439,7 +445,7 @@ struct Row {
 
   // The tokens of `kept` with values in [low, top], no more than kFew, ranked by block 0; the last
   // kept one is the `count`-th of them, or the first up to which `above` and their weights reach
-  // `goal`.
+  // `goal`. Where they are more than kFew after all, nothing is ranked and the result is 0.
   __device__ uint64_t rank_few(const Kept &kept, float hi_value, float lo_value, int count,
                                double above, double goal) {
     Shared &first = *cluster.map_shared_rank(&sh, 0);
@@ -453,8 +459,9 @@ struct Row {
       }
     });
     cluster.sync();
+    if (first.few_n > kFew) return 0;
     if (rank == 0) {
-      const int n = min(sh.few_n, kFew), tid = threadIdx.x, lane = tid & 31;
+      const int n = sh.few_n, tid = threadIdx.x, lane = tid & 31;
       uint64_t e = 0;
       int place = 0;
       if (tid < n) {
@@ -517,6 +524,25 @@ struct Row {
   // Keeps the first k.
   __device__ void keep_count(Kept &kept, unsigned k) {
     float hi = top, lo = low;
+    const unsigned threads = blocks * kThreads;
+    if (hi > lo && k <= threads / 4 * 3 && part.vectors >= 2 * kThreads) {
+      // No fewer than k tokens are as large as the k-th of the threads' largest, and few more: those
+      // below (by two bins, for the rounding) need not be counted.
+      const Bins bins(hi, lo);
+      clear_bins();
+      if (bins.has(mine)) atomicAdd(&sh.bins[bins.of(mine)], 1u);
+      scan_bins();
+      const int bin = first_bin(k);
+      if (bin < kBins) lo = fmaxf(lo, hi - (bin + 2) / (bins.up * bins.per));
+      cluster.sync();
+      if (k <= kFew / 2) {
+        const uint64_t border = rank_few(kept, hi, lo, k, 0.0, -1.0);
+        if (border) {
+          limit(kept, border);
+          return;
+        }
+      }
+    }
     for (int level = 0; hi > lo && level < kLevels; ++level) {
       const Bins bins(hi, lo);
       clear_bins();
@@ -614,6 +640,7 @@ __device__ __forceinline__ void sample_row(const Arguments &a, Shared &sh, int r
       if (x[i] > -INFINITY) e.low = fminf(e.low, x[i]);
     }
   }
+  const float mine = e.top;
   const auto join = [](Extent p, const Extent &q) {
     return Extent{max_nan(p.top, q.top), fminf(p.low, q.low)};
   };
@@ -641,7 +668,11 @@ __device__ __forceinline__ void sample_row(const Arguments &a, Shared &sh, int r
     cluster.sync();  // a block's extent is read until here
     return;
   }
-  Row<T> r{part, sh, cluster, blocks, rank, e.top, e.low, kLog2e / temperature};
+  // No larger than gives the logit next below the largest 2^-200 of its weight, so that as an f32 number
+  // the floor, too, is above 2^-1000.
+  const double scale = fmin(kLog2e / temperature, kSteep / fabs(static_cast<double>(e.top)));
+  const float floor = floor_of(e.top, scale);
+  Row<T> r{part, sh, cluster, blocks, rank, e.top, e.low, mine, scale, floor};
   Kept kept{-INFINITY, -kLargest, 0};
   const auto write = [&](int column, double w, double all) {
     a.tokens[row] = column;
@@ -691,7 +722,7 @@ __device__ __noinline__ void sample_rare_row(const Arguments &a, Shared &sh, int
 
 // Rows without limits. A block takes a row and goes over it once, a run of it a warp, with each warp's weights
 // by the largest logit of the first that it has met (and by a larger one, its sum scaled, where later ones'
-// weights pass 2^500). Then all of the block goes over the run of the warp that has the token.
+// weights pass 2^400). Then all of the block goes over the run of the warp that has the token.
 //
 // Ten 64-bit instructions a token bound it, 20 cycles of a quarter of an SM for 32 tokens, and one in eight
 // of those for its conversion: 2000 rows of 50257 bf16 logits take 131 us, where these alone take 56 and
@@ -714,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) draw_kernel(const __grid_con
   const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
   const double scale = kLog2e / temperature;
   // What is none of an ordinary row goes by the definition: also u = 0, for which weights must be 0 that
-  // are 2^-1000 here, and any that is not finite.
+  // are 2^-500 here, and any that is not finite.
   if (!(u > 0.0f && u < 1.0f && scale > 1e-30 && scale < 1e30)) {
     sample_rare_row<T>(a, sh, row);
     return;
@@ -725,9 +756,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) draw_kernel(const __grid_con
 
   const float scale_f = static_cast<float>(scale);
   float ref = -INFINITY, floor = -INFINITY;  // of the warp
-  double sum = 0.0, off = 0.0;
+  double sum = 0.0, ref_d = 0.0;
   const auto weigh = [&](float x) {
-    return power_of_two(sh.power, fma(static_cast<double>(fmaxf(x, floor)), scale, off));
+    return power_of_two(sh.power, static_cast<double>(fmaxf(x, floor)) - ref_d, scale);
   };
   const auto take = [&](const uint4 *raw, auto number) {
     constexpr int n = decltype(number)::value;
@@ -739,15 +770,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm) draw_kernel(const __grid_con
 #pragma unroll
       for (int i = 0; i < N; ++i) top = max_nan(top, x[i]);
     }
-    if (__any_sync(kAll, !((top - ref) * scale_f <= 500.0f))) {
+    if (__any_sync(kAll, !((top - ref) * scale_f <= 400.0f))) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(kAll, top, o));
-      if (!(top < INFINITY)) odd = 1;
+      if (!(top < INFINITY && fabsf(top) * scale_f < static_cast<float>(kSteep)) && top != -INFINITY) odd = 1;
       if (top == -INFINITY || odd) return;  // all of them are
       sum = ref == -INFINITY ? 0.0 : sum * exp2(fmax((static_cast<double>(ref) - top) * scale, -2000.0));
       ref = top;
-      off = -static_cast<double>(ref) * scale;
-      floor = fmaxf(-kLargest, __double2float_ru(ref - 1000.0 / scale));
+      ref_d = ref;
+      floor = floor_of(ref, scale);
     }
 #pragma unroll
     for (int k = 0; k < n; ++k) {
@@ -812,8 +843,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) draw_kernel(const __grid_con
   double start = owner ? __shfl_sync(kAll, upto, owner - 1) : 0.0;
   const double owner_by = __shfl_sync(kAll, by, owner);
   ref = __shfl_sync(kAll, mine, owner);
-  off = -static_cast<double>(ref) * scale;
-  floor = fmaxf(-kLargest, __double2float_ru(ref - 1000.0 / scale));
+  ref_d = ref;
+  floor = floor_of(ref, scale);
   const int each = (part.vectors + kThreads - 1) / kThreads * 32;
   const int begin = min(owner * each, part.vectors), end = min(begin + each, part.vectors);
   for (int v0 = begin; v0 < end; v0 += kThreads) {
