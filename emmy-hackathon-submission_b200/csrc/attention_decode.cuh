@@ -27,6 +27,13 @@
 // take 265 us (3.4 TB/s), bound by the instructions' latency at two warps a scheduler; 32-bit FMA
 // from shared memory took 735.
 //
+// Over a cache in 8 bits the products are turned, S^T = K Q^T and O^T = V^T P^T, so that keys and values
+// go in as the f16 numbers that their bytes become and eight rows of queries fill an operand; a pair has
+// 8 or 16 rows. Queries go in as one f16 number, by a power of two of their row (f32 ones as two), scores
+// are multiplied by their keys' scales in 32 bits, and weights by their values' before they are rounded.
+// Half the bytes of 16 bits, and three blocks an SM, as turning bytes to numbers takes the time that copies
+// leave: 48 sequences of up to 32768 keys, 64 heads on 8 of 128 in bf16, take 266 us (5.2 TB/s).
+//
 // Several queries' heads make more rows, 16 to a pair of their own, so each of their groups of 16
 // reads the keys again, from L2. What some row of a step must not see has weight 0 there; values
 // that are not finite are zeroed in such steps, and added again at the end for rows that see them. In

@@ -1,5 +1,6 @@
 """Calling the C ABI's operators on PyTorch tensors: the checks of arguments that
-``ptxgen.cache``, ``ptxgen.attention`` and ``ptxgen.logprob`` share, and the call itself.
+``ptxgen.cache``, ``ptxgen.attention``, ``ptxgen.sampling`` and ``ptxgen.logprob`` share, and the call
+itself.
 
 Single-token calls last a few microseconds on the GPU, so the host's part counts: the stream is
 asked for as a plain integer, and the device is only switched where it has to be.
