@@ -71,8 +71,14 @@ constexpr float kGrow = 8.0f;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 // What a cache holds: numbers of the type T; f16 ones whatever T is, as 2^-k (keys) and 2^-v (values) of
-// what they are, with the ints k and v for each page, of kKeys keys, at k_scale; or ones of 8 bits.
-enum Held { kOfType, kShifted, kBytes };
+// what they are, with the ints k and v for each page, of kKeys keys, at k_scale; the whole numbers of 8
+// bits as f16 ones, with Scales for each page there; or the 8 bits.
+enum Held { kOfType, kShifted, kWhole, kBytes };
+
+struct Scales {
+  int shift, unused[3];
+  float k[128], v[128];  // v's as 2^-shift of what they are, 1 at most
+};
 
 template <int DIM, Held HELD>
 struct Plan {
@@ -80,8 +86,10 @@ struct Plan {
   static constexpr int atom = 1024, chunks = DIM / 64, group = chunks * atom;
   static constexpr int tile = 16 * group;
   static constexpr int raw = HELD == kBytes ? kKeys * DIM : 0;  // keys or values in 8 bits, on their way
-  static constexpr int stages = DIM == 128 ? HELD == kBytes ? 4 : 5 : 8;
-  static constexpr int q = 0, ring = 2 * tile, raws = ring + stages * tile, bars = raws + 2 * raw;
+  static constexpr int stages = DIM == 128 ? HELD >= kWhole ? 4 : 5 : 8;
+  static constexpr int scales = HELD == kWhole ? 8 * 1024 : 0;  // a step's, for each warp of rows
+  static constexpr int q = 0, ring = 2 * tile, raws = ring + stages * tile, ks = raws + 2 * raw,
+                       bars = ks + scales;
   // over half an SM's shared memory, so that no other block that takes all its tensor memory
   // is resident beside this one
   static constexpr int bytes = 1024 + bars + 256;
@@ -358,12 +366,13 @@ __device__ __noinline__ void add_values(const Attention &a, const int *pages, in
 // Without TMA the maps and `boxes` are empty.
 // TREE: a sequence's new tokens are a tree. Where numbers are SHIFTED, queries are brought into f16 too, by
 // row; a row's scores are in powers of 2, with v added to them, so that its weights are what they are times
-// 2^v as its maximum is, and l takes them times 2^-v.
+// 2^v as its maximum is, and l takes them times 2^-v. Where they are WHOLE, scores are multiplied by their
+// keys' scales, and weights by their values' before they are rounded.
 template <class T, int DIM, bool TMA, bool TREE, Held HELD>
 __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
     prompt_kernel(const __grid_constant__ Attention a, const __grid_constant__ CUtensorMap k_map,
                   const __grid_constant__ CUtensorMap v_map, int run) {
-  constexpr bool SHIFTED = HELD != kOfType, K8 = HELD == kBytes;
+  constexpr bool SHIFTED = HELD != kOfType, K8 = HELD == kBytes, WHOLE = HELD == kWhole;
   using P = Plan<DIM, HELD>;
   using C = std::conditional_t<SHIFTED, __half, T>;  // what products are of
   static_assert(!(TMA && K8), "keys in 8 bits come by cp.async");
@@ -791,6 +800,17 @@ __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
                                              head * a.ks_head);
     };
     int2 next = shifts_of(0);
+    float4 *const ks = reinterpret_cast<float4 *>(smem + P::ks) + warp * 64;
+    float4 next_k = {}, next_v = {};
+    const auto scales_of = [&](int j) {
+      if (!WHOLE || j >= steps) return;
+      const Scales &x = *reinterpret_cast<const Scales *>(
+          a.k_scale + t.pages[blocks.key_block(b0 + j)] * a.ks_page + head * a.ks_head);
+      next.y = x.shift;
+      next_k = reinterpret_cast<const float4 *>(x.k)[lane];
+      next_v = reinterpret_cast<const float4 *>(x.v)[lane];
+    };
+    scales_of(0);
     const float m_to_2 = SHIFTED ? 1.0f : c;  // brings m into powers of 2
     const bool active = i < tiles;
     bool ok = true;
@@ -802,7 +822,17 @@ __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
         shift = next;
         next = shifts_of(j + 1);
       }
-      const float to_2 = SHIFTED ? c * pg::power_of_2(min(max(q_shift + shift.x, -126), 127)) : c;
+      if constexpr (WHOLE) {
+        __syncwarp();  // the last step's have been read
+        ks[lane] = make_float4(next_k.x * c, next_k.y * c, next_k.z * c, next_k.w * c);
+        ks[32 + lane] = next_v;
+        shift = next;
+        scales_of(j + 1);
+        __syncwarp();
+      }
+      const float to_2 = WHOLE     ? 1.0f
+                         : SHIFTED ? c * pg::power_of_2(min(max(q_shift + shift.x, -126), 127))
+                                   : c;
       const float plus = static_cast<float>(shift.y);
       float s[kKeys];
       uint32_t *const s_bits = reinterpret_cast<uint32_t *>(s);
@@ -811,6 +841,14 @@ __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
       wait_loads();
 #pragma unroll
       for (int k = 0; k < 4; ++k) tie(s_bits + 32 * k);
+      if constexpr (WHOLE) {
+#pragma unroll
+        for (int k = 0; k < kKeys / 4; ++k) {
+          const float4 x = ks[k];
+          mul(Two(s[4 * k], s[4 * k + 1]), Two(x.x, x.y)).get(s[4 * k], s[4 * k + 1]);
+          mul(Two(s[4 * k + 2], s[4 * k + 3]), Two(x.z, x.w)).get(s[4 * k + 2], s[4 * k + 3]);
+        }
+      }
       const int key0 = blocks.key_block(b0 + j) * kKeys;
       if (static_cast<unsigned>(j - whole) >= wholes) {
         asm volatile("" ::: "memory");  // a branch, not predicated instructions in every block
@@ -888,6 +926,10 @@ __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
           y = pg::exp2_fast(y);
           z = pg::exp2_fast(z);
           sum[e & 1] = add(sum[e & 1], Two(y, z));
+          if constexpr (WHOLE) {
+            const float2 by = reinterpret_cast<const float2 *>(ks + 32)[32 * k + e];
+            mul(Two(y, z), Two(by.x, by.y)).get(y, z);
+          }
           x[e] = Type<C>::pack(y, z);
         }
         tmem_store(s_at + 32 * k, x);
@@ -1070,15 +1112,17 @@ int launch_prompt(Attention a, int max_len, int64_t partial_bytes, int sms, cuda
   }
 }
 
+template <class T, bool TREE, Held HELD>
+int run_prompt_of(const Attention &a, int max_len, int64_t partial_bytes, int sms, cudaStream_t stream) {
+  return a.dim <= 64 ? launch_prompt<T, 64, TREE, HELD>(a, max_len, partial_bytes, sms, stream)
+                     : launch_prompt<T, 128, TREE, HELD>(a, max_len, partial_bytes, sms, stream);
+}
+
 template <bool TREE, Held HELD>
 int run_prompt(const Attention &a, bool bf16, int max_len, int64_t partial_bytes, int sms,
                cudaStream_t stream) {
-  if (bf16)
-    return a.dim <= 64
-               ? launch_prompt<__nv_bfloat16, 64, TREE, HELD>(a, max_len, partial_bytes, sms, stream)
-               : launch_prompt<__nv_bfloat16, 128, TREE, HELD>(a, max_len, partial_bytes, sms, stream);
-  return a.dim <= 64 ? launch_prompt<__half, 64, TREE, HELD>(a, max_len, partial_bytes, sms, stream)
-                     : launch_prompt<__half, 128, TREE, HELD>(a, max_len, partial_bytes, sms, stream);
+  return bf16 ? run_prompt_of<__nv_bfloat16, TREE, HELD>(a, max_len, partial_bytes, sms, stream)
+              : run_prompt_of<__half, TREE, HELD>(a, max_len, partial_bytes, sms, stream);
 }
 
 }  // namespace

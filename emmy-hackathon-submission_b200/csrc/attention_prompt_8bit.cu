@@ -6,12 +6,15 @@
 // a 16-bit cache with pages of 128 tokens, as many kv heads at a time as there is room for, and the kernel
 // runs over that.
 //
-// Either way they are widened to f16 for both types of results, as 2^-e of what they are, with one e for
+// For f16 results the whole numbers are what is widened, scores are multiplied by each key's scale and
+// weights by each value's, so that only these are rounded, as over 16 bits. Elsewhere, for bf16 results or
+// without room in the workspace, numbers go to f16 as 2^-e of what they are, with one e for
 // the keys, and one for the values, of a page of a head or of a block's part. bf16 would lose too much:
 // keys rounded to it change a score of 8 by a hundredth, and results by three times as much as all other
-// roundings together. (The whole numbers, with scores multiplied by each key's scale, lose nothing, but the
-// rows' threads took a third longer for it: two sequences of 2048 new tokens and up to 8192 keys, 32 heads
-// on 8 of 128 in bf16, 605 us so and 490 us in f16.)
+// roundings together. In f16 they add little to bf16 results (1.8e-3 off with their own rounding of 1.6e-3)
+// but would make f16 ones 4.9e-4 off, where theirs is 2.1e-4. The rows' threads bound it, so whole numbers
+// cost: two sequences of 2048 new tokens and up to 8192 keys, 32 heads on 8 of 128, take 490 us in bf16 and
+// 675 us in f16.
 #include "attention_prompt.cuh"
 
 namespace {
@@ -28,8 +31,9 @@ constexpr int kFewRounds = 3;
 
 // Block (i, h): keys 128 i.. of the batch's sequences, each with `blocks` such blocks, of kv head first + h;
 // block (i, heads + h) the values. HBM bounds it: a byte read and two written.
+template <bool WHOLE>
 __global__ void __launch_bounds__(kWiden)
-    widen_kernel(Attention a, int blocks, int first, int heads, char *k_to, char *v_to, int2 *shifts,
+    widen_kernel(Attention a, int blocks, int first, int heads, char *k_to, char *v_to, char *scales,
                  int *table, int *lens) {
   pg::wait_for_earlier_kernels();
   const int b = blockIdx.x / blocks, block = blockIdx.x - b * blocks;
@@ -76,9 +80,12 @@ __global__ void __launch_bounds__(kWiden)
   __syncthreads();
   const int shift = shift_of(top, values);
   const float by = pg::power_of_2(-shift);
+  const int64_t at_scales = static_cast<int64_t>(blockIdx.x) * heads + head;
+  Scales *const whole = reinterpret_cast<Scales *>(scales) + at_scales;
   if (!threadIdx.x) {
-    int2 *const to = shifts + static_cast<int64_t>(blockIdx.x) * heads + head;
-    (values ? to->y : to->x) = shift;
+    int2 *const to = reinterpret_cast<int2 *>(scales) + at_scales;
+    if (!WHOLE) (values ? to->y : to->x) = shift;
+    else if (values) whole->shift = shift + 8;
   }
   constexpr int kAhead = 4;  // loads a thread has in flight
   for (int i0 = threadIdx.x; i0 < kKeys * pieces; i0 += kWiden * kAhead) {
@@ -104,7 +111,15 @@ __global__ void __launch_bounds__(kWiden)
       const int i = i0 + u * kWiden;
       if (i >= kKeys * pieces) continue;
       uint4 out[2];
-      widen(raw[u], scale[u] * by, out);
+      if constexpr (WHOLE) {  // a scale that is not finite goes into the numbers
+        const bool finite = fabsf(scale[u]) < INFINITY;
+        widen(raw[u], finite ? 1.0f : scale[u], out);
+        if (i % pieces == 0)
+          (values ? whole->v : whole->k)[i / pieces] =
+              values ? finite ? scale[u] * by * 0x1p-8f : 0.0f : finite ? scale[u] : 1.0f;
+      } else {
+        widen(raw[u], scale[u] * by, out);
+      }
       to[2 * i] = out[0], to[2 * i + 1] = out[1];
     }
   }
@@ -120,18 +135,26 @@ int widen_first(Attention a, bool bf16, int max_len, int heads, int blocks, int 
     Attention b = a;
     const int64_t head_bytes = static_cast<int64_t>(kKeys) * a.dim * 2;
     char *const v = k + pages * n * head_bytes;
-    int2 *const shifts = reinterpret_cast<int2 *>(v + pages * n * head_bytes);
-    int rc = pg::launch<widen_kernel>("widen_kernel", dim3(pages, 2 * n), kWiden, 0, stream, a, blocks, first,
-                                      n, k, v, shifts, table, lens);
+    char *const scales = v + pages * n * head_bytes;
+    const auto widen_all = [&](auto whole) {
+      return pg::launch<widen_kernel<decltype(whole)::value>>("widen_kernel", dim3(pages, 2 * n), kWiden, 0,
+                                                              stream, a, blocks, first, n, k, v, scales, table,
+                                                              lens);
+    };
+    int rc = bf16 ? widen_all(std::false_type()) : widen_all(std::true_type());
     if (rc) return rc;
     b.q += first * a.group * a.q_head, b.out += first * a.group * a.out_head;
-    b.k = k, b.v = v, b.k_scale = reinterpret_cast<char *>(shifts);
+    b.k = k, b.v = v, b.k_scale = scales;
     b.k_head = b.v_head = head_bytes, b.k_page = b.v_page = n * head_bytes;
-    b.ks_head = 8, b.ks_page = n * 8;
+    b.ks_head = bf16 ? sizeof(int2) : sizeof(Scales), b.ks_page = n * b.ks_head;
     b.table = table, b.table_row = blocks, b.lens = lens, b.slots = nullptr;
     b.slot_rows = a.batch, b.heads = n, b.page_size = kKeys, b.width = blocks, b.pages = pages;
-    rc = a.mask ? run_prompt<true, kShifted>(b, bf16, max_len, kPartsBytes, sms, stream)
-                : run_prompt<false, kShifted>(b, bf16, max_len, kPartsBytes, sms, stream);
+    if (bf16)
+      rc = a.mask ? run_prompt_of<__nv_bfloat16, true, kShifted>(b, max_len, kPartsBytes, sms, stream)
+                  : run_prompt_of<__nv_bfloat16, false, kShifted>(b, max_len, kPartsBytes, sms, stream);
+    else
+      rc = a.mask ? run_prompt_of<__half, true, kWhole>(b, max_len, kPartsBytes, sms, stream)
+                  : run_prompt_of<__half, false, kWhole>(b, max_len, kPartsBytes, sms, stream);
     if (rc) return rc;
   }
   return PG_OK;
@@ -145,12 +168,14 @@ int prompt_8bit(const Attention &a, bool bf16, int max_len, int64_t partial_byte
                 cudaStream_t stream) {
   const int64_t blocks = (max_len + kKeys - 1ll) / kKeys, pages = a.batch * blocks;
   const int64_t room = partial_bytes - kPartsBytes - 4 * (pages + a.batch) - 256;
-  const int64_t each = pages * (kKeys * a.dim * 4ll + 8);  // of a kv head: keys, values and shifts
+  // of a kv head: keys, values and scales
+  const int64_t each = pages * (kKeys * a.dim * 4ll + (bf16 ? sizeof(int2) : sizeof(Scales)));
   int64_t heads = room > 0 ? room / each : 0;
   heads = heads < a.heads ? heads : a.heads;
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
-  if (heads >= 1 && pages <= INT32_MAX / 2 && rows >= kWidenRows * a.batch &&
-      (heads * kFewRounds >= a.heads || heads * rows >= static_cast<int64_t>(kRows) * sms)) {
+  if (heads >= 1 && pages <= INT32_MAX / 2 &&
+      (!bf16 || (rows >= kWidenRows * a.batch &&
+                 (heads * kFewRounds >= a.heads || heads * rows >= static_cast<int64_t>(kRows) * sms)))) {
     const int64_t rounds = (a.heads + heads - 1) / heads;  // as even as they come
     return widen_first(a, bf16, max_len, static_cast<int>((a.heads + rounds - 1) / rounds),
                        static_cast<int>(blocks), sms, stream);

@@ -14,10 +14,14 @@ bf16, 2^-11 f16, 2^-24 f32):
 * a bf16 result over 8 bits has its weights as one f16 number each, 2^-12 of itself off, independently:
   six times the root of that variance, 3.5 2^-12 S, more;
 * tiles of many rows round each weight once, independently: six times the root of that variance more,
-  3.5 e S, is met by one in 10^9 results. Over 8 bits weights, keys and values are in f16 for both types,
-  e = 2^-11 for these: half a step each, again at random, so the values add 1.75 e S, and a score has a
-  variance of c^2, c = e / 12^(1/2) times the scale and (sum q^2 k^2)^(1/2), the weights that much of
-  themselves and the result 6 c (S + |o|) with the largest c.
+  3.5 e S, is met by one in 10^9 results. Over 8 bits that is a weight times its value's scale, in f16
+  for both types, e = 2^-11 here. For f16 results keys and values are exact; a product below f16's normal
+  numbers is 2^-25 off with weights held at 2^7 and scales at 1 or less of a page's largest, doubled at
+  most, and numbers up to 127: 2^-32 2 127 s = 2^-31 max |v| for each of n keys. For bf16 ones (and f16
+  ones without room to widen in) keys and values are rounded to f16, too: half a step each, again at
+  random, so the values add 1.75 e S, and a score has a variance of c^2, c = e / 12^(1/2) times the scale
+  and (sum q^2 k^2)^(1/2), the weights that much of themselves and the result 6 c (S + |o|) with the
+  largest c.
 
 Heads above 128 are summed in f32 in order: n^(1/2) 2^-24 of the largest sum, within 4e-5 A at 4000."""
 
@@ -136,7 +140,8 @@ class Batch:
             out[r, sees] = True
         return torch.from_numpy(out).cuda()
 
-    def hold(self, got, window=0, sinks=0, tiles=False, scale=None, but=None) -> None:
+    def hold(self, got, window=0, sinks=0, tiles=False, scale=None, but=None,
+             rounded=False) -> None:
         import torch
 
         scale = self.dim ** -0.5 if scale is None else scale
@@ -169,7 +174,9 @@ class Batch:
                 e = UNIT["float16"] if self.bits8 else e
                 if tiles:
                     bound = bound + 3.5 * e * m
-                if tiles and self.bits8:
+                if tiles and self.bits8 and self.dtype is torch.float16:
+                    bound = bound + 2.0 ** -31 * n * float(v.abs().max())
+                if tiles and self.bits8 and (rounded or self.dtype is torch.bfloat16):
                     c = torch.einsum("tgd,kd->tgk", q[:, h] ** 2, k ** 2).sqrt()
                     c = c.masked_fill(~seen[:, None], 0.0).amax(-1, keepdim=True) * abs(scale)
                     bound = bound + 1.75 * e * m + 6 * c * e / 12 ** 0.5 * (m + o.abs())
@@ -330,16 +337,17 @@ def test_prompts_with_queries_of_any_size(ws, lens, news, max_len, size, dtype) 
 
 
 @pytest.mark.gpu
-def test_wide_tables_and_larger_workspaces(ws) -> None:
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_wide_tables_and_larger_workspaces(ws, dtype) -> None:
     """A table for far more tokens than there are: nothing of the workspace goes by it."""
     import torch
 
-    b = Batch([1500, 1000], [900, 700], 2, 4, 128, 16, "bfloat16", True)
+    b = Batch([1500, 1000], [900, 700], 2, 4, 128, 16, dtype, True)
     want = b.run(ws, max_len=1500)
     table = torch.full((2, 1 << 16), -1, dtype=torch.int32, device="cuda")
     table[:, :b.table.shape[1]] = b.table
     b.table, narrow = table, b.table
-    b.hold(b.run(ws), tiles=True)
+    b.hold(b.run(ws), tiles=True, rounded=True)
     b.table = narrow
     large = attention.Workspace(size=200 << 20)
     assert torch.equal(b.run(large, max_len=1500), want)
