@@ -172,6 +172,7 @@ int prompt_8bit(const Attention &a, bool bf16, int max_len, int64_t partial_byte
   const int64_t each = pages * (kKeys * a.dim * 4ll + (bf16 ? sizeof(int2) : sizeof(Scales)));
   int64_t heads = room > 0 ? room / each : 0;
   heads = heads < a.heads ? heads : a.heads;
+  heads = heads < 32767 ? heads : 32767;  // twice as many rows of blocks
   const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
   if (heads >= 1 && pages <= INT32_MAX / 2 &&
       (!bf16 || (rows >= kWidenRows * a.batch &&

@@ -357,6 +357,18 @@ def test_wide_tables_and_larger_workspaces(ws, dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_sequences_longer_than_max_len(cuda, dtype) -> None:
+    w = attention.Workspace()
+    b = Batch([1500, 1000], [900, 700], 2, 4, 128, 16, dtype, True)
+    got = b.run(w, max_len=1000)
+    with pytest.raises(CacheError) as e:
+        w.check()
+    assert e.value.bits == cache_module.TOO_LONG
+    b.hold(got, tiles=True, but=0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("news,masked", [([1, 1, 1], False), ([9, 9, 9], False), ([70, 60, 50], False),
                                          ([900, 400, 800], False), ([5, 6, 7], True), ([64, 60, 50], True)])
