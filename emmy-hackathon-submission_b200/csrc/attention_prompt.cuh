@@ -367,7 +367,7 @@ __device__ __noinline__ void add_values(const Attention &a, const int *pages, in
 // TREE: a sequence's new tokens are a tree. Where numbers are SHIFTED, queries are brought into f16 too, by
 // row; a row's scores are in powers of 2, with v added to them, so that its weights are what they are times
 // 2^v as its maximum is, and l takes them times 2^-v. Where they are WHOLE, scores are multiplied by their
-// keys' scales, and weights by their values' before they are rounded.
+// keys' scales, and weights by their values', which makes two f16 numbers: the rounded one and the rest.
 template <class T, int DIM, bool TMA, bool TREE, Held HELD>
 __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
     prompt_kernel(const __grid_constant__ Attention a, const __grid_constant__ CUtensorMap k_map,
@@ -702,6 +702,12 @@ __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
           mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k,
                  operand(v_at + k * 2 * P::group, P::group, P::atom), o_desc, add || k > 0,
                  elected);
+        if constexpr (WHOLE) {
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 64 + 8 * k,
+                   operand(v_at + k * 2 * P::group, P::group, P::atom), o_desc, true, elected);
+        }
       };
       const auto wait = [&](uint32_t bar, uint32_t parity) {
         return __all_sync(0xffffffffu, bar_wait(bar, parity, failed, a.status));
@@ -918,7 +924,7 @@ __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
       const Two c2(to_2, to_2), base2(base, base);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        uint32_t x[32];
+        uint32_t x[32], rest[WHOLE ? 32 : 1];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           float y, z;
@@ -931,8 +937,10 @@ __global__ void __launch_bounds__(HELD == kBytes ? kThreads8 : kThreads, 1)
             mul(Two(y, z), Two(by.x, by.y)).get(y, z);
           }
           x[e] = Type<C>::pack(y, z);
+          if constexpr (WHOLE) rest[e] = Type<C>::pack(y - Type<C>::low(x[e]), z - Type<C>::high(x[e]));
         }
         tmem_store(s_at + 32 * k, x);
+        if constexpr (WHOLE) tmem_store(s_at + 64 + 32 * k, rest);  // the scores there have been read
       }
       {
         float y, z;

@@ -7,14 +7,15 @@
 // runs over that.
 //
 // For f16 results the whole numbers are what is widened, scores are multiplied by each key's scale and
-// weights by each value's, so that only these are rounded, as over 16 bits. Elsewhere, for bf16 results or
+// weights by each value's, which go in as two f16 numbers, so that nothing but the result is rounded.
+// Elsewhere, for bf16 results or
 // without room in the workspace, numbers go to f16 as 2^-e of what they are, with one e for
 // the keys, and one for the values, of a page of a head or of a block's part. bf16 would lose too much:
 // keys rounded to it change a score of 8 by a hundredth, and results by three times as much as all other
 // roundings together. In f16 they add little to bf16 results (1.8e-3 off with their own rounding of 1.6e-3)
 // but would make f16 ones 4.9e-4 off, where theirs is 2.1e-4. The rows' threads bound it, so whole numbers
 // cost: two sequences of 2048 new tokens and up to 8192 keys, 32 heads on 8 of 128, take 490 us in bf16 and
-// 675 us in f16.
+// 892 us in f16 (675 with one number a weight, and results up to 1.5 times as far off).
 #include "attention_prompt.cuh"
 
 namespace {

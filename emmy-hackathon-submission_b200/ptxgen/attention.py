@@ -20,8 +20,8 @@ of its own branch, which ``mask`` names (``branches`` makes it of the tokens' pa
 Over a cache in 8 bits, ``k_scale`` and ``v_scale`` [pages, kv_heads, page_size] are one layer's scales
 (``PagedCache.k_scale[layer]``) and k and v int8. For few rows keys and values are what they stand for, and
 only the weights' products with the values' scales are rounded, to f16 numbers (one each for bf16 results,
-else two). For prompts of many rows, as below, that is one f16 number for both types, and bf16 ones have
-keys and values rounded to f16, too, as have f16 ones where the workspace has no room for one kv head's keys
+else two). Prompts of many rows, as below, with bf16 results have keys and values rounded to f16, too, as
+have f16 ones (and one number a weight) where the workspace has no room for one kv head's keys
 and values in 16 bits (96000 tokens of heads of 128 in all, by ``max_len`` or the table's width, in one of
 the default size). What is below 2^-22 of the largest scale loses digits there. A key or value whose scale is not finite makes the results
 that see it NaN. ``max_len`` must not be below a length then: such a sequence is cut, and ``Workspace.check``

@@ -391,9 +391,9 @@ int pg_attention(const pg_attention_args *args, uint64_t stream);
  * stands for its numbers times the float32 at k_scale + page * k_scale_page + head * k_scale_head + 4 r,
  * v_scale likewise (pg_cache8_write). dtype is the queries' and the result's. For few rows the numbers go
  * into the products as they are, and a weight times its value's scale as one f16 number for bf16 results
- * and two for others. For 16-bit types and many rows, as above, it is one f16 number, and for bf16 (and f16
- * where the workspace has no room for a kv head's keys and values in 16 bits, max_len or the table's width
- * of them a sequence) keys and values are rounded to f16, too. A workspace of more than
+ * and two for others. For many rows, as above, and bf16 keys and values are rounded to f16, too; so they are
+ * for f16, and weights go in as one number, where the workspace has no room for a kv head's keys and values
+ * in 16 bits, max_len or the table's width of them a sequence. A workspace of more than
  * PG_ATTENTION_WORKSPACE bytes is made use of; a sequence longer than max_len is then cut
  * (PG_CACHE_TOO_LONG). A scale that is not finite makes the result of the rows
  * that see it NaN.

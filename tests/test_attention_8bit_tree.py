@@ -14,14 +14,14 @@ bf16, 2^-11 f16, 2^-24 f32):
 * a bf16 result over 8 bits has its weights as one f16 number each, 2^-12 of itself off, independently:
   six times the root of that variance, 3.5 2^-12 S, more;
 * tiles of many rows round each weight once, independently: six times the root of that variance more,
-  3.5 e S, is met by one in 10^9 results. Over 8 bits that is a weight times its value's scale, in f16
-  for both types, e = 2^-11 here. For f16 results keys and values are exact; a product below f16's normal
-  numbers is 2^-25 off with weights held at 2^7 and scales at 1 or less of a page's largest, doubled at
-  most, and numbers up to 127: 2^-32 2 127 s = 2^-31 max |v| for each of n keys. For bf16 ones (and f16
-  ones without room to widen in) keys and values are rounded to f16, too: half a step each, again at
-  random, so the values add 1.75 e S, and a score has a variance of c^2, c = e / 12^(1/2) times the scale
-  and (sum q^2 k^2)^(1/2), the weights that much of themselves and the result 6 c (S + |o|) with the
-  largest c.
+  3.5 e S, is met by one in 10^9 results. Over 8 bits that is in f16 for bf16 results, e = 2^-11 here, and
+  keys and values are rounded to f16, too: half a step each, again at random, so the values add 1.75 e S,
+  and a score has a variance of c^2, c = e / 12^(1/2) times the scale and (sum q^2 k^2)^(1/2), the weights
+  that much of themselves and the result 6 c (S + |o|) with the largest c. So it is for f16 results without
+  room to widen in; with it, keys and values are exact there, and a weight times its value's scale goes in
+  as two f16 numbers, 2^-22 of itself off, but for what is below f16's normal numbers: 2^-25, with weights
+  held at 2^7, scales at half a page's largest or less and numbers up to 127, 2^-32 2 127 s = 2^-31 max |v|
+  for each of n keys.
 
 Heads above 128 are summed in f32 in order: n^(1/2) 2^-24 of the largest sum, within 4e-5 A at 4000."""
 
@@ -172,7 +172,8 @@ class Batch:
                     bound = bound + 3.5 * 2.0 ** -12 * m
                 # the tiles' products over 8 bits are in f16 for both types
                 e = UNIT["float16"] if self.bits8 else e
-                if tiles:
+                whole = self.bits8 and self.dtype is torch.float16 and not rounded
+                if tiles and not whole:
                     bound = bound + 3.5 * e * m
                 if tiles and self.bits8 and self.dtype is torch.float16:
                     bound = bound + 2.0 ** -31 * n * float(v.abs().max())
